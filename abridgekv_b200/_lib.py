@@ -50,6 +50,12 @@ SIGNATURES: dict[str, tuple] = {
         [c_vpp, c_vpp, c_vpp, c_i64p, c_vpp, c_i64p, c_vpp, c_int, c_int, c_int, c_int, c_int,
          c_int, c_int, C.c_float, c_int, c_vp, c_size, c_vp],
     ),
+    "abkv_decode_window_workspace_size": (c_size, [c_int] * 8 + [c_i32p, c_i32p, c_int]),
+    "abkv_decode_window": (
+        c_int,
+        [c_vpp, c_vpp, c_vpp, c_i64p, c_vpp, c_i64p, c_vpp, c_int, c_int, c_int, c_int, c_int,
+         c_int, c_int, C.c_float, c_int, c_i32p, c_i32p, c_vpp, c_i64p, c_int, c_int, c_vp, c_size, c_vp],
+    ),
     "abkv_decode_noalloc": (
         c_int,
         [c_vpp, c_vpp, c_vpp, c_i64p, c_vpp, c_i64p, c_vpp, c_int, c_int, c_int, c_int, c_int,

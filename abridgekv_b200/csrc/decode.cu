@@ -35,6 +35,7 @@
 // call with another plan may find the previous call's partials there), so a
 // workspace is ready for any later call on the same stream; concurrent calls
 // must not share a workspace.  Every mbarrier wait is bounded.
+#include <algorithm>
 #include <cstring>
 #include <mutex>
 
@@ -111,6 +112,7 @@ struct DecodeParams {
   int num_items;
   int warp_epi;  // 1: per-warp epilogue (one consumer warp per KV head, 16-byte aligned outputs)
   static constexpr bool kHasSide = false;
+  static constexpr bool kHasWin = false;
 };
 
 // Parameters of the packed-sidecar decode.  The plain decode is compiled from
@@ -120,6 +122,42 @@ struct SideDecodeParams : DecodeParams {
   SideArgs side[kMaxLayers];
   static constexpr bool kHasSide = true;
 };
+
+// Window, sinks and weight accumulators of one layer (abkv_decode_window).
+struct WinArgs {
+  float* weights;  // [B][units][w_cap] accumulators, or null
+  int64_t w_sb, w_su;
+  int window;      // visible rows: [slen - window, slen) and [0, sinks); 0 = every row
+  int sinks;
+  int w_cap;
+};
+
+// Parameters of the windowed / weight-accumulating decode.  The producer walks VIRTUAL tiles: the
+// tiles that hold sink rows, then those that hold window rows, so nothing else is loaded.
+struct WinDecodeParams : DecodeParams {
+  WinArgs win[kMaxLayers];
+  float* logits;  // [layers of the launch][B][Hq][lrows] scores (log2 units) by virtual row, or null
+  float* lse2;    // [layers][B][Hq] log-sum-exp (log2 units) of the finished rows, with logits
+  int lrows;
+  int units;      // accumulator rows per sequence: Hkv, or 1 (summed over all heads)
+  static constexpr bool kHasWin = true;
+};
+
+// Virtual-tile map of a sequence of n rows under (window, sinks): virtual tile v is cache tile
+// v < ns ? v : v + shift, and n_tiles virtual tiles cover every visible row.
+struct WinSpan {
+  int lo, ns, shift, n_tiles;
+};
+__device__ __forceinline__ WinSpan win_span(int n, int window, int sinks) {
+  WinSpan w;
+  const int ntl = (n + kTile - 1) / kTile;
+  w.lo = (window > 0 && n > window) ? n - window : 0;
+  const int s = min(sinks, w.lo);
+  w.ns = (s + kTile - 1) / kTile;
+  w.shift = max(w.lo / kTile - w.ns, 0);
+  w.n_tiles = ntl - w.shift;
+  return w;
+}
 
 // A group is either main tiles (16 rows x all KV heads; ok bit per tile, warp w
 // takes head w % Hkv of tile w / Hkv) or sidecar tiles of ONE KV head (the
@@ -291,7 +329,15 @@ __device__ void producer(const Prm& p, uint8_t* smem) {
         b = rem - li * p.B;
         slen = clamp_seq_len(p, p.layer[li], b, chunk == 0);
         // chunks [0, nside) cover the sidecar rows, head after head; the rest the main rows
-        const int ntl = (slen + kTile - 1) / kTile;
+        int ntl = (slen + kTile - 1) / kTile;
+        if constexpr (Prm::kHasWin) {
+          const WinArgs& W = p.win[li];
+          if (W.weights && slen > W.w_cap) {  // the accumulators hold fewer rows than the sequence
+            if (chunk == 0) set_error(p.err, ABKV_DEVERR_SEQ_OOB);
+            slen = W.w_cap;
+          }
+          ntl = win_span(slen, W.window, W.sinks).n_tiles;
+        }
         if constexpr (Prm::kHasSide) {
           const SideArgs& S = p.side[li];
           nside = scount = 0;
@@ -377,14 +423,28 @@ __device__ void producer(const Prm& p, uint8_t* smem) {
       }
     }
     // ---- main item: tiles of 16 rows x all KV heads through the block table
-    const int ntl = (slen + kTile - 1) / kTile;
+    int ntl = (slen + kTile - 1) / kTile;
+    WinSpan ws{0, 0, 0, 0};
+    if constexpr (Prm::kHasWin) {
+      ws = win_span(slen, p.win[li].window, p.win[li].sinks);
+      ntl = ws.n_tiles;
+    }
     const int tile0 = (chunk - nside) * p.chunk_tiles;
     const int tile1 = min(tile0 + p.chunk_tiles, ntl);
     const int ntiles = max(0, tile1 - tile0);
     const int page0 = tile0 * kTile / P;
-    const int npages = ntiles ? (tile1 * kTile + P - 1) / P - page0 : 0;
-    const int32_t* bt = L.bt + (int64_t)b * L.bt_stride + page0;
-    for (int i = lane; i < npages; i += 32) s_pages[i] = __ldg(bt + i);
+    if constexpr (Prm::kHasWin) {
+      // one page id per virtual tile (the chunk may jump from the sinks to the window)
+      const int32_t* bt = L.bt + (int64_t)b * L.bt_stride;
+      for (int i = lane; i < ntiles; i += 32) {
+        const int v = tile0 + i, t = v < ws.ns ? v : v + ws.shift;
+        s_pages[i] = __ldg(bt + (int64_t)t * kTile / P);
+      }
+    } else {
+      const int npages = ntiles ? (tile1 * kTile + P - 1) / P - page0 : 0;
+      const int32_t* bt = L.bt + (int64_t)b * L.bt_stride + page0;
+      for (int i = lane; i < npages; i += 32) s_pages[i] = __ldg(bt + i);
+    }
     __syncwarp();
     const int ngroups = max(1, (ntiles + nsub - 1) / nsub);
     for (int grp = 0; grp < ngroups; ++grp, ++gq) {
@@ -396,7 +456,10 @@ __device__ void producer(const Prm& p, uint8_t* smem) {
       int64_t pg = -1;
       if (lane < nt) {
         const int t = tg0 + lane;
-        pg = s_pages[(P == kTile ? t : t * kTile / P) - page0];
+        if constexpr (Prm::kHasWin)
+          pg = s_pages[t - tile0];
+        else
+          pg = s_pages[(P == kTile ? t : t * kTile / P) - page0];
         if (pg < 0 || pg >= L.num_blocks) {
           set_error(p.err, ABKV_DEVERR_PAGE_OOB);
           pg = -1;
@@ -423,7 +486,8 @@ __device__ void producer(const Prm& p, uint8_t* smem) {
       }
       __syncwarp();  // the expected byte count is posted before any copy can complete
       if (pg >= 0) {
-        const int t = tg0 + lane;
+        int t = tg0 + lane;
+        if constexpr (Prm::kHasWin) t = t < ws.ns ? t : t + ws.shift;
         uint8_t* dst = smem + kOffStage + (size_t)st * kStageBytes + (size_t)lane * 2 * tile_half;
         const __nv_bfloat16* ksrc = L.kv + pg * page_elems + (int64_t)((t * kTile) % P) * row_elems;
         bulk_g2s(dst, ksrc, (uint32_t)tile_half, &full[st]);
@@ -460,8 +524,8 @@ __device__ void producer(const Prm& p, uint8_t* smem) {
 // = dim 8g + 64 hh + 2i, o[4 hh + i][2 + jh] = the next dim); the row statistics
 // of query head r sit in lanes 4r..4r+3.  Arithmetic as the shared-memory merge
 // (one warp: weight exp2(0) = 1) and combine, so both epilogues give the same bits.
-template <int D, bool kGather>
-__device__ __forceinline__ void warp_epilogue(const DecodeParams& p, const LayerArgs& L, const StageMeta& M, int h,
+template <int D, class Prm, bool kGather>
+__device__ __forceinline__ void warp_epilogue(const Prm& p, const LayerArgs& L, const StageMeta& M, int h,
                                               int lane, const float (&o)[D / 16][4], float m_run, float l_run) {
   constexpr int kVH = D / 64;
   const int g = lane >> 2, c = lane & 3, G = p.G;
@@ -481,6 +545,9 @@ __device__ __forceinline__ void warp_epilogue(const DecodeParams& p, const Layer
       const int head = 2 * c + jh;
       if (head >= G) continue;
       const float Ls = lh[jh];
+      if constexpr (Prm::kHasWin) {
+        if (p.lse2 && g == 0) p.lse2[lb * p.Hq + h * G + head] = Ls > 0.f ? mh[jh] + log2f(Ls) : -INFINITY;
+      }
 #pragma unroll
       for (int hh = 0; hh < kVH; ++hh) {
         float v[8];
@@ -550,6 +617,9 @@ __device__ __forceinline__ void warp_epilogue(const DecodeParams& p, const Layer
         acc[hh][4] += f * bq.x; acc[hh][5] += f * bq.y; acc[hh][6] += f * bq.z; acc[hh][7] += f * bq.w;
       }
     }
+    if constexpr (Prm::kHasWin) {
+      if (p.lse2 && g == 0) p.lse2[lb * p.Hq + hr] = Ls > 0.f ? Mu + log2f(Ls) : -INFINITY;
+    }
 #pragma unroll
     for (int hh = 0; hh < kVH; ++hh) {
       float v[8];
@@ -616,11 +686,24 @@ __device__ void consumer(const Prm& p, uint8_t* smem) {
       // main tile: row T of KV head h at T * row_bytes + h * D * 2 of tile sub, rows < seq_len;
       // sidecar tile w: 16 slots of the item's head, K then V, rows < pages * quota
       const bool ok = (M.bits >> my_tile) & 1;
-      const int tok0 = (M.t0 + my_tile) * kTile;
+      int tok0 = (M.t0 + my_tile) * kTile;
+      int w_lo = 0, w_sinks = 0;
+      if constexpr (Prm::kHasWin) {
+        const WinSpan ws = win_span(M.seq_len, p.win[M.li].window, p.win[M.li].sinks);
+        if (M.t0 + my_tile >= ws.ns) tok0 += ws.shift * kTile;
+        w_lo = ws.lo;
+        w_sinks = p.win[M.li].sinks;
+      }
       int seq_len = M.seq_len;
       if constexpr (Prm::kHasSide) {
         if (side_grp) seq_len *= p.side[M.li].q[hw];
       }
+      auto row_ok = [&](int T) -> bool {  // row T of the tile is visible
+        if constexpr (Prm::kHasWin)
+          return tok0 + T < seq_len && (tok0 + T >= w_lo || tok0 + T < w_sinks);
+        else
+          return tok0 + T < seq_len;
+      };
       const int rstride = side_grp ? D * 2 : row_bytes;
       const int head_tile = kTile * D * 2;
       const uint8_t* kb = smem + kOffStage + (size_t)st * kStageBytes +
@@ -632,7 +715,7 @@ __device__ void consumer(const Prm& p, uint8_t* smem) {
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt) {
         const int T = 8 * nt + g;
-        const bool valid = ok && (tok0 + T < seq_len);
+        const bool valid = ok && row_ok(T);
         uint32_t kr[kQC][4];
 #pragma unroll
         for (int m = 0; m < kQC; ++m) {
@@ -654,9 +737,17 @@ __device__ void consumer(const Prm& p, uint8_t* smem) {
       for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const bool valid = ok && (tok0 + 8 * nt + 2 * c + j < seq_len);
+          const bool valid = ok && row_ok(8 * nt + 2 * c + j);
           x[nt][j] = valid ? s[nt][j] * sl2 : -INFINITY;
         }
+      if constexpr (Prm::kHasWin) {
+        if (p.logits && g < G) {  // the scores wait for the log-sum-exp of the whole row
+          float* lg = p.logits + (((int64_t)M.li * p.B + M.b) * p.Hq + hw * G + g) * p.lrows +
+                      (M.t0 + my_tile) * kTile + 2 * c;
+          *reinterpret_cast<float2*>(lg) = make_float2(x[0][0], x[0][1]);
+          *reinterpret_cast<float2*>(lg + 8) = make_float2(x[1][0], x[1][1]);
+        }
+      }
       float tmax = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
       tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 1));
       tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 2));
@@ -689,7 +780,7 @@ __device__ void consumer(const Prm& p, uint8_t* smem) {
         for (int i = 0; i < 4; ++i) {
           const int T = 2 * c + (i & 1) + 8 * (i >> 1);
           uint4 v = make_uint4(0, 0, 0, 0);
-          if (ok && (tok0 + T < seq_len)) v = lds128(vb + T * rstride + (64 * hh + 8 * g) * 2);
+          if (ok && row_ok(T)) v = lds128(vb + T * rstride + (64 * hh + 8 * g) * 2);
           vr[i][0] = v.x; vr[i][1] = v.y; vr[i][2] = v.z; vr[i][3] = v.w;
         }
 #pragma unroll
@@ -706,7 +797,7 @@ __device__ void consumer(const Prm& p, uint8_t* smem) {
     if (!(M.bits & kLast)) continue;
     if constexpr (!Prm::kHasSide) {
       if (p.warp_epi) {
-        warp_epilogue<D, kGather>(p, L, M, h, lane, o, m_run, l_run);
+        warp_epilogue<D, Prm, kGather>(p, L, M, h, lane, o, m_run, l_run);
         continue;
       }
     }
@@ -769,6 +860,9 @@ __device__ void consumer(const Prm& p, uint8_t* smem) {
       if (n_chunks == 1) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) store_out<D, kGather>(p, L, M.b, hr, d0 + k, val[k]);
+        if constexpr (Prm::kHasWin) {
+          if (p.lse2 && d0 == 0) p.lse2[lb * p.Hq + hr] = Ls > 0.f ? Mu + log2f(Ls) : -INFINITY;
+        }
       } else {
         *reinterpret_cast<float4*>(p.part_o + (prow + hr) * D + d0) = make_float4(val[0], val[1], val[2], val[3]);
         if (d0 == 0) p.part_lse[prow + hr] = Ls > 0.f ? Mu + log2f(Ls) : -INFINITY;
@@ -810,6 +904,9 @@ __device__ void consumer(const Prm& p, uint8_t* smem) {
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) store_out<D, kGather>(p, L, M.b, hr, d0 + k, Ls > 0.f ? Os[k] / Ls : 0.f);
+          if constexpr (Prm::kHasWin) {
+            if (p.lse2 && d0 == 0) p.lse2[lb * p.Hq + hr] = Ls > 0.f ? Mu + log2f(Ls) : -INFINITY;
+          }
         }
         if (threadIdx.x == 0) p.counters[lb] = 0;  // ready for the next call on this workspace
       }
@@ -842,6 +939,34 @@ __global__ void __launch_bounds__(kThreads, 1) decode_split_kernel(const __grid_
   }
 }
 
+// w[b][u][row] += sum over the query heads of unit u of softmax weight 2^(score - lse2), heads in order:
+// thread = (virtual row, unit) of one (layer, sequence).  Rows of a visible tile that the window hides
+// scored -inf and add nothing.
+constexpr int kWeightRows = 128;
+__global__ void __launch_bounds__(kWeightRows) decode_weights_kernel(const __grid_constant__ WinDecodeParams p) {
+  const int li = blockIdx.z / p.units, u = blockIdx.z % p.units, b = blockIdx.y;
+  const LayerArgs& L = p.layer[li];
+  const WinArgs& W = p.win[li];
+  const int n = min(clamp_seq_len(p, L, b, false), W.w_cap);
+  const WinSpan ws = win_span(n, W.window, W.sinks);
+  const int vr = blockIdx.x * kWeightRows + threadIdx.x;
+  if (blockIdx.x * kWeightRows >= ws.n_tiles * kTile) return;  // CTA-uniform
+  const int nh = p.Hq / p.units, h0 = u * nh;
+  const float* lse2 = p.lse2 + ((int64_t)(p.layer_base + li) * p.B + b) * p.Hq + h0;
+  const int row = vr < ws.ns * kTile ? vr : vr + ws.shift * kTile;
+  if (vr >= ws.n_tiles * kTile || row >= n) return;
+  const float* lg = p.logits + (((int64_t)li * p.B + b) * p.Hq + h0) * p.lrows + vr;
+  float acc = 0.f;
+#pragma unroll 8
+  for (int h = 0; h < nh; ++h) {
+    const float x = __ldcg(lg + (int64_t)h * p.lrows), l = __ldcg(lse2 + h);
+    acc += l == -INFINITY ? 0.f : exp2f(x - l);
+  }
+  float* w = W.weights + b * W.w_sb + u * W.w_su + row;
+  *w += acc;
+}
+
+constexpr int kMinWindowChunkTiles = 4;
 constexpr int kMaxAutoChunkTiles = 384;  // 6144 cache rows
 
 int auto_chunk_tiles(int num_layers, int num_seqs, int max_tiles, int page_tiles, int num_kv_heads) {
@@ -1184,6 +1309,175 @@ extern "C" int abkv_decode_gather(const void* const* q, const void* const* kv,
   return launch_decode(q, kv, block_tables, bt_strides, seq_lens, num_blocks, out, num_layers, num_seqs,
                        num_q_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq, scale, chunk_tokens,
                        workspace, workspace_bytes, stream, g);
+}
+
+// ---------------------------------------------------------------------------
+// Decode under a sliding window with sinks, optionally accumulating attention weights
+// (abkv_decode_window): the persistent kernel above over virtual tiles, then, for the layers that
+// accumulate, decode_weights_kernel.
+namespace abkv {
+namespace {
+// Layers per launch of a weight-accumulating call: their scores (4 bytes a query head and row) wait
+// in the workspace for the rows' log-sum-exp, so the workspace stays near this size.
+constexpr int64_t kLogitBytes = 64 << 20;
+
+struct WindowPlan {
+  int group;  // layers per launch; every launch reuses the same scratch
+  int chunk_tiles, max_chunks, lrows;
+  size_t off_lse, off_part_o, off_lse2, off_logits, total, counter_bytes;
+};
+
+int plan_window(int num_layers, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                int max_pages, int chunk_tokens, const int32_t* windows, const int32_t* sinks, bool weighted,
+                WindowPlan* plan) {
+  if (num_layers <= 0 || num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || page_size <= 0 ||
+      max_pages <= 0 || num_q_heads % num_kv_heads || chunk_tokens < 0 || chunk_tokens % kTile)
+    return ABKV_ERR_INVALID_ARG;
+  if ((head_dim != 64 && head_dim != kD) || page_size % kTile != 0 || num_seqs > 65535 ||
+      kWarps % num_kv_heads != 0 || num_q_heads / num_kv_heads > kMaxG)
+    return ABKV_ERR_UNSUPPORTED;
+  const int64_t rows_cap = (int64_t)max_pages * page_size;
+  if (rows_cap > ((int64_t)1 << 30)) return ABKV_ERR_UNSUPPORTED;
+  const int64_t max_tiles = rows_cap / kTile;
+  int64_t vt = 1;
+  for (int l = 0; l < num_layers; ++l) {
+    const int64_t w = windows ? windows[l] : 0, s = sinks ? sinks[l] : 0;
+    if (w < 0 || s < 0) return ABKV_ERR_INVALID_ARG;
+    // sink tiles + window tiles (one more where the window starts inside a tile)
+    const int64_t need = w == 0 ? max_tiles : (s + kTile - 1) / kTile + (w + kTile - 1) / kTile + 1;
+    vt = std::max(vt, std::min(need, max_tiles));
+  }
+  plan->lrows = (int)(vt * kTile);
+  plan->group = num_layers < kMaxLayers ? num_layers : kMaxLayers;
+  const int64_t layer_logits = (int64_t)num_seqs * num_q_heads * plan->lrows * 4;
+  if (weighted) plan->group = (int)std::max<int64_t>(1, std::min<int64_t>(plan->group, kLogitBytes / layer_logits));
+  int ct;
+  if (chunk_tokens) {
+    ct = chunk_tokens / kTile;
+  } else {
+    ct = 128;
+    while (ct > kMinWindowChunkTiles && plan->group * (int64_t)num_seqs * vt / ct < 148 * 4) ct >>= 1;
+  }
+  if (ct > kMaxChunkPages) return ABKV_ERR_UNSUPPORTED;
+  plan->chunk_tiles = ct;
+  plan->max_chunks = (int)((vt + ct - 1) / ct);
+  if ((int64_t)plan->max_chunks * plan->group * num_seqs > INT32_MAX) return ABKV_ERR_UNSUPPORTED;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  const size_t lb = (size_t)plan->group * num_seqs;
+  const size_t rows = plan->max_chunks > 1 ? lb * plan->max_chunks * num_q_heads : 0;
+  plan->counter_bytes = rows ? up(lb * num_kv_heads * 4) : 0;
+  plan->off_lse = kWsHeader + plan->counter_bytes;
+  plan->off_part_o = plan->off_lse + up(rows * 4);
+  plan->off_lse2 = plan->off_part_o + up(rows * head_dim * 4);
+  plan->off_logits = plan->off_lse2 + (weighted ? up(lb * num_q_heads * 4) : 0);
+  plan->total = plan->off_logits + (weighted ? up(lb * num_q_heads * (size_t)plan->lrows * 4) : 0);
+  return ABKV_OK;
+}
+}  // namespace
+}  // namespace abkv
+
+extern "C" size_t abkv_decode_window_workspace_size(int num_layers, int num_seqs, int num_q_heads, int num_kv_heads,
+                                                    int head_dim, int page_size, int max_pages_per_seq,
+                                                    int chunk_tokens, const int32_t* windows, const int32_t* sinks,
+                                                    int weighted) {
+  WindowPlan plan;
+  if (plan_window(num_layers, num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq,
+                  chunk_tokens, windows, sinks, weighted != 0, &plan) != ABKV_OK)
+    return 0;
+  return plan.total;
+}
+
+extern "C" int abkv_decode_window(const void* const* q, const void* const* kv, const int32_t* const* block_tables,
+                                  const int64_t* bt_strides, const int32_t* const* seq_lens,
+                                  const int64_t* num_blocks, void* const* out, int num_layers, int num_seqs,
+                                  int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                                  int max_pages_per_seq, float scale, int chunk_tokens, const int32_t* windows,
+                                  const int32_t* sinks, float* const* weights, const int64_t* weight_strides,
+                                  int weight_rows, int weight_units, void* workspace, size_t workspace_bytes,
+                                  void* stream) {
+  if (!q || !kv || !block_tables || !bt_strides || !seq_lens || !num_blocks || !out || !(scale > 0.f))
+    return ABKV_ERR_INVALID_ARG;
+  WindowPlan plan;
+  const int st = plan_window(num_layers, num_seqs, num_q_heads, num_kv_heads, head_dim, page_size,
+                             max_pages_per_seq, chunk_tokens, windows, sinks, weights != nullptr, &plan);
+  if (st != ABKV_OK) return st;
+  if (weights && (!weight_strides || weight_rows <= 0 || (weight_units != 1 && weight_units != num_kv_heads)))
+    return ABKV_ERR_INVALID_ARG;
+  if (!workspace || workspace_bytes < plan.total || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return ABKV_ERR_WORKSPACE;
+  bool out16 = true;
+  for (int l = 0; l < num_layers; ++l) {
+    if (!q[l] || !kv[l] || !block_tables[l] || !seq_lens[l] || !out[l] || bt_strides[l] <= 0 || num_blocks[l] <= 0 ||
+        (weights && !weights[l]))
+      return ABKV_ERR_INVALID_ARG;
+    if (((reinterpret_cast<uintptr_t>(q[l]) | reinterpret_cast<uintptr_t>(kv[l])) & 15) ||
+        (reinterpret_cast<uintptr_t>(block_tables[l]) & 3) || (reinterpret_cast<uintptr_t>(out[l]) & 1))
+      return ABKV_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(out[l]) & 15) out16 = false;
+  }
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  int dev = 0, num_sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || num_sms <= 0)
+    return ABKV_ERR_CUDA;
+  char* ws = static_cast<char*>(workspace);
+  WinDecodeParams prm;
+  memset(&prm, 0, sizeof(prm));
+  prm.gather.out_row = (int64_t)num_q_heads * head_dim;
+  prm.gather.world = 1;
+  prm.err = reinterpret_cast<int32_t*>(ws);
+  prm.work = reinterpret_cast<int32_t*>(ws + 64);
+  const bool split = plan.max_chunks > 1;
+  prm.counters = split ? reinterpret_cast<int32_t*>(ws + kWsHeader) : nullptr;
+  prm.part_lse = split ? reinterpret_cast<float*>(ws + plan.off_lse) : nullptr;
+  prm.part_o = split ? reinterpret_cast<float*>(ws + plan.off_part_o) : nullptr;
+  prm.lse2 = weights ? reinterpret_cast<float*>(ws + plan.off_lse2) : nullptr;
+  prm.logits = weights ? reinterpret_cast<float*>(ws + plan.off_logits) : nullptr;
+  prm.lrows = plan.lrows;
+  prm.units = weights ? weight_units : 1;
+  prm.scale_log2 = scale * 1.4426950408889634f;
+  prm.B = num_seqs;
+  prm.Hq = num_q_heads;
+  prm.Hkv = num_kv_heads;
+  prm.G = num_q_heads / num_kv_heads;
+  prm.P = page_size;
+  prm.chunk_tiles = plan.chunk_tiles;
+  prm.max_chunks = plan.max_chunks;
+  prm.max_rows = max_pages_per_seq * page_size;
+  prm.warp_epi = num_kv_heads == kWarps && out16 ? 1 : 0;
+  // other entry points leave their own data where the chunk counters are; every launch below
+  // leaves them at zero again
+  if (split && cudaMemsetAsync(prm.counters, 0, plan.counter_bytes, s) != cudaSuccess) return ABKV_ERR_CUDA;
+  for (int l0 = 0; l0 < num_layers; l0 += plan.group) {
+    const int nl = std::min(plan.group, num_layers - l0);
+    for (int i = 0; i < nl; ++i) {
+      LayerArgs& a = prm.layer[i];
+      a.q = static_cast<const __nv_bfloat16*>(q[l0 + i]);
+      a.kv = static_cast<const __nv_bfloat16*>(kv[l0 + i]);
+      a.bt = block_tables[l0 + i];
+      a.seq_lens = seq_lens[l0 + i];
+      a.out = static_cast<__nv_bfloat16*>(out[l0 + i]);
+      a.bt_stride = bt_strides[l0 + i];
+      a.num_blocks = num_blocks[l0 + i];
+      WinArgs& w = prm.win[i];
+      w.window = windows ? windows[l0 + i] : 0;
+      w.sinks = sinks ? sinks[l0 + i] : 0;
+      w.weights = weights ? weights[l0 + i] : nullptr;
+      w.w_sb = weights ? weight_strides[2 * (l0 + i)] : 0;
+      w.w_su = weights ? weight_strides[2 * (l0 + i) + 1] : 0;
+      w.w_cap = weight_rows;
+    }
+    prm.nl = nl;
+    prm.num_items = plan.max_chunks * nl * num_seqs;
+    const int rc = launch_kernel<WinDecodeParams, false>(prm, head_dim, std::min(prm.num_items, num_sms), s);
+    if (rc != ABKV_OK) return rc;
+    if (weights) {
+      const dim3 grid((plan.lrows + kWeightRows - 1) / kWeightRows, num_seqs, nl * prm.units);
+      decode_weights_kernel<<<grid, kWeightRows, 0, s>>>(prm);
+    }
+  }
+  if (cudaGetLastError() != cudaSuccess) return ABKV_ERR_CUDA;
+  return ABKV_OK;
 }
 
 // ---------------------------------------------------------------------------

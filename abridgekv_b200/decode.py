@@ -24,7 +24,7 @@ from typing import Sequence
 import torch
 
 from . import _lib
-from .workspace import Workspace, default_workspace
+from .workspace import Workspace, call_workspace, default_workspace
 
 def _check_cuda(name: str, t: torch.Tensor, dtype: torch.dtype | None = None) -> None:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -127,6 +127,124 @@ def _call_decode(lib, queries, kv_caches, block_tables, seq_lens, outs, L, B, Hq
         L, B, Hq, Hkv, D, page, max_pages_per_seq, float(scale), chunk_tokens,
         ws.ptr(), ws.nbytes, s.cuda_stream,
     )
+
+
+def _per_layer(name: str, value, L: int) -> list[int]:
+    """An int (or None) for every layer, or one entry per layer; None counts as 0."""
+    if value is None or isinstance(value, int):
+        value = [value] * L
+    out = [0 if v is None else int(v) for v in value]
+    if len(out) != L:
+        raise ValueError(f"{name} must be one number or one per layer ({L})")
+    if any(v < 0 or v > 0x7FFFFFFF for v in out):
+        raise ValueError(f"{name} must lie in [0, 2^31), got {out}")
+    return out
+
+
+def _decode_window(queries, kv_caches, block_tables, seq_lens, weights, window, num_sinks, scale, outputs,
+                   max_pages_per_seq, chunk_tokens, workspace, stream):
+    L = len(queries)
+    B, Hq, Hkv, D, page, outs = _validate(queries, kv_caches, block_tables, seq_lens, outputs)
+    device = queries[0].device
+    for ts in (queries, kv_caches, block_tables, seq_lens, outs, weights or ()):
+        if any(t.device != device for t in ts):
+            raise ValueError("every tensor of the call must be on the queries' device")
+    windows, sinks = _per_layer("window", window, L), _per_layer("num_sinks", num_sinks, L)
+    if max_pages_per_seq is None:
+        max_pages_per_seq = max(int(bt.shape[1]) for bt in block_tables)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    w_ptrs = w_strides = None
+    w_rows, units = 0, 1
+    if weights is not None:
+        if len(weights) != L:
+            raise ValueError("weights must hold one accumulator tensor per layer")
+        w_rows, units = int(weights[0].shape[-1]), int(weights[0].shape[1])
+        for w in weights:
+            _check_cuda("weights", w, torch.float32)
+            if w.dim() != 3 or w.shape[0] < B or w.shape[1] != units or w.shape[2] != w_rows or w.stride(2) != 1:
+                raise ValueError("every weights tensor must be [>=B, Hkv or 1, rows] with contiguous rows, "
+                                 f"got {tuple(w.shape)}")
+            if (B > 1 and w.stride(0) < w_rows) or (units > 1 and w.stride(1) < w_rows):
+                raise ValueError("the rows of weights must not overlap")
+        if units not in (1, Hkv):
+            raise ValueError(f"weights must hold one row per KV head ({Hkv}) or one per sequence, got {units}")
+        if len({w.data_ptr() for w in weights}) != L:
+            raise ValueError("every layer needs its own weights tensor")
+        w_ptrs = _lib.ptr_array([w.data_ptr() for w in weights])
+        w_strides = _lib.i64_array([x for w in weights for x in (w.stride(0), w.stride(1))])
+    if B == 0:
+        return outs
+    lib = _lib.lib()
+    win, snk = _lib.i32_array(windows), _lib.i32_array(sinks)
+    need = lib.abkv_decode_window_workspace_size(L, B, Hq, Hkv, D, page, max_pages_per_seq, chunk_tokens, win, snk,
+                                                 int(weights is not None))
+    if need == 0:
+        raise _lib.AbkvError("abkv_decode_window_workspace_size", 3,
+                             f"unsupported shape (B={B}, Hq={Hq}, Hkv={Hkv}, D={D}, page={page}, "
+                             f"chunk_tokens={chunk_tokens})")
+    s = torch.cuda.current_stream(device) if stream is None else stream
+    ws = call_workspace(device, s, need, workspace)
+    with torch.cuda.device(device):
+        st = lib.abkv_decode_window(
+            _lib.ptr_array([q.data_ptr() for q in queries]), _lib.ptr_array([kv.data_ptr() for kv in kv_caches]),
+            _lib.ptr_array([bt.data_ptr() for bt in block_tables]),
+            _lib.i64_array([bt.stride(0) for bt in block_tables]),
+            _lib.ptr_array([sl.data_ptr() for sl in seq_lens]), _lib.i64_array([kv.shape[0] for kv in kv_caches]),
+            _lib.ptr_array([o.data_ptr() for o in outs]), L, B, Hq, Hkv, D, page, max_pages_per_seq, float(scale),
+            chunk_tokens, win, snk, w_ptrs, w_strides, w_rows, units, ws.ptr(), ws.nbytes, s.cuda_stream)
+    _lib.check("abkv_decode_window", st)
+    return outs
+
+
+def paged_decode_window(
+    queries: Sequence[torch.Tensor],
+    kv_caches: Sequence[torch.Tensor],
+    block_tables: Sequence[torch.Tensor],
+    seq_lens: Sequence[torch.Tensor],
+    *,
+    window: int | None | Sequence[int | None],
+    num_sinks: int | Sequence[int] = 0,
+    scale: float | None = None,
+    outputs: Sequence[torch.Tensor] | None = None,
+    max_pages_per_seq: int | None = None,
+    chunk_tokens: int = 0,
+    workspace: Workspace | None = None,
+    stream: torch.cuda.Stream | None = None,
+) -> list[torch.Tensor]:
+    """``paged_decode`` under a sliding window with sinks (``abkv_decode_window``): the query of a
+    sequence of n rows sees its last ``window`` rows (its own among them) and its first
+    ``num_sinks`` rows.  ``window`` and ``num_sinks`` are one number, or one per layer; a window of
+    None or 0 shows every row, so layers with and without a window share a launch.  Pages that hold
+    no visible row are never read, and their block-table entries may be stale (freed pages)."""
+    return _decode_window(queries, kv_caches, block_tables, seq_lens, None, window, num_sinks, scale, outputs,
+                          max_pages_per_seq, chunk_tokens, workspace, stream)
+
+
+def paged_decode_weighted(
+    queries: Sequence[torch.Tensor],
+    kv_caches: Sequence[torch.Tensor],
+    block_tables: Sequence[torch.Tensor],
+    seq_lens: Sequence[torch.Tensor],
+    weights: Sequence[torch.Tensor],
+    *,
+    window: int | None | Sequence[int | None] = None,
+    num_sinks: int | Sequence[int] = 0,
+    scale: float | None = None,
+    outputs: Sequence[torch.Tensor] | None = None,
+    max_pages_per_seq: int | None = None,
+    chunk_tokens: int = 0,
+    workspace: Workspace | None = None,
+    stream: torch.cuda.Stream | None = None,
+) -> list[torch.Tensor]:
+    """``paged_decode_window`` that also adds every visible row's attention weight to ``weights``.
+
+    weights[l]: fp32 [>=B, units, rows], rows contiguous and at least as many as the longest
+    sequence (a longer sequence sets the workspace's SEQ_OOB bit and is cut): with units = Hkv,
+    unit u collects KV head u's query heads; with units = 1, all query heads.  The sums are taken in
+    head order, so repeated calls give the same bits.  ``compaction.evict_by_weight`` reads them."""
+    return _decode_window(queries, kv_caches, block_tables, seq_lens, list(weights), window, num_sinks, scale,
+                          outputs, max_pages_per_seq, chunk_tokens, workspace, stream)
 
 
 def attend_decode_batched(

@@ -52,3 +52,28 @@ def default_workspace(device: torch.device) -> Workspace:
     if ws is None:
         ws = _per_device[idx] = Workspace(torch.device("cuda", idx))
     return ws
+
+
+_per_stream: dict[tuple[int, int], Workspace] = {}
+
+
+def call_workspace(device: torch.device, stream: torch.cuda.Stream, nbytes: int,
+                   workspace: Workspace | None = None) -> Workspace:
+    """The workspace of one call: the caller's, else one that no other stream and no CUDA graph uses.
+
+    The device's default stream takes ``default_workspace`` (whose error word the caller reads there); any other
+    stream has its own.  A call under stream capture gets a fresh one from the graph's memory pool, zeroed
+    at every replay: two graphs never share it, and no later growth frees it under them.  (To read the
+    error word of a captured or side-stream call, pass a workspace of your own.)"""
+    if workspace is not None:
+        return workspace.ensure(nbytes)
+    with torch.cuda.device(device), torch.cuda.stream(stream):
+        if torch.cuda.is_current_stream_capturing():
+            return Workspace(device, nbytes)
+        if stream.cuda_stream == 0:
+            return default_workspace(device).ensure(nbytes)
+        key = (default_workspace(device).device.index, stream.cuda_stream)
+        ws = _per_stream.get(key)
+        if ws is None:
+            ws = _per_stream[key] = Workspace(torch.device("cuda", key[0]), nbytes)
+        return ws.ensure(nbytes)

@@ -107,6 +107,46 @@ int abkv_decode(const void* const* q, const void* const* kv,
                 int chunk_tokens, void* workspace, size_t workspace_bytes,
                 void* stream);
 
+/* Decode under a sliding window with sinks, and accumulation of attention
+ * weights.  No counterpart in the reference: the training-free ways of
+ * bounding a KV cache (a window with a few first tokens that stay visible, or
+ * eviction by accumulated weight) next to its learned compression.
+ * Arguments as abkv_decode, and per layer l (HOST arrays):
+ *   windows[l], sinks[l]  the query (at position seq_len - 1) sees row j iff
+ *       j >= seq_len - windows[l] or j < sinks[l]; windows[l] = 0 shows every
+ *       row (then sinks[l] says nothing); windows / sinks NULL = all 0.  Pages
+ *       that hold no visible row are never looked up: their block-table
+ *       entries may be stale.
+ *   weights[l]  (weights NULL = none) DEVICE float accumulators: for a visible
+ *       row j of sequence b,
+ *         weights[l][b * weight_strides[2l] + u * weight_strides[2l+1] + j]
+ *           += sum over the query heads of unit u of their softmax weight of j
+ *       with weight_units = num_kv_heads (unit u = KV head u's query heads) or
+ *       1 (all query heads), each sum taken in head order.  weight_rows rows
+ *       are addressable per unit; a longer sequence sets ABKV_DEVERR_SEQ_OOB
+ *       and is cut there.  Other elements are not touched.
+ * chunk_tokens: a multiple of 16, at most 8192 (0 = automatic).  A call with
+ * weights keeps scores in the workspace (about 64 MiB, or one layer's
+ * 4 x num_seqs x num_q_heads x visible rows if that is more) and runs its
+ * layers in as many launches as that takes. */
+size_t abkv_decode_window_workspace_size(int num_layers, int num_seqs, int num_q_heads,
+                                         int num_kv_heads, int head_dim, int page_size,
+                                         int max_pages_per_seq, int chunk_tokens,
+                                         const int32_t* windows, const int32_t* sinks,
+                                         int weighted);
+
+int abkv_decode_window(const void* const* q, const void* const* kv,
+                       const int32_t* const* block_tables, const int64_t* bt_strides,
+                       const int32_t* const* seq_lens, const int64_t* num_blocks,
+                       void* const* out, int num_layers, int num_seqs,
+                       int num_q_heads, int num_kv_heads, int head_dim,
+                       int page_size, int max_pages_per_seq, float scale,
+                       int chunk_tokens, const int32_t* windows,
+                       const int32_t* sinks, float* const* weights,
+                       const int64_t* weight_strides, int weight_rows,
+                       int weight_units, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 /* Decode that allocates nothing and takes no workspace.  No counterpart in the
  * reference: it exists for callers that cannot allocate device memory when
  * they decode (an engine that has reserved all of HBM for its KV cache, an
