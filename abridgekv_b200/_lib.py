@@ -103,6 +103,10 @@ SIGNATURES: dict[str, tuple] = {
                              c_vp, c_size, c_vp]),
     "abkv_gather_rows": (c_int, [c_vpp, c_vpp, c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64, c_vp,
                                  c_vp, c_size, c_vp]),
+    "abkv_evict_by_weight_workspace_size": (c_size, [c_int, c_int, c_int, c_i32p]),
+    "abkv_evict_by_weight": (c_int, [c_vpp, c_vpp, c_i64p, c_vpp, c_i64p, c_vpp, c_vpp, c_i64p, c_vpp, c_i64p, c_int,
+                                     c_vpp, c_i64p, c_int, c_vpp, c_i32p, c_int, c_int, c_int, c_int, c_int, c_int,
+                                     c_int, c_int, c_int, c_int, c_vp, c_size, c_vp]),
     "abkv_store_kv": (c_int, [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_int, c_i64, c_int, c_int, c_int,
                               c_vp, c_int, c_vp, c_size, c_vp]),
     "abkv_prefill_masked": (c_int, [c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i32p, c_vp,

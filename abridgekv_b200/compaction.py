@@ -10,6 +10,8 @@
   ``_execute_kv_copy_group`` (:1194-1220): one batch.
 * ``evict_columns(K, V, keep_cols)`` mirrors ``KVStore.evict``
   (abridgekv/gen_compress.py:72-77) for all layers in one launch.
+* ``evict_by_weight(...)`` picks the kept rows itself, by accumulated attention
+  weight, and compacts the paged caches, the weights and the lengths.
 
 Both paged layouts are accepted, detected like the reference: a leading dim of
 2 is the FlashAttention layout ``[2, num_blocks, page, Hkv, D]``, otherwise
@@ -20,13 +22,14 @@ from __future__ import annotations
 
 import itertools
 from collections.abc import Sequence as _SequenceABC
+from dataclasses import dataclass
 from typing import Hashable, Sequence
 
 import numpy as np
 import torch
 
 from . import _lib
-from .workspace import Workspace, default_workspace
+from .workspace import Workspace, call_workspace, default_workspace
 
 
 class CopyOps(_SequenceABC):
@@ -230,3 +233,113 @@ def evict_columns(K: Sequence[torch.Tensor], V: Sequence[torch.Tensor], keep_col
     _lib.check("abkv_gather_rows", st)
     L = len(K)
     return outs[:L], outs[L:]
+
+
+@dataclass(frozen=True)
+class Evicted:
+    """What ``evict_by_weight`` leaves, one entry per layer."""
+
+    seq_lens: list[torch.Tensor]            # [B] int32 new lengths
+    weights: list[torch.Tensor]             # [B, units, rows] fp32: the kept rows' weights, then zeros
+    keep: list[torch.Tensor] | None         # [B, units, budget] int32 kept rows in order, then -1
+
+
+def evict_by_weight(kv_caches: Sequence[torch.Tensor], block_tables: Sequence[torch.Tensor],
+                    seq_lens: Sequence[torch.Tensor], weights: Sequence[torch.Tensor], *,
+                    budget: int | Sequence[int], num_sinks: int = 0, num_recent: int = 0,
+                    dst_block_tables: Sequence[torch.Tensor] | None = None, return_keep: bool = False,
+                    in_place_weights: bool = False, workspace: Workspace | None = None,
+                    stream: torch.cuda.Stream | None = None) -> Evicted:
+    """Bring every sequence back to ``budget`` rows by accumulated attention weight (``abkv_evict_by_weight``).
+
+    Of a sequence of n > budget rows, the first ``num_sinks``, the last ``num_recent`` and the
+    heaviest of the others stay, in their order (ties to the lower row); a shorter sequence
+    keeps all.  kv_caches[l]: paged, either layout, 2-byte elements; block_tables[l]: [>=B, pages] int32;
+    seq_lens[l]: [B] int32; weights[l]: fp32 [>=B, units, rows] as ``decode.paged_decode_weighted`` and
+    ``codestep.paged_prompt_weights`` accumulate them: with units = Hkv every KV head keeps its
+    own rows, with units = 1 all heads keep the same.  ``budget``: one number, or one per layer.
+
+    Rows move inside the sequence's own pages (the pages past the new length are then free), or,
+    with ``dst_block_tables``, into the pages of those tables, which must be other pages of the same
+    caches.  The new weights are new tensors of ``weights``' shape, or ``weights`` themselves with
+    ``in_place_weights``.  ``seq_lens`` stays as it was; go on with the returned lengths."""
+    L = len(kv_caches)
+    if L == 0 or not (L == len(block_tables) == len(seq_lens) == len(weights)):
+        raise ValueError("per-layer argument lists must be non-empty and of equal length")
+    if dst_block_tables is not None and len(dst_block_tables) != L:
+        raise ValueError("dst_block_tables must hold one table per layer")
+    budgets = [int(budget)] * L if isinstance(budget, int) else [int(x) for x in budget]
+    if len(budgets) != L:
+        raise ValueError(f"budget must be one number or one per layer ({L})")
+    num_sinks, num_recent = int(num_sinks), int(num_recent)
+    if num_sinks < 0 or num_recent < 0 or any(m <= 0 or num_sinks + num_recent > m or m > 1 << 30 for m in budgets):
+        raise ValueError("every budget must be positive and hold num_sinks + num_recent rows (both >= 0), "
+                         f"got budget {budgets}, num_sinks {num_sinks}, num_recent {num_recent}")
+    dev = kv_caches[0].device
+    layout, _, page, hkv, d = _layout_of(kv_caches[0])
+    B = int(seq_lens[0].shape[0])
+    units, rows = int(weights[0].shape[1]) if weights[0].dim() == 3 else 0, int(weights[0].shape[-1])
+
+    def check(name, t, dtype):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or (dtype is not None and t.dtype != dtype):
+            raise TypeError(f"{name} must be a{'' if dtype is None else ' ' + str(dtype)} CUDA tensor "
+                            "(libabkv has no CPU path)")
+        if t.device != dev:
+            raise ValueError(f"{name} must be on the caches' device")
+
+    for l in range(L):
+        kv, w = kv_caches[l], weights[l]
+        check("kv_cache", kv, None)
+        if _layout_of(kv)[0] != layout or _layout_of(kv)[2:] != (page, hkv, d) or not kv.is_contiguous():
+            raise ValueError("every KV cache must be contiguous and share layout, page size, heads and head size")
+        if kv.element_size() != 2:
+            raise TypeError("the caches must hold 2-byte elements")
+        for name, bt in (("block_table", block_tables[l]),) + (
+                (("dst_block_table", dst_block_tables[l]),) if dst_block_tables is not None else ()):
+            check(name, bt, torch.int32)
+            if bt.dim() != 2 or bt.shape[0] < B or not bt.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous [>=B, max_pages] tensor")
+        check("seq_lens", seq_lens[l], torch.int32)
+        if tuple(seq_lens[l].shape) != (B,) or not seq_lens[l].is_contiguous():
+            raise ValueError("seq_lens must be a contiguous [B] tensor, the same B for every layer")
+        check("weights", w, torch.float32)
+        if w.dim() != 3 or w.shape[0] < B or w.shape[1] != units or w.shape[2] != rows or (rows > 1 and
+                                                                                           w.stride(2) != 1):
+            raise ValueError("every weights tensor must be [>=B, Hkv or 1, rows] with contiguous rows")
+        if in_place_weights and ((w.shape[0] > 1 and w.stride(0) < rows) or (units > 1 and w.stride(1) < rows)):
+            raise ValueError("the rows of weights must not overlap")
+    if units not in (1, hkv):
+        raise ValueError(f"weights must hold one row per KV head ({hkv}) or one per sequence, got {units}")
+    if len({kv.data_ptr() for kv in kv_caches}) != L and dst_block_tables is None:
+        raise ValueError("every layer needs its own cache tensor")
+    if in_place_weights and len({w.data_ptr() for w in weights}) != L:
+        raise ValueError("every layer needs its own weights tensor")
+    s = torch.cuda.current_stream(dev) if stream is None else stream
+    lib = _lib.lib()
+    with torch.cuda.device(dev), torch.cuda.stream(s):
+        new = [torch.empty(B, dtype=torch.int32, device=dev) for _ in range(L)]
+        outs = list(weights) if in_place_weights else [torch.empty((B, units, rows), dtype=torch.float32, device=dev)
+                                                       for _ in range(L)]
+        keep = [torch.empty((B, units, m), dtype=torch.int32, device=dev) for m in budgets] if return_keep else None
+        result = Evicted(new, outs, keep)
+        if B == 0:
+            return result
+        if rows == 0:
+            raise ValueError("weights must hold at least one row")
+        c_budget = _lib.i32_array(budgets)
+        need = 256 if return_keep else lib.abkv_evict_by_weight_workspace_size(L, B, units, c_budget)
+        ws = call_workspace(dev, s, need, workspace)
+        pa, ia = _lib.ptr_array, _lib.i64_array
+        st = lib.abkv_evict_by_weight(
+            pa([t.data_ptr() for t in kv_caches]), pa([t.data_ptr() for t in block_tables]),
+            ia([t.stride(0) for t in block_tables]),
+            pa([t.data_ptr() for t in dst_block_tables]) if dst_block_tables is not None else None,
+            ia([t.stride(0) for t in dst_block_tables]) if dst_block_tables is not None else None,
+            pa([t.data_ptr() for t in seq_lens]), pa([t.data_ptr() for t in new]),
+            ia([_layout_of(t)[1] for t in kv_caches]), pa([t.data_ptr() for t in weights]),
+            ia([x for t in weights for x in (t.stride(0), t.stride(1))]), rows, pa([t.data_ptr() for t in outs]),
+            ia([x for t in outs for x in (t.stride(0), t.stride(1))]), rows,
+            pa([t.data_ptr() for t in keep]) if keep is not None else None, c_budget, L, B, units, layout, hkv, d, page,
+            max(int(t.shape[1]) for t in block_tables), num_sinks, num_recent, ws.ptr(), ws.nbytes, s.cuda_stream)
+    _lib.check("abkv_evict_by_weight", st)
+    return result

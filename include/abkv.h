@@ -414,6 +414,48 @@ int abkv_gather_rows(const void* const* src, void* const* dst, int num_tensors,
                      int64_t row_bytes, const int64_t* keep, void* workspace,
                      size_t workspace_bytes, void* stream);
 
+/* Eviction by accumulated attention weight (the accumulators of
+ * abkv_decode_window / abkv_prompt_weights).  No counterpart in the reference,
+ * whose KVStore.evict takes the kept columns from its block layout.
+ * For layer l (HOST arrays of num_layers entries), sequence b of n =
+ * seq_lens[l][b] rows and unit u (weight_units = num_kv_heads: every KV head
+ * keeps its own rows; 1: all heads keep the same rows):
+ *   n <= budgets[l]: every row is kept.  Otherwise the first num_sinks rows, the
+ *   last num_recent rows and, of the others, the heaviest by
+ *   weights[l][b * weight_strides[2l] + u * weight_strides[2l+1] + row] up to
+ *   budgets[l] rows in all (ties to the lower row; NaN counts as -inf).
+ * Kept rows stay in order: kept row i moves to row i of block_tables[l] (in
+ * place) or, with dst_block_tables, to row i of that table's pages in the same
+ * cache, which must not be pages of any source table (not checked).
+ * new_lens[l][b] = min(n, budget) (another buffer than seq_lens[l]).
+ * weights_out[l] (weights[l] itself with the same strides, or a buffer that does
+ * not overlap it) gets the kept rows' weights, then zeros up to weight_out_rows.
+ * keep (optional): keep[l] DEVICE [num_seqs][weight_units][budgets[l]] kept
+ * rows, then -1.  num_sinks + num_recent <= budgets[l].
+ * Supported: head_dim 64 or 128, num_kv_heads in {1,2,4,8}, 2-byte elements, both
+ * paged layouts (kv_layout as abkv_compact), num_seqs <= 8191.
+ * A length past the table or the weights sets ABKV_DEVERR_SEQ_OOB and is cut; a
+ * page id out of range sets ABKV_DEVERR_PAGE_OOB and its rows do not move.
+ * workspace: abkv_evict_by_weight_workspace_size (256 bytes with keep). */
+size_t abkv_evict_by_weight_workspace_size(int num_layers, int num_seqs, int weight_units,
+                                           const int32_t* budgets);
+
+int abkv_evict_by_weight(void* const* kv, const int32_t* const* block_tables,
+                         const int64_t* bt_strides,
+                         const int32_t* const* dst_block_tables,
+                         const int64_t* dst_strides,
+                         const int32_t* const* seq_lens, int32_t* const* new_lens,
+                         const int64_t* num_blocks, const float* const* weights,
+                         const int64_t* weight_strides, int weight_rows,
+                         float* const* weights_out,
+                         const int64_t* weight_out_strides, int weight_out_rows,
+                         int32_t* const* keep, const int32_t* budgets,
+                         int num_layers, int num_seqs, int weight_units,
+                         int kv_layout, int num_kv_heads, int head_dim,
+                         int page_size, int max_pages_per_seq, int num_sinks,
+                         int num_recent, void* workspace, size_t workspace_bytes,
+                         void* stream);
+
 /* The step's new K / V rows into the paged cache, before attention: the
  * slot write vLLM's attention backend makes at the start of
  * AttentionImpl.forward (reshape_and_cache_flash in vLLM 0.13.0, the
