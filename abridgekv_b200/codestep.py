@@ -25,7 +25,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .workspace import Workspace, default_workspace
+from .workspace import Workspace, call_workspace, default_workspace, on_stream
 
 
 def _layout_of(kv: torch.Tensor, num_kv_heads: int) -> tuple[int, int, int]:
@@ -160,6 +160,103 @@ def paged_prefill(query: torch.Tensor, kv_cache: torch.Tensor, block_table: torc
                                                ws.nbytes, s.cuda_stream)
     _lib.check("abkv_paged_prefill" + ("_packed" if sidecar is not None else ""), st)
     return out
+
+
+def _window(window, num_sinks) -> tuple[int, int]:
+    w, s = 0 if window is None else int(window), int(num_sinks)
+    if not (0 <= w <= 0x7FFFFFFF and 0 <= s <= 0x7FFFFFFF):
+        raise ValueError(f"window and num_sinks must lie in [0, 2^31), got {window} and {num_sinks}")
+    return w, s
+
+
+def _same_device(query, **tensors) -> None:
+    for name, t in tensors.items():
+        if t is not None and t.device != query.device:
+            raise ValueError(f"{name} must be on the query's device")
+
+
+def paged_prefill_window(query: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor,
+                         seq_lens: torch.Tensor, query_start_loc: torch.Tensor, *, max_query_len: int,
+                         num_kv_heads: int, window: int | None, num_sinks: int = 0, scale: float | None = None,
+                         num_requests: int | None = None, out: torch.Tensor | None = None, return_lse: bool = False,
+                         workspace: Workspace | None = None, stream: torch.cuda.Stream | None = None):
+    """``paged_prefill`` under a sliding window with sinks (``abkv_paged_prefill_window``): the row at
+    position p of its request sees cache rows j <= p with j > p - window or j < num_sinks.  A window
+    of None or 0 shows every row j <= p.  Pages that hold no visible row are never read, and their
+    block-table entries may be stale (freed pages).
+
+    Returns out [T, Hq, D], or (out, lse) with ``return_lse``: lse [T, Hq] fp32, the natural-log
+    log-sum-exp of each row's scaled scores, which ``paged_prompt_weights`` takes.  Rows of no request
+    are left untouched (in a new lse: NaN)."""
+    window, num_sinks = _window(window, num_sinks)
+    with on_stream(stream):  # what the call allocates belongs to the stream that uses it
+        head, out, R, nb, page, T, scale = _prepare(query, kv_cache, block_table, seq_lens, query_start_loc, None,
+                                                    scale, None, num_requests, out, num_kv_heads=num_kv_heads)
+        lse = torch.full((T, query.shape[1]), float("nan"), dtype=torch.float32, device=query.device) \
+            if return_lse else None
+    _same_device(query, kv_cache=kv_cache, block_table=block_table, seq_lens=seq_lens, out=out,
+                 query_start_loc=query_start_loc)
+    if int(max_query_len) <= 0 or int(max_query_len) > T:
+        raise ValueError(f"max_query_len must be in [1, T={T}]")
+    dev = query.device
+    s = torch.cuda.current_stream(dev) if stream is None else stream
+    ws = call_workspace(dev, s, 256, workspace)
+    with torch.cuda.device(dev):
+        st = _lib.lib().abkv_paged_prefill_window(
+            *head[:6], lse.data_ptr() if lse is not None else None, *head[6:], int(max_query_len), T, scale, window,
+            num_sinks, ws.ptr(), ws.nbytes, s.cuda_stream)
+    _lib.check("abkv_paged_prefill_window", st)
+    return (out, lse) if return_lse else out
+
+
+def paged_prompt_weights(query: torch.Tensor, lse: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor,
+                         seq_lens: torch.Tensor, query_start_loc: torch.Tensor, weights: torch.Tensor, *,
+                         max_query_len: int, num_kv_heads: int, observe: int | None = None, window: int | None = None,
+                         num_sinks: int = 0, scale: float | None = None, num_requests: int | None = None,
+                         workspace: Workspace | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+    """Add the attention weights of prompt rows to per-row accumulators (``abkv_prompt_weights``).
+
+    The arguments of ``paged_prefill_window`` (same window, num_sinks and scale) plus the ``lse`` [T, Hq] it
+    returned.  Request r's counted rows are its last ``observe`` query rows (None: all of them); every
+    cache row that they see collects their softmax weight in ``weights`` [>=R, units, rows] fp32 (rows
+    contiguous, at least as many as the longest sequence): unit u = KV head u's query heads, or one unit
+    for all heads.  The sums' order is fixed, so repeated calls give the same bits.  Returns weights."""
+    window, num_sinks = _window(window, num_sinks)
+    obs = 0 if observe is None else int(observe)
+    if observe is not None and obs <= 0:
+        raise ValueError(f"observe must be positive (or None for every row), got {observe}")
+    for name, t in (("lse", lse), ("weights", weights)):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32:
+            raise TypeError(f"{name} must be a float32 CUDA tensor")
+    head, _, R, nb, page, T, scale = _prepare(query, kv_cache, block_table, seq_lens, query_start_loc, None, scale,
+                                              None, num_requests, query, num_kv_heads=num_kv_heads)
+    _same_device(query, kv_cache=kv_cache, block_table=block_table, seq_lens=seq_lens, lse=lse, weights=weights,
+                 query_start_loc=query_start_loc)
+    Hq, Hkv, D = query.shape[1], int(num_kv_heads), query.shape[2]
+    if tuple(lse.shape) != (T, Hq) or not lse.is_contiguous():
+        raise ValueError(f"lse must be the attention's contiguous [{T}, {Hq}] log-sum-exp")
+    if weights.dim() != 3 or weights.shape[0] < R or weights.shape[1] not in (1, Hkv) or weights.shape[2] == 0 or \
+            weights.stride(2) != 1:
+        raise ValueError(f"weights must be [>=R, Hkv or 1, rows] with contiguous rows, got {tuple(weights.shape)}")
+    units, rows = int(weights.shape[1]), int(weights.shape[2])
+    if (R > 1 and weights.stride(0) < rows) or (units > 1 and weights.stride(1) < rows):
+        raise ValueError("the rows of weights must not overlap")
+    if int(max_query_len) <= 0 or int(max_query_len) > T:
+        raise ValueError(f"max_query_len must be in [1, T={T}]")
+    dev = query.device
+    s = torch.cuda.current_stream(dev) if stream is None else stream
+    lib = _lib.lib()
+    max_rows = min(int(block_table.shape[1]) * page, rows)
+    if R == 0 or max_rows == 0:
+        return weights
+    ws = call_workspace(dev, s, lib.abkv_prompt_weights_workspace_size(R, Hkv, max_rows, units), workspace)
+    with torch.cuda.device(dev):
+        st = lib.abkv_prompt_weights(
+            query.data_ptr(), query.stride(0), query.stride(1), lse.data_ptr(), *head[6:14], weights.data_ptr(),
+            weights.stride(0), weights.stride(1), rows, units, R, Hq, Hkv, D, int(max_query_len), max_rows, T, obs,
+            scale, window, num_sinks, ws.ptr(), ws.nbytes, s.cuda_stream)
+    _lib.check("abkv_prompt_weights", st)
+    return weights
 
 
 def check_op_ownership(ops: np.ndarray, op_offsets: np.ndarray, block_table_host, seq_lens_host,

@@ -71,14 +71,15 @@ constexpr int kOffKV = 2 * kQBytes;
 constexpr int kOffBar = kOffKV + kStages * kStageBytes;
 // mbarriers (u64 slots from kOffBar): q_full, kv_full[kStages], kv_empty[kStages] (one
 // arrival per head's P.V), s_full[head][S buffer], p_full[head][S buffer], o_done[head],
-// o_full[head], v_zero[2] (head A's softmax warps have zeroed the V rows past the valid rows
-// of the last sidecar tile / the last cache tile: head B's P.V of that tile waits for it),
+// o_full[head], v_zero[3] (head A's softmax warps have zeroed the V rows past the valid rows
+// of the last sidecar tile / the last cache tile: head B's P.V of that tile waits for it; under a
+// window, one per tile that holds rows hidden from the whole query tile, in tile order),
 // then the TMEM address.  p_full is double-buffered like S: a head's softmax may finish tile j+1
 // before the MMA thread has taken tile j's P, and one barrier per buffer keeps the
 // two arrivals in different barriers (a parity wait cannot tell phases 2 apart).
 constexpr int kBarKvFull = 1, kBarKvEmpty = kBarKvFull + kStages, kBarSFull = kBarKvEmpty + kStages,
               kBarPFull = kBarSFull + 4, kBarODone = kBarPFull + 4, kBarOFull = kBarODone + 2,
-              kBarVZero = kBarOFull + 2, kBarTmem = kBarVZero + 2;
+              kBarVZero = kBarOFull + 2, kBarTmem = kBarVZero + 3;
 static_assert((kBarTmem + 1) * 8 <= 256, "barrier area");
 constexpr int kOffList = kOffBar + 256;         // visited key tiles (tile indices)
 constexpr int kMaxKeyTiles = 2048;              // keys up to 2048 x 64 = 128K rows
@@ -130,6 +131,10 @@ struct alignas(64) CodeStepParams {
   int64_t side_bt_stride, side_pages;
   int side_off[8], side_q[8];
   int has_side;
+  // window mode (kWin, causal): the row at position p sees cache rows j <= p with j > p - window
+  // (window 0: all) or j < n_sink; lse (optional): [T][H] natural-log log-sum-exp of the rows
+  int window, n_sink;
+  float* lse;
 };
 
 // The last CTA of request blockIdx.z applies that request's copy ops.  Every CTA of the request
@@ -294,6 +299,11 @@ __device__ __forceinline__ void softmax_half(const CodeStepParams& p, int lim, i
   tmem_wait_st();
 }
 
+// kWin: the causal mode under a sliding window with sinks (abkv_paged_prefill_window).  The key tiles
+// hidden from every row of the query tile are not visited (rows [n_sink, w_lo) are hidden from all of
+// them); in a visited tile, 16-row slices inside that range are not loaded -- their pages may be freed --
+// and its V rows are zeroed; the rest is the per-row hole of softmax_half.
+template <bool kWin>
 __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_constant__ CodeStepParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -309,7 +319,8 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar + kBarTmem);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int qt = blockIdx.x;  // query tile of the request's code rows
+  // query tile of the request's rows; without a window the last tiles see the most keys: first
+  const int qt = kWin ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x;
   const int hk = blockIdx.y / p.npairs, hp = blockIdx.y % p.npairs;
   const int hA = hk * p.G + 2 * hp;
   const int hB = (2 * hp + 1 < p.G) ? hA + 1 : -1;  // odd group size: the last pair has one head
@@ -317,6 +328,9 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
   int kt_end = 0, seq_len = 0, leffA = 0, leffB = 0, hole_s = 0, hole_e = 0;
   int qlen = p.Kc;  // the request's query rows (all Kc code rows in the code step)
   int n_side = 0, side_tiles = 0;  // sidecar rows of this CTA's KV head, in 64-row tiles
+  // kWin: rows [n_sink, w_lo) are hidden from the whole query tile; visited tile i is key tile
+  // i < w_ns ? i : i + w_shift
+  int w_lo = 0, w_ns = 0, w_shift = 0;
   {
     // every thread reads the same values, so an early return is CTA-uniform and
     // happens before any barrier, TMEM allocation or copy
@@ -338,7 +352,8 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
     // trim identity: a head with quota q sees rows [0, seq_len - (Kc - q)) --
     // its own code slots >= q are the last Kc - q rows of the request
     int sl = __ldg(p.seq_lens + b);
-    const int64_t cap = min(p.bt_stride * (int64_t)p.page, (int64_t)kMaxKeyTiles * kBN);
+    const int64_t cap = kWin ? min(p.bt_stride * (int64_t)p.page, (int64_t)INT32_MAX - kBN)
+                             : min(p.bt_stride * (int64_t)p.page, (int64_t)kMaxKeyTiles * kBN);
     if (sl < qlen || (int64_t)sl > cap) {
       if (threadIdx.x == 0) set_error(p.err, ABKV_DEVERR_SEQ_OOB);
       sl = sl < qlen ? qlen : (int)cap;
@@ -374,7 +389,13 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
       n_side = cnt * p.side_q[hk];
     }
     side_tiles = (n_side + kBN - 1) / kBN;
-    if (side_tiles + kt_end > kMaxKeyTiles) {  // the tile list would not hold them: skip the request
+    if constexpr (kWin) {
+      if (p.window > 0) w_lo = max(0, seq_len - qlen + qt * kBM - p.window + 1);
+      const int sinks = min(p.n_sink, w_lo);
+      w_ns = (sinks + kBN - 1) / kBN;
+      w_shift = max(w_lo / kBN - w_ns, 0);
+    }
+    if (side_tiles + kt_end - w_shift > kMaxKeyTiles) {  // the tile list would not hold them: skip the request
       if (threadIdx.x == 0) set_error(p.err, ABKV_DEVERR_SEQ_OOB);
       return;
     }
@@ -391,8 +412,8 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
     for (int i = 0; i < 2; ++i) {
       mbar_init(&o_done[i], 1);
       mbar_init(&o_full[i], 1);
-      mbar_init(&v_zero[i], 256);
     }
+    for (int i = 0; i < 3; ++i) mbar_init(&v_zero[i], 256);
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)),
@@ -404,14 +425,18 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
   int32_t* s_nlist = s_list + kMaxKeyTiles;
   if (warp == 2) {
     int n = 0;
+    if constexpr (kWin) {
+      n = kt_end - w_shift;
+      for (int i = lane; i < n; i += 32) s_list[i] = i < w_ns ? i : i + w_shift;
+    }
     // sidecar tiles first (entry -(t + 1) = sidecar tile t), all visible
-    for (int base = 0; base < side_tiles; base += 32) {
+    for (int base = 0; !kWin && base < side_tiles; base += 32) {
       const int t = base + lane;
       const uint32_t m = __ballot_sync(0xffffffffu, t < side_tiles);
       if (t < side_tiles) s_list[n + __popc(m & ((1u << lane) - 1u))] = -(t + 1);
       n += __popc(m);
     }
-    for (int base = 0; base < kt_end; base += 32) {
+    for (int base = 0; !kWin && base < kt_end; base += 32) {
       const int kt = base + lane;
       // tiles entirely inside the exclusion range are skipped for both heads
       const bool vis = kt < kt_end && !(kt * kBN >= hole_s && kt * kBN + kBN <= hole_e);
@@ -466,6 +491,7 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
         }
         const int row0 = s_list[j] * kBN + 16 * (lane & 3);
         if (row0 >= seq_len) return -1;
+        if (kWin && row0 >= p.n_sink && row0 + 16 <= w_lo) return -1;  // hidden from every row of the tile
         const int v = __ldg(p.bt + (int64_t)b * p.bt_stride + row0 / p.page);
         if (v < 0 || (int64_t)v >= p.num_blocks) {
           set_error(p.err, ABKV_DEVERR_PAGE_OOB);
@@ -525,8 +551,23 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
       // head B's P.V of a partial tile (the last sidecar tile, the last cache tile) waits
       // until head A's softmax warps have zeroed its V rows past the valid rows; the two
       // tile indices, read before any MMA is issued
-      int jz0 = -1, jz1 = -1;
-      if (hs == 1) {
+      int jz0 = -1, jz1 = -1, jz2 = -1;
+      if (kWin) {
+        // tiles with rows hidden from the whole query tile: the one the sinks end in, the one the
+        // window starts in, the last (each once, in order)
+        if (hs == 1) {
+          int t0 = -1, t1 = -1, t2 = -1;
+          if (w_lo > p.n_sink && p.n_sink % kBN) t0 = p.n_sink / kBN;
+          if (w_lo > p.n_sink && w_lo % kBN) t1 = w_lo / kBN;
+          if (seq_len % kBN && (seq_len - 1) / kBN == kt_end - 1) t2 = kt_end - 1;
+          if (t1 == t0) t1 = -1;
+          if (t2 == t0 || t2 == t1) t2 = -1;
+          auto idx = [&](int t) { return t < 0 ? -1 : (t < w_ns ? t : t - w_shift); };
+          jz0 = idx(t0);
+          jz1 = idx(t1);
+          jz2 = idx(t2);
+        }
+      } else if (hs == 1) {
         if (n_side % kBN) jz0 = side_tiles - 1;
         if (n_tiles > side_tiles && (seq_len % kBN) && s_list[n_tiles - 1] == (seq_len - 1) / kBN) jz1 = n_tiles - 1;
       }
@@ -557,6 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
         issue_s(sbase + 64 * t, t);
         umma_commit(&s_full[2 * hs + t]);
       }
+      int nz = 0;  // kWin: zeroed tiles waited for
       for (int j = 0; j < n && !dead; ++j) {
         const int st = j % kStages, st2 = (j + 2) % kStages;
         const bool more = j + 2 < n;
@@ -565,8 +607,12 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
         // softmax(j) has released
         if (more && !wait_or_abort(&kv_full[st2], (uint32_t)(((j + 2) / kStages) & 1), dead, p.err)) break;
         if (!wait_or_abort(&p_full[2 * hs + (j & 1)], (uint32_t)((j >> 1) & 1), dead, p.err)) break;
-        if (j == jz0 && !wait_or_abort(&v_zero[0], 0, dead, p.err)) break;
-        if (j == jz1 && !wait_or_abort(&v_zero[1], 0, dead, p.err)) break;
+        if constexpr (kWin) {
+          if ((j == jz0 || j == jz1 || j == jz2) && !wait_or_abort(&v_zero[nz++], 0, dead, p.err)) break;
+        } else {
+          if (j == jz0 && !wait_or_abort(&v_zero[0], 0, dead, p.err)) break;
+          if (j == jz1 && !wait_or_abort(&v_zero[1], 0, dead, p.err)) break;
+        }
         tc_fence_after();
         issue_pv(sbase + 64 * (j & 1) + kPCol, st, j == 0);
         umma_commit(&o_done[hs]);
@@ -600,9 +646,15 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
       // causal: row q sees seq_len - qlen + q + 1 keys (rows past the request's
       // last row, which are never written, take the last row's limit)
       const int leff = p.causal ? seq_len - qlen + min(q, qlen - 1) + 1 : (head_slot ? leffB : leffA);
+      // kWin: rows [n_sink, p - window + 1) are hidden from the row at position p
+      if (kWin && p.window > 0 && leff - p.window > p.n_sink) {
+        hole_s = p.n_sink;
+        hole_e = leff - p.window;
+      }
+      int nz = 0;
       for (int j = 0; j < n_tiles; ++j) {
         const int e = s_list[j];
-        const bool side = e < 0;  // sidecar tile -(e + 1): every query row sees its rows
+        const bool side = !kWin && e < 0;  // sidecar tile -(e + 1): every query row sees its rows
         const int lim = side ? min(max(n_side - (-e - 1) * kBN, 0), kBN) : min(max(leff - e * kBN, 0), kBN);
         // valid rows of the tile: the rest was not loaded (V zeroed below)
         const int valid = side ? n_side - (-e - 1) * kBN : seq_len - e * kBN;
@@ -613,7 +665,21 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
                                    wait_or_abort(&s_full[2 * head_slot + (j & 1)], (uint32_t)((j >> 1) & 1), dead, p.err));
         if (!ok) dead = true;
         tc_fence_after();
-        if (ok && head_slot == 0 && valid < kBN) {
+        if constexpr (kWin) {
+          // V rows at or past seq_len, or hidden from every row of the query tile (w_hs .. w_he)
+          const int w_hs = max(p.n_sink - e * kBN, 0), w_he = min(w_lo - e * kBN, kBN);
+          if (ok && head_slot == 0 && (valid < kBN || w_hs < w_he)) {
+            uint8_t* vb = smem + kOffKV + (j % kStages) * kStageBytes + kKVHalf;
+            for (int idx = sw * 32 + lane; idx < 2 * kBN * 8; idx += 256) {
+              const int r = (idx >> 3) & (kBN - 1);
+              if (r >= valid || (r >= w_hs && r < w_he))
+                *reinterpret_cast<uint4*>(vb + (idx >> 9) * (kKVHalf / 2) + r * 128 + (idx & 7) * 16) =
+                    make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            mbar_arrive_one(&v_zero[nz++]);
+          }
+        } else if (ok && head_slot == 0 && valid < kBN) {
           // V rows at or past seq_len (or the sidecar segment's end): stale page
           // slots or unloaded slices become zeros before either head's P.V reads
           // them (P is 0 there, but 0 * NaN would not be)
@@ -654,6 +720,9 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
         // quota and the exclusion hide everything) is written as zeros
         const bool none = !(l > 0.f);
         const float inv = none ? 0.f : 1.f / l;
+        if (kWin && p.lse && half == 0 && q < qlen)
+          p.lse[(int64_t)(__ldg(p.q_start + b) + q) * p.H + h] =
+              none ? -INFINITY : (st.m_run + log2f(l)) * 0.6931471805599453f;  // natural log
         __nv_bfloat16* orow =
             p.out + (int64_t)(__ldg(p.q_start + b) + q) * p.o_ss + (int64_t)h * p.o_sh + 64 * half;
 #pragma unroll 1
@@ -725,6 +794,12 @@ struct CommitArgs {
   int32_t* count;      // device [R], zeroed
 };
 
+// Window of the causal mode (abkv_paged_prefill_window).
+struct WindowOpts {
+  int window, n_sink;
+  float* lse;
+};
+
 int code_step_launch(const void* q, int64_t q_row_stride, int64_t q_head_stride, void* out,
                      int64_t out_row_stride, int64_t out_head_stride, const int32_t* q_start,
                      const void* kv_cache, int kv_layout, int64_t num_blocks, int page_size,
@@ -732,7 +807,7 @@ int code_step_launch(const void* q, int64_t q_row_stride, int64_t q_head_stride,
                      const int32_t* excluded, const int32_t* quota_per_kv_head, int R, int Hq,
                      int Hkv, int head_dim, int K_code, int T, float scale, void* workspace,
                      size_t workspace_bytes, void* stream, const CommitArgs* commit, int causal_max_qlen = 0,
-                     const abkv_sidecar_t* side = nullptr);
+                     const abkv_sidecar_t* side = nullptr, const WindowOpts* win = nullptr);
 
 constexpr size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 size_t commit_workspace(int R, int64_t n_ops) {
@@ -764,6 +839,21 @@ extern "C" int abkv_paged_prefill(const void* q, int64_t q_row_stride, int64_t q
                           kv_cache, kv_layout, num_blocks, page_size, block_table, bt_stride, seq_lens, nullptr,
                           nullptr, R, Hq, Hkv, head_dim, 0, T, scale, workspace, workspace_bytes, stream, nullptr,
                           max_query_len);
+}
+
+extern "C" int abkv_paged_prefill_window(const void* q, int64_t q_row_stride, int64_t q_head_stride, void* out,
+                                         int64_t out_row_stride, int64_t out_head_stride, float* lse,
+                                         const int32_t* query_start_loc, const void* kv_cache, int kv_layout,
+                                         int64_t num_blocks, int page_size, const int32_t* block_table,
+                                         int64_t bt_stride, const int32_t* seq_lens, int R, int Hq, int Hkv,
+                                         int head_dim, int max_query_len, int T, float scale, int window,
+                                         int num_sinks, void* workspace, size_t workspace_bytes, void* stream) {
+  if (max_query_len <= 0 || window < 0 || num_sinks < 0) return ABKV_ERR_INVALID_ARG;
+  const WindowOpts win{window, num_sinks, lse};
+  return code_step_launch(q, q_row_stride, q_head_stride, out, out_row_stride, out_head_stride, query_start_loc,
+                          kv_cache, kv_layout, num_blocks, page_size, block_table, bt_stride, seq_lens, nullptr,
+                          nullptr, R, Hq, Hkv, head_dim, 0, T, scale, workspace, workspace_bytes, stream, nullptr,
+                          max_query_len, nullptr, &win);
 }
 
 extern "C" int abkv_code_step_attention_packed(
@@ -862,7 +952,7 @@ int code_step_launch(const void* q, int64_t q_row_stride, int64_t q_head_stride,
                      const int32_t* excluded, const int32_t* quota_per_kv_head, int R, int Hq,
                      int Hkv, int head_dim, int K_code, int T, float scale, void* workspace,
                      size_t workspace_bytes, void* stream, const CommitArgs* commit, int causal_max_qlen,
-                     const abkv_sidecar_t* side) {
+                     const abkv_sidecar_t* side, const WindowOpts* win) {
   const bool causal = causal_max_qlen > 0;  // abkv_paged_prefill: no quotas, no exclusion, no copies
   if (!q || !out || !q_start || !kv_cache || !block_table || !seq_lens || (!causal && !quota_per_kv_head))
     return ABKV_ERR_INVALID_ARG;
@@ -971,8 +1061,15 @@ int code_step_launch(const void* q, int64_t q_row_stride, int64_t q_head_stride,
     prm.side_pages = side->num_pages;
     prm.has_side = 1;
   }
-  if (cudaFuncSetAttribute(codestep_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) !=
-      cudaSuccess)
+  auto kernel = codestep_kernel<false>;
+  if (win) {
+    if (!causal || side || commit) return ABKV_ERR_INVALID_ARG;
+    prm.window = win->window;
+    prm.n_sink = win->n_sink;
+    prm.lse = win->lse;
+    kernel = codestep_kernel<true>;
+  }
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) != cudaSuccess)
     return ABKV_ERR_CUDA;
   if (commit) {
     prm.cops = commit->ops;
@@ -983,7 +1080,7 @@ int code_step_launch(const void* q, int64_t q_row_stride, int64_t q_head_stride,
     prm.ctas_per_req = (K_code / kBM) * Hkv * prm.npairs;
   }
   dim3 grid(causal ? (causal_max_qlen + kBM - 1) / kBM : K_code / kBM, Hkv * prm.npairs, R);
-  codestep_kernel<<<grid, kThreads, kSmemBytes, reinterpret_cast<cudaStream_t>(stream)>>>(prm);
+  kernel<<<grid, kThreads, kSmemBytes, reinterpret_cast<cudaStream_t>(stream)>>>(prm);
   if (cudaGetLastError() != cudaSuccess) return ABKV_ERR_CUDA;
   return ABKV_OK;
 }

@@ -1,0 +1,476 @@
+// Attention weights of prompt rows over the paged KV cache, summed per cache row, on 5th-generation
+// tensor cores (tcgen05 + TMEM) for sm_100a.
+//
+// For KV head h of a request of n rows, cache row j, and the request's counted query rows i (its last
+// `observe` rows, or all) at positions p_i = n - qlen + i:
+//   w[j] += sum over i and the query heads g of h, where j <= p_i and (no window or j > p_i - window or
+//           j < sinks), of exp(scale q_ig . k_j - lse_ig)
+// with lse the log-sum-exp that the attention of these rows returned, so one pass over the keys is
+// enough and nothing is rescaled.
+//
+// A tile of S^T = K Q^T (128 cache rows x 128 query columns) per step: the accumulator's lanes are
+// cache rows, so the sum over queries is a sum over a thread's own registers, no reduction across lanes
+// and no second product.  The 128 columns are 4 units of 32 consecutive query rows of one head (so a
+// group of 4 heads x 32 observed rows is one full tile).  19 warps:
+//   warp 0      K tiles (eight 16-row page slices, 2-stage ring) by cp.async.bulk.tensor, 128B swizzle
+//   warp 18     Q tiles (four 32-row boxes, 4-stage ring); where every counted row of a request fits one
+//               tile, it is loaded once for all cache tiles of a (request, head) run
+//   warp 1      TMEM owner (4 S^T buffers) and issuer of tcgen05.mma
+//   warps 2..17 thread = one cache row and one unit's 32 columns: x = S scale log2(e) - lse log2(e), 2^x, sum
+// The exponentials bound it: 128 x 128 of them take 1024 clocks of the SM's 16 a clock, the tile's MMAs
+// 256 (head_dim 128).  Work items are (cache tile, KV head, request); a CTA per SM takes them round
+// robin, the cache tiles that the most rows see first -- or, where Q stays resident, a contiguous run.
+// The sum's order is fixed (units, then the four column groups), so results repeat bit for bit.
+// With one accumulator row for all heads, per-head sums go through the workspace and are added in head order.
+// Every mbarrier wait is bounded and records ABKV_DEVERR_TIMEOUT on expiry.
+#include <algorithm>
+#include <cstring>
+
+#include "tcgen05.cuh"
+
+namespace abkv {
+namespace {
+using namespace tc;
+
+constexpr int kM = 128, kN = 128, kD = 128;  // cache rows, query columns, head_dim
+constexpr int kUnit = 32;                    // query rows of a unit
+constexpr int kThreads = 608;
+constexpr int kWarpQ = 18;
+constexpr int kKStages = 2, kQStages = 4, kSBufs = 4;
+constexpr uint32_t kIdescS = idesc_bf16_m128(kN, false);
+constexpr int kTileBytes = kM * kD * 2;  // 2 atoms of [128 rows][128 B]
+constexpr int kOffK = 0;
+constexpr int kOffQ = kOffK + kKStages * kTileBytes;
+constexpr int kOffLse = kOffQ + kQStages * kTileBytes;  // 16 warps x 32 floats
+constexpr int kOffAcc = kOffLse + 16 * 32 * 4;          // [2 items][4 column groups][128 rows] partial sums
+constexpr int kOffBar = kOffAcc + 2 * 4 * kM * 4;
+constexpr int kBarKFull = 0, kBarKEmpty = kBarKFull + kKStages, kBarQFull = kBarKEmpty + kKStages,
+              kBarQEmpty = kBarQFull + kQStages, kBarSFull = kBarQEmpty + kQStages, kBarSEmpty = kBarSFull + kSBufs,
+              kBarTmem = kBarSEmpty + kSBufs;
+constexpr int kSmemBytes = kOffBar + 8 * (kBarTmem + 1) + 1024;
+static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+
+struct alignas(64) PromptParams {
+  CUtensorMap tm_q, tm_k;  // q [T][H][D] in boxes of 32 rows; K/V planes of the paged cache
+  const float* lse;        // [T][H]
+  const int32_t* bt;
+  const int32_t* seq_lens;
+  const int32_t* q_start;
+  float* w;      // [R][units][w_rows], or the per-head sums of the workspace
+  float* w_out;  // [R][1][...]: set when w is the workspace
+  int64_t w_sb, w_su, out_sb;
+  int32_t* err;
+  int64_t bt_stride, num_blocks;
+  int page, fa_layout, T, H, Hkv, G, R, w_rows, max_tiles, n_items, observe, window, n_sink;
+  int max_query_len;
+  float scale_log2;
+};
+
+// One request as every role sees it.
+struct Req {
+  int q0, nq, n, p0;  // first counted query row, counted rows, cache rows, position of the first counted row
+};
+
+// Most counted rows of a request that the launch is laid out for.
+__device__ __forceinline__ int most_rows(const PromptParams& p) {
+  return p.observe > 0 ? min(p.observe, p.max_query_len) : p.max_query_len;
+}
+
+__device__ __forceinline__ Req load_req(const PromptParams& p, int r, bool report) {
+  Req x;
+  const int a = __ldg(p.q_start + r), e = __ldg(p.q_start + r + 1);
+  const int qlen = e - a;
+  x.q0 = x.nq = x.n = x.p0 = 0;
+  if (a < 0 || qlen < 0 || e > p.T) {
+    if (report) set_error(p.err, ABKV_DEVERR_RANGE);
+    return x;
+  }
+  const int n = __ldg(p.seq_lens + r);
+  const int64_t cap = p.bt_stride * (int64_t)p.page;
+  if (n < qlen || (int64_t)n > cap || n > p.w_rows) {
+    if (report) set_error(p.err, ABKV_DEVERR_SEQ_OOB);
+    return x;  // nothing of the request is counted
+  }
+  x.nq = min(qlen, most_rows(p));
+  if (report && qlen > p.max_query_len && x.nq < (p.observe > 0 ? min(qlen, p.observe) : qlen))
+    set_error(p.err, ABKV_DEVERR_RANGE);  // max_query_len understated: only the last rows are counted
+  x.q0 = e - x.nq;
+  x.n = n;
+  x.p0 = n - x.nq;
+  return x;
+}
+
+// Work of one item: the contiguous range [u0, u1) of units (unit = chunk * G + head) whose rows see a row
+// of cache tile kt; empty when there is none.
+__device__ __forceinline__ void item_units(const PromptParams& p, const Req& x, int kt, bool resident, int& u0,
+                                           int& u1) {
+  const int k0 = kt * kM;
+  u0 = u1 = 0;
+  if (x.nq == 0 || k0 >= x.n) return;
+  const int chunks = (x.nq + kUnit - 1) / kUnit;
+  // chunk c holds positions p0 + 32 c .. : the first whose last row reaches the tile, the last whose
+  // first row's window still does
+  const int k1 = min(k0 + kM, x.n) - 1;
+  int c0 = k0 <= x.p0 ? 0 : (k0 - x.p0) / kUnit;  // its last row is at or past k0
+  int c1 = chunks;
+  if (p.window > 0 && k0 >= p.n_sink) {
+    // p - window < k1 for the chunk's first row p = p0 + 32 c
+    const int64_t lim = (int64_t)k1 + p.window - x.p0;  // 32 c < lim
+    c1 = lim <= 0 ? 0 : (int)min((int64_t)chunks, (lim + kUnit - 1) / kUnit);
+  }
+  if (c0 >= c1) return;
+  u0 = resident ? 0 : c0 * p.G;
+  u1 = resident ? chunks * p.G : c1 * p.G;
+}
+
+// Item sequence of a CTA; resident: Q of a whole request fits one tile (same answer for every request,
+// from the host's bound on the counted rows).
+struct Items {
+  int i, end, step;
+};
+__device__ __forceinline__ Items my_items(const PromptParams& p, bool resident) {
+  Items t;
+  if (resident) {  // contiguous: (request, head) outermost
+    const int per = (p.n_items + (int)gridDim.x - 1) / (int)gridDim.x;
+    t.i = min(p.n_items, (int)blockIdx.x * per);
+    t.end = min(p.n_items, t.i + per);
+    t.step = 1;
+  } else {
+    t.i = blockIdx.x;
+    t.end = p.n_items;
+    t.step = gridDim.x;
+  }
+  return t;
+}
+__device__ __forceinline__ void item_at(const PromptParams& p, bool resident, int i, int& r, int& hk, int& kt) {
+  const int rh = p.R * p.Hkv;
+  int g;
+  if (resident) {
+    g = i / p.max_tiles;
+    kt = i - g * p.max_tiles;
+  } else {
+    kt = i / rh;
+    g = i - kt * rh;
+  }
+  r = g / p.Hkv;
+  hk = g - r * p.Hkv;
+}
+
+__global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __grid_constant__ PromptParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kOffBar);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar + kBarTmem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool resident = (int64_t)((most_rows(p) + kUnit - 1) / kUnit) * p.G <= kN / kUnit;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBarTmem; ++i) mbar_init(&bar[i], i >= kBarSEmpty ? 16 : 1);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)),
+                 "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  bool dead = false;
+  const Items it = my_items(p, resident);
+
+  if (warp == 0) {
+    // ---------------- K producer: lane i < 8 owns 16-row slice i ----------------
+    int kc = 0;
+    for (int i = it.i; i < it.end && !dead; i += it.step) {
+      int r, hk, kt, u0, u1;
+      item_at(p, resident, i, r, hk, kt);
+      const Req x = load_req(p, r, kt == 0 && hk == 0 && lane == 0);
+      item_units(p, x, kt, resident, u0, u1);
+      if (u0 >= u1) continue;
+      const int row0 = kt * kM + 16 * lane;
+      int pg = -1;
+      if (lane < 8 && row0 < x.n) {
+        // a slice hidden from every counted row is not looked up: its page may be freed
+        const bool hidden = p.window > 0 && row0 >= p.n_sink && row0 + 16 <= x.p0 - p.window + 1;
+        if (!hidden) {
+          pg = __ldg(p.bt + (int64_t)r * p.bt_stride + row0 / p.page);
+          if (pg < 0 || (int64_t)pg >= p.num_blocks) {
+            set_error(p.err, ABKV_DEVERR_PAGE_OOB);
+            pg = -1;
+          }
+        }
+      }
+      const int st = kc % kKStages;
+      const uint32_t valid = __ballot_sync(0xffffffffu, pg >= 0);
+      bool ok = true;
+      if (lane == 0) {
+        ok = wait_or_abort(&bar[kBarKEmpty + st], (uint32_t)(((kc / kKStages) & 1) ^ 1), dead, p.err);
+        if (ok) mbar_expect_tx(&bar[kBarKFull + st], (uint32_t)__popc(valid) * 2u * 2048u);
+      }
+      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+      if (pg >= 0) {
+        uint8_t* kb = smem + kOffK + st * kTileBytes + lane * 2048;
+        const int plane = p.fa_layout ? pg : 2 * pg;
+        tma_load_4d(kb, &p.tm_k, 0, hk, row0 % p.page, plane, &bar[kBarKFull + st]);
+        tma_load_4d(kb + kTileBytes / 2, &p.tm_k, 64, hk, row0 % p.page, plane, &bar[kBarKFull + st]);
+      }
+      ++kc;
+    }
+  } else if (warp == kWarpQ) {
+    // ---------------- Q producer ----------------
+    if (lane == 0) {
+      int qc = 0, last_g = -1;
+      for (int i = it.i; i < it.end && !dead; i += it.step) {
+        int r, hk, kt, u0, u1;
+        item_at(p, resident, i, r, hk, kt);
+        const Req x = load_req(p, r, false);
+        item_units(p, x, kt, resident, u0, u1);
+        if (u0 >= u1) continue;
+        if (resident && last_g == r * p.Hkv + hk) continue;  // this tile is loaded
+        last_g = r * p.Hkv + hk;
+        for (int u = u0; u < u1; u += 4, ++qc) {
+          const int st = qc % kQStages, nu = min(4, u1 - u);
+          if (!wait_or_abort(&bar[kBarQEmpty + st], (uint32_t)(((qc / kQStages) & 1) ^ 1), dead, p.err)) break;
+          mbar_expect_tx(&bar[kBarQFull + st], (uint32_t)nu * 2u * 4096u);
+          for (int c = 0; c < nu; ++c) {
+            const int chunk = (u + c) / p.G, h = hk * p.G + (u + c) % p.G;
+            uint8_t* qb = smem + kOffQ + st * kTileBytes + c * 4096;
+            tma_load_4d(qb, &p.tm_q, 0, h, x.q0 + chunk * kUnit, 0, &bar[kBarQFull + st]);
+            tma_load_4d(qb + kTileBytes / 2, &p.tm_q, 64, h, x.q0 + chunk * kUnit, 0, &bar[kBarQFull + st]);
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer ----------------
+    if (lane == 0) {
+      int kc = 0, qc = 0, sc = 0, last_g = -1;
+      for (int i = it.i; i < it.end && !dead; i += it.step) {
+        int r, hk, kt, u0, u1;
+        item_at(p, resident, i, r, hk, kt);
+        const Req x = load_req(p, r, false);
+        item_units(p, x, kt, resident, u0, u1);
+        if (u0 >= u1) continue;
+        const int ks = kc % kKStages;
+        if (!wait_or_abort(&bar[kBarKFull + ks], (uint32_t)((kc / kKStages) & 1), dead, p.err)) break;
+        const uint64_t dk = desc_kmajor_sw128(smem_u32(smem + kOffK + ks * kTileBytes));
+        const bool fresh = !resident || last_g != r * p.Hkv + hk;
+        if (resident && fresh && last_g >= 0) {
+          umma_commit(&bar[kBarQEmpty + qc % kQStages]);  // the previous run's Q tile
+          ++qc;
+        }
+        last_g = r * p.Hkv + hk;
+        for (int u = u0; u < u1 && !dead; u += 4) {
+          const int qs = qc % kQStages, sb = sc % kSBufs;
+          if (fresh && !wait_or_abort(&bar[kBarQFull + qs], (uint32_t)((qc / kQStages) & 1), dead, p.err)) break;
+          if (!wait_or_abort(&bar[kBarSEmpty + sb], (uint32_t)(((sc / kSBufs) & 1) ^ 1), dead, p.err)) break;
+          tc_fence_after();
+          const uint64_t dq = desc_kmajor_sw128(smem_u32(smem + kOffQ + qs * kTileBytes));
+#pragma unroll
+          for (int kk = 0; kk < kD / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * (kTileBytes / 2) + (kk & 3) * 32;
+            umma(tmem + 128 * sb, desc_advance(dk, off), desc_advance(dq, off), kIdescS, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(&bar[kBarSFull + sb]);
+          ++sc;
+          if (!resident) {
+            umma_commit(&bar[kBarQEmpty + qs]);
+            ++qc;
+          }
+        }
+        umma_commit(&bar[kBarKEmpty + ks]);
+        ++kc;
+      }
+    }
+  } else {
+    // ---------------- exponentials and sums: lane = cache row, warp group = unit of the tile ----------------
+    const int sw = warp - 2, cg = sw >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    float* s_lse = reinterpret_cast<float*>(smem + kOffLse) + sw * 32;
+    float* s_acc = reinterpret_cast<float*>(smem + kOffAcc);
+    const float sl2 = p.scale_log2;
+    int sc = 0, ic = 0;
+    for (int i = it.i; i < it.end; i += it.step) {
+      int r, hk, kt, u0, u1;
+      item_at(p, resident, i, r, hk, kt);
+      const Req x = load_req(p, r, false);
+      item_units(p, x, kt, resident, u0, u1);
+      if (u0 >= u1) continue;
+      const int key = kt * kM + row;
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int u = u0; u < u1; u += 4, ++sc) {
+        const int sb = sc % kSBufs, un = u + cg;
+        const bool live = un < u1;  // warp-uniform: the tile has this unit
+        const int chunk = un / p.G, h = hk * p.G + un % p.G;
+        if (live) {
+          const int t = min(x.q0 + chunk * kUnit + lane, p.T - 1);
+          s_lse[lane] = __ldg(p.lse + (int64_t)t * p.H + h) * 1.4426950408889634f;
+        }
+        __syncwarp();
+        const bool ok = __all_sync(0xffffffffu,
+                                   wait_or_abort(&bar[kBarSFull + sb], (uint32_t)((sc / kSBufs) & 1), dead, p.err));
+        if (!ok) dead = true;
+        tc_fence_after();
+        if (ok && live) {
+          float s[32];
+          tmem_ld32(tmem + lane_base + 128 * sb + 32 * cg, s);
+          tmem_wait_ld();
+          tc_fence_before();
+          if (lane == 0) mbar_arrive_one(&bar[kBarSEmpty + sb]);  // the buffer's columns are in registers
+          // visible columns [a, e): rows at or past the key, inside its window, and counted
+          const int pc = x.p0 + chunk * kUnit;
+          const int a = max(key - pc, 0);
+          int e = min(kUnit, x.nq - chunk * kUnit);
+          if (p.window > 0 && key >= p.n_sink) e = (int)min((int64_t)e, (int64_t)key + p.window - pc);
+          const uint32_t mask = (a >= e || e <= 0) ? 0u : (0xFFFFFFFFu >> (32 - e)) & (0xFFFFFFFFu << a);
+          const bool full = __all_sync(0xffffffffu, mask == 0xFFFFFFFFu);
+          if (full) {
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+              const float4 l = *reinterpret_cast<const float4*>(s_lse + c);
+              acc[0] += fast_exp2(fmaf(s[c], sl2, -l.x));
+              acc[1] += fast_exp2(fmaf(s[c + 1], sl2, -l.y));
+              acc[2] += fast_exp2(fmaf(s[c + 2], sl2, -l.z));
+              acc[3] += fast_exp2(fmaf(s[c + 3], sl2, -l.w));
+            }
+          } else {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+              const float v = fast_exp2(fmaf(s[c], sl2, -s_lse[c]));
+              acc[c & 3] += (mask >> c) & 1u ? v : 0.f;
+            }
+          }
+        } else {
+          if (lane == 0) mbar_arrive_one(&bar[kBarSEmpty + sb]);
+        }
+        __syncwarp();  // s_lse is rewritten by the next step
+      }
+      // the four column groups of a cache row, added in order
+      float* sa = s_acc + (ic & 1) * 4 * kM;
+      sa[cg * kM + row] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+      named_bar_sync(1, 512);
+      if (cg == 0 && key < x.n && !dead) {
+        float* w = p.w + (int64_t)r * p.w_sb + (int64_t)hk * p.w_su + key;
+        const float add = (sa[row] + sa[kM + row]) + (sa[2 * kM + row] + sa[3 * kM + row]);
+        *w = p.w_out ? add : *w + add;
+      }
+      ++ic;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u));
+  }
+}
+
+// One accumulator row for all heads: w_out[r][row] += the per-head sums in head order.
+__global__ void prompt_weights_heads_kernel(const __grid_constant__ PromptParams p) {
+  const int r = blockIdx.y;
+  const Req x = load_req(p, r, false);
+  const int row = blockIdx.x * blockDim.x + threadIdx.x;
+  if (row >= x.n || x.nq == 0) return;
+  float acc = 0.f;
+  for (int h = 0; h < p.Hkv; ++h) {
+    // a tile no counted row sees was not written
+    int u0, u1;
+    item_units(p, x, row / kM, false, u0, u1);
+    if (u0 < u1) acc += __ldcg(p.w + (int64_t)r * p.w_sb + (int64_t)h * p.w_su + row);
+  }
+  p.w_out[(int64_t)r * p.out_sb + row] += acc;
+}
+
+}  // namespace
+}  // namespace abkv
+
+using namespace abkv;
+
+extern "C" size_t abkv_prompt_weights_workspace_size(int R, int num_kv_heads, int64_t max_rows, int weight_units) {
+  if (R <= 0 || num_kv_heads <= 0 || max_rows <= 0 || weight_units <= 0) return 0;
+  return 256 + (weight_units == 1 && num_kv_heads > 1 ? (size_t)R * num_kv_heads * max_rows * 4 : 0);
+}
+
+extern "C" int abkv_prompt_weights(const void* q, int64_t q_row_stride, int64_t q_head_stride, const float* lse,
+                                   const int32_t* query_start_loc, const void* kv_cache, int kv_layout,
+                                   int64_t num_blocks, int page_size, const int32_t* block_table, int64_t bt_stride,
+                                   const int32_t* seq_lens, float* weights, int64_t weight_seq_stride,
+                                   int64_t weight_unit_stride, int weight_rows, int weight_units, int R, int Hq,
+                                   int Hkv, int head_dim, int max_query_len, int max_rows, int T, int observe,
+                                   float scale, int window, int num_sinks, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  if (!q || !lse || !query_start_loc || !kv_cache || !block_table || !seq_lens || !weights) return ABKV_ERR_INVALID_ARG;
+  if (R <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || T <= 0 || num_blocks <= 0 || bt_stride <= 0 ||
+      !(scale > 0.f) || (kv_layout != 0 && kv_layout != 1) || max_query_len <= 0 || max_query_len > T || max_rows <= 0 ||
+      observe < 0 || window < 0 || num_sinks < 0 || weight_rows <= 0 || (weight_units != 1 && weight_units != Hkv) ||
+      q_row_stride <= 0 || q_head_stride <= 0)
+    return ABKV_ERR_INVALID_ARG;
+  if (head_dim != kD || page_size <= 0 || page_size % 16 || 2 * num_blocks > INT32_MAX || R > 65535)
+    return ABKV_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(kv_cache)) & 15) return ABKV_ERR_INVALID_ARG;
+  const size_t need = abkv_prompt_weights_workspace_size(R, Hkv, max_rows, weight_units);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return ABKV_ERR_WORKSPACE;
+  PromptParams prm;
+  std::memset(&prm, 0, sizeof(prm));
+  {
+    const cuuint64_t dims[4] = {(cuuint64_t)kD, (cuuint64_t)Hq, (cuuint64_t)T, 1};
+    const cuuint64_t gstr[3] = {(cuuint64_t)q_head_stride * 2, (cuuint64_t)q_row_stride * 2,
+                                (cuuint64_t)q_row_stride * 2 * (cuuint64_t)T};
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)kUnit, 1};
+    const int st = tc::encode_tiled_4d(&prm.tm_q, q, dims, gstr, box);
+    if (st != ABKV_OK) return st;
+  }
+  {
+    const cuuint64_t row = (cuuint64_t)Hkv * kD * 2;
+    const cuuint64_t dims[4] = {(cuuint64_t)kD, (cuuint64_t)Hkv, (cuuint64_t)page_size, (cuuint64_t)(2 * num_blocks)};
+    const cuuint64_t gstr[3] = {(cuuint64_t)kD * 2, row, row * (cuuint64_t)page_size};
+    const cuuint32_t box[4] = {64, 1, 16, 1};
+    const int st = tc::encode_tiled_4d(&prm.tm_k, kv_cache, dims, gstr, box);
+    if (st != ABKV_OK) return st;
+  }
+  const bool shared = weight_units == 1 && Hkv > 1;
+  prm.lse = lse;
+  prm.bt = block_table;
+  prm.seq_lens = seq_lens;
+  prm.q_start = query_start_loc;
+  prm.w = shared ? reinterpret_cast<float*>(static_cast<char*>(workspace) + 256) : weights;
+  prm.w_sb = shared ? (int64_t)Hkv * max_rows : weight_seq_stride;
+  prm.w_su = shared ? max_rows : weight_unit_stride;
+  prm.w_out = shared ? weights : nullptr;
+  prm.out_sb = weight_seq_stride;
+  prm.err = static_cast<int32_t*>(workspace);
+  prm.bt_stride = bt_stride;
+  prm.num_blocks = num_blocks;
+  prm.page = page_size;
+  prm.fa_layout = kv_layout;
+  prm.T = T;
+  prm.H = Hq;
+  prm.Hkv = Hkv;
+  prm.G = Hq / Hkv;
+  prm.R = R;
+  prm.w_rows = std::min(weight_rows, max_rows);
+  prm.max_tiles = (max_rows - 1) / kM + 1;
+  const int64_t items = (int64_t)prm.max_tiles * R * Hkv;
+  if (items > INT32_MAX / 2) return ABKV_ERR_UNSUPPORTED;
+  prm.n_items = (int)items;
+  prm.observe = observe;
+  prm.window = window;
+  prm.n_sink = num_sinks;
+  prm.max_query_len = max_query_len;
+  prm.scale_log2 = scale * 1.4426950408889634f;
+  int dev = 0, num_sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || num_sms <= 0)
+    return ABKV_ERR_CUDA;
+  if (cudaFuncSetAttribute(prompt_weights_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) !=
+      cudaSuccess)
+    return ABKV_ERR_CUDA;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  prompt_weights_kernel<<<std::min(prm.n_items, num_sms), kThreads, kSmemBytes, s>>>(prm);
+  if (shared) prompt_weights_heads_kernel<<<dim3((max_rows + 255) / 256, R), 256, 0, s>>>(prm);
+  if (cudaGetLastError() != cudaSuccess) return ABKV_ERR_CUDA;
+  return ABKV_OK;
+}

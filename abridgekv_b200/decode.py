@@ -24,7 +24,7 @@ from typing import Sequence
 import torch
 
 from . import _lib
-from .workspace import Workspace, call_workspace, default_workspace
+from .workspace import Workspace, call_workspace, default_workspace, on_stream
 
 def _check_cuda(name: str, t: torch.Tensor, dtype: torch.dtype | None = None) -> None:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -144,7 +144,8 @@ def _per_layer(name: str, value, L: int) -> list[int]:
 def _decode_window(queries, kv_caches, block_tables, seq_lens, weights, window, num_sinks, scale, outputs,
                    max_pages_per_seq, chunk_tokens, workspace, stream):
     L = len(queries)
-    B, Hq, Hkv, D, page, outs = _validate(queries, kv_caches, block_tables, seq_lens, outputs)
+    with on_stream(stream):
+        B, Hq, Hkv, D, page, outs = _validate(queries, kv_caches, block_tables, seq_lens, outputs)
     device = queries[0].device
     for ts in (queries, kv_caches, block_tables, seq_lens, outs, weights or ()):
         if any(t.device != device for t in ts):

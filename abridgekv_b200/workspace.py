@@ -7,6 +7,7 @@ outside any kernel; a grown buffer starts with a clean error word).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
@@ -52,6 +53,11 @@ def default_workspace(device: torch.device) -> Workspace:
     if ws is None:
         ws = _per_device[idx] = Workspace(torch.device("cuda", idx))
     return ws
+
+
+def on_stream(stream: torch.cuda.Stream | None):
+    """The context in which a call's outputs are allocated: the stream that writes them."""
+    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
 
 
 _per_stream: dict[tuple[int, int], Workspace] = {}

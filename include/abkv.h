@@ -593,6 +593,59 @@ int abkv_paged_prefill(const void* q, int64_t q_row_stride,
                        void* workspace, size_t workspace_bytes,
                        void* stream);
 
+/* abkv_paged_prefill under a sliding window with sinks (no counterpart in the
+ * reference; see abkv_decode_window): the row at position p of its request sees
+ * cache rows j <= p with j > p - window or j < num_sinks; window = 0 shows every
+ * j <= p.  lse (optional): DEVICE [T][Hq] float, the natural-log log-sum-exp of
+ * the scaled scores of each written row.  Pages that hold no row visible to any
+ * of a request's query rows are never looked up.  seq_lens[r] in [qlen,
+ * bt_stride * page]; one 128-row query tile may visit 2048 64-row key tiles
+ * (rows of a request beyond that set ABKV_DEVERR_SEQ_OOB and stay unwritten): with a
+ * window, window + num_sinks up to 130,000; without one, 131,072 rows.  Other
+ * arguments as abkv_paged_prefill. */
+int abkv_paged_prefill_window(const void* q, int64_t q_row_stride,
+                              int64_t q_head_stride, void* out,
+                              int64_t out_row_stride, int64_t out_head_stride,
+                              float* lse, const int32_t* query_start_loc,
+                              const void* kv_cache, int kv_layout,
+                              int64_t num_blocks, int page_size,
+                              const int32_t* block_table, int64_t bt_stride,
+                              const int32_t* seq_lens, int R, int Hq, int Hkv,
+                              int head_dim, int max_query_len, int T,
+                              float scale, int window, int num_sinks,
+                              void* workspace, size_t workspace_bytes,
+                              void* stream);
+
+/* Attention weights of prompt rows, summed per cache row (no counterpart in the
+ * reference; the prompt's part of the accumulators of abkv_decode_window).
+ * Request r's counted rows are its last `observe` query rows (0 = all) of rows
+ * query_start_loc[r] .. query_start_loc[r+1]-1, whose keys are the last cache
+ * rows as in abkv_paged_prefill; lse [T][Hq] is what abkv_paged_prefill_window
+ * returned for them with the same scale, window and num_sinks.  For a cache row
+ * j and unit u,
+ *   weights[r * weight_seq_stride + u * weight_unit_stride + j] +=
+ *     sum over the counted rows that see j and the query heads of u of
+ *     exp(scale q.k_j - lse)
+ * (weight_units = Hkv, or 1 for all heads).  The order of the sum is fixed.
+ * max_query_len >= every qlen, max_rows >= every seq_lens[r] (they bound the launch);
+ * a request with seq_lens[r] < qlen, or more rows than the table, max_rows or
+ * weight_rows hold, sets ABKV_DEVERR_SEQ_OOB and is not counted.  head_dim 128,
+ * page_size a multiple of 16. */
+size_t abkv_prompt_weights_workspace_size(int R, int num_kv_heads, int64_t max_rows,
+                                          int weight_units);
+
+int abkv_prompt_weights(const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                        const float* lse, const int32_t* query_start_loc,
+                        const void* kv_cache, int kv_layout, int64_t num_blocks,
+                        int page_size, const int32_t* block_table,
+                        int64_t bt_stride, const int32_t* seq_lens,
+                        float* weights, int64_t weight_seq_stride,
+                        int64_t weight_unit_stride, int weight_rows,
+                        int weight_units, int R, int Hq, int Hkv, int head_dim,
+                        int max_query_len, int max_rows, int T, int observe,
+                        float scale, int window, int num_sinks, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 /* The code step and the causal paged attention of requests that hold packed
  * sidecar pages (per-head quotas): PackedKVSidecar._attend_request_vectorized
  * with layer_pages (third_party/vllm_overlay/vllm/v1/worker/
