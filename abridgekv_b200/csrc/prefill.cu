@@ -47,6 +47,11 @@
 //               tile j+2 overwrites P(j) after P.V(j) read it: tcgen05.mma
 //               operations of one thread run in issue order.
 // Every mbarrier wait is bounded and records ABKV_DEVERR_TIMEOUT on expiry.
+//
+// kWin (abkv_window_attention): the same kernel under a causal sliding window with sinks instead of the
+// block mask, for any S: row q sees keys j <= q with j > q - window or j < n_sink.  Key tiles hidden from
+// the whole query tile are not visited; inside a tile a row's hidden keys are its causal tail and the hole
+// [n_sink, q - window + 1).  Rows past S are read as zeros and clipped by the output's tensor map.
 #include <cstring>
 
 #include "prefill_mask.cuh"
@@ -113,6 +118,7 @@ struct alignas(64) PrefillParams {
   int quota[kMaxHeads];
   int B, H, Hkv, G, npairs, S, C, KL, per, n_qtiles;
   float scale_log2;
+  int window, n_sink;  // kWin
 };
 
 // Softmax of one (head, 64-key tile) for query row `row` (= TMEM lane), columns
@@ -122,8 +128,9 @@ struct alignas(64) PrefillParams {
 // so both take the same lazy-rescale decision and reference maximum; each keeps
 // the row sum of its own columns and rescales its own half of O (D / 2 columns).
 // P (bf16, 16 words) goes into this half's columns of the upper half of the S buffer.
-template <int D>
-__device__ __forceinline__ void softmax_half(const PrefillParams& p, int lim, int half, int row, uint32_t tmem_s,
+// kHole: columns [hs, he) are hidden as well.
+template <int D, bool kHole>
+__device__ __forceinline__ void softmax_half(const PrefillParams& p, int lim, int hs, int he, int half, int row, uint32_t tmem_s,
                                              uint32_t tmem_o, uint32_t lane_base, int j, uint64_t* o_done,
                                              bool& dead, SoftmaxState& st, float* xm_mine, const float* xm_other,
                                              int pair_bar, bool live) {
@@ -137,10 +144,11 @@ __device__ __forceinline__ void softmax_half(const PrefillParams& p, int lim, in
   tmem_ld32(tmem_s + lane_base + c0, t);
   tmem_wait_ld();
   // visible columns of this half as a bit mask (bit i: column c0 + i visible, i.e. c0 + i < lim)
-  const int nv = lim - c0;
-  const uint32_t vm = nv >= 32 ? 0xFFFFFFFFu : (nv <= 0 ? 0u : ((1u << nv) - 1u));
+  auto below = [](int n) -> uint32_t { return n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : ((1u << n) - 1u)); };
+  uint32_t vm = below(lim - c0);
+  if (kHole) vm &= below(hs - c0) | ~below(he - c0);
   auto vis = [&](int c) { return ((vm >> (c - c0)) & 1u) != 0u; };
-  const bool full = lim == kBN;
+  const bool full = kHole ? __all_sync(0xffffffffu, vm == 0xFFFFFFFFu) : lim == kBN;
   float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // independent chains
   if (full) {
 #pragma unroll
@@ -211,7 +219,7 @@ __device__ __forceinline__ bool visit_tile(const PrefillParams& p, int hA, int h
   return tile_class_t<kBM, kBN>(p, hA, qt, kt, pl) != 0 || (hB >= 0 && tile_class_t<kBM, kBN>(p, hB, qt, kt, pl) != 0);
 }
 
-template <int D>
+template <int D, bool kWin>
 __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_constant__ PrefillParams p) {
   using LY = Layout<D>;
   constexpr int kQBytes = LY::kQBytes, kKVHalf = LY::kKVHalf, kStageBytes = LY::kStageBytes;
@@ -236,8 +244,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   const int hB = (2 * hp + 1 < p.G) ? hA + 1 : -1;  // odd group size: the last pair has one head
   const int b = blockIdx.z;
   const int pl = p.prompt_len ? __ldg(p.prompt_len + b) : 0;
-  const int qb = qt * kBM / p.per;
-  const int kt_end = (qb + 1) * p.per / kBN;  // key tiles beyond the query's block are never visible
+  const int qb = kWin ? 0 : qt * kBM / p.per;
+  // key tiles beyond the query's block (kWin: past its last row) are never visible
+  const int kt_end = kWin ? (min(qt * kBM + kBM, p.S) + kBN - 1) / kBN : (qb + 1) * p.per / kBN;
+  // kWin: keys [n_sink, w_lo) are hidden from the whole query tile; visited tile i is key tile
+  // i < w_ns ? i : i + w_shift
+  int w_ns = 0, w_shift = 0;
+  if constexpr (kWin) {
+    const int w_lo = max(0, qt * kBM - p.window + 1);
+    w_ns = (min(p.n_sink, w_lo) + kBN - 1) / kBN;
+    w_shift = max(w_lo / kBN - w_ns, 0);
+  }
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -272,7 +289,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   int32_t* s_nlist = s_list + kMaxKeyTiles;
   if (warp == 2) {
     int n = 0;
-    for (int base = 0; base < kt_end; base += 32) {
+    if constexpr (kWin) {
+      n = kt_end - w_shift;
+      for (int i = lane; i < n; i += 32) s_list[i] = i < w_ns ? i : i + w_shift;
+    }
+    for (int base = 0; !kWin && base < kt_end; base += 32) {
       const int kt = base + lane;
       const bool vis = kt < kt_end && visit_tile(p, hA, hB, qt, kt, pl);
       const uint32_t m = __ballot_sync(0xffffffffu, vis);
@@ -296,7 +317,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     if (lane == 0) {
       for (int j = 0; j < n_tiles; ++j) {
         const int e = s_list[j];
-        const int k0 = (e >> 16) * p.per + (e & 0xFFFF);
+        const int k0 = kWin ? e * kBN : (e >> 16) * p.per + (e & 0xFFFF);
         const int st = j % kStages;
         if (!wait_or_abort(&kv_empty[st], (uint32_t)(((j / kStages) & 1) ^ 1), dead, p.err)) break;
         uint8_t* kbuf = smem + kOffKV + st * kStageBytes;
@@ -376,11 +397,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     float* xsum = reinterpret_cast<float*>(smem + LY::kOffXchg + kXchgMax) + head_slot * 256;  // [half][128]
     if (h >= 0) {
       SoftmaxState st{-INFINITY, 0.f};  // l_run: the row sum of this warp's columns
-      const int qbr = q / p.per, qwr = q - qbr * p.per, quota = p.quota[h];
+      const int qbr = kWin ? 0 : q / p.per, qwr = kWin ? 0 : q - qbr * p.per, quota = kWin ? 0 : p.quota[h];
       for (int j = 0; j < n_tiles; ++j) {
         const int e = s_list[j];
-        const int kb = e >> 16, kw0 = e & 0xFFFF;
-        const int lim = tile_limit_t<kBN>(p, quota, q, qbr, qwr, kb, kw0, kb * p.per + kw0, pl);
+        int lim, hs = 0, he = 0;
+        if constexpr (kWin) {
+          lim = min(max(q + 1 - e * kBN, 0), kBN);
+          hs = p.n_sink - e * kBN;
+          he = q - p.window + 1 - e * kBN;
+        } else {
+          const int kb = e >> 16, kw0 = e & 0xFFFF;
+          lim = tile_limit_t<kBN>(p, quota, q, qbr, qwr, kb, kw0, kb * p.per + kw0, pl);
+        }
         // warp-uniform (tcgen05.ld is a warp-collective); a warp that gave up waiting keeps
         // going through the tiles without their work, so both warps of the pair meet at the
         // same named barriers
@@ -389,7 +417,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         if (!ok) dead = true;
         tc_fence_after();
         float* xm = xmax + ((j & 1) * 2 + head_slot) * 256;  // parity j: tile j + 2 reuses it after both
-        softmax_half<D>(p, lim, half, row, tmem_h + 64 * (j & 1), tmem_o, lane_base, j, &o_done[head_slot], dead,
+        softmax_half<D, kWin>(p, lim, hs, he, half, row, tmem_h + 64 * (j & 1), tmem_o, lane_base, j, &o_done[head_slot], dead,
                         st, xm + half * 128, xm + (1 - half) * 128, pair_bar, ok);
         tc_fence_before();  // P's tcgen05.st completed (wait::st) before the arrival
         mbar_arrive_one(&p_full[2 * head_slot + (j & 1)]);
@@ -425,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
                           pack_bf16x2(t[v8 * 8 + 4] * inv, t[v8 * 8 + 5] * inv),
                           pack_bf16x2(t[v8 * 8 + 6] * inv, t[v8 * 8 + 7] * inv));
         }
-        if (p.lse && half == 0) {
+        if (p.lse && half == 0 && (!kWin || q < p.S)) {
           const float lse2 = l > 0.f ? st.m_run + log2f(l) : -INFINITY;
           p.lse[((int64_t)b * p.H + h) * p.S + q] = lse2 * 0.6931471805599453f;  // natural log
         }
@@ -513,7 +541,7 @@ extern "C" int abkv_prefill_masked(const void* q, const int64_t* q_strides, cons
   prm.per = C + K_layout;
   prm.n_qtiles = S / kBM;
   prm.scale_log2 = scale * 1.4426950408889634f;
-  auto kernel = head_dim == 64 ? prefill_kernel<64> : prefill_kernel<128>;
+  auto kernel = head_dim == 64 ? prefill_kernel<64, false> : prefill_kernel<128, false>;
   const int smem = head_dim == 64 ? Layout<64>::kSmem : Layout<128>::kSmem;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
       cudaSuccess)
@@ -525,3 +553,47 @@ extern "C" int abkv_prefill_masked(const void* q, const int64_t* q_strides, cons
   return ABKV_OK;
 }
 
+
+extern "C" int abkv_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                     const void* v, const int64_t* v_strides, void* out, const int64_t* out_strides,
+                                     float* lse, int B, int H, int Hkv, int S, int head_dim, float scale, int window,
+                                     int num_sinks, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !k || !v || !out || !q_strides || !k_strides || !v_strides || !out_strides) return ABKV_ERR_INVALID_ARG;
+  if (B <= 0 || H <= 0 || Hkv <= 0 || S <= 0 || H % Hkv != 0 || !(scale > 0.f) || window <= 0 || num_sinks < 0)
+    return ABKV_ERR_INVALID_ARG;
+  if ((head_dim != 64 && head_dim != 128) || H > kMaxHeads || B > 65535 || S > kMaxKeyTiles * kBN)
+    return ABKV_ERR_UNSUPPORTED;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
+       reinterpret_cast<uintptr_t>(out)) & 15)
+    return ABKV_ERR_INVALID_ARG;
+  if (!workspace || workspace_bytes < 256 || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return ABKV_ERR_WORKSPACE;
+  PrefillParams prm;
+  std::memset(&prm, 0, sizeof(prm));
+  int st = make_map(&prm.tm_q, q, B, H, S, head_dim, q_strides, kBM);
+  if (st == ABKV_OK) st = make_map(&prm.tm_k, k, B, Hkv, S, head_dim, k_strides, kBN);
+  if (st == ABKV_OK) st = make_map(&prm.tm_v, v, B, Hkv, S, head_dim, v_strides, kBN);
+  if (st == ABKV_OK) st = make_map(&prm.tm_out, out, B, H, S, head_dim, out_strides, kBM);
+  if (st != ABKV_OK) return st;
+  prm.lse = lse;
+  prm.err = static_cast<int32_t*>(workspace);
+  prm.B = B;
+  prm.H = H;
+  prm.Hkv = Hkv;
+  prm.G = H / Hkv;
+  prm.npairs = (prm.G + 1) / 2;
+  prm.S = S;
+  prm.n_qtiles = (S + kBM - 1) / kBM;
+  prm.scale_log2 = scale * 1.4426950408889634f;
+  // a window past S hides nothing, sinks past S are every key: keep the tile arithmetic in 32 bits
+  prm.window = window < S ? window : S;
+  prm.n_sink = num_sinks < S ? num_sinks : S;
+  auto kernel = head_dim == 64 ? prefill_kernel<64, true> : prefill_kernel<128, true>;
+  const int smem = head_dim == 64 ? Layout<64>::kSmem : Layout<128>::kSmem;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return ABKV_ERR_CUDA;
+  if (Hkv * prm.npairs > 65535) return ABKV_ERR_UNSUPPORTED;
+  kernel<<<dim3(prm.n_qtiles, Hkv * prm.npairs, B), kThreads, smem, reinterpret_cast<cudaStream_t>(stream)>>>(prm);
+  if (cudaGetLastError() != cudaSuccess) return ABKV_ERR_CUDA;
+  return ABKV_OK;
+}

@@ -11,7 +11,8 @@ materialising a BlockMask.
 ``flex_attention_forward`` (the attention function CompressLM forces with
 ``_attn_implementation = "flex_attention"``, compress_forward.py:248) and is
 registered under the name ``"abkv_sm100"``.  It expects ``attention_mask`` to
-be a :class:`CompressMask` descriptor: CompressLM's per-layer dispatch hook
+be a :class:`CompressMask` descriptor (or a :class:`WindowMask` for a layer
+under a causal sliding window with sinks, ``window_attention``): CompressLM's per-layer dispatch hook
 (compress_forward.py:557-564) can hand each layer its own descriptor exactly as
 it hands each layer its own BlockMask today.
 """
@@ -24,7 +25,7 @@ from typing import Sequence
 import torch
 
 from . import _lib
-from .workspace import Workspace, default_workspace
+from .workspace import Workspace, call_workspace, default_workspace, on_stream
 
 TILE = 128
 
@@ -167,14 +168,145 @@ def prefill_masked_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, 
     return PrefillMaskedAttention.apply(q, k, v, C, K_layout, quota_per_head, prompt_len, scale)
 
 
+@dataclass(frozen=True)
+class WindowMask:
+    """A causal sliding window with sinks: row i sees keys j <= i with j > i - window or j < num_sinks."""
+
+    window: int
+    num_sinks: int = 0
+
+
+def _window_args(q, k, v, window, num_sinks, scale):
+    for name, t in (("query", q), ("key", k), ("value", v)):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.bfloat16:
+            raise TypeError(f"{name} must be a bf16 CUDA tensor (libabkv has no CPU path)")
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be 4-D")
+        if t.device != q.device:
+            raise ValueError(f"{name} must be on the query's device")
+    B, H, S, D = q.shape
+    Hkv = k.shape[1]
+    if tuple(k.shape) != (B, Hkv, S, D) or tuple(v.shape) != (B, Hkv, S, D):
+        raise ValueError("key/value must be [B, Hkv, S, D] matching the query")
+    if Hkv == 0 or H % Hkv:
+        raise ValueError("the KV heads must divide the query heads")
+    window, num_sinks = int(window), int(num_sinks)
+    if not (1 <= window <= 0x7FFFFFFF and 0 <= num_sinks <= 0x7FFFFFFF):
+        raise ValueError(f"window must be at least 1 and num_sinks at least 0, got {window} and {num_sinks}")
+    return window, num_sinks, 1.0 / math.sqrt(D) if scale is None else float(scale)
+
+
+def _tma_ready(t: torch.Tensor) -> torch.Tensor:
+    """t itself where the copy engine can address it (16-byte rows and base, no broadcast dimension),
+    else a contiguous copy."""
+    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(
+        t.size(i) == 1 or (t.stride(i) > 0 and t.stride(i) % 8 == 0) for i in range(3))
+    return t if ok else t.contiguous() if not t.is_contiguous() else t.clone()
+
+
+def _packed_strides(t: torch.Tensor) -> "_lib.C.Array":
+    """Element strides (batch, head, seq); a dimension of one element gets a legal one."""
+    return _lib.i64_array([t.stride(i) if t.size(i) > 1 else t.size(1) * t.size(2) * t.size(3) for i in range(3)])
+
+
+def window_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int, num_sinks: int = 0,
+                   scale: float | None = None, return_lse: bool = False, workspace: Workspace | None = None,
+                   stream: torch.cuda.Stream | None = None):
+    """Causal attention under a sliding window with sinks (``abkv_window_attention``): row i sees keys
+    j <= i with j > i - window or j < num_sinks.  q [B, H, S, D], k/v [B, Hkv, S, D] bf16 (any strides;
+    what the copy engine cannot address is copied first), D 64 or 128, any S up to 131072, finite values.
+    Returns out [B, H, S, D] (stored as [B, S, H, D]), and lse [B, H, S] fp32 with ``return_lse``."""
+    window, num_sinks, scale = _window_args(q, k, v, window, num_sinks, scale)
+    B, H, S, D = q.shape
+    with torch.cuda.device(q.device), on_stream(stream):
+        out = torch.empty((B, S, H, D), dtype=torch.bfloat16, device=q.device).transpose(1, 2)
+        lse = torch.empty((B, H, S), dtype=torch.float32, device=q.device) if return_lse else None
+        if out.numel():
+            q, k, v = _tma_ready(q), _tma_ready(k), _tma_ready(v)
+            s = torch.cuda.current_stream(q.device)
+            ws = call_workspace(q.device, s, 256, workspace)
+            st = _lib.lib().abkv_window_attention(
+                q.data_ptr(), _packed_strides(q), k.data_ptr(), _packed_strides(k), v.data_ptr(), _packed_strides(v),
+                out.data_ptr(), _packed_strides(out), lse.data_ptr() if lse is not None else None, B, H, k.shape[1], S, D,
+                scale, window, num_sinks, ws.ptr(), ws.nbytes, s.cuda_stream)
+            _lib.check("abkv_window_attention", st)
+    return (out, lse) if return_lse else out
+
+
+def window_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, dout: torch.Tensor,
+                    lse: torch.Tensor, *, window: int, num_sinks: int = 0, scale: float | None = None,
+                    workspace: Workspace | None = None, stream: torch.cuda.Stream | None = None):
+    """Gradients (dq, dk, dv) of ``window_forward`` for the upstream gradient ``dout``, from the forward's
+    output and log-sum-exp (``abkv_window_attention_backward``).  dq's parts are added in no fixed order."""
+    window, num_sinks, scale = _window_args(q, k, v, window, num_sinks, scale)
+    B, H, S, D = q.shape
+    for name, t in (("out", out), ("dout", dout)):
+        if not isinstance(t, torch.Tensor) or t.device != q.device or t.dtype != torch.bfloat16:
+            raise TypeError(f"{name} must be a bf16 tensor on the query's device")
+        if tuple(t.shape) != (B, H, S, D):
+            raise ValueError("out and dout must be [B, H, S, D] like the query")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (B, H, S) or not lse.is_contiguous() or \
+            lse.device != q.device:
+        raise ValueError("lse must be the forward's contiguous float32 [B, H, S] log-sum-exp")
+    with torch.cuda.device(q.device), on_stream(stream):
+        q, k, v, out, dout = (_tma_ready(t) for t in (q, k, v, out, dout))
+        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+        if dq.numel() == 0:
+            return dq, dk, dv
+        lib = _lib.lib()
+        need = lib.abkv_window_attention_backward_workspace_size(B, H, S, D)
+        if need == 0:
+            raise _lib.AbkvError("abkv_window_attention_backward_workspace_size", 3, f"unsupported shape D={D}")
+        s = torch.cuda.current_stream(q.device)
+        ws = call_workspace(q.device, s, need, workspace)
+        args = [x for t in (q, k, v, out, dout) for x in (t.data_ptr(), _packed_strides(t))] + [lse.data_ptr()] + [
+            x for t in (dq, dk, dv) for x in (t.data_ptr(), _packed_strides(t))]
+        st = lib.abkv_window_attention_backward(*args, B, H, k.shape[1], S, D, scale, window, num_sinks, ws.ptr(),
+                                                ws.nbytes, s.cuda_stream)
+    _lib.check("abkv_window_attention_backward", st)
+    return dq, dk, dv
+
+
+class WindowAttention(torch.autograd.Function):
+    """window_forward with its backward: the forward keeps its output and log-sum-exp."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, window, num_sinks, scale):
+        out, lse = window_forward(q, k, v, window=window, num_sinks=num_sinks, scale=scale, return_lse=True)
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.args = (window, num_sinks, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        window, num_sinks, scale = ctx.args
+        dq, dk, dv = window_backward(q, k, v, out, dout, lse, window=window, num_sinks=num_sinks, scale=scale)
+        return dq, dk, dv, None, None, None
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int, num_sinks: int = 0,
+                     scale: float | None = None) -> torch.Tensor:
+    """Differentiable ``window_forward`` (forward and backward on the tcgen05 kernels).  To capture forward
+    and backward into a CUDA graph, release any eager autograd graph of the same leaf tensors first (torch
+    ends the capture otherwise, as for every operator)."""
+    return WindowAttention.apply(q, k, v, window, num_sinks, scale)
+
+
 def abkv_attention_forward(module, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
                            attention_mask, scaling: float | None = None, dropout: float = 0.0,
                            softcap: float | None = None, s_aux=None, **kwargs):
     """transformers AttentionInterface function: (attn_output [B, S, H, D], None)."""
-    if not isinstance(attention_mask, CompressMask):
-        raise TypeError("abkv_sm100 attention needs a CompressMask descriptor as attention_mask")
+    if not isinstance(attention_mask, (CompressMask, WindowMask)):
+        raise TypeError("abkv_sm100 attention needs a CompressMask (or WindowMask) descriptor as attention_mask")
     if dropout != 0.0 or softcap is not None or s_aux is not None:
-        raise ValueError("abkv_sm100 attention supports no dropout, softcap or attention sinks")
+        raise ValueError("abkv_sm100 attention supports no dropout, softcap or learned sink logits")
+    if isinstance(attention_mask, WindowMask):
+        kw = dict(window=attention_mask.window, num_sinks=attention_mask.num_sinks, scale=scaling)
+        train = torch.is_grad_enabled() and any(t.requires_grad for t in (query, key, value))
+        out = (window_attention if train else window_forward)(query, key, value, **kw)
+        return out.transpose(1, 2), None
     kw = dict(C=attention_mask.C, K_layout=attention_mask.K_layout,
               quota_per_head=attention_mask.quota_per_head, prompt_len=attention_mask.prompt_len, scale=scaling)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (query, key, value)):

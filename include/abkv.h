@@ -525,6 +525,35 @@ int abkv_prefill_masked_backward(
     int K_layout, float scale, void* workspace, size_t workspace_bytes,
     void* stream);
 
+/* Causal attention under a sliding window with sinks, and its gradients (no
+ * counterpart in the reference: the training form of abkv_paged_prefill_window).
+ * Layouts, strides, lse and the backward's arguments as abkv_prefill_masked and its
+ * backward; row i sees keys j <= i with j > i - window or j < num_sinks (window
+ * >= 1, so every row sees itself).  Any S from 1 to 131072, head_dim 64 or 128,
+ * H <= 128.  All of q, k, v and dout must be finite: a tile multiplies hidden
+ * rows by zero.  The backward adds dq's parts in no fixed order (32-bit rounding
+ * differs between runs); dk and dv repeat bit for bit.  Its workspace:
+ * abkv_window_attention_backward_workspace_size(B, H, S, head_dim) bytes. */
+int abkv_window_attention(const void* q, const int64_t* q_strides, const void* k,
+                          const int64_t* k_strides, const void* v,
+                          const int64_t* v_strides, void* out,
+                          const int64_t* out_strides, float* lse, int B, int H,
+                          int Hkv, int S, int head_dim, float scale, int window,
+                          int num_sinks, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+size_t abkv_window_attention_backward_workspace_size(int B, int H, int S,
+                                                     int head_dim);
+int abkv_window_attention_backward(
+    const void* q, const int64_t* q_strides, const void* k,
+    const int64_t* k_strides, const void* v, const int64_t* v_strides,
+    const void* out, const int64_t* out_strides, const void* dout,
+    const int64_t* dout_strides, const float* lse, void* dq,
+    const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
+    const int64_t* dv_strides, int B, int H, int Hkv, int S, int head_dim,
+    float scale, int window, int num_sinks, void* workspace,
+    size_t workspace_bytes, void* stream);
+
 /* ========================================================================
  * 5. Code step: K_code code queries per request over the paged cache (tcgen05).
  *
