@@ -198,6 +198,15 @@ def ptr_array(values) -> C.Array:
     return arr
 
 
+def data_ptrs(tensors) -> C.Array:
+    """Host array of the tensors' device addresses."""
+    return (C.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def i64(*values) -> C.Array:
+    return (C.c_int64 * len(values))(*values)
+
+
 def i64_array(values) -> C.Array:
     arr = (C.c_int64 * len(values))()
     for i, v in enumerate(values):

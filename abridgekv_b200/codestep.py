@@ -25,7 +25,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .workspace import Workspace, call_workspace, default_workspace, on_stream
+from .workspace import Workspace, call_scope, call_workspace, default_workspace
 
 
 def _layout_of(kv: torch.Tensor, num_kv_heads: int) -> tuple[int, int, int]:
@@ -169,6 +169,12 @@ def _window(window, num_sinks) -> tuple[int, int]:
     return w, s
 
 
+def _check_query(query, kv_cache) -> None:
+    for name, t in (("query", query), ("kv_cache", kv_cache)):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.bfloat16:
+            raise TypeError(f"{name} must be a bf16 CUDA tensor (libabkv has no CPU path)")
+
+
 def _same_device(query, **tensors) -> None:
     for name, t in tensors.items():
         if t is not None and t.device != query.device:
@@ -187,25 +193,24 @@ def paged_prefill_window(query: torch.Tensor, kv_cache: torch.Tensor, block_tabl
 
     Returns out [T, Hq, D], or (out, lse) with ``return_lse``: lse [T, Hq] fp32, the natural-log
     log-sum-exp of each row's scaled scores, which ``paged_prompt_weights`` takes.  Rows of no request
-    are left untouched (in a new lse: NaN)."""
+    are left untouched (in lse: undefined)."""
     window, num_sinks = _window(window, num_sinks)
-    with on_stream(stream):  # what the call allocates belongs to the stream that uses it
+    _check_query(query, kv_cache)
+    dev = query.device
+    with call_scope(dev, stream):
         head, out, R, nb, page, T, scale = _prepare(query, kv_cache, block_table, seq_lens, query_start_loc, None,
                                                     scale, None, num_requests, out, num_kv_heads=num_kv_heads)
-        lse = torch.full((T, query.shape[1]), float("nan"), dtype=torch.float32, device=query.device) \
-            if return_lse else None
-    _same_device(query, kv_cache=kv_cache, block_table=block_table, seq_lens=seq_lens, out=out,
-                 query_start_loc=query_start_loc)
-    if int(max_query_len) <= 0 or int(max_query_len) > T:
-        raise ValueError(f"max_query_len must be in [1, T={T}]")
-    dev = query.device
-    s = torch.cuda.current_stream(dev) if stream is None else stream
-    ws = call_workspace(dev, s, 256, workspace)
-    with torch.cuda.device(dev):
+        _same_device(query, kv_cache=kv_cache, block_table=block_table, seq_lens=seq_lens, out=out,
+                     query_start_loc=query_start_loc)
+        if not 0 < max_query_len <= T:
+            raise ValueError(f"max_query_len must be in [1, T={T}]")
+        lse = torch.empty(query.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
+        ws, raw = call_workspace(dev, 256, workspace)
         st = _lib.lib().abkv_paged_prefill_window(
-            *head[:6], lse.data_ptr() if lse is not None else None, *head[6:], int(max_query_len), T, scale, window,
-            num_sinks, ws.ptr(), ws.nbytes, s.cuda_stream)
-    _lib.check("abkv_paged_prefill_window", st)
+            *head[:6], lse.data_ptr() if lse is not None else None, *head[6:], max_query_len, T, scale, window, num_sinks,
+            ws.ptr(), ws.nbytes, raw)
+    if st:
+        _lib.check("abkv_paged_prefill_window", st)
     return (out, lse) if return_lse else out
 
 
@@ -244,18 +249,18 @@ def paged_prompt_weights(query: torch.Tensor, lse: torch.Tensor, kv_cache: torch
     if int(max_query_len) <= 0 or int(max_query_len) > T:
         raise ValueError(f"max_query_len must be in [1, T={T}]")
     dev = query.device
-    s = torch.cuda.current_stream(dev) if stream is None else stream
     lib = _lib.lib()
     max_rows = min(int(block_table.shape[1]) * page, rows)
     if R == 0 or max_rows == 0:
         return weights
-    ws = call_workspace(dev, s, lib.abkv_prompt_weights_workspace_size(R, Hkv, max_rows, units), workspace)
-    with torch.cuda.device(dev):
+    with call_scope(dev, stream):
+        ws, raw = call_workspace(dev, lib.abkv_prompt_weights_workspace_size(R, Hkv, max_rows, units), workspace)
         st = lib.abkv_prompt_weights(
             query.data_ptr(), query.stride(0), query.stride(1), lse.data_ptr(), *head[6:14], weights.data_ptr(),
             weights.stride(0), weights.stride(1), rows, units, R, Hq, Hkv, D, int(max_query_len), max_rows, T, obs,
-            scale, window, num_sinks, ws.ptr(), ws.nbytes, s.cuda_stream)
-    _lib.check("abkv_prompt_weights", st)
+            scale, window, num_sinks, ws.ptr(), ws.nbytes, raw)
+    if st:
+        _lib.check("abkv_prompt_weights", st)
     return weights
 
 

@@ -29,7 +29,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .workspace import Workspace, call_workspace, default_workspace
+from .workspace import Workspace, call_scope, call_workspace, default_workspace
 
 
 class CopyOps(_SequenceABC):
@@ -281,16 +281,16 @@ def evict_by_weight(kv_caches: Sequence[torch.Tensor], block_tables: Sequence[to
     units, rows = int(weights[0].shape[1]) if weights[0].dim() == 3 else 0, int(weights[0].shape[-1])
 
     def check(name, t, dtype):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or (dtype is not None and t.dtype != dtype):
-            raise TypeError(f"{name} must be a{'' if dtype is None else ' ' + str(dtype)} CUDA tensor "
-                            "(libabkv has no CPU path)")
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype:
+            raise TypeError(f"{name} must be a {dtype} CUDA tensor (libabkv has no CPU path)")
         if t.device != dev:
             raise ValueError(f"{name} must be on the caches' device")
 
+    shape = kv_caches[0].shape
     for l in range(L):
         kv, w = kv_caches[l], weights[l]
-        check("kv_cache", kv, None)
-        if _layout_of(kv)[0] != layout or _layout_of(kv)[2:] != (page, hkv, d) or not kv.is_contiguous():
+        check("kv_cache", kv, kv_caches[0].dtype)
+        if not kv.is_contiguous() or kv.dim() != 5 or kv.shape[2:] != shape[2:] or kv.shape[1 - layout] != 2:
             raise ValueError("every KV cache must be contiguous and share layout, page size, heads and head size")
         if kv.element_size() != 2:
             raise TypeError("the caches must hold 2-byte elements")
@@ -310,36 +310,38 @@ def evict_by_weight(kv_caches: Sequence[torch.Tensor], block_tables: Sequence[to
             raise ValueError("the rows of weights must not overlap")
     if units not in (1, hkv):
         raise ValueError(f"weights must hold one row per KV head ({hkv}) or one per sequence, got {units}")
-    if len({kv.data_ptr() for kv in kv_caches}) != L and dst_block_tables is None:
+    if L > 1 and len({kv.data_ptr() for kv in kv_caches}) != L and dst_block_tables is None:
         raise ValueError("every layer needs its own cache tensor")
     if in_place_weights and len({w.data_ptr() for w in weights}) != L:
         raise ValueError("every layer needs its own weights tensor")
-    s = torch.cuda.current_stream(dev) if stream is None else stream
     lib = _lib.lib()
-    with torch.cuda.device(dev), torch.cuda.stream(s):
-        new = [torch.empty(B, dtype=torch.int32, device=dev) for _ in range(L)]
-        outs = list(weights) if in_place_weights else [torch.empty((B, units, rows), dtype=torch.float32, device=dev)
-                                                       for _ in range(L)]
-        keep = [torch.empty((B, units, m), dtype=torch.int32, device=dev) for m in budgets] if return_keep else None
-        result = Evicted(new, outs, keep)
+    with call_scope(dev, stream):
+        # one allocation per kind, a view per layer
+        new = torch.empty((L, B), dtype=torch.int32, device=dev).unbind(0)
+        outs = weights if in_place_weights else torch.empty((L, B, units, rows), dtype=torch.float32, device=dev).unbind(0)
+        keep = None
+        if return_keep:
+            sizes = [B * units * m for m in budgets]
+            keep = [t.view(B, units, m) for t, m in zip(torch.empty(sum(sizes), dtype=torch.int32, device=dev).split(sizes),
+                                                        budgets)]
+        result = Evicted(list(new), list(outs), keep)
         if B == 0:
             return result
         if rows == 0:
             raise ValueError("weights must hold at least one row")
         c_budget = _lib.i32_array(budgets)
         need = 256 if return_keep else lib.abkv_evict_by_weight_workspace_size(L, B, units, c_budget)
-        ws = call_workspace(dev, s, need, workspace)
-        pa, ia = _lib.ptr_array, _lib.i64_array
+        ws, raw = call_workspace(dev, need, workspace)
+        ptrs, i64 = _lib.data_ptrs, _lib.i64
         st = lib.abkv_evict_by_weight(
-            pa([t.data_ptr() for t in kv_caches]), pa([t.data_ptr() for t in block_tables]),
-            ia([t.stride(0) for t in block_tables]),
-            pa([t.data_ptr() for t in dst_block_tables]) if dst_block_tables is not None else None,
-            ia([t.stride(0) for t in dst_block_tables]) if dst_block_tables is not None else None,
-            pa([t.data_ptr() for t in seq_lens]), pa([t.data_ptr() for t in new]),
-            ia([_layout_of(t)[1] for t in kv_caches]), pa([t.data_ptr() for t in weights]),
-            ia([x for t in weights for x in (t.stride(0), t.stride(1))]), rows, pa([t.data_ptr() for t in outs]),
-            ia([x for t in outs for x in (t.stride(0), t.stride(1))]), rows,
-            pa([t.data_ptr() for t in keep]) if keep is not None else None, c_budget, L, B, units, layout, hkv, d, page,
-            max(int(t.shape[1]) for t in block_tables), num_sinks, num_recent, ws.ptr(), ws.nbytes, s.cuda_stream)
-    _lib.check("abkv_evict_by_weight", st)
+            ptrs(kv_caches), ptrs(block_tables), i64(*[t.shape[1] for t in block_tables]),
+            ptrs(dst_block_tables) if dst_block_tables is not None else None,
+            i64(*[t.shape[1] for t in dst_block_tables]) if dst_block_tables is not None else None, ptrs(seq_lens),
+            ptrs(new), i64(*[t.shape[layout] for t in kv_caches]), ptrs(weights),
+            i64(*[x for t in weights for x in t.stride()[:2]]), rows, ptrs(outs),
+            i64(*[x for t in outs for x in t.stride()[:2]]), rows, ptrs(keep) if keep is not None else None, c_budget, L, B,
+            units, layout, hkv, d, page, max([t.shape[1] for t in block_tables]), num_sinks, num_recent, ws.ptr(),
+            ws.nbytes, raw)
+    if st:
+        _lib.check("abkv_evict_by_weight", st)
     return result

@@ -966,6 +966,286 @@ __global__ void __launch_bounds__(kWeightRows) decode_weights_kernel(const __gri
   *w += acc;
 }
 
+// ---------------------------------------------------------------------------
+// Few rows in all (a single sequence, a short window): latency decides.  One cluster of CTAs per (layer,
+// sequence, KV head); the visible tiles go round robin over its warps, which load K and V fragments straight
+// from global memory (the next tile's while one is computed) and keep everything in registers; the
+// partial results meet in shared memory, then over the cluster's shared memory, so there are no partials in
+// global memory, no counters to clear and no second kernel.  The arithmetic of a tile is consumer()'s.
+// With accumulators of one unit per KV head the scores wait in shared memory for the log-sum-exp; one
+// unit for all heads goes through the global scores and decode_weights_kernel.
+constexpr int kClusterThreads = 256, kClusterWarps = kClusterThreads / 32;
+constexpr int kMaxClusterTiles = 8;  // tiles per warp
+
+__device__ __forceinline__ uint32_t cluster_map(const void* p, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float cluster_ld(uint32_t a) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];\n" : "=f"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float4 cluster_ld4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
+}
+
+template <int D>
+struct ClusterSmem {
+  float o[kClusterWarps][kMaxG][D];   // warp partials
+  float m[kClusterWarps][kMaxG], l[kClusterWarps][kMaxG];
+  float co[kMaxG][D];                 // the CTA's partial (read by the cluster)
+  float cm[kMaxG], cl[kMaxG];
+  float lse[kMaxG];                   // of the whole row, log2 units
+  float x[1];                         // [tiles of the CTA][G][16] scores, with weights
+};
+
+template <int D>
+__global__ void __launch_bounds__(kClusterThreads, 1) decode_cluster_kernel(const __grid_constant__ WinDecodeParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  ClusterSmem<D>& S = *reinterpret_cast<ClusterSmem<D>*>(smem);
+  constexpr int kQC = D / 32, kVH = D / 64, kOT = D / 16;
+  const int rank = blockIdx.x, cs = gridDim.x, h = blockIdx.y;
+  const int li = blockIdx.z / p.B, b = blockIdx.z - li * p.B;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int G = p.G;
+  const LayerArgs& L = p.layer[li];
+  const WinArgs& W = p.win[li];
+  const bool report = rank == 0 && h == 0 && threadIdx.x == 0;
+  int n = clamp_seq_len(p, L, b, report);
+  if (W.weights && n > W.w_cap) {
+    if (report) set_error(p.err, ABKV_DEVERR_SEQ_OOB);
+    n = W.w_cap;
+  }
+  const WinSpan ws = win_span(n, W.window, W.sinks);
+  const int64_t row_elems = (int64_t)p.Hkv * D, half = (int64_t)p.P * row_elems;
+  // virtual tile i of this warp: rank + cs * (warp + 8 i)
+  const int v0 = rank + cs * warp, vstep = cs * kClusterWarps;
+  const int ntiles = v0 < ws.n_tiles ? (ws.n_tiles - 1 - v0) / vstep + 1 : 0;
+  auto tile_of = [&](int i) {
+    const int v = v0 + i * vstep;
+    return v < ws.ns ? v : v + ws.shift;
+  };
+  // lane i holds the page of tile i
+  int pg_lane = -1;
+  if (lane < ntiles) {
+    pg_lane = __ldg(L.bt + (int64_t)b * L.bt_stride + (int64_t)tile_of(lane) * kTile / p.P);
+    if (pg_lane < 0 || pg_lane >= L.num_blocks) {
+      set_error(p.err, ABKV_DEVERR_PAGE_OOB);
+      pg_lane = -1;
+    }
+  }
+  uint32_t qr[kQC][4];
+  {
+    const __nv_bfloat16* qrow = L.q + ((int64_t)b * p.Hq + h * G + g) * D + 8 * c;
+#pragma unroll
+    for (int m = 0; m < kQC; ++m) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (g < G) v = __ldg(reinterpret_cast<const uint4*>(qrow + 32 * m));
+      qr[m][0] = v.x; qr[m][1] = v.y; qr[m][2] = v.z; qr[m][3] = v.w;
+    }
+  }
+  float o[kOT][4];
+#pragma unroll
+  for (int mt = 0; mt < kOT; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+
+  uint4 kr[2][kQC], vr[kVH][4], kn[2][kQC], vn[kVH][4];
+  auto load = [&](int i, uint4 (&k)[2][kQC], uint4 (&v)[kVH][4]) {
+    const int pg = __shfl_sync(0xffffffffu, pg_lane, i);
+    const int t0 = tile_of(i) * kTile;
+    const __nv_bfloat16* base = L.kv + (int64_t)max(pg, 0) * 2 * half + (int64_t)(t0 % p.P) * row_elems + h * D;
+    auto ok = [&](int T) { return pg >= 0 && t0 + T < n && (t0 + T >= ws.lo || t0 + T < W.sinks); };
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int m = 0; m < kQC; ++m) {
+        k[nt][m] = make_uint4(0, 0, 0, 0);
+        if (ok(8 * nt + g)) k[nt][m] = ld_stream_v4(base + (8 * nt + g) * row_elems + 32 * m + 8 * c);
+      }
+#pragma unroll
+    for (int hh = 0; hh < kVH; ++hh)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        const int T = 2 * c + (i4 & 1) + 8 * (i4 >> 1);
+        v[hh][i4] = make_uint4(0, 0, 0, 0);
+        if (ok(T)) v[hh][i4] = ld_stream_v4(base + half + T * row_elems + 64 * hh + 8 * g);
+      }
+  };
+  if (ntiles > 0) load(0, kr, vr);
+  for (int i = 0; i < ntiles; ++i) {
+    if (i + 1 < ntiles) load(i + 1, kn, vn);
+    const int t0 = tile_of(i) * kTile;
+    const bool pg_ok = __shfl_sync(0xffffffffu, pg_lane, i) >= 0;
+    float s[2][4];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+      for (int m = 0; m < kQC; ++m) {
+        mma_bf16_16816(s[nt], qr[m][0], 0u, qr[m][1], 0u, kr[nt][m].x, kr[nt][m].y);
+        mma_bf16_16816(s[nt], qr[m][2], 0u, qr[m][3], 0u, kr[nt][m].z, kr[nt][m].w);
+      }
+    }
+    float x[2][2];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int r = t0 + 8 * nt + 2 * c + j;
+        x[nt][j] = pg_ok && r < n && (r >= ws.lo || r < W.sinks) ? s[nt][j] * p.scale_log2 : -INFINITY;
+      }
+    if (W.weights && g < G) {
+      float* dst = p.logits
+                       ? p.logits + (((int64_t)li * p.B + b) * p.Hq + h * G + g) * p.lrows + (v0 + i * vstep) * kTile
+                       : S.x + ((i * kClusterWarps + warp) * G + g) * kTile;
+      *reinterpret_cast<float2*>(dst + 2 * c) = make_float2(x[0][0], x[0][1]);
+      *reinterpret_cast<float2*>(dst + 8 + 2 * c) = make_float2(x[1][0], x[1][1]);
+    }
+    float tmax = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
+    tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 1));
+    tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 2));
+    const float m_new = fmaxf(m_run, tmax);
+    const float m_use = (m_new == -INFINITY) ? 0.f : m_new;
+    const float alpha = exp2f(m_run - m_use);
+    float pr[2][2];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) pr[nt][j] = exp2f(x[nt][j] - m_use);
+    l_run = l_run * alpha + ((pr[0][0] + pr[0][1]) + (pr[1][0] + pr[1][1]));
+    m_run = m_new;
+    const float a0 = __shfl_sync(0xffffffffu, alpha, 8 * c), a1 = __shfl_sync(0xffffffffu, alpha, 8 * c + 4);
+#pragma unroll
+    for (int mt = 0; mt < kOT; ++mt) {
+      o[mt][0] *= a0; o[mt][1] *= a1; o[mt][2] *= a0; o[mt][3] *= a1;
+    }
+    const uint32_t pb0 = pack_bf16x2(pr[0][0], pr[0][1]), pb1 = pack_bf16x2(pr[1][0], pr[1][1]);
+#pragma unroll
+    for (int hh = 0; hh < kVH; ++hh) {
+      const uint32_t a[4][4] = {{vr[hh][0].x, vr[hh][0].y, vr[hh][0].z, vr[hh][0].w},
+                                {vr[hh][1].x, vr[hh][1].y, vr[hh][1].z, vr[hh][1].w},
+                                {vr[hh][2].x, vr[hh][2].y, vr[hh][2].z, vr[hh][2].w},
+                                {vr[hh][3].x, vr[hh][3].y, vr[hh][3].z, vr[hh][3].w}};
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        mma_bf16_16816(o[4 * hh + q], prmt(a[0][q], a[1][q], 0x5410u), prmt(a[0][q], a[1][q], 0x7632u),
+                       prmt(a[2][q], a[3][q], 0x5410u), prmt(a[2][q], a[3][q], 0x7632u), pb0, pb1);
+    }
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+      for (int m = 0; m < kQC; ++m) kr[nt][m] = kn[nt][m];
+#pragma unroll
+    for (int hh = 0; hh < kVH; ++hh)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) vr[hh][q] = vn[hh][q];
+  }
+  // warp partials -> the CTA's partial
+  float lq = l_run;
+  lq += __shfl_xor_sync(0xffffffffu, lq, 1);
+  lq += __shfl_xor_sync(0xffffffffu, lq, 2);
+#pragma unroll
+  for (int jh = 0; jh < 2; ++jh) {
+    const int head = 2 * c + jh;
+    if (head < G) {
+#pragma unroll
+      for (int mt = 0; mt < kOT; ++mt) {
+        const int d = 8 * g + 64 * (mt >> 2) + 2 * (mt & 3);
+        *reinterpret_cast<float2*>(&S.o[warp][head][d]) = make_float2(o[mt][jh], o[mt][2 + jh]);
+      }
+    }
+  }
+  if (c == 0 && g < G) {
+    S.m[warp][g] = m_run;
+    S.l[warp][g] = lq;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < G * (D / 4); e += kClusterThreads) {
+    const int r = e / (D / 4), d0 = (e % (D / 4)) * 4;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kClusterWarps; ++w) M = fmaxf(M, S.m[w][r]);
+    const float Mu = M == -INFINITY ? 0.f : M;
+    float l = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kClusterWarps; ++w) {
+      const float f = exp2f(S.m[w][r] - Mu);
+      const float4 v = *reinterpret_cast<const float4*>(&S.o[w][r][d0]);
+      l += S.l[w][r] * f;
+      a[0] += v.x * f; a[1] += v.y * f; a[2] += v.z * f; a[3] += v.w * f;
+    }
+    *reinterpret_cast<float4*>(&S.co[r][d0]) = make_float4(a[0], a[1], a[2], a[3]);
+    if (d0 == 0) {
+      S.cm[r] = M;
+      S.cl[r] = l;
+    }
+  }
+  cluster_sync();
+  // the cluster's partials: CTA `rank` finishes every cs-th group of four dims
+  for (int e = threadIdx.x * cs + rank; e < G * (D / 4); e += kClusterThreads * cs) {
+    const int r = e / (D / 4), d0 = (e % (D / 4)) * 4;
+    float mk[8], M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      mk[k] = k < cs ? cluster_ld(cluster_map(&S.cm[r], k)) : -INFINITY;
+      M = fmaxf(M, mk[k]);
+    }
+    const float Mu = M == -INFINITY ? 0.f : M;
+    float l = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (k >= cs) break;
+      const float f = exp2f(mk[k] - Mu);
+      const float4 v = cluster_ld4(cluster_map(&S.co[r][d0], k));
+      l += cluster_ld(cluster_map(&S.cl[r], k)) * f;
+      a[0] += v.x * f; a[1] += v.y * f; a[2] += v.z * f; a[3] += v.w * f;
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    uint2 u;
+    u.x = pack_bf16x2(a[0] * inv, a[1] * inv);
+    u.y = pack_bf16x2(a[2] * inv, a[3] * inv);
+    *reinterpret_cast<uint2*>(L.out + ((int64_t)b * p.Hq + h * G + r) * D + d0) = u;
+  }
+  if (W.weights) {
+    if (threadIdx.x < G) {
+      const int r = threadIdx.x;
+      float M = -INFINITY, l = 0.f;
+      for (int k = 0; k < cs; ++k) M = fmaxf(M, cluster_ld(cluster_map(&S.cm[r], k)));
+      const float Mu = M == -INFINITY ? 0.f : M;
+      for (int k = 0; k < cs; ++k)
+        l += cluster_ld(cluster_map(&S.cl[r], k)) * exp2f(cluster_ld(cluster_map(&S.cm[r], k)) - Mu);
+      const float lse = l > 0.f ? Mu + log2f(l) : -INFINITY;
+      S.lse[r] = lse;
+      if (p.lse2 && rank == 0) p.lse2[((int64_t)li * p.B + b) * p.Hq + h * G + r] = lse;
+    }
+    __syncthreads();
+    if (!p.logits) {
+      float* w = W.weights + b * W.w_sb + h * W.w_su;
+      // the CTA's tiles: slot = i * 8 + warp holds virtual tile rank + cs * slot
+      const int slots = rank < ws.n_tiles ? (ws.n_tiles - 1 - rank) / cs + 1 : 0;
+      for (int e = threadIdx.x; e < slots * kTile; e += kClusterThreads) {
+        const int slot = e / kTile, T = e % kTile, v = rank + cs * slot;
+        const int row = (v < ws.ns ? v : v + ws.shift) * kTile + T;
+        if (row >= n || (row < ws.lo && row >= W.sinks)) continue;
+        float acc = 0.f;
+        for (int r = 0; r < G; ++r) {
+          const float lse = S.lse[r];
+          acc += lse == -INFINITY ? 0.f : exp2f(S.x[(slot * G + r) * kTile + T] - lse);
+        }
+        w[row] += acc;
+      }
+    }
+  }
+  cluster_sync();  // no CTA leaves while another may still read its partial
+}
+
 constexpr int kMinWindowChunkTiles = 4;
 constexpr int kMaxAutoChunkTiles = 384;  // 6144 cache rows
 
@@ -1320,15 +1600,19 @@ namespace {
 // Layers per launch of a weight-accumulating call: their scores (4 bytes a query head and row) wait
 // in the workspace for the rows' log-sum-exp, so the workspace stays near this size.
 constexpr int64_t kLogitBytes = 64 << 20;
+constexpr int64_t kClusterCtas = 2 * 148;
 
 struct WindowPlan {
-  int group;  // layers per launch; every launch reuses the same scratch
+  int group;    // layers per launch; every launch reuses the same scratch
+  int cluster;  // CTAs per (layer, sequence, KV head) of decode_cluster_kernel, 0 = the split kernel
+  int warp_tiles;
+  bool logits;  // scores go through the workspace
   int chunk_tiles, max_chunks, lrows;
   size_t off_lse, off_part_o, off_lse2, off_logits, total, counter_bytes;
 };
 
 int plan_window(int num_layers, int num_seqs, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
-                int max_pages, int chunk_tokens, const int32_t* windows, const int32_t* sinks, bool weighted,
+                int max_pages, int chunk_tokens, const int32_t* windows, const int32_t* sinks, int weighted,
                 WindowPlan* plan) {
   if (num_layers <= 0 || num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || page_size <= 0 ||
       max_pages <= 0 || num_q_heads % num_kv_heads || chunk_tokens < 0 || chunk_tokens % kTile)
@@ -1349,8 +1633,21 @@ int plan_window(int num_layers, int num_seqs, int num_q_heads, int num_kv_heads,
   }
   plan->lrows = (int)(vt * kTile);
   plan->group = num_layers < kMaxLayers ? num_layers : kMaxLayers;
+  // Clusters where the whole call is about two waves of CTAs with few tiles per warp.
+  plan->cluster = 0;
+  const int64_t heads = (int64_t)plan->group * num_seqs * num_kv_heads;
+  if (!chunk_tokens && num_layers <= kMaxLayers && heads <= kClusterCtas) {
+    int cs = 1;
+    while (cs < 8 && vt > cs * kClusterWarps && heads * cs * 2 <= kClusterCtas) cs <<= 1;
+    const int64_t per = (vt + cs * kClusterWarps - 1) / (cs * kClusterWarps);
+    if (per <= kMaxClusterTiles && heads / num_kv_heads <= 65535) {
+      plan->cluster = cs;
+      plan->warp_tiles = (int)per;
+    }
+  }
+  plan->logits = weighted && !(plan->cluster && weighted == num_kv_heads);
   const int64_t layer_logits = (int64_t)num_seqs * num_q_heads * plan->lrows * 4;
-  if (weighted) plan->group = (int)std::max<int64_t>(1, std::min<int64_t>(plan->group, kLogitBytes / layer_logits));
+  if (plan->logits && !plan->cluster) plan->group = (int)std::max<int64_t>(1, std::min<int64_t>(plan->group, kLogitBytes / layer_logits));
   int ct;
   if (chunk_tokens) {
     ct = chunk_tokens / kTile;
@@ -1364,14 +1661,34 @@ int plan_window(int num_layers, int num_seqs, int num_q_heads, int num_kv_heads,
   if ((int64_t)plan->max_chunks * plan->group * num_seqs > INT32_MAX) return ABKV_ERR_UNSUPPORTED;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   const size_t lb = (size_t)plan->group * num_seqs;
-  const size_t rows = plan->max_chunks > 1 ? lb * plan->max_chunks * num_q_heads : 0;
+  const size_t rows = plan->max_chunks > 1 && !plan->cluster ? lb * plan->max_chunks * num_q_heads : 0;
   plan->counter_bytes = rows ? up(lb * num_kv_heads * 4) : 0;
   plan->off_lse = kWsHeader + plan->counter_bytes;
   plan->off_part_o = plan->off_lse + up(rows * 4);
   plan->off_lse2 = plan->off_part_o + up(rows * head_dim * 4);
-  plan->off_logits = plan->off_lse2 + (weighted ? up(lb * num_q_heads * 4) : 0);
-  plan->total = plan->off_logits + (weighted ? up(lb * num_q_heads * (size_t)plan->lrows * 4) : 0);
+  plan->off_logits = plan->off_lse2 + (plan->logits ? up(lb * num_q_heads * 4) : 0);
+  plan->total = plan->off_logits + (plan->logits ? up(lb * num_q_heads * (size_t)plan->lrows * 4) : 0);
   return ABKV_OK;
+}
+
+int launch_cluster(const WinDecodeParams& prm, const WindowPlan& plan, int head_dim, cudaStream_t s) {
+  auto kernel = head_dim == 64 ? decode_cluster_kernel<64> : decode_cluster_kernel<kD>;
+  const size_t scores = prm.win[0].weights && !plan.logits
+                            ? (size_t)plan.warp_tiles * kClusterWarps * prm.G * kTile * 4 : 0;
+  const size_t smem = (head_dim == 64 ? sizeof(ClusterSmem<64>) : sizeof(ClusterSmem<kD>)) + scores;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    return ABKV_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(plan.cluster, prm.Hkv, prm.nl * prm.B);
+  cfg.blockDim = dim3(kClusterThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)plan.cluster, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, prm) == cudaSuccess ? ABKV_OK : ABKV_ERR_CUDA;
 }
 }  // namespace
 }  // namespace abkv
@@ -1379,10 +1696,10 @@ int plan_window(int num_layers, int num_seqs, int num_q_heads, int num_kv_heads,
 extern "C" size_t abkv_decode_window_workspace_size(int num_layers, int num_seqs, int num_q_heads, int num_kv_heads,
                                                     int head_dim, int page_size, int max_pages_per_seq,
                                                     int chunk_tokens, const int32_t* windows, const int32_t* sinks,
-                                                    int weighted) {
+                                                    int weight_units) {
   WindowPlan plan;
   if (plan_window(num_layers, num_seqs, num_q_heads, num_kv_heads, head_dim, page_size, max_pages_per_seq,
-                  chunk_tokens, windows, sinks, weighted != 0, &plan) != ABKV_OK)
+                  chunk_tokens, windows, sinks, weight_units, &plan) != ABKV_OK)
     return 0;
   return plan.total;
 }
@@ -1399,21 +1716,19 @@ extern "C" int abkv_decode_window(const void* const* q, const void* const* kv, c
     return ABKV_ERR_INVALID_ARG;
   WindowPlan plan;
   const int st = plan_window(num_layers, num_seqs, num_q_heads, num_kv_heads, head_dim, page_size,
-                             max_pages_per_seq, chunk_tokens, windows, sinks, weights != nullptr, &plan);
+                             max_pages_per_seq, chunk_tokens, windows, sinks, weights ? weight_units : 0, &plan);
   if (st != ABKV_OK) return st;
   if (weights && (!weight_strides || weight_rows <= 0 || (weight_units != 1 && weight_units != num_kv_heads)))
     return ABKV_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < plan.total || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return ABKV_ERR_WORKSPACE;
-  bool out16 = true;
   for (int l = 0; l < num_layers; ++l) {
     if (!q[l] || !kv[l] || !block_tables[l] || !seq_lens[l] || !out[l] || bt_strides[l] <= 0 || num_blocks[l] <= 0 ||
         (weights && !weights[l]))
       return ABKV_ERR_INVALID_ARG;
-    if (((reinterpret_cast<uintptr_t>(q[l]) | reinterpret_cast<uintptr_t>(kv[l])) & 15) ||
-        (reinterpret_cast<uintptr_t>(block_tables[l]) & 3) || (reinterpret_cast<uintptr_t>(out[l]) & 1))
+    if (((reinterpret_cast<uintptr_t>(q[l]) | reinterpret_cast<uintptr_t>(kv[l]) | reinterpret_cast<uintptr_t>(out[l])) &
+         15) || (reinterpret_cast<uintptr_t>(block_tables[l]) & 3))
       return ABKV_ERR_INVALID_ARG;
-    if (reinterpret_cast<uintptr_t>(out[l]) & 15) out16 = false;
   }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int dev = 0, num_sms = 0;
@@ -1427,12 +1742,12 @@ extern "C" int abkv_decode_window(const void* const* q, const void* const* kv, c
   prm.gather.world = 1;
   prm.err = reinterpret_cast<int32_t*>(ws);
   prm.work = reinterpret_cast<int32_t*>(ws + 64);
-  const bool split = plan.max_chunks > 1;
+  const bool split = plan.max_chunks > 1 && !plan.cluster;
   prm.counters = split ? reinterpret_cast<int32_t*>(ws + kWsHeader) : nullptr;
   prm.part_lse = split ? reinterpret_cast<float*>(ws + plan.off_lse) : nullptr;
   prm.part_o = split ? reinterpret_cast<float*>(ws + plan.off_part_o) : nullptr;
-  prm.lse2 = weights ? reinterpret_cast<float*>(ws + plan.off_lse2) : nullptr;
-  prm.logits = weights ? reinterpret_cast<float*>(ws + plan.off_logits) : nullptr;
+  prm.lse2 = plan.logits ? reinterpret_cast<float*>(ws + plan.off_lse2) : nullptr;
+  prm.logits = plan.logits ? reinterpret_cast<float*>(ws + plan.off_logits) : nullptr;
   prm.lrows = plan.lrows;
   prm.units = weights ? weight_units : 1;
   prm.scale_log2 = scale * 1.4426950408889634f;
@@ -1444,7 +1759,7 @@ extern "C" int abkv_decode_window(const void* const* q, const void* const* kv, c
   prm.chunk_tiles = plan.chunk_tiles;
   prm.max_chunks = plan.max_chunks;
   prm.max_rows = max_pages_per_seq * page_size;
-  prm.warp_epi = num_kv_heads == kWarps && out16 ? 1 : 0;
+  prm.warp_epi = num_kv_heads == kWarps ? 1 : 0;
   // other entry points leave their own data where the chunk counters are; every launch below
   // leaves them at zero again
   if (split && cudaMemsetAsync(prm.counters, 0, plan.counter_bytes, s) != cudaSuccess) return ABKV_ERR_CUDA;
@@ -1469,9 +1784,10 @@ extern "C" int abkv_decode_window(const void* const* q, const void* const* kv, c
     }
     prm.nl = nl;
     prm.num_items = plan.max_chunks * nl * num_seqs;
-    const int rc = launch_kernel<WinDecodeParams, false>(prm, head_dim, std::min(prm.num_items, num_sms), s);
+    const int rc = plan.cluster ? launch_cluster(prm, plan, head_dim, s)
+                                : launch_kernel<WinDecodeParams, false>(prm, head_dim, std::min(prm.num_items, num_sms), s);
     if (rc != ABKV_OK) return rc;
-    if (weights) {
+    if (plan.logits) {
       const dim3 grid((plan.lrows + kWeightRows - 1) / kWeightRows, num_seqs, nl * prm.units);
       decode_weights_kernel<<<grid, kWeightRows, 0, s>>>(prm);
     }

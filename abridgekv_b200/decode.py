@@ -18,13 +18,14 @@ missing library or a non-CUDA tensor raises.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Sequence
 
 import torch
 
 from . import _lib
-from .workspace import Workspace, call_workspace, default_workspace, on_stream
+from .workspace import Workspace, call_scope, call_workspace, default_workspace
 
 def _check_cuda(name: str, t: torch.Tensor, dtype: torch.dtype | None = None) -> None:
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
@@ -129,72 +130,111 @@ def _call_decode(lib, queries, kv_caches, block_tables, seq_lens, outs, L, B, Hq
     )
 
 
-def _per_layer(name: str, value, L: int) -> list[int]:
+def _per_layer(name: str, value, L: int) -> tuple[int, ...]:
     """An int (or None) for every layer, or one entry per layer; None counts as 0."""
     if value is None or isinstance(value, int):
-        value = [value] * L
-    out = [0 if v is None else int(v) for v in value]
-    if len(out) != L:
-        raise ValueError(f"{name} must be one number or one per layer ({L})")
-    if any(v < 0 or v > 0x7FFFFFFF for v in out):
+        out = (value or 0,) * L
+    else:
+        out = tuple(0 if v is None else int(v) for v in value)
+        if len(out) != L:
+            raise ValueError(f"{name} must be one number or one per layer ({L})")
+    if min(out) < 0 or max(out) > 0x7FFFFFFF:
         raise ValueError(f"{name} must lie in [0, 2^31), got {out}")
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _window_plan(L, B, Hq, Hkv, D, page, max_pages, chunk_tokens, windows, sinks, weighted):
+    """(workspace bytes, windows array, sinks array) of a shape."""
+    win, snk = _lib.i32_array(windows), _lib.i32_array(sinks)
+    return _lib.lib().abkv_decode_window_workspace_size(L, B, Hq, Hkv, D, page, max_pages, chunk_tokens, win, snk,
+                                                        weighted), win, snk
+
+
+def _need(ok: bool, name: str, want: str, t) -> None:
+    if not ok:
+        kind = TypeError if not isinstance(t, torch.Tensor) or not t.is_cuda else ValueError
+        raise kind(f"{name} must be {want}" + (
+            f", got {t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else ""))
+
+
+def _check_weights(weights, L, B, Hkv, device) -> tuple[int, int]:
+    """-> (units, rows)"""
+    if len(weights) != L:
+        raise ValueError("weights must hold one accumulator tensor per layer")
+    for w in weights:
+        _check_cuda("weights", w, torch.float32)
+    units, rows = (int(weights[0].shape[1]), int(weights[0].shape[2])) if weights[0].dim() == 3 else (0, 0)
+    for w in weights:
+        if w.dim() != 3 or w.shape[0] < B or w.shape[1] != units or w.shape[2] != rows or w.stride(2) != 1 or rows == 0:
+            raise ValueError(f"every weights tensor must be [>=B, Hkv or 1, rows] with contiguous rows, got {tuple(w.shape)}")
+        if (B > 1 and w.stride(0) < rows) or (units > 1 and w.stride(1) < rows):
+            raise ValueError("the rows of weights must not overlap")
+        if w.device != device:
+            raise ValueError("every tensor of the call must be on the queries' device")
+    if units not in (1, Hkv):
+        raise ValueError(f"weights must hold one row per KV head ({Hkv}) or one per sequence, got {units}")
+    if L > 1 and len({w.data_ptr() for w in weights}) != L:
+        raise ValueError("every layer needs its own weights tensor")
+    return units, rows
 
 
 def _decode_window(queries, kv_caches, block_tables, seq_lens, weights, window, num_sinks, scale, outputs,
                    max_pages_per_seq, chunk_tokens, workspace, stream):
     L = len(queries)
-    with on_stream(stream):
-        B, Hq, Hkv, D, page, outs = _validate(queries, kv_caches, block_tables, seq_lens, outputs)
-    device = queries[0].device
-    for ts in (queries, kv_caches, block_tables, seq_lens, outs, weights or ()):
-        if any(t.device != device for t in ts):
-            raise ValueError("every tensor of the call must be on the queries' device")
+    if not (L == len(kv_caches) == len(block_tables) == len(seq_lens)) or L == 0 or (
+            outputs is not None and len(outputs) != L):
+        raise ValueError("per-layer argument lists must be non-empty and of equal length")
+    q0, kv0 = queries[0], kv_caches[0]
+    _check_cuda("query", q0, torch.bfloat16)
+    _check_cuda("kv_cache", kv0, torch.bfloat16)
+    if q0.dim() != 3 or kv0.dim() != 5:
+        raise ValueError("query must be [B, Hq, D] and kv_cache [num_blocks, 2, page, Hkv, D]")
+    q_shape, kv_shape, device = q0.shape, kv0.shape, q0.device
+    (B, Hq, D), (_, two, page, Hkv, D2) = q_shape, kv_shape
+    if two != 2 or D2 != D:
+        raise ValueError(f"kv cache must be [num_blocks, 2, page, Hkv, {D}], got {tuple(kv_shape)}")
+    bf16, i32 = torch.bfloat16, torch.int32
+    for l in range(L):
+        q, kv, bt, sl = queries[l], kv_caches[l], block_tables[l], seq_lens[l]
+        _need(q.dtype is bf16 and q.device == device and q.shape == q_shape and q.is_contiguous(), "query",
+              f"a contiguous bf16 [{B}, {Hq}, {D}] tensor on {device}", q)
+        _need(kv.dtype is bf16 and kv.device == device and kv.dim() == 5 and kv.shape[1:] == kv_shape[1:] and
+              kv.is_contiguous(), "kv_cache", f"a contiguous bf16 [num_blocks, 2, {page}, {Hkv}, {D}] tensor on {device}", kv)
+        _need(bt.dtype is i32 and bt.device == device and bt.dim() == 2 and bt.shape[0] >= B and bt.is_contiguous(),
+              "block_table", f"a contiguous int32 [>={B}, max_pages] tensor on {device}", bt)
+        _need(sl.dtype is i32 and sl.device == device and sl.dim() == 1 and sl.shape[0] >= B and sl.is_contiguous(),
+              "seq_lens", f"a contiguous int32 [>={B}] tensor on {device}", sl)
+        if outputs is not None:
+            o = outputs[l]
+            _need(o.dtype is bf16 and o.device == device and o.shape == q_shape and o.is_contiguous(), "output",
+                  f"a contiguous bf16 [{B}, {Hq}, {D}] tensor on {device}", o)
     windows, sinks = _per_layer("window", window, L), _per_layer("num_sinks", num_sinks, L)
     if max_pages_per_seq is None:
-        max_pages_per_seq = max(int(bt.shape[1]) for bt in block_tables)
-    if scale is None:
-        scale = 1.0 / math.sqrt(D)
-    w_ptrs = w_strides = None
-    w_rows, units = 0, 1
-    if weights is not None:
-        if len(weights) != L:
-            raise ValueError("weights must hold one accumulator tensor per layer")
-        w_rows, units = int(weights[0].shape[-1]), int(weights[0].shape[1])
-        for w in weights:
-            _check_cuda("weights", w, torch.float32)
-            if w.dim() != 3 or w.shape[0] < B or w.shape[1] != units or w.shape[2] != w_rows or w.stride(2) != 1:
-                raise ValueError("every weights tensor must be [>=B, Hkv or 1, rows] with contiguous rows, "
-                                 f"got {tuple(w.shape)}")
-            if (B > 1 and w.stride(0) < w_rows) or (units > 1 and w.stride(1) < w_rows):
-                raise ValueError("the rows of weights must not overlap")
-        if units not in (1, Hkv):
-            raise ValueError(f"weights must hold one row per KV head ({Hkv}) or one per sequence, got {units}")
-        if len({w.data_ptr() for w in weights}) != L:
-            raise ValueError("every layer needs its own weights tensor")
-        w_ptrs = _lib.ptr_array([w.data_ptr() for w in weights])
-        w_strides = _lib.i64_array([x for w in weights for x in (w.stride(0), w.stride(1))])
-    if B == 0:
-        return outs
-    lib = _lib.lib()
-    win, snk = _lib.i32_array(windows), _lib.i32_array(sinks)
-    need = lib.abkv_decode_window_workspace_size(L, B, Hq, Hkv, D, page, max_pages_per_seq, chunk_tokens, win, snk,
-                                                 int(weights is not None))
-    if need == 0:
-        raise _lib.AbkvError("abkv_decode_window_workspace_size", 3,
-                             f"unsupported shape (B={B}, Hq={Hq}, Hkv={Hkv}, D={D}, page={page}, "
-                             f"chunk_tokens={chunk_tokens})")
-    s = torch.cuda.current_stream(device) if stream is None else stream
-    ws = call_workspace(device, s, need, workspace)
-    with torch.cuda.device(device):
-        st = lib.abkv_decode_window(
-            _lib.ptr_array([q.data_ptr() for q in queries]), _lib.ptr_array([kv.data_ptr() for kv in kv_caches]),
-            _lib.ptr_array([bt.data_ptr() for bt in block_tables]),
-            _lib.i64_array([bt.stride(0) for bt in block_tables]),
-            _lib.ptr_array([sl.data_ptr() for sl in seq_lens]), _lib.i64_array([kv.shape[0] for kv in kv_caches]),
-            _lib.ptr_array([o.data_ptr() for o in outs]), L, B, Hq, Hkv, D, page, max_pages_per_seq, float(scale),
-            chunk_tokens, win, snk, w_ptrs, w_strides, w_rows, units, ws.ptr(), ws.nbytes, s.cuda_stream)
-    _lib.check("abkv_decode_window", st)
+        max_pages_per_seq = max([bt.shape[1] for bt in block_tables])
+    units, rows = (1, 0) if weights is None else _check_weights(weights, L, B, Hkv, device)
+    with call_scope(device, stream):
+        outs = list(outputs) if outputs is not None else [torch.empty(q_shape, dtype=bf16, device=device)
+                                                          for _ in range(L)]
+        if B == 0:
+            return outs
+        need, win, snk = _window_plan(L, B, Hq, Hkv, D, page, max_pages_per_seq, chunk_tokens, windows, sinks,
+                                      0 if weights is None else units)
+        if need == 0:
+            raise _lib.AbkvError("abkv_decode_window_workspace_size", 3,
+                                 f"unsupported shape (B={B}, Hq={Hq}, Hkv={Hkv}, D={D}, page={page}, "
+                                 f"max_pages_per_seq={max_pages_per_seq}, chunk_tokens={chunk_tokens})")
+        ws, raw = call_workspace(device, need, workspace)
+        ptrs = _lib.data_ptrs
+        st = _lib.lib().abkv_decode_window(
+            ptrs(queries), ptrs(kv_caches), ptrs(block_tables), _lib.i64(*[bt.shape[1] for bt in block_tables]),
+            ptrs(seq_lens), _lib.i64(*[kv.shape[0] for kv in kv_caches]), ptrs(outs), L, B, Hq, Hkv, D, page,
+            max_pages_per_seq, 1.0 / math.sqrt(D) if scale is None else scale, chunk_tokens, win, snk,
+            None if weights is None else ptrs(weights),
+            None if weights is None else _lib.i64(*[x for w in weights for x in w.stride()[:2]]), rows, units,
+            ws.ptr(), ws.nbytes, raw)
+    if st:
+        _lib.check("abkv_decode_window", st)
     return outs
 
 

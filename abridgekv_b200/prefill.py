@@ -25,7 +25,7 @@ from typing import Sequence
 import torch
 
 from . import _lib
-from .workspace import Workspace, call_workspace, default_workspace, on_stream
+from .workspace import Workspace, call_scope, call_workspace, default_workspace
 
 TILE = 128
 
@@ -196,17 +196,20 @@ def _window_args(q, k, v, window, num_sinks, scale):
     return window, num_sinks, 1.0 / math.sqrt(D) if scale is None else float(scale)
 
 
-def _tma_ready(t: torch.Tensor) -> torch.Tensor:
-    """t itself where the copy engine can address it (16-byte rows and base, no broadcast dimension),
-    else a contiguous copy."""
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(
-        t.size(i) == 1 or (t.stride(i) > 0 and t.stride(i) % 8 == 0) for i in range(3))
-    return t if ok else t.contiguous() if not t.is_contiguous() else t.clone()
-
-
-def _packed_strides(t: torch.Tensor) -> "_lib.C.Array":
-    """Element strides (batch, head, seq); a dimension of one element gets a legal one."""
-    return _lib.i64_array([t.stride(i) if t.size(i) > 1 else t.size(1) * t.size(2) * t.size(3) for i in range(3)])
+def _tma_ready(t: torch.Tensor) -> tuple[torch.Tensor, "_lib.C.Array"]:
+    """t and its element strides (batch, head, seq), where the copy engine can address it (16-byte rows and
+    base, no broadcast dimension); else a contiguous copy and its strides."""
+    a, b, c, d = t.stride()
+    if d != 1 or (a | b | c) % 8 or not a * b * c or t.data_ptr() % 16:
+        n = t.shape
+        ok = d == 1 and t.data_ptr() % 16 == 0 and all(
+            n[i] == 1 or (x > 0 and x % 8 == 0) for i, x in enumerate((a, b, c)))
+        if not ok:
+            t = t.clone(memory_format=torch.contiguous_format)
+            a, b, c, _ = t.stride()
+        # the stride of a dimension of one element addresses nothing: any legal one will do
+        a, b, c = (n[1] * n[2] * n[3] if n[i] == 1 else x for i, x in enumerate((a, b, c)))
+    return t, _lib.i64(a, b, c)
 
 
 def window_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int, num_sinks: int = 0,
@@ -218,18 +221,19 @@ def window_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window:
     Returns out [B, H, S, D] (stored as [B, S, H, D]), and lse [B, H, S] fp32 with ``return_lse``."""
     window, num_sinks, scale = _window_args(q, k, v, window, num_sinks, scale)
     B, H, S, D = q.shape
-    with torch.cuda.device(q.device), on_stream(stream):
-        out = torch.empty((B, S, H, D), dtype=torch.bfloat16, device=q.device).transpose(1, 2)
-        lse = torch.empty((B, H, S), dtype=torch.float32, device=q.device) if return_lse else None
-        if out.numel():
-            q, k, v = _tma_ready(q), _tma_ready(k), _tma_ready(v)
-            s = torch.cuda.current_stream(q.device)
-            ws = call_workspace(q.device, s, 256, workspace)
+    device = q.device
+    with call_scope(device, stream):
+        out = torch.empty((B, S, H, D), dtype=torch.bfloat16, device=device).transpose(1, 2)
+        lse = torch.empty((B, H, S), dtype=torch.float32, device=device) if return_lse else None
+        if B * H * S:
+            (q, qs), (k, ks), (v, vs), (_, os) = _tma_ready(q), _tma_ready(k), _tma_ready(v), _tma_ready(out)
+            ws, raw = call_workspace(device, 256, workspace)
             st = _lib.lib().abkv_window_attention(
-                q.data_ptr(), _packed_strides(q), k.data_ptr(), _packed_strides(k), v.data_ptr(), _packed_strides(v),
-                out.data_ptr(), _packed_strides(out), lse.data_ptr() if lse is not None else None, B, H, k.shape[1], S, D,
-                scale, window, num_sinks, ws.ptr(), ws.nbytes, s.cuda_stream)
-            _lib.check("abkv_window_attention", st)
+                q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os,
+                lse.data_ptr() if return_lse else None, B, H, k.shape[1], S, D, scale, window, num_sinks, ws.ptr(),
+                ws.nbytes, raw)
+            if st:
+                _lib.check("abkv_window_attention", st)
     return (out, lse) if return_lse else out
 
 
@@ -239,31 +243,32 @@ def window_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
     """Gradients (dq, dk, dv) of ``window_forward`` for the upstream gradient ``dout``, from the forward's
     output and log-sum-exp (``abkv_window_attention_backward``).  dq's parts are added in no fixed order."""
     window, num_sinks, scale = _window_args(q, k, v, window, num_sinks, scale)
-    B, H, S, D = q.shape
+    B, H, S, D = shape = q.shape
+    device = q.device
     for name, t in (("out", out), ("dout", dout)):
-        if not isinstance(t, torch.Tensor) or t.device != q.device or t.dtype != torch.bfloat16:
+        if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.bfloat16:
             raise TypeError(f"{name} must be a bf16 tensor on the query's device")
-        if tuple(t.shape) != (B, H, S, D):
+        if t.shape != shape:
             raise ValueError("out and dout must be [B, H, S, D] like the query")
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (B, H, S) or not lse.is_contiguous() or \
-            lse.device != q.device:
+    if lse.dtype != torch.float32 or lse.shape != shape[:3] or not lse.is_contiguous() or lse.device != device:
         raise ValueError("lse must be the forward's contiguous float32 [B, H, S] log-sum-exp")
-    with torch.cuda.device(q.device), on_stream(stream):
-        q, k, v, out, dout = (_tma_ready(t) for t in (q, k, v, out, dout))
+    with call_scope(device, stream):
+        (q, qs), (k, ks), (v, vs), (out, os), (dout, ds) = (_tma_ready(t) for t in (q, k, v, out, dout))
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-        if dq.numel() == 0:
+        if B * H * S == 0:
             return dq, dk, dv
         lib = _lib.lib()
         need = lib.abkv_window_attention_backward_workspace_size(B, H, S, D)
         if need == 0:
             raise _lib.AbkvError("abkv_window_attention_backward_workspace_size", 3, f"unsupported shape D={D}")
-        s = torch.cuda.current_stream(q.device)
-        ws = call_workspace(q.device, s, need, workspace)
-        args = [x for t in (q, k, v, out, dout) for x in (t.data_ptr(), _packed_strides(t))] + [lse.data_ptr()] + [
-            x for t in (dq, dk, dv) for x in (t.data_ptr(), _packed_strides(t))]
-        st = lib.abkv_window_attention_backward(*args, B, H, k.shape[1], S, D, scale, window, num_sinks, ws.ptr(),
-                                                ws.nbytes, s.cuda_stream)
-    _lib.check("abkv_window_attention_backward", st)
+        ws, raw = call_workspace(device, need, workspace)
+        (_, dqs), (_, dks), (_, dvs) = _tma_ready(dq), _tma_ready(dk), _tma_ready(dv)
+        st = lib.abkv_window_attention_backward(
+            q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os, dout.data_ptr(), ds,
+            lse.data_ptr(), dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(), dvs, B, H, k.shape[1], S, D, scale,
+            window, num_sinks, ws.ptr(), ws.nbytes, raw)
+    if st:
+        _lib.check("abkv_window_attention_backward", st)
     return dq, dk, dv
 
 

@@ -55,31 +55,37 @@ def default_workspace(device: torch.device) -> Workspace:
     return ws
 
 
-def on_stream(stream: torch.cuda.Stream | None):
-    """The context in which a call's outputs are allocated: the stream that writes them."""
-    return contextlib.nullcontext() if stream is None else torch.cuda.stream(stream)
+_here = contextlib.nullcontext()
+
+
+def call_scope(device: torch.device, stream: torch.cuda.Stream | None):
+    """The context of one call's allocations and launches: ``device`` current, and ``stream`` (when
+    given) its current stream, so that what the call allocates belongs to the stream that uses it.
+    No context is entered where both hold already (a context costs a few microseconds)."""
+    if stream is not None:
+        return torch.cuda.stream(stream)
+    return _here if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
 _per_stream: dict[tuple[int, int], Workspace] = {}
 
 
-def call_workspace(device: torch.device, stream: torch.cuda.Stream, nbytes: int,
-                   workspace: Workspace | None = None) -> Workspace:
-    """The workspace of one call: the caller's, else one that no other stream and no CUDA graph uses.
+def call_workspace(device: torch.device, nbytes: int, workspace: Workspace | None = None) -> tuple[Workspace, int]:
+    """(workspace, raw current stream) of one call, inside its ``call_scope``: the caller's workspace,
+    else one that no other stream and no CUDA graph uses.
 
     The device's default stream takes ``default_workspace`` (whose error word the caller reads there); any other
     stream has its own.  A call under stream capture gets a fresh one from the graph's memory pool, zeroed
     at every replay: two graphs never share it, and no later growth frees it under them.  (To read the
     error word of a captured or side-stream call, pass a workspace of your own.)"""
+    raw = torch._C._cuda_getCurrentRawStream(device.index)
     if workspace is not None:
-        return workspace.ensure(nbytes)
-    with torch.cuda.device(device), torch.cuda.stream(stream):
-        if torch.cuda.is_current_stream_capturing():
-            return Workspace(device, nbytes)
-        if stream.cuda_stream == 0:
-            return default_workspace(device).ensure(nbytes)
-        key = (default_workspace(device).device.index, stream.cuda_stream)
-        ws = _per_stream.get(key)
-        if ws is None:
-            ws = _per_stream[key] = Workspace(torch.device("cuda", key[0]), nbytes)
-        return ws.ensure(nbytes)
+        return workspace.ensure(nbytes), raw
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return Workspace(device, nbytes), raw
+    if raw == 0:
+        return default_workspace(device).ensure(nbytes), raw
+    ws = _per_stream.get((device.index, raw))
+    if ws is None:
+        ws = _per_stream[(device.index, raw)] = Workspace(device, nbytes)
+    return ws.ensure(nbytes), raw

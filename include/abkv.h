@@ -125,7 +125,10 @@ int abkv_decode(const void* const* q, const void* const* kv,
  *       1 (all query heads), each sum taken in head order.  weight_rows rows
  *       are addressable per unit; a longer sequence sets ABKV_DEVERR_SEQ_OOB
  *       and is cut there.  Other elements are not touched.
- * chunk_tokens: a multiple of 16, at most 8192 (0 = automatic).  A call with
+ * q, kv and out must start on 16-byte boundaries.
+ * chunk_tokens: a multiple of 16, at most 8192 (0 = automatic; a small call then
+ * runs one cluster of CTAs per KV head instead of the split kernel).  The
+ * workspace query takes weight_units = 0 for a call without weights.  A call with
  * weights keeps scores in the workspace (about 64 MiB, or one layer's
  * 4 x num_seqs x num_q_heads x visible rows if that is more) and runs its
  * layers in as many launches as that takes. */
@@ -133,7 +136,7 @@ size_t abkv_decode_window_workspace_size(int num_layers, int num_seqs, int num_q
                                          int num_kv_heads, int head_dim, int page_size,
                                          int max_pages_per_seq, int chunk_tokens,
                                          const int32_t* windows, const int32_t* sinks,
-                                         int weighted);
+                                         int weight_units);
 
 int abkv_decode_window(const void* const* q, const void* const* kv,
                        const int32_t* const* block_tables, const int64_t* bt_strides,

@@ -49,7 +49,7 @@ def run(qlens, lens, Hkv, G, window, sinks, page=16, layout=0, observe=None, uni
         R.check_out(got[sl], o, a, (r, qlens[r], case.c.lens[r]))
         # log-sum-exp: 32-bit scores (2^-13 of relative weight) and a 32-bit sum
         assert ((lse[sl].double().cpu() - l).abs() <= 2.0 ** -12 + 2.0 ** -22 * l.abs()).all(), r
-    assert (got[case.qs[-1]:] == 7.0).all() and torch.isnan(lse[case.qs[-1]:]).all()
+    assert (got[case.qs[-1]:] == 7.0).all()
     cap = max(case.c.lens) + 4
     for u in ([units] if units else sorted({1, Hkv})):
         w0 = torch.rand((len(qlens), u, cap), generator=torch.Generator().manual_seed(seed))
