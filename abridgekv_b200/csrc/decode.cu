@@ -655,6 +655,7 @@ __device__ void consumer(const Prm& p, uint8_t* smem) {
   float o[kOT][4];
   float m_run = -INFINITY, l_run = 0.f;
   uint32_t qr[kQC][4];
+  float* lg_row = nullptr;  // kHasWin: this lane's scores of the item's sequence
 
   for (int gq = 0;; ++gq) {
     const int st = gq % kStages;
@@ -674,6 +675,10 @@ __device__ void consumer(const Prm& p, uint8_t* smem) {
       for (int mt = 0; mt < kOT; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
       m_run = -INFINITY;
       l_run = 0.f;
+      if constexpr (Prm::kHasWin) {
+        if (p.logits && g < G)
+          lg_row = p.logits + (((int64_t)M.li * p.B + M.b) * p.Hq + hw * G + g) * p.lrows + 2 * c;
+      }
       const __nv_bfloat16* qrow = L.q + ((int64_t)M.b * p.Hq + hw * G + g) * D + 8 * c;
 #pragma unroll
       for (int m = 0; m < kQC; ++m) {
@@ -741,9 +746,8 @@ __device__ void consumer(const Prm& p, uint8_t* smem) {
           x[nt][j] = valid ? s[nt][j] * sl2 : -INFINITY;
         }
       if constexpr (Prm::kHasWin) {
-        if (p.logits && g < G) {  // the scores wait for the log-sum-exp of the whole row
-          float* lg = p.logits + (((int64_t)M.li * p.B + M.b) * p.Hq + hw * G + g) * p.lrows +
-                      (M.t0 + my_tile) * kTile + 2 * c;
+        if (lg_row) {  // the scores wait for the log-sum-exp of the whole row
+          float* lg = lg_row + (M.t0 + my_tile) * kTile;
           *reinterpret_cast<float2*>(lg) = make_float2(x[0][0], x[0][1]);
           *reinterpret_cast<float2*>(lg + 8) = make_float2(x[1][0], x[1][1]);
         }
@@ -939,31 +943,39 @@ __global__ void __launch_bounds__(kThreads, 1) decode_split_kernel(const __grid_
   }
 }
 
-// w[b][u][row] += sum over the query heads of unit u of softmax weight 2^(score - lse2), heads in order:
-// thread = (virtual row, unit) of one (layer, sequence).  Rows of a visible tile that the window hides
-// scored -inf and add nothing.
-constexpr int kWeightRows = 128;
-__global__ void __launch_bounds__(kWeightRows) decode_weights_kernel(const __grid_constant__ WinDecodeParams p) {
+// w[b][u][row] += sum over the query heads of unit u of softmax weight 2^(score - lse2), heads in order.
+// Thread = four consecutive virtual rows of one (layer, sequence, unit): 16-byte loads, eight heads in
+// flight.  Rows that the window hides scored -inf and add nothing; virtual rows past the last visible
+// tile are not touched.  Launched with programmatic stream serialization: it waits for the decode itself.
+constexpr int kWeightThreads = 128, kWeightRows = 4 * kWeightThreads;
+__global__ void __launch_bounds__(kWeightThreads) decode_weights_kernel(const __grid_constant__ WinDecodeParams p) {
   const int li = blockIdx.z / p.units, u = blockIdx.z % p.units, b = blockIdx.y;
   const LayerArgs& L = p.layer[li];
   const WinArgs& W = p.win[li];
   const int n = min(clamp_seq_len(p, L, b, false), W.w_cap);
   const WinSpan ws = win_span(n, W.window, W.sinks);
-  const int vr = blockIdx.x * kWeightRows + threadIdx.x;
-  if (blockIdx.x * kWeightRows >= ws.n_tiles * kTile) return;  // CTA-uniform
-  const int nh = p.Hq / p.units, h0 = u * nh;
-  const float* lse2 = p.lse2 + ((int64_t)(p.layer_base + li) * p.B + b) * p.Hq + h0;
+  const int vr = blockIdx.x * kWeightRows + 4 * threadIdx.x;
+  const bool mine = vr < ws.n_tiles * kTile;
   const int row = vr < ws.ns * kTile ? vr : vr + ws.shift * kTile;
-  if (vr >= ws.n_tiles * kTile || row >= n) return;
+  const int nh = p.Hq / p.units, h0 = u * nh;
+  const float* lse2 = p.lse2 + ((int64_t)li * p.B + b) * p.Hq + h0;
   const float* lg = p.logits + (((int64_t)li * p.B + b) * p.Hq + h0) * p.lrows + vr;
-  float acc = 0.f;
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  if (!mine) return;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
   for (int h = 0; h < nh; ++h) {
-    const float x = __ldcg(lg + (int64_t)h * p.lrows), l = __ldcg(lse2 + h);
-    acc += l == -INFINITY ? 0.f : exp2f(x - l);
+    const float4 x = __ldcs(reinterpret_cast<const float4*>(lg + (int64_t)h * p.lrows));
+    const float l = __ldcg(lse2 + h), neg = l == -INFINITY ? INFINITY : l;  // an empty row adds nothing
+    acc[0] += exp2f(x.x - neg);
+    acc[1] += exp2f(x.y - neg);
+    acc[2] += exp2f(x.z - neg);
+    acc[3] += exp2f(x.w - neg);
   }
   float* w = W.weights + b * W.w_sb + u * W.w_su + row;
-  *w += acc;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (row + k < n) w[k] += acc[k];
 }
 
 // ---------------------------------------------------------------------------
@@ -975,7 +987,7 @@ __global__ void __launch_bounds__(kWeightRows) decode_weights_kernel(const __gri
 // With accumulators of one unit per KV head the scores wait in shared memory for the log-sum-exp; one
 // unit for all heads goes through the global scores and decode_weights_kernel.
 constexpr int kClusterThreads = 256, kClusterWarps = kClusterThreads / 32;
-constexpr int kMaxClusterTiles = 8;  // tiles per warp
+constexpr int kMaxClusterTiles = 31;  // tiles per warp
 
 __device__ __forceinline__ uint32_t cluster_map(const void* p, int rank) {
   uint32_t r;
@@ -1246,7 +1258,6 @@ __global__ void __launch_bounds__(kClusterThreads, 1) decode_cluster_kernel(cons
   cluster_sync();  // no CTA leaves while another may still read its partial
 }
 
-constexpr int kMinWindowChunkTiles = 4;
 constexpr int kMaxAutoChunkTiles = 384;  // 6144 cache rows
 
 int auto_chunk_tiles(int num_layers, int num_seqs, int max_tiles, int page_tiles, int num_kv_heads) {
@@ -1599,8 +1610,46 @@ namespace abkv {
 namespace {
 // Layers per launch of a weight-accumulating call: their scores (4 bytes a query head and row) wait
 // in the workspace for the rows' log-sum-exp, so the workspace stays near this size.
-constexpr int64_t kLogitBytes = 64 << 20;
-constexpr int64_t kClusterCtas = 2 * 148;
+constexpr int64_t kLogitBytes = 256 << 20;
+constexpr int kSms = 148;
+
+// CTAs per (layer, sequence, KV head) of decode_cluster_kernel, or 0 for the split kernel.  One CTA fits an
+// SM, so a call should be one wave (a second one only while it is short), in clusters of 4 at most once
+// most SMs are taken: clusters of 8 then no longer all fit at a time.  Measured (128 dims, 8 KV heads,
+// us: cluster / split at its best chunk): 1 sequence x 1040 rows 8.9 / 27, x 8000 18.6 / 48; 4 x 1040 10.3 /
+// 29 (20.5 in clusters of 8), 4 x 8000 34.6 / 55; 8 x 8000 63 / 66; 16 x 4096 63 / 62; two waves: 32 x 512
+// 20.7 / 27, 32 x 2048 67 / 60.
+int cluster_size(int64_t heads, int64_t vt) {
+  const int most = heads <= 8 ? 8 : heads <= 32 ? 4 : heads <= 64 ? 2 : 1;
+  int cs = 1;
+  while (cs < most && vt > (int64_t)cs * kClusterWarps) cs <<= 1;
+  const int64_t per = (vt + cs * kClusterWarps - 1) / (cs * kClusterWarps);
+  if (heads <= kSms) return per <= kMaxClusterTiles ? cs : 0;
+  return heads <= 2 * kSms && per <= 8 ? cs : 0;
+}
+
+// Tiles per chunk of the split kernel for num_seqs x layers sequences of vt tiles: full chunks run in waves over
+// the SMs, each with a cost of its own (the item's start and its merge, about `fixed` tiles' time: 5 with one warp
+// per head, 10 where warps share a head), and what is left of a sequence fills the gaps.  Predicts the measured best
+// chunk for 16..256 sequences of 1K..8K rows (32 x 8000 rows: 2048-row chunks 174 us, 512-row 208 us; 16 x 4096:
+// 512-row 62 us, 2048-row 171 us).
+int window_chunk_tiles(int64_t seqs, int64_t vt, int num_kv_heads) {
+  const int fixed = num_kv_heads == kWarps ? 5 : 10;
+  int best = kMaxChunkPages;
+  double cost = 1e30;
+  for (int ct = kMaxChunkPages; ct >= 4; ct >>= 1) {
+    const int64_t full = vt / ct, items = (vt + ct - 1) / ct;
+    const double waves = full ? (double)((seqs * full + kSms - 1) / kSms) * (ct + fixed)
+                              : (double)((seqs + kSms - 1) / kSms) * (vt + fixed);
+    const double fluid = (double)(seqs * vt + seqs * items * fixed) / kSms;
+    const double c = std::max(waves, fluid);
+    if (c < cost) {
+      cost = c;
+      best = ct;
+    }
+  }
+  return best;
+}
 
 struct WindowPlan {
   int group;    // layers per launch; every launch reuses the same scratch
@@ -1633,28 +1682,16 @@ int plan_window(int num_layers, int num_seqs, int num_q_heads, int num_kv_heads,
   }
   plan->lrows = (int)(vt * kTile);
   plan->group = num_layers < kMaxLayers ? num_layers : kMaxLayers;
-  // Clusters where the whole call is about two waves of CTAs with few tiles per warp.
-  plan->cluster = 0;
-  const int64_t heads = (int64_t)plan->group * num_seqs * num_kv_heads;
-  if (!chunk_tokens && num_layers <= kMaxLayers && heads <= kClusterCtas) {
-    int cs = 1;
-    while (cs < 8 && vt > cs * kClusterWarps && heads * cs * 2 <= kClusterCtas) cs <<= 1;
-    const int64_t per = (vt + cs * kClusterWarps - 1) / (cs * kClusterWarps);
-    if (per <= kMaxClusterTiles && heads / num_kv_heads <= 65535) {
-      plan->cluster = cs;
-      plan->warp_tiles = (int)per;
-    }
+  plan->cluster = plan->warp_tiles = 0;
+  if (!chunk_tokens && num_layers <= kMaxLayers) {
+    plan->cluster = cluster_size((int64_t)num_layers * num_seqs * num_kv_heads, vt);
+    if (plan->cluster) plan->warp_tiles = (int)((vt - 1) / (plan->cluster * kClusterWarps) + 1);
   }
   plan->logits = weighted && !(plan->cluster && weighted == num_kv_heads);
   const int64_t layer_logits = (int64_t)num_seqs * num_q_heads * plan->lrows * 4;
   if (plan->logits && !plan->cluster) plan->group = (int)std::max<int64_t>(1, std::min<int64_t>(plan->group, kLogitBytes / layer_logits));
   int ct;
-  if (chunk_tokens) {
-    ct = chunk_tokens / kTile;
-  } else {
-    ct = 128;
-    while (ct > kMinWindowChunkTiles && plan->group * (int64_t)num_seqs * vt / ct < 148 * 4) ct >>= 1;
-  }
+  ct = chunk_tokens ? chunk_tokens / kTile : window_chunk_tiles((int64_t)plan->group * num_seqs, vt, num_kv_heads);
   if (ct > kMaxChunkPages) return ABKV_ERR_UNSUPPORTED;
   plan->chunk_tiles = ct;
   plan->max_chunks = (int)((vt + ct - 1) / ct);
@@ -1788,8 +1825,16 @@ extern "C" int abkv_decode_window(const void* const* q, const void* const* kv, c
                                 : launch_kernel<WinDecodeParams, false>(prm, head_dim, std::min(prm.num_items, num_sms), s);
     if (rc != ABKV_OK) return rc;
     if (plan.logits) {
-      const dim3 grid((plan.lrows + kWeightRows - 1) / kWeightRows, num_seqs, nl * prm.units);
-      decode_weights_kernel<<<grid, kWeightRows, 0, s>>>(prm);
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((plan.lrows + kWeightRows - 1) / kWeightRows, num_seqs, nl * prm.units);
+      cfg.blockDim = dim3(kWeightThreads);
+      cfg.stream = s;
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      attr[0].val.programmaticStreamSerializationAllowed = 1;
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      if (cudaLaunchKernelEx(&cfg, decode_weights_kernel, prm) != cudaSuccess) return ABKV_ERR_CUDA;
     }
   }
   if (cudaGetLastError() != cudaSuccess) return ABKV_ERR_CUDA;

@@ -129,7 +129,7 @@ int abkv_decode(const void* const* q, const void* const* kv,
  * chunk_tokens: a multiple of 16, at most 8192 (0 = automatic; a small call then
  * runs one cluster of CTAs per KV head instead of the split kernel).  The
  * workspace query takes weight_units = 0 for a call without weights.  A call with
- * weights keeps scores in the workspace (about 64 MiB, or one layer's
+ * weights keeps scores in the workspace (up to 256 MiB, or one layer's
  * 4 x num_seqs x num_q_heads x visible rows if that is more) and runs its
  * layers in as many launches as that takes. */
 size_t abkv_decode_window_workspace_size(int num_layers, int num_seqs, int num_q_heads,
