@@ -316,15 +316,11 @@ def evict_by_weight(kv_caches: Sequence[torch.Tensor], block_tables: Sequence[to
         raise ValueError("every layer needs its own weights tensor")
     lib = _lib.lib()
     with call_scope(dev, stream):
-        # one allocation per kind, a view per layer
-        new = torch.empty((L, B), dtype=torch.int32, device=dev).unbind(0)
-        outs = weights if in_place_weights else torch.empty((L, B, units, rows), dtype=torch.float32, device=dev).unbind(0)
-        keep = None
-        if return_keep:
-            sizes = [B * units * m for m in budgets]
-            keep = [t.view(B, units, m) for t, m in zip(torch.empty(sum(sizes), dtype=torch.int32, device=dev).split(sizes),
-                                                        budgets)]
-        result = Evicted(list(new), list(outs), keep)
+        new = [torch.empty(B, dtype=torch.int32, device=dev) for _ in range(L)]
+        outs = list(weights) if in_place_weights else [torch.empty((B, units, rows), dtype=torch.float32, device=dev)
+                                                       for _ in range(L)]
+        keep = [torch.empty((B, units, m), dtype=torch.int32, device=dev) for m in budgets] if return_keep else None
+        result = Evicted(new, outs, keep)
         if B == 0:
             return result
         if rows == 0:

@@ -183,4 +183,6 @@ def test_refusals():
     with pytest.raises(TypeError, match="block_table"):
         ev(kv, [bt[0].long()], sl, w, budget=8)
     with pytest.raises(_lib.AbkvError):
+        ev(kv, bt, sl, w, budget=8, dst_block_tables=bt)
+    with pytest.raises(_lib.AbkvError):
         ev([torch.zeros((4, 2, 16, 2, 32), dtype=torch.bfloat16, device="cuda")], bt, sl, w, budget=8)
