@@ -8,9 +8,9 @@
 //
 // Two kernels.  select: one CTA per unit.  The weights become order-preserving 32-bit keys (-0 as
 // +0, NaN as -inf), are held in shared memory, and the (m - sinks - recent)-th largest key is found by
-// three histogram passes over 11, 11 and 10 key bits.  A warp first groups equal digits (attention
-// weights share few exponents: one shared-memory add per distinct digit instead of up to 32 on one
-// address).  Then every warp walks its contiguous share of the rows twice, counting and emitting by
+// histogram passes over 11, 11 and 10 key bits, of which the last are left out once they decide nothing
+// (plain shared-memory adds, one per warp where its rows share the digit; grouping equal digits first with
+// match.any was 1.3 to 3 us slower on 1311 and 8190 rows).  Then every warp walks its contiguous share of the rows twice, counting and emitting by
 // ballot, so the kept list comes out in row order with one scan over the warps.
 // move: bound by memory, so as many bytes in flight as fit: rows go through a shared-memory ring (see
 // evict_move_kernel).
@@ -140,8 +140,14 @@ __global__ void __launch_bounds__(kSelThreads, 1) evict_select_kernel(const __gr
           const uint32_t k = i < e ? key_at(i) : 0u;
           const bool in = i < e && (k & mask) == prefix;
           const uint32_t digit = in ? (k >> shift) & dmask : 0xFFFFFFFFu;
-          const uint32_t peers = __match_any_sync(0xffffffffu, digit);
-          if (in && lane == __ffs(peers) - 1) atomicAdd(&s_hist[digit], __popc(peers));
+          // one add where the warp's rows share a digit (rows never attended to, ties)
+          const uint32_t act = __ballot_sync(0xffffffffu, in);
+          const uint32_t first = __shfl_sync(0xffffffffu, digit, act ? __ffs(act) - 1 : 0);
+          if (__all_sync(0xffffffffu, !in || digit == first)) {
+            if (act && lane == 0) atomicAdd(&s_hist[first], __popc(act));
+          } else if (in) {
+            atomicAdd(&s_hist[digit], 1);
+          }
         }
         __syncthreads();
         // thread t holds bins kBins - 1 - 2t and kBins - 2 - 2t: a running count from the largest digit
