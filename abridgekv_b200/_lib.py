@@ -117,10 +117,10 @@ SIGNATURES: dict[str, tuple] = {
                                              c_i64p, c_vp, c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_i32p,
                                              c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_int, C.c_float,
                                              c_vp, c_size, c_vp]),
-    "abkv_window_attention": (c_int, [c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_vp, c_int, c_int, c_int,
-                                      c_int, c_int, C.c_float, c_int, c_int, c_vp, c_size, c_vp]),
+    "abkv_window_attention": (c_int, [c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_vp, c_i64p, c_vp, c_vp, c_int, c_int,
+                                      c_int, c_int, c_int, C.c_float, c_int, c_int, c_vp, c_size, c_vp]),
     "abkv_window_attention_backward_workspace_size": (c_size, [c_int, c_int, c_int, c_int]),
-    "abkv_window_attention_backward": (c_int, [c_vp, c_i64p] * 5 + [c_vp] + [c_vp, c_i64p] * 3 +
+    "abkv_window_attention_backward": (c_int, [c_vp, c_i64p] * 4 + [c_vp] + [c_vp, c_i64p] + [c_vp] + [c_vp, c_i64p] * 3 +
                                        [c_int, c_int, c_int, c_int, c_int, C.c_float, c_int, c_int, c_vp, c_size,
                                         c_vp]),
     "abkv_code_step_attention": (c_int, [c_vp, c_i64, c_i64, c_vp, c_i64, c_i64, c_vp, c_vp, c_int, c_i64, c_int,

@@ -119,6 +119,7 @@ struct alignas(64) PrefillParams {
   int B, H, Hkv, G, npairs, S, C, KL, per, n_qtiles;
   float scale_log2;
   int window, n_sink;  // kWin
+  int8_t* out_lo;      // kWin, optional: [B][H][S][D] the eight mantissa bits after out's
 };
 
 // Softmax of one (head, 64-key tile) for query row `row` (= TMEM lane), columns
@@ -213,6 +214,17 @@ __device__ __forceinline__ void softmax_half(const PrefillParams& p, int lim, in
     }
   }
   tmem_wait_st();
+}
+
+// The eight mantissa bits below the bf16 rounding of four floats: the difference of the bit patterns, in units
+// of 2^8 (bit patterns of one sign are ordered like the values, so adding it back needs no exponent).
+__device__ __forceinline__ uint32_t low_bits4(float a, float b, float c, float d) {
+  auto one = [](float x) -> uint32_t {
+    const int32_t hi = (int32_t)((uint32_t)__bfloat16_as_ushort(__float2bfloat16(x)) << 16);
+    const int32_t diff = (__float_as_int(x) - hi + 128) >> 8;  // in [-128, 128]
+    return (uint32_t)min(diff, 127) & 0xFFu;
+  };
+  return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
 }
 
 __device__ __forceinline__ bool visit_tile(const PrefillParams& p, int hA, int hB, int qt, int kt, int pl) {
@@ -445,6 +457,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             for (int i = 0; i < 32; ++i) t[i] = 0.f;
           }
           const int d0 = (D / 2) * half + 32 * c4;  // first dim of these 32
+          if (kWin && p.out_lo && q < p.S) {
+            uint4 lo[2];
+            uint32_t* l = reinterpret_cast<uint32_t*>(lo);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              l[i] = low_bits4(t[4 * i] * inv, t[4 * i + 1] * inv, t[4 * i + 2] * inv, t[4 * i + 3] * inv);
+            uint4* dst = reinterpret_cast<uint4*>(p.out_lo + (((int64_t)b * p.H + h) * p.S + q) * D + d0);
+            dst[0] = lo[0];
+            dst[1] = lo[1];
+          }
           uint8_t* atom = stage + (d0 / 64) * (kQBytes / kAtoms);
 #pragma unroll
           for (int v8 = 0; v8 < 4; ++v8)
@@ -556,15 +578,15 @@ extern "C" int abkv_prefill_masked(const void* q, const int64_t* q_strides, cons
 
 extern "C" int abkv_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                                      const void* v, const int64_t* v_strides, void* out, const int64_t* out_strides,
-                                     float* lse, int B, int H, int Hkv, int S, int head_dim, float scale, int window,
-                                     int num_sinks, void* workspace, size_t workspace_bytes, void* stream) {
+                                     void* out_lo, float* lse, int B, int H, int Hkv, int S, int head_dim,
+                                     float scale, int window, int num_sinks, void* workspace, size_t workspace_bytes, void* stream) {
   if (!q || !k || !v || !out || !q_strides || !k_strides || !v_strides || !out_strides) return ABKV_ERR_INVALID_ARG;
   if (B <= 0 || H <= 0 || Hkv <= 0 || S <= 0 || H % Hkv != 0 || !(scale > 0.f) || window <= 0 || num_sinks < 0)
     return ABKV_ERR_INVALID_ARG;
   if ((head_dim != 64 && head_dim != 128) || H > kMaxHeads || B > 65535 || S > kMaxKeyTiles * kBN)
     return ABKV_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
-       reinterpret_cast<uintptr_t>(out)) & 15)
+       reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_lo)) & 15)
     return ABKV_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < 256 || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return ABKV_ERR_WORKSPACE;
@@ -576,6 +598,7 @@ extern "C" int abkv_window_attention(const void* q, const int64_t* q_strides, co
   if (st == ABKV_OK) st = make_map(&prm.tm_out, out, B, H, S, head_dim, out_strides, kBM);
   if (st != ABKV_OK) return st;
   prm.lse = lse;
+  prm.out_lo = static_cast<int8_t*>(out_lo);
   prm.err = static_cast<int32_t*>(workspace);
   prm.B = B;
   prm.H = H;

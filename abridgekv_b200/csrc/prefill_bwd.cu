@@ -37,11 +37,6 @@
 // further down, which cuts each pair into two 64-query units so that two units
 // are in flight in TMEM at once.
 // Every mbarrier wait is bounded and records ABKV_DEVERR_TIMEOUT on expiry.
-//
-// kWin (abkv_window_attention_backward): both kernels under a causal sliding window with sinks, for any S.
-// The query tiles that see a key tile are a contiguous range (to the end for the sinks' tiles), so the pairs
-// need no list; a query's hidden keys inside the tile are its causal tail and the hole up to its window.
-// Rows past S load as zeros, are masked, and are clipped by the accumulator's [B*H][S][D] map.
 #include <cstring>
 #include <type_traits>
 
@@ -99,41 +94,12 @@ struct alignas(64) BwdParams {
   int quota[kMaxHeads];
   int B, H, Hkv, G, S, C, KL, per, n_tiles;
   float scale, scale_log2;
-  int window, n_sink;  // kWin
 };
-
-// kWin: the pairs of key tile kt are query tiles [first, first + count / G) x the G heads, heads fastest.
-struct WinPairs {
-  int first, count;
-};
-__device__ __forceinline__ WinPairs win_pairs(const BwdParams& p, int kt) {
-  WinPairs w;
-  w.first = kt;
-  int last = p.n_tiles - 1;
-  // the tile's last key k sees queries q < k + window
-  if (kt * kT >= p.n_sink) last = min(last, (min(kt * kT + kT, p.S) - 1 + p.window - 1) / kT);
-  w.count = (last - kt + 1) * p.G;
-  return w;
-}
-// The 128 keys from k0 that query q sees: [0, lim) without [n_sink - k0, he), as lim | he << 16 (0 past S).
-__device__ __forceinline__ int win_limits(const BwdParams& p, int q, int k0) {
-  if (q >= p.S) return 0;
-  const int lim = min(max(q + 1 - k0, 0), kT), he = min(max(q - p.window + 1 - k0, 0), kT);
-  return lim | (he << 16);
-}
-__device__ __forceinline__ bool win_visible(int limits, int row, bool sink) {
-  return row < (limits & 0xFFFF) && (sink || row >= (limits >> 16));
-}
 
 // global[tile at (x, y)] += shared box (f32 add by the TMA engine), tracked by the bulk group.
 __device__ __forceinline__ void tma_reduce_add_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
   asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];\n"
                ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(src)
-               : "memory");
-}
-__device__ __forceinline__ void tma_reduce_add_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
-  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2, %3}], [%4];\n"
-               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(src)
                : "memory");
 }
 // Packed fp32 pairs: (a0, a1) * (b0, b1) + (c0, c1) and (a0 - b0, a1 - b1) * (c0, c1).
@@ -168,7 +134,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       : "memory");
 }
 
-template <int D, bool kWin>
+template <int D>
 __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_kernel(const __grid_constant__ BwdParams p) {
   using LY = Layout<D>;
   constexpr int kAtoms = LY::kAtoms, kTileBytes = LY::kTileBytes;
@@ -186,9 +152,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_kernel(const __grid_c
   const int kt = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   const int G = p.G;
   const int pl = p.prompt_len ? __ldg(p.prompt_len + b) : 0;
-  const int kb = kWin ? 0 : kt * kT / p.per, kw0 = kWin ? 0 : kt * kT - kb * p.per;
-  // query tiles of earlier blocks never see this key tile
-  const int qt_first = kWin ? kt : kb * p.per / kT;
+  const int kb = kt * kT / p.per, kw0 = kt * kT - kb * p.per;
+  const int qt_first = kb * p.per / kT;  // query tiles of earlier blocks never see this key tile
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBarTmem; ++i) mbar_init(&bar[i], (i == kBarP || i == kBarFree) ? 256 : 1);
@@ -198,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_kernel(const __grid_c
                  "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
   }
-  if (!kWin && warp == 2) {  // the (query tile, head) pairs this key tile contributes to, by ballot
+  if (warp == 2) {  // the (query tile, head) pairs this key tile contributes to, by ballot
     int n = 0;
     const int total = (p.n_tiles - qt_first) * G;
     for (int base = 0; base < total; base += 32) {
@@ -219,9 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_kernel(const __grid_c
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  const int n_pairs = kWin ? win_pairs(p, kt).count : *s_n;
-  // pair i as (query tile << 8 | head)
-  auto pair_at = [&](int i) -> int { return kWin ? ((qt_first + i / G) << 8) | (i % G) : s_list[i]; };
+  const int n_pairs = *s_n;
   bool dead = false;
 
   if (warp == 0) {
@@ -233,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_kernel(const __grid_c
         tma_load_4d(smem + LY::kOffV + a * (kTileBytes / kAtoms), &p.tm_v, 64 * a, kt * kT, hk, b, &bar[kBarKV]);
       }
       for (int i = 0; i < n_pairs; ++i) {
-        const int e = pair_at(i);
+        const int e = s_list[i];
         const int qt = e >> 8, h = hk * G + (e & 0xFF);
         if (!wait_or_abort(&bar[kBarQDE], (uint32_t)((i & 1) ^ 1), dead, p.err)) break;
         mbar_expect_tx(&bar[kBarQD], 2 * kTileBytes);
@@ -305,26 +268,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_kernel(const __grid_c
     const int row = quarter * 32 + lane;  // key row (P / dS phase), query row (dQ read-back)
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const float sl2 = p.scale_log2, scale = p.scale;
-    const bool sink = kWin && kt * kT + row < p.n_sink;  // this thread's key is a sink
     const uint32_t ds_row = smem_u32(smem + LY::kOffDS) + hf * (kT * 128) + row * 128;  // atom column hf
     for (int i = 0; i < n_pairs; ++i) {
       const uint32_t par = (uint32_t)(i & 1);
-      const int e = pair_at(i);
+      const int e = s_list[i];
       const int qt = e >> 8, h = hk * G + (e & 0xFF);
       if (hf == 0) {  // the 128 query rows of this pair: log2-domain lse, Di and the visible-key prefix
         const int q = qt * kT + row;
         const int64_t rr = ((int64_t)b * p.H + h) * p.S + q;
-        if constexpr (kWin) {
-          const bool in = q < p.S;
-          s_lse2[row] = in ? __ldg(p.lse + rr) * 1.4426950408889634f : 0.f;
-          s_di[row] = in ? __ldg(p.di + rr) : 0.f;
-          s_lim[row] = win_limits(p, q, kt * kT);
-        } else {
-          const int qb = q / p.per, qw = q - qb * p.per;
-          s_lse2[row] = __ldg(p.lse + rr) * 1.4426950408889634f;
-          s_di[row] = __ldg(p.di + rr);
-          s_lim[row] = tile_limit_fast(p, p.quota[h], q, qb, qw, kb, kw0, kt * kT, pl);
-        }
+        const int qb = q / p.per, qw = q - qb * p.per;
+        s_lse2[row] = __ldg(p.lse + rr) * 1.4426950408889634f;
+        s_di[row] = __ldg(p.di + rr);
+        s_lim[row] = tile_limit_fast(p, p.quota[h], q, qb, qw, kb, kw0, kt * kT, pl);
       }
       softmax_bar();
       const bool ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarS], par, dead, p.err));
@@ -360,8 +315,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_kernel(const __grid_c
             const int cc = 8 * c8 + j;
             float x0, x1;
             fma2v(x0, x1, sv[cc], sv[cc + 1], sl2, sl2, -lse[j], -lse[j + 1]);
-            pv[j] = (kWin ? win_visible(lim[j], row, sink) : row < lim[j]) ? fast_exp2(x0) : 0.f;
-            pv[j + 1] = (kWin ? win_visible(lim[j + 1], row, sink) : row < lim[j + 1]) ? fast_exp2(x1) : 0.f;
+            pv[j] = row < lim[j] ? fast_exp2(x0) : 0.f;
+            pv[j + 1] = row < lim[j + 1] ? fast_exp2(x1) : 0.f;
             // dS = (dP - Di) * (P * scale)
             submul2(dsv[j], dsv[j + 1], dpv[cc], dpv[cc + 1], di[j], di[j + 1], pv[j] * scale, pv[j + 1] * scale);
           }
@@ -416,13 +371,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_kernel(const __grid_c
         softmax_bar();  // every row of this half is staged
         if (issuer) {
           if (!dead) {
-            if constexpr (kWin) {
-              tma_reduce_add_3d(&p.tm_dq, stage, 64 * half, qt * kT, b * p.H + h);
-              tma_reduce_add_3d(&p.tm_dq, stage + kT * 128, 64 * half + 32, qt * kT, b * p.H + h);
-            } else {
-              tma_reduce_add_2d(&p.tm_dq, stage, 64 * half, y0);
-              tma_reduce_add_2d(&p.tm_dq, stage + kT * 128, 64 * half + 32, y0);
-            }
+            tma_reduce_add_2d(&p.tm_dq, stage, 64 * half, y0);
+            tma_reduce_add_2d(&p.tm_dq, stage + kT * 128, 64 * half + 32, y0);
             bulk_commit();
           }
           if (half + 1 < D / 64) bulk_wait_read();
@@ -455,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_kernel(const __grid_c
           pk.y = pack_bf16x2(t[v8 * 8 + 2], t[v8 * 8 + 3]);
           pk.z = pack_bf16x2(t[v8 * 8 + 4], t[v8 * 8 + 5]);
           pk.w = pack_bf16x2(t[v8 * 8 + 6], t[v8 * 8 + 7]);
-          if (!kWin || key < p.S) *reinterpret_cast<uint4*>(outr + c4 * 32 + v8 * 8) = pk;
+          *reinterpret_cast<uint4*>(outr + c4 * 32 + v8 * 8) = pk;
         }
       }
     }
@@ -518,7 +468,6 @@ constexpr int kUBarKV = 0, kUBarQD = 1, kUBarQDE = kUBarQD + kQSlots, kUBarS = k
               kUBarTmem = kUBarAcc + 1;
 static_assert((kUBarTmem + 1) * 8 <= 256, "barrier area");
 
-template <bool kWin>
 __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_unit_kernel(const __grid_constant__ BwdParams p) {
   using LY = LayoutU;
   extern __shared__ uint8_t smem_raw[];
@@ -536,8 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_unit_kernel(const __g
   const int kt = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
   const int G = p.G;
   const int pl = p.prompt_len ? __ldg(p.prompt_len + b) : 0;
-  const int kb = kWin ? 0 : kt * kT / p.per, kw0 = kWin ? 0 : kt * kT - kb * p.per;
-  const int qt_first = kWin ? kt : kb * p.per / kT;
+  const int kb = kt * kT / p.per, kw0 = kt * kT - kb * p.per;
+  const int qt_first = kb * p.per / kT;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kUBarTmem; ++i) {
@@ -550,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_unit_kernel(const __g
                  "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
   }
-  if (!kWin && warp == 2) {  // the (query tile, head) pairs this key tile contributes to, by ballot
+  if (warp == 2) {  // the (query tile, head) pairs this key tile contributes to, by ballot
     int n = 0;
     const int total = (p.n_tiles - qt_first) * G;
     for (int base = 0; base < total; base += 32) {
@@ -571,9 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_unit_kernel(const __g
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  const int n_units = 2 * (kWin ? win_pairs(p, kt).count : *s_n);
-  // pair i as (query tile << 8 | head)
-  auto pair_at = [&](int i) -> int { return kWin ? ((qt_first + i / G) << 8) | (i % G) : s_list[i]; };
+  const int n_units = 2 * *s_n;
   bool dead = false;
 
   if (warp == 0) {
@@ -585,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_unit_kernel(const __g
         tma_load_4d(smem + LY::kOffV + a * (LY::kKV / 2), &p.tm_v, 64 * a, kt * kT, hk, b, &bar[kUBarKV]);
       }
       for (int u = 0; u < n_units; ++u) {
-        const int e = pair_at(u >> 1);
+        const int e = s_list[u >> 1];
         const int qrow = (e >> 8) * kT + kU * (u & 1), h = hk * G + (e & 0xFF);
         const int qs = u % kQSlots, use = u / kQSlots;
         // slot qs is free once the dV / dK MMAs of unit u - 3 ran (immediate for the first use)
@@ -676,7 +623,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_unit_kernel(const __g
     const int row = quarter * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const float sl2 = p.scale_log2;
-    const bool sink = kWin && kt * kT + row < p.n_sink;  // this thread's key is a sink
     const bool issuer = threadIdx.x == 64;
     const uint32_t stage = smem_u32(smem + LY::kOffStage);
     // dQ^T of unit v: read out of its TMEM buffer (lane = dim, query columns [32 hf, 32 hf + 32))
@@ -695,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_unit_kernel(const __g
     };
     auto reduce_dq = [&](int v) {
       const int s = v & 1, i = v >> 1;
-      const int e = pair_at(i);
+      const int e = s_list[i];
       const int qt = e >> 8, h = hk * G + (e & 0xFF);
       if (issuer) bulk_wait_read();  // the previous unit's reductions have read the staging buffer
       softmax_bar();
@@ -711,16 +657,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_unit_kernel(const __g
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       softmax_bar();  // the unit's dQ is staged
       if (issuer && !dead) {
-        if constexpr (kWin) {
+        const int y0 = (int)(((int64_t)b * p.H + h) * p.S + qt * kT + kU * s);
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (qt * kT + kU * s < p.S)
-              tma_reduce_add_3d(&p.tm_dq, stage + c * (kU * 128), 32 * c, qt * kT + kU * s, b * p.H + h);
-        } else {
-          const int y0 = (int)(((int64_t)b * p.H + h) * p.S + qt * kT + kU * s);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tma_reduce_add_2d(&p.tm_dq, stage + c * (kU * 128), 32 * c, y0);
-        }
+        for (int c = 0; c < 4; ++c) tma_reduce_add_2d(&p.tm_dq, stage + c * (kU * 128), 32 * c, y0);
         bulk_commit();
       }
     };
@@ -731,21 +670,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_unit_kernel(const __g
     float n_lse = 0.f, n_di = 0.f;
     int n_lim = 0;
     auto fetch_rows = [&](int u) {
-      const int e = pair_at(u >> 1);
+      const int e = s_list[u >> 1];
       const int qt = e >> 8, h = hk * G + (e & 0xFF);
       const int q = qt * kT + kU * (u & 1) + row;
       const int64_t rr = ((int64_t)b * p.H + h) * p.S + q;
-      if constexpr (kWin) {
-        const bool in = q < p.S;
-        n_lse = in ? __ldg(p.lse + rr) : 0.f;
-        n_di = in ? __ldg(p.di + rr) : 0.f;
-        n_lim = win_limits(p, q, kt * kT);
-      } else {
-        const int qb = q / p.per, qw = q - qb * p.per;
-        n_lse = __ldg(p.lse + rr);
-        n_di = __ldg(p.di + rr);
-        n_lim = tile_limit_fast(p, p.quota[h], q, qb, qw, kb, kw0, kt * kT, pl);
-      }
+      const int qb = q / p.per, qw = q - qb * p.per;
+      n_lse = __ldg(p.lse + rr);
+      n_di = __ldg(p.di + rr);
+      n_lim = tile_limit_fast(p, p.quota[h], q, qb, qw, kb, kw0, kt * kT, pl);
     };
     if (stager && n_units > 0) fetch_rows(0);
     for (int u = 0; u < n_units; ++u) {
@@ -755,8 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_unit_kernel(const __g
         s_di[kU * s + row] = n_di;
         s_lim[kU * s + row] = n_lim;
         // the stagers are lane quarters 0 and 1 (rows 0..63), one warp each
-        // kWin: lim = 128 and no hole (he = 0)
-        const bool all = __all_sync(0xffffffffu, kWin ? n_lim == kT : n_lim >= kT);
+        const bool all = __all_sync(0xffffffffu, n_lim >= kT);
         if (lane == 0) s_allvis[2 * s + quarter] = all;
       }
       softmax_bar();
@@ -804,8 +735,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_unit_kernel(const __g
               pv[j] = fast_exp2(x0);
               pv[j + 1] = fast_exp2(x1);
               if constexpr (!kAll) {
-                pv[j] = (kWin ? win_visible(lim[j], row, sink) : row < lim[j]) ? pv[j] : 0.f;
-                pv[j + 1] = (kWin ? win_visible(lim[j + 1], row, sink) : row < lim[j + 1]) ? pv[j + 1] : 0.f;
+                pv[j] = row < lim[j] ? pv[j] : 0.f;
+                pv[j + 1] = row < lim[j + 1] ? pv[j + 1] : 0.f;
               }
               submul2(dsv[j], dsv[j + 1], dpv[cc], dpv[cc + 1], di[j], di[j + 1], pv[j], pv[j + 1]);
             }
@@ -861,7 +792,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_bwd_unit_kernel(const __g
           pk.y = pack_bf16x2(t[v8 * 8 + 2], t[v8 * 8 + 3]);
           pk.z = pack_bf16x2(t[v8 * 8 + 4], t[v8 * 8 + 5]);
           pk.w = pack_bf16x2(t[v8 * 8 + 6], t[v8 * 8 + 7]);
-          if (!kWin || key < p.S) *reinterpret_cast<uint4*>(outr + c4 * 32 + v8 * 8) = pk;
+          *reinterpret_cast<uint4*>(outr + c4 * 32 + v8 * 8) = pk;
         }
       }
     }
@@ -1031,7 +962,7 @@ extern "C" int abkv_prefill_masked_backward(
         static_cast<const __nv_bfloat16*>(dout), dout_strides[0], dout_strides[1], dout_strides[2], di, B, H, S,
         head_dim);
   }
-  auto kernel = head_dim == 64 ? prefill_bwd_kernel<64, false> : prefill_bwd_unit_kernel<false>;
+  auto kernel = head_dim == 64 ? prefill_bwd_kernel<64> : prefill_bwd_unit_kernel;
   const int smem = head_dim == 64 ? Layout<64>::kSmem : LayoutU::kSmem;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return ABKV_ERR_CUDA;
@@ -1043,94 +974,6 @@ extern "C" int abkv_prefill_masked_backward(
                                                                   S, head_dim,
                                                                   head_dim == 128 ? scale : 1.f);
   }
-  if (cudaGetLastError() != cudaSuccess) return ABKV_ERR_CUDA;
-  return ABKV_OK;
-}
-
-extern "C" size_t abkv_window_attention_backward_workspace_size(int B, int H, int S, int head_dim) {
-  return abkv_prefill_masked_backward_workspace_size(B, H, S, head_dim);
-}
-
-extern "C" int abkv_window_attention_backward(
-    const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
-    const int64_t* v_strides, const void* out, const int64_t* out_strides, const void* dout,
-    const int64_t* dout_strides, const float* lse, void* dq, const int64_t* dq_strides, void* dk,
-    const int64_t* dk_strides, void* dv, const int64_t* dv_strides, int B, int H, int Hkv, int S, int head_dim,
-    float scale, int window, int num_sinks, void* workspace, size_t workspace_bytes, void* stream) {
-  const void* ptrs[9] = {q, k, v, out, dout, dq, dk, dv, lse};
-  for (const void* x : ptrs)
-    if (!x) return ABKV_ERR_INVALID_ARG;
-  const int64_t* strs[8] = {q_strides, k_strides, v_strides, out_strides, dout_strides, dq_strides, dk_strides,
-                            dv_strides};
-  for (const int64_t* x : strs)
-    if (!x) return ABKV_ERR_INVALID_ARG;
-  if (B <= 0 || H <= 0 || Hkv <= 0 || S <= 0 || H % Hkv != 0 || !(scale > 0.f) || window <= 0 || num_sinks < 0)
-    return ABKV_ERR_INVALID_ARG;
-  if ((head_dim != 64 && head_dim != 128) || H > kMaxHeads || B > 65535 || S > (1 << 17)) return ABKV_ERR_UNSUPPORTED;
-  if ((int64_t)B * H * S > INT32_MAX) return ABKV_ERR_UNSUPPORTED;
-  for (int i = 0; i < 8; ++i)
-    if (reinterpret_cast<uintptr_t>(ptrs[i]) & 15) return ABKV_ERR_INVALID_ARG;
-  for (int i = 3; i < 8; ++i)
-    if (strs[i][0] % 8 || strs[i][1] % 8 || strs[i][2] % 8) return ABKV_ERR_INVALID_ARG;
-  const size_t need = bwd_workspace(B, H, S, head_dim);
-  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))
-    return ABKV_ERR_WORKSPACE;
-  char* ws = static_cast<char*>(workspace);
-  const size_t rows = (size_t)B * H * S;
-  float* dq_acc = reinterpret_cast<float*>(ws + kWsHeader);
-  float* di = reinterpret_cast<float*>(ws + kWsHeader + (rows * head_dim * 4 + 255) / 256 * 256);
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  BwdParams prm;
-  std::memset(&prm, 0, sizeof(prm));
-  const int qrows = head_dim == 128 ? kU : kT;
-  int st = make_map(&prm.tm_q, q, B, H, S, head_dim, q_strides, qrows);
-  if (st == ABKV_OK) st = make_map(&prm.tm_do, dout, B, H, S, head_dim, dout_strides, qrows);
-  if (st == ABKV_OK) st = make_map(&prm.tm_k, k, B, Hkv, S, head_dim, k_strides, kT);
-  if (st == ABKV_OK) st = make_map(&prm.tm_v, v, B, Hkv, S, head_dim, v_strides, kT);
-  if (st == ABKV_OK) {
-    // [B*H][S][D]: a box that runs past S is clipped instead of reaching the next head's rows
-    const cuuint64_t dims[3] = {(cuuint64_t)head_dim, (cuuint64_t)S, (cuuint64_t)B * H};
-    const cuuint64_t gstr[2] = {(cuuint64_t)head_dim * 4, (cuuint64_t)head_dim * 4 * S};
-    const cuuint32_t box[3] = {32, (cuuint32_t)qrows, 1};
-    st = tc::encode_tiled(&prm.tm_dq, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, dq_acc, dims, gstr, box,
-                          CU_TENSOR_MAP_SWIZZLE_128B);
-  }
-  if (st != ABKV_OK) return st;
-  prm.lse = lse;
-  prm.di = di;
-  prm.dq_acc = dq_acc;
-  prm.dk = static_cast<__nv_bfloat16*>(dk);
-  prm.dv = static_cast<__nv_bfloat16*>(dv);
-  prm.dk_sb = dk_strides[0];
-  prm.dk_sh = dk_strides[1];
-  prm.dk_ss = dk_strides[2];
-  prm.dv_sb = dv_strides[0];
-  prm.dv_sh = dv_strides[1];
-  prm.dv_ss = dv_strides[2];
-  prm.err = reinterpret_cast<int32_t*>(ws);
-  prm.B = B;
-  prm.H = H;
-  prm.Hkv = Hkv;
-  prm.G = H / Hkv;
-  prm.S = S;
-  prm.n_tiles = (S + kT - 1) / kT;
-  prm.scale = scale;
-  prm.scale_log2 = scale * 1.4426950408889634f;
-  prm.window = window < S ? window : S;
-  prm.n_sink = num_sinks < S ? num_sinks : S;
-  if (cudaMemsetAsync(dq_acc, 0, rows * head_dim * 4, s) != cudaSuccess) return ABKV_ERR_CUDA;
-  rowdot_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(
-      static_cast<const __nv_bfloat16*>(out), out_strides[0], out_strides[1], out_strides[2],
-      static_cast<const __nv_bfloat16*>(dout), dout_strides[0], dout_strides[1], dout_strides[2], di, B, H, S, head_dim);
-  auto kernel = head_dim == 64 ? prefill_bwd_kernel<64, true> : prefill_bwd_unit_kernel<true>;
-  const int smem = head_dim == 64 ? Layout<64>::kSmem : LayoutU::kSmem;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return ABKV_ERR_CUDA;
-  kernel<<<dim3(prm.n_tiles, Hkv, B), kThreads, smem, s>>>(prm);
-  const int64_t n = (int64_t)rows * (head_dim / 8);
-  dq_store_kernel<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(dq_acc, static_cast<__nv_bfloat16*>(dq), dq_strides[0],
-                                                              dq_strides[1], dq_strides[2], B, H, S, head_dim,
-                                                              head_dim == 128 ? scale : 1.f);
   if (cudaGetLastError() != cudaSuccess) return ABKV_ERR_CUDA;
   return ABKV_OK;
 }

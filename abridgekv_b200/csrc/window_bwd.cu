@@ -1,0 +1,721 @@
+// Backward of the training attention under a sliding window with sinks (abkv_window_attention_backward) on
+// 5th-generation tensor cores (tcgen05 + TMEM) for sm_100a.
+//
+// Row i sees keys j <= i with j > i - window or j < n_sink.  With P = exp(scale q k^T - lse) on the visible
+// pairs (lse from the forward), dP = dO V^T and Di = rowsum(dO * O):
+//   dS = P (dP - Di)      dV = sum P^T dO      dK = scale sum dS^T Q      dQ = scale dS K
+//
+// Two kernels instead of one.  A key-stationary kernel (dK, dV: four products a tile) and a query-stationary one
+// (dQ: three) recompute S and dP once each -- seven products a tile instead of five -- but every sum
+// stays in TMEM: no fp32 accumulator of dQ in memory (its zeroing, a 64 KiB reduction per tile pair, its
+// conversion) and no order-dependent additions, so all gradients repeat bit for bit.  Measured at 2 x 32 heads x
+// 4096 rows x 128 dims, window 1024: see the table at the entry point.
+//
+// Both work on 128 x 128 tiles (S and dP products with N = 128: with N = 64 the operands' shared-memory reads,
+// not the tensor core, set the pace).  18 warps: 0 the TMA producer, 1 the issuer of tcgen05.mma and owner of the
+// TMEM, 2..17 threads of TMEM lanes -- warp group cg = (warp - 2) / 4 takes columns [32 cg, 32 cg + 32) of
+// every tile, the warp's lane quarter 32 of its rows.  The four warps of a quarter meet at a named barrier between
+// reading a score tile and writing bf16 operands over it.  The element-wise half of a tile (16,384
+// exponentials, 1024 clocks) runs beside the products of its neighbours:
+//   dK/dV:  S(0) dP(0) | dV(u) S(u+1) | dK(u) dP(u+1) | ...    threads: P(u) then dS(u)
+//   dQ:     S(0) dP(0) S(1) | dQ(u) dP(u+1) S(u+2) | ...       threads: P(u) in registers, dS(u)
+// Every mbarrier wait is bounded and records ABKV_DEVERR_TIMEOUT on expiry.
+#include <algorithm>
+#include <cstring>
+
+#include "tcgen05.cuh"
+
+namespace abkv {
+namespace {
+using namespace tc;
+
+constexpr int kT = 128;          // tile rows (keys and queries)
+constexpr int kThreads = 576;    // 18 warps
+constexpr int kWorkers = 512;    // threads of TMEM lanes
+constexpr int kLong = 3, kShort = 2;  // ring depth of the operand used twice, and of the one released early
+constexpr uint32_t kIdescS = idesc_bf16_m128(kT, false);
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D>
+struct Lay {
+  static constexpr int kAtoms = D / 64;
+  static constexpr int kTile = kT * D * 2;         // [128][D] bf16: D / 64 atom columns of [128 rows][128 B]
+  static constexpr int kAtom = kTile / kAtoms;
+  static constexpr int kOffA = 0;                  // stationary operands (K, V or Q, dO)
+  static constexpr int kOffB = kTile;
+  static constexpr int kOffLong = 2 * kTile;       // Q (dK/dV kernel) or K (dQ kernel)
+  static constexpr int kOffShort = kOffLong + kLong * kTile;  // dO or V
+  static constexpr int kOffStat = kOffShort + kShort * kTile;  // [2 tiles][4 column groups][lse2, di][32]
+  static constexpr int kOffBar = kOffStat + 2 * 4 * 2 * 32 * 4;
+  static constexpr int kSmem = kOffBar + 256;      // the base is 1024-byte aligned (checked by the kernels)
+  static constexpr int kRedStride = D + 4;         // fp32 rows of the cluster reduction (in the rings)
+  static constexpr uint32_t kIdescAcc = idesc_bf16_m128(D, true);
+};
+static_assert(Lay<128>::kSmem <= 227 * 1024, "shared memory");
+static_assert(2 * kT * Lay<128>::kRedStride * 4 <= (kLong + kShort) * Lay<128>::kTile, "cluster reduction");
+static_assert(2 * kT * Lay<64>::kRedStride * 4 <= (kLong + kShort) * Lay<64>::kTile, "cluster reduction");
+
+// barriers: stationary operands, long ring full / empty, short ring full / empty, S full (two in the dQ kernel),
+// dP full, P ready, dS ready, accumulators complete, then the TMEM address
+constexpr int kBarA = 0, kBarLF = 1, kBarLE = kBarLF + kLong, kBarSF = kBarLE + kLong, kBarSE = kBarSF + kShort,
+              kBarS = kBarSE + kShort, kBarDP = kBarS + 2, kBarP = kBarDP + 1, kBarDS = kBarP + 1,
+              kBarAcc = kBarDS + 1, kBarTmem = kBarAcc + 1;
+static_assert((kBarTmem + 1) * 8 <= 256, "barrier area");
+
+struct alignas(64) WinBwdParams {
+  CUtensorMap tm_q, tm_k, tm_v, tm_do;
+  const float* lse;  // [B][H][S], natural log
+  const float* di;   // [B][H][S]
+  __nv_bfloat16 *dq, *dk, *dv;
+  int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
+  int32_t* err;
+  int B, H, Hkv, G, S, n_tiles, window, n_sink, cluster;
+  float scale, scale_log2;
+};
+
+__device__ __forceinline__ uint32_t below(int n) {  // bits [0, n)
+  return n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : ((1u << n) - 1u));
+}
+
+template <int D>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, int row, int head, int b, uint64_t* bar) {
+#pragma unroll
+  for (int a = 0; a < Lay<D>::kAtoms; ++a) tma_load_4d(dst + a * Lay<D>::kAtom, map, 64 * a, row, head, b, bar);
+}
+
+// D(128 x 128) = A B^T over head_dim, both K-major tiles in shared memory.
+template <int D>
+__device__ __forceinline__ void issue_scores(uint32_t tmem, uint32_t a, uint32_t b) {
+  const uint64_t da = desc_kmajor_sw128(a), db = desc_kmajor_sw128(b);
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) {
+    const uint32_t off = (kk >> 2) * Lay<D>::kAtom + (kk & 3) * 32;
+    umma(tmem, desc_advance(da, off), desc_advance(db, off), kIdescS, kk > 0 ? 1u : 0u);
+  }
+}
+// D(128 x head_dim) += A B: A bf16 in TMEM (128 x 128), B a [128][D] tile read MN-major.
+template <int D>
+__device__ __forceinline__ void issue_accumulate(uint32_t tmem, uint32_t a, uint32_t b, bool first) {
+  const uint64_t db = desc_mnmajor_sw128(b, Lay<D>::kAtom);
+#pragma unroll
+  for (int kk = 0; kk < kT / 16; ++kk)
+    umma_tmem_a(tmem, a + kk * 8, desc_advance(db, kk * 2048), Lay<D>::kIdescAcc, (!first || kk > 0) ? 1u : 0u);
+}
+
+__device__ __forceinline__ void alloc_tmem(uint32_t* s_tmem) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)), "r"(512u));
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
+}
+
+// x = a * b + c on a pair with one b and a pair of c; (a - b) * c on pairs.
+__device__ __forceinline__ void fma_pair(float& d0, float& d1, float a0, float a1, float b, float c0, float c1) {
+  asm("{\n .reg .b64 x, y, z, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mov.b64 z, {%5, %6};\n"
+      " fma.rn.f32x2 r, x, y, z;\n mov.b64 {%0, %1}, r;\n}\n"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void sub_mul_pair(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0,
+                                             float c1) {
+  asm("{\n .reg .b64 x, y, z, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " sub.rn.f32x2 r, x, y;\n mul.rn.f32x2 r, r, z;\n mov.b64 {%0, %1}, r;\n}\n"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
+}
+__device__ __forceinline__ float4 peer_ld4(uint32_t local, int rank) {
+  uint32_t a;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(a) : "r"(local), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];\n" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+  return v;
+}
+
+// ---------------------------------------------------------------------------
+// dK and dV of one 128-key tile of one KV head: walks the (query tile, head) pairs that see it.  A cluster of
+// p.cluster CTAs shares the pairs and adds its parts, in rank order, through its shared memory.
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_constant__ WinBwdParams p) {
+  using LY = Lay<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {  // the 128B swizzle needs it; the same answer in every thread of the launch
+    if (threadIdx.x == 0) set_error(p.err, ABKV_DEVERR_RANGE);
+    return;
+  }
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + LY::kOffBar);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar + kBarTmem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % p.cluster, hk = blockIdx.x / p.cluster, b = blockIdx.y, kt = blockIdx.z;
+  // query tiles kt .. last see the key tile (its last key k: queries < k + window); the sinks' tiles: all
+  int last = p.n_tiles - 1;
+  if (kt * kT >= p.n_sink) last = min(last, (min(kt * kT + kT, p.S) - 1 + p.window - 1) / kT);
+  const int pairs = (last - kt + 1) * p.G;
+  const int n = pairs > rank ? (pairs - rank - 1) / p.cluster + 1 : 0;  // this CTA's
+  auto pair_at = [&](int u, int& qt, int& h) {
+    const int i = rank + u * p.cluster;
+    qt = kt + i / p.G;
+    h = hk * p.G + i % p.G;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBarTmem; ++i) mbar_init(&bar[i], (i == kBarP || i == kBarDS) ? kWorkers : 1);
+  }
+  if (warp == 1) alloc_tmem(s_tmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;  // S^T [0,128), dP^T [128,256), dV [256,..), dK [384,..)
+  bool dead = false;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      mbar_expect_tx(&bar[kBarA], 2 * LY::kTile);
+      load_tile<D>(smem + LY::kOffA, &p.tm_k, kt * kT, hk, b, &bar[kBarA]);
+      load_tile<D>(smem + LY::kOffB, &p.tm_v, kt * kT, hk, b, &bar[kBarA]);
+      for (int u = 0; u < n; ++u) {
+        int qt, h;
+        pair_at(u, qt, h);
+        const int l = u % kLong, s = u % kShort;
+        if (!wait_or_abort(&bar[kBarLE + l], (uint32_t)(((u / kLong) & 1) ^ 1), dead, p.err)) break;
+        mbar_expect_tx(&bar[kBarLF + l], LY::kTile);
+        load_tile<D>(smem + LY::kOffLong + l * LY::kTile, &p.tm_q, qt * kT, h, b, &bar[kBarLF + l]);
+        if (!wait_or_abort(&bar[kBarSE + s], (uint32_t)(((u / kShort) & 1) ^ 1), dead, p.err)) break;
+        mbar_expect_tx(&bar[kBarSF + s], LY::kTile);
+        load_tile<D>(smem + LY::kOffShort + s * LY::kTile, &p.tm_do, qt * kT, h, b, &bar[kBarSF + s]);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      const uint32_t k = smem_u32(smem + LY::kOffA), v = smem_u32(smem + LY::kOffB);
+      auto q_at = [&](int u) { return smem_u32(smem + LY::kOffLong + (u % kLong) * LY::kTile); };
+      auto do_at = [&](int u) { return smem_u32(smem + LY::kOffShort + (u % kShort) * LY::kTile); };
+      auto scores = [&](int u) -> bool {  // S^T(u)
+        if (!wait_or_abort(&bar[kBarLF + u % kLong], (uint32_t)((u / kLong) & 1), dead, p.err)) return false;
+        tc_fence_after();
+        issue_scores<D>(tmem, k, q_at(u));
+        umma_commit(&bar[kBarS]);
+        return true;
+      };
+      auto dscores = [&](int u) -> bool {  // dP^T(u)
+        if (!wait_or_abort(&bar[kBarSF + u % kShort], (uint32_t)((u / kShort) & 1), dead, p.err)) return false;
+        tc_fence_after();
+        issue_scores<D>(tmem + 128, v, do_at(u));
+        umma_commit(&bar[kBarDP]);
+        return true;
+      };
+      if (wait_or_abort(&bar[kBarA], 0, dead, p.err) && scores(0) && dscores(0)) {
+        for (int u = 0; u < n; ++u) {
+          const uint32_t par = (uint32_t)(u & 1);
+          // P^T(u) is ready: dV, then the next scores over it (one thread's MMAs run in issue order)
+          if (!wait_or_abort(&bar[kBarP], par, dead, p.err)) break;
+          tc_fence_after();
+          issue_accumulate<D>(tmem + 256, tmem, do_at(u), u == 0);
+          umma_commit(&bar[kBarSE + u % kShort]);  // dO(u): its last use
+          if (u + 1 < n && !scores(u + 1)) break;
+          if (!wait_or_abort(&bar[kBarDS], par, dead, p.err)) break;
+          tc_fence_after();
+          issue_accumulate<D>(tmem + 384, tmem + 128, q_at(u), u == 0);
+          umma_commit(&bar[kBarLE + u % kLong]);
+          if (u + 1 < n && !dscores(u + 1)) break;
+        }
+      }
+      umma_commit(&bar[kBarAcc]);
+    }
+  } else {
+    const int sw = warp - 2, cg = sw >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane, key = kt * kT + row;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const int qbar = 1 + quarter;  // the four warps of this lane quarter
+    // the four warps of a column group share its queries' statistics: quarter 0 writes them, two tiles deep
+    float* stat = reinterpret_cast<float*>(smem + LY::kOffStat) + cg * 64;
+    const float sl2 = p.scale_log2;
+    const bool sink = key < p.n_sink;
+    // lane c holds the statistics of the next pair's query 32 cg + c
+    float n_lse = 0.f, n_di = 0.f;
+    auto fetch = [&](int u) {
+      int qt, h;
+      pair_at(u, qt, h);
+      const int q = qt * kT + 32 * cg + lane;
+      const int64_t r = ((int64_t)b * p.H + h) * p.S + q;
+      n_lse = q < p.S ? __ldg(p.lse + r) * kLog2e : 0.f;
+      n_di = q < p.S ? __ldg(p.di + r) : 0.f;
+    };
+    const bool stager = quarter == 0;
+    if (stager && n > 0) fetch(0);
+    for (int u = 0; u < n; ++u) {
+      const uint32_t par = (uint32_t)(u & 1);
+      int qt, h;
+      pair_at(u, qt, h);
+      float *s_lse = stat + (u & 1) * 256, *s_di = s_lse + 32;
+      if (stager) {
+        s_lse[lane] = n_lse;
+        s_di[lane] = n_di;
+        if (u + 1 < n) fetch(u + 1);
+      }
+      named_bar_sync(5 + cg, 128);
+      // visible queries of this key among the warp's 32: q >= key, q < key + window (or a sink), q < S
+      const int q0 = qt * kT + 32 * cg;
+      const int e = sink ? p.S : min(p.S, key + p.window);
+      const uint32_t mask = below(e - q0) & ~below(key - q0);
+      const bool full = __all_sync(0xffffffffu, mask == 0xFFFFFFFFu);
+      bool ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarS], par, dead, p.err));
+      if (!ok) dead = true;
+      tc_fence_after();
+      float pv[32];
+      uint32_t w[16];
+      if (ok) {
+        tmem_ld32(tmem + lane_base + 32 * cg, pv);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 l = *reinterpret_cast<const float4*>(s_lse + c);
+          fma_pair(pv[c], pv[c + 1], pv[c], pv[c + 1], sl2, -l.x, -l.y);
+          fma_pair(pv[c + 2], pv[c + 3], pv[c + 2], pv[c + 3], sl2, -l.z, -l.w);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) pv[c + j] = fast_exp2(pv[c + j]);
+        }
+        if (!full) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) pv[c] = (mask >> c) & 1u ? pv[c] : 0.f;
+        }
+#pragma unroll
+        for (int c = 0; c < 16; ++c) w[c] = pack_bf16x2(pv[2 * c], pv[2 * c + 1]);
+      }
+      tc_fence_before();
+      named_bar_sync(qbar, 128);  // every warp of the quarter has read its columns
+      tc_fence_after();
+      if (ok) {
+        tmem_st16(tmem + lane_base + 16 * cg, w);
+        tmem_wait_st();
+      }
+      tc_fence_before();
+      mbar_arrive_one(&bar[kBarP]);
+      ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarDP], par, dead, p.err));
+      if (!ok) dead = true;
+      tc_fence_after();
+      if (ok) {
+        float dp[32];
+        tmem_ld32(tmem + lane_base + 128 + 32 * cg, dp);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 d = *reinterpret_cast<const float4*>(s_di + c);
+          sub_mul_pair(dp[c], dp[c + 1], dp[c], dp[c + 1], d.x, d.y, pv[c], pv[c + 1]);
+          sub_mul_pair(dp[c + 2], dp[c + 3], dp[c + 2], dp[c + 3], d.z, d.w, pv[c + 2], pv[c + 3]);
+          w[c / 2] = pack_bf16x2(dp[c], dp[c + 1]);
+          w[c / 2 + 1] = pack_bf16x2(dp[c + 2], dp[c + 3]);
+        }
+      }
+      tc_fence_before();
+      named_bar_sync(qbar, 128);
+      tc_fence_after();
+      if (ok) {
+        tmem_st16(tmem + lane_base + 128 + 16 * cg, w);
+        tmem_wait_st();
+      }
+      tc_fence_before();
+      mbar_arrive_one(&bar[kBarDS]);
+    }
+    if (n > 0) {
+      if (!__all_sync(0xffffffffu, wait_or_abort(&bar[kBarAcc], 0, dead, p.err))) dead = true;
+      tc_fence_after();
+    }
+    // dV (cg 0, 1) and dK (cg 2, 3): this warp's D / 2 columns of its rows
+    const bool is_dk = cg >= 2;
+    const int c0 = (cg & 1) * (D / 2);
+    const uint32_t col = (is_dk ? 384u : 256u) + c0;
+    const float gs = is_dk ? p.scale : 1.f;
+    float* red = reinterpret_cast<float*>(smem + LY::kOffLong) + ((is_dk ? kT : 0) + row) * LY::kRedStride;
+    __nv_bfloat16* out = is_dk ? p.dk + (int64_t)b * p.dk_sb + (int64_t)hk * p.dk_sh + (int64_t)key * p.dk_ss
+                               : p.dv + (int64_t)b * p.dv_sb + (int64_t)hk * p.dv_sh + (int64_t)key * p.dv_ss;
+#pragma unroll 1
+    for (int c = 0; c < D / 2; c += 32) {
+      float t[32];
+      if (n > 0) {
+        tmem_ld32(tmem + lane_base + col + c, t);
+        tmem_wait_ld();
+      }
+      if (n == 0) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) t[j] = 0.f;
+      }
+      if (p.cluster > 1) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+          *reinterpret_cast<float4*>(red + c0 + c + j) = make_float4(t[j], t[j + 1], t[j + 2], t[j + 3]);
+      } else if (key < p.S && !dead) {
+#pragma unroll
+        for (int v8 = 0; v8 < 4; ++v8) {
+          uint4 pk;
+          pk.x = pack_bf16x2(t[v8 * 8 + 0] * gs, t[v8 * 8 + 1] * gs);
+          pk.y = pack_bf16x2(t[v8 * 8 + 2] * gs, t[v8 * 8 + 3] * gs);
+          pk.z = pack_bf16x2(t[v8 * 8 + 4] * gs, t[v8 * 8 + 5] * gs);
+          pk.w = pack_bf16x2(t[v8 * 8 + 6] * gs, t[v8 * 8 + 7] * gs);
+          *reinterpret_cast<uint4*>(out + c0 + c + v8 * 8) = pk;
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u));
+  if (p.cluster > 1) {
+    cluster_barrier();
+    // this CTA's share of the rows of [dV; dK], eight dims a thread, the parts in rank order
+    const int rows = 2 * kT / p.cluster;
+    const uint32_t base = smem_u32(smem + LY::kOffLong);
+    for (int i = threadIdx.x; i < rows * (D / 8); i += kThreads) {
+      const int rr = rank * rows + i / (D / 8), d0 = (i % (D / 8)) * 8;
+      const bool is_dk = rr >= kT;
+      const int key = kt * kT + (is_dk ? rr - kT : rr);
+      if (key >= p.S) continue;
+      float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      for (int c = 0; c < p.cluster; ++c) {
+        const uint32_t at = base + (rr * LY::kRedStride + d0) * 4;
+        const float4 x = peer_ld4(at, c), y = peer_ld4(at + 16, c);
+        a[0] += x.x; a[1] += x.y; a[2] += x.z; a[3] += x.w;
+        a[4] += y.x; a[5] += y.y; a[6] += y.z; a[7] += y.w;
+      }
+      const float gs = is_dk ? p.scale : 1.f;
+      uint4 pk;
+      pk.x = pack_bf16x2(a[0] * gs, a[1] * gs);
+      pk.y = pack_bf16x2(a[2] * gs, a[3] * gs);
+      pk.z = pack_bf16x2(a[4] * gs, a[5] * gs);
+      pk.w = pack_bf16x2(a[6] * gs, a[7] * gs);
+      __nv_bfloat16* out = is_dk ? p.dk + (int64_t)b * p.dk_sb + (int64_t)hk * p.dk_sh + (int64_t)key * p.dk_ss
+                                 : p.dv + (int64_t)b * p.dv_sb + (int64_t)hk * p.dv_sh + (int64_t)key * p.dv_ss;
+      *reinterpret_cast<uint4*>(out + d0) = pk;
+    }
+    cluster_barrier();  // no CTA leaves while another reads its part
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dQ of one 128-query tile of one head: walks the key tiles it sees (the sinks', then the window's).
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_constant__ WinBwdParams p) {
+  using LY = Lay<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023u) {  // the 128B swizzle needs it; the same answer in every thread of the launch
+    if (threadIdx.x == 0) set_error(p.err, ABKV_DEVERR_RANGE);
+    return;
+  }
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + LY::kOffBar);
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar + kBarTmem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.x, b = blockIdx.y, qt = p.n_tiles - 1 - (int)blockIdx.z;  // the longest first
+  const int hk = h / p.G;
+  // keys [n_sink, w_lo) are hidden from the whole tile; visited tile i is key tile i < ns ? i : i + shift
+  const int w_lo = max(0, qt * kT - p.window + 1);
+  const int ns = (min(p.n_sink, w_lo) + kT - 1) / kT, shift = max(w_lo / kT - ns, 0);
+  const int n = qt + 1 - shift;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBarTmem; ++i) mbar_init(&bar[i], i == kBarDS ? kWorkers : 1);
+  }
+  if (warp == 1) alloc_tmem(s_tmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;  // S [0,128) [128,256), dP [256,384), dQ [384,..)
+  bool dead = false;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_expect_tx(&bar[kBarA], 2 * LY::kTile);
+      load_tile<D>(smem + LY::kOffA, &p.tm_q, qt * kT, h, b, &bar[kBarA]);
+      load_tile<D>(smem + LY::kOffB, &p.tm_do, qt * kT, h, b, &bar[kBarA]);
+      for (int u = 0; u < n; ++u) {
+        const int row = (u < ns ? u : u + shift) * kT;
+        const int l = u % kLong, s = u % kShort;
+        if (!wait_or_abort(&bar[kBarLE + l], (uint32_t)(((u / kLong) & 1) ^ 1), dead, p.err)) break;
+        mbar_expect_tx(&bar[kBarLF + l], LY::kTile);
+        load_tile<D>(smem + LY::kOffLong + l * LY::kTile, &p.tm_k, row, hk, b, &bar[kBarLF + l]);
+        if (!wait_or_abort(&bar[kBarSE + s], (uint32_t)(((u / kShort) & 1) ^ 1), dead, p.err)) break;
+        mbar_expect_tx(&bar[kBarSF + s], LY::kTile);
+        load_tile<D>(smem + LY::kOffShort + s * LY::kTile, &p.tm_v, row, hk, b, &bar[kBarSF + s]);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t q = smem_u32(smem + LY::kOffA), dout = smem_u32(smem + LY::kOffB);
+      auto k_at = [&](int u) { return smem_u32(smem + LY::kOffLong + (u % kLong) * LY::kTile); };
+      auto scores = [&](int u) -> bool {  // S(u) into buffer u % 2: dS(u - 2) has been formed from it
+        if (!wait_or_abort(&bar[kBarLF + u % kLong], (uint32_t)((u / kLong) & 1), dead, p.err)) return false;
+        tc_fence_after();
+        issue_scores<D>(tmem + 128 * (u & 1), q, k_at(u));
+        umma_commit(&bar[kBarS + (u & 1)]);
+        return true;
+      };
+      auto dscores = [&](int u) -> bool {  // dP(u), over dS(u - 1) which dQ has read
+        if (!wait_or_abort(&bar[kBarSF + u % kShort], (uint32_t)((u / kShort) & 1), dead, p.err)) return false;
+        tc_fence_after();
+        issue_scores<D>(tmem + 256, dout, smem_u32(smem + LY::kOffShort + (u % kShort) * LY::kTile));
+        umma_commit(&bar[kBarDP]);
+        umma_commit(&bar[kBarSE + u % kShort]);  // V(u): its only use
+        return true;
+      };
+      if (wait_or_abort(&bar[kBarA], 0, dead, p.err) && scores(0) && dscores(0) && (n == 1 || scores(1))) {
+        for (int u = 0; u < n; ++u) {
+          if (!wait_or_abort(&bar[kBarDS], (uint32_t)(u & 1), dead, p.err)) break;
+          tc_fence_after();
+          issue_accumulate<D>(tmem + 384, tmem + 256, k_at(u), u == 0);
+          umma_commit(&bar[kBarLE + u % kLong]);
+          if (u + 1 < n && !dscores(u + 1)) break;
+          if (u + 2 < n && !scores(u + 2)) break;
+        }
+      }
+      umma_commit(&bar[kBarAcc]);
+    }
+  } else {
+    const int sw = warp - 2, cg = sw >> 2, quarter = warp & 3;
+    const int row = quarter * 32 + lane, q = qt * kT + row;
+    const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+    const int qbar = 1 + quarter;
+    const float sl2 = p.scale_log2;
+    const int64_t r = ((int64_t)b * p.H + h) * p.S + q;
+    const bool in = q < p.S;
+    const float nl = in ? -__ldg(p.lse + r) * kLog2e : 0.f, di = in ? __ldg(p.di + r) : 0.f;
+    for (int u = 0; u < n; ++u) {
+      const int k0 = (u < ns ? u : u + shift) * kT + 32 * cg;
+      // visible keys of this row among the warp's 32: k <= q without [n_sink, q - window + 1)
+      const uint32_t mask = in ? below(q + 1 - k0) & (below(p.n_sink - k0) | ~below(q - p.window + 1 - k0)) : 0u;
+      const bool full = __all_sync(0xffffffffu, mask == 0xFFFFFFFFu);
+      bool ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarS + (u & 1)], (uint32_t)((u >> 1) & 1), dead, p.err));
+      if (!ok) dead = true;
+      tc_fence_after();
+      float pv[32];
+      if (ok) {
+        tmem_ld32(tmem + lane_base + 128 * (u & 1) + 32 * cg, pv);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          ffma2(pv[c], pv[c + 1], pv[c], pv[c + 1], sl2, nl);
+          pv[c] = fast_exp2(pv[c]);
+          pv[c + 1] = fast_exp2(pv[c + 1]);
+        }
+        if (!full) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) pv[c] = (mask >> c) & 1u ? pv[c] : 0.f;
+        }
+      }
+      ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarDP], (uint32_t)(u & 1), dead, p.err));
+      if (!ok) dead = true;
+      tc_fence_after();
+      uint32_t w[16];
+      if (ok) {
+        float dp[32];
+        tmem_ld32(tmem + lane_base + 256 + 32 * cg, dp);
+        tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          sub_mul_pair(dp[c], dp[c + 1], dp[c], dp[c + 1], di, di, pv[c], pv[c + 1]);
+          w[c / 2] = pack_bf16x2(dp[c], dp[c + 1]);
+        }
+      }
+      tc_fence_before();
+      named_bar_sync(qbar, 128);
+      tc_fence_after();
+      if (ok) {
+        tmem_st16(tmem + lane_base + 256 + 16 * cg, w);
+        tmem_wait_st();
+      }
+      tc_fence_before();
+      mbar_arrive_one(&bar[kBarDS]);
+    }
+    if (!__all_sync(0xffffffffu, wait_or_abort(&bar[kBarAcc], 0, dead, p.err))) dead = true;
+    tc_fence_after();
+    // this warp's D / 4 columns of its rows
+    __nv_bfloat16* out = p.dq + (int64_t)b * p.dq_sb + (int64_t)h * p.dq_sh + (int64_t)q * p.dq_ss + cg * (D / 4);
+    float t[32];
+    tmem_ld32(tmem + lane_base + 384 + cg * (D / 4), t);  // D 64: the upper 16 columns are the next group's
+    tmem_wait_ld();
+    if (in && !dead) {
+#pragma unroll
+      for (int v8 = 0; v8 < D / 32; ++v8) {
+        uint4 pk;
+        pk.x = pack_bf16x2(t[v8 * 8 + 0] * p.scale, t[v8 * 8 + 1] * p.scale);
+        pk.y = pack_bf16x2(t[v8 * 8 + 2] * p.scale, t[v8 * 8 + 3] * p.scale);
+        pk.z = pack_bf16x2(t[v8 * 8 + 4] * p.scale, t[v8 * 8 + 5] * p.scale);
+        pk.w = pack_bf16x2(t[v8 * 8 + 6] * p.scale, t[v8 * 8 + 7] * p.scale);
+        *reinterpret_cast<uint4*>(out + v8 * 8) = pk;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u));
+}
+
+// Di = rowsum(dO * O) in fp32: D / 8 lanes per row, eight dims a lane.  O is the forward's bf16 output with,
+// optionally, the next eight bits of its mantissa (out_lo): Di enters every dS of its row alike, and with
+// O rounded to bf16 it would be the largest error of dQ and dK after dS's own rounding.
+template <int D>
+__global__ void __launch_bounds__(256) window_rowdot_kernel(const __nv_bfloat16* __restrict__ o, int64_t o_sb,
+                                                            int64_t o_sh, int64_t o_ss, const int8_t* __restrict__ lo,
+                                                            const __nv_bfloat16* __restrict__ dout, int64_t d_sb,
+                                                            int64_t d_sh, int64_t d_ss, float* di, int B, int H, int S) {
+  constexpr int kL = D / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t r = i / kL;
+  const int d0 = (int)(i % kL) * 8;
+  const bool live = r < (int64_t)B * H * S;
+  float acc = 0.f;
+  if (live) {
+    // rows in memory order of [B][S][H]: neighbouring rows of a warp are neighbours there
+    const int h = (int)(r % H);
+    const int64_t bs = r / H;
+    const int q = (int)(bs % S), b = (int)(bs / S);
+    const uint4 x = ld_stream_v4(o + b * o_sb + h * o_sh + q * o_ss + d0);
+    const uint4 y = ld_stream_v4(dout + b * d_sb + h * d_sh + q * d_ss + d0);
+    const int64_t rr = ((int64_t)b * H + h) * S + q;
+    uint2 l = make_uint2(0, 0);
+    if (lo) l = __ldcs(reinterpret_cast<const uint2*>(lo + rr * D + d0));
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t xb = k & 1 ? xs[k / 2] & 0xFFFF0000u : xs[k / 2] << 16;
+      const uint32_t yb = k & 1 ? ys[k / 2] & 0xFFFF0000u : ys[k / 2] << 16;
+      const int32_t low = (int32_t)(int8_t)((k < 4 ? l.x : l.y) >> (8 * (k & 3)));
+      acc = fmaf(__int_as_float((int32_t)xb + (low << 8)), __uint_as_float(yb), acc);
+    }
+    (void)rr;
+  }
+#pragma unroll
+  for (int s = kL / 2; s; s >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, s);
+  if (live && d0 == 0) {
+    const int h = (int)(r % H);
+    const int64_t bs = r / H;
+    di[((bs / S) * H + h) * S + bs % S] = acc;
+  }
+}
+
+int make_map(CUtensorMap* m, const void* base, int B, int heads, int S, int D, const int64_t* strides) {
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)heads, (cuuint64_t)B};
+  const cuuint64_t gstr[3] = {(cuuint64_t)strides[2] * 2, (cuuint64_t)strides[1] * 2, (cuuint64_t)strides[0] * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)kT, 1, 1};
+  return tc::encode_tiled_4d(m, base, dims, gstr, box);
+}
+
+constexpr size_t kWsHeader = 256;
+constexpr int kSms = 148;
+
+template <int D>
+int launch(const WinBwdParams& prm, const void* out, const int64_t* os, const int8_t* lo, const void* dout,
+           const int64_t* ds, float* di, cudaStream_t s) {
+  const int64_t threads = (int64_t)prm.B * prm.H * prm.S * (D / 8);
+  window_rowdot_kernel<D><<<(unsigned)((threads + 255) / 256), 256, 0, s>>>(
+      static_cast<const __nv_bfloat16*>(out), os[0], os[1], os[2], lo, static_cast<const __nv_bfloat16*>(dout), ds[0],
+      ds[1], ds[2], di, prm.B, prm.H, prm.S);
+  if (cudaFuncSetAttribute(window_dkdv_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::kSmem) !=
+          cudaSuccess ||
+      cudaFuncSetAttribute(window_dq_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::kSmem) !=
+          cudaSuccess)
+    return ABKV_ERR_CUDA;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(prm.Hkv * prm.cluster, prm.B, prm.n_tiles);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Lay<D>::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim = {(unsigned)prm.cluster, 1, 1};
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, window_dkdv_kernel<D>, prm) != cudaSuccess) return ABKV_ERR_CUDA;
+  window_dq_kernel<D><<<dim3(prm.H, prm.B, prm.n_tiles), kThreads, Lay<D>::kSmem, s>>>(prm);
+  return cudaGetLastError() == cudaSuccess ? ABKV_OK : ABKV_ERR_CUDA;
+}
+
+// CTAs that share a key tile's pairs: while the launch leaves SMs idle, or the sinks' tile (which every query tile
+// sees) would outlast the rest of the launch.
+int pick_cluster(const WinBwdParams& p) {
+  const int64_t most = (int64_t)(p.n_sink > 0 ? p.n_tiles : std::min(p.n_tiles, (p.window + kT - 2) / kT + 1)) * p.G;
+  const int64_t usual = (int64_t)std::min(p.n_tiles, (p.window + kT - 2) / kT + 1) * p.G;
+  const int64_t ctas = (int64_t)p.n_tiles * p.Hkv * p.B;
+  int cs = 1;
+  while (cs < 8 && most >= 2 * cs &&
+         (ctas * 2 * cs <= kSms || 4 * most > 5 * cs * std::max<int64_t>(usual, ctas * usual / kSms)))
+    cs *= 2;
+  return cs;
+}
+
+}  // namespace
+}  // namespace abkv
+
+using namespace abkv;
+
+extern "C" size_t abkv_window_attention_backward_workspace_size(int B, int H, int S, int head_dim) {
+  if (B <= 0 || H <= 0 || S <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
+  return kWsHeader + ((size_t)B * H * S * 4 + 255) / 256 * 256;
+}
+
+extern "C" int abkv_window_attention_backward(
+    const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+    const int64_t* v_strides, const void* out, const int64_t* out_strides, const void* out_lo, const void* dout,
+    const int64_t* dout_strides, const float* lse, void* dq, const int64_t* dq_strides, void* dk,
+    const int64_t* dk_strides, void* dv, const int64_t* dv_strides, int B, int H, int Hkv, int S, int head_dim,
+    float scale, int window, int num_sinks, void* workspace, size_t workspace_bytes, void* stream) {
+  const void* ptrs[9] = {q, k, v, out, dout, dq, dk, dv, lse};
+  for (const void* x : ptrs)
+    if (!x) return ABKV_ERR_INVALID_ARG;
+  const int64_t* strs[8] = {q_strides, k_strides, v_strides, out_strides, dout_strides, dq_strides, dk_strides,
+                            dv_strides};
+  for (const int64_t* x : strs)
+    if (!x) return ABKV_ERR_INVALID_ARG;
+  if (B <= 0 || H <= 0 || Hkv <= 0 || S <= 0 || H % Hkv != 0 || !(scale > 0.f) || window <= 0 || num_sinks < 0)
+    return ABKV_ERR_INVALID_ARG;
+  if ((head_dim != 64 && head_dim != 128) || H > 128 || B > 65535 || S > (1 << 17)) return ABKV_ERR_UNSUPPORTED;
+  if ((int64_t)B * H * S > INT32_MAX) return ABKV_ERR_UNSUPPORTED;
+  for (int i = 0; i < 8; ++i)
+    if (reinterpret_cast<uintptr_t>(ptrs[i]) & 15) return ABKV_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(out_lo) & 15) return ABKV_ERR_INVALID_ARG;
+  for (int i = 3; i < 8; ++i)
+    if (strs[i][0] % 8 || strs[i][1] % 8 || strs[i][2] % 8) return ABKV_ERR_INVALID_ARG;
+  const size_t need = abkv_window_attention_backward_workspace_size(B, H, S, head_dim);
+  if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return ABKV_ERR_WORKSPACE;
+  WinBwdParams prm;
+  std::memset(&prm, 0, sizeof(prm));
+  int st = make_map(&prm.tm_q, q, B, H, S, head_dim, q_strides);
+  if (st == ABKV_OK) st = make_map(&prm.tm_do, dout, B, H, S, head_dim, dout_strides);
+  if (st == ABKV_OK) st = make_map(&prm.tm_k, k, B, Hkv, S, head_dim, k_strides);
+  if (st == ABKV_OK) st = make_map(&prm.tm_v, v, B, Hkv, S, head_dim, v_strides);
+  if (st != ABKV_OK) return st;
+  float* di = reinterpret_cast<float*>(static_cast<char*>(workspace) + kWsHeader);
+  prm.lse = lse;
+  prm.di = di;
+  prm.dq = static_cast<__nv_bfloat16*>(dq);
+  prm.dk = static_cast<__nv_bfloat16*>(dk);
+  prm.dv = static_cast<__nv_bfloat16*>(dv);
+  prm.dq_sb = dq_strides[0];
+  prm.dq_sh = dq_strides[1];
+  prm.dq_ss = dq_strides[2];
+  prm.dk_sb = dk_strides[0];
+  prm.dk_sh = dk_strides[1];
+  prm.dk_ss = dk_strides[2];
+  prm.dv_sb = dv_strides[0];
+  prm.dv_sh = dv_strides[1];
+  prm.dv_ss = dv_strides[2];
+  prm.err = static_cast<int32_t*>(workspace);
+  prm.B = B;
+  prm.H = H;
+  prm.Hkv = Hkv;
+  prm.G = H / Hkv;
+  prm.S = S;
+  prm.n_tiles = (S + kT - 1) / kT;
+  prm.scale = scale;
+  prm.scale_log2 = scale * kLog2e;
+  // a window past S hides nothing, sinks past S are every key: keep the tile arithmetic in 32 bits
+  prm.window = window < S ? window : S;
+  prm.n_sink = num_sinks < S ? num_sinks : S;
+  prm.cluster = pick_cluster(prm);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int8_t* lo = static_cast<const int8_t*>(out_lo);
+  return head_dim == 64 ? launch<64>(prm, out, out_strides, lo, dout, dout_strides, di, s)
+                        : launch<128>(prm, out, out_strides, lo, dout, dout_strides, di, s);
+}

@@ -213,35 +213,40 @@ def _tma_ready(t: torch.Tensor) -> tuple[torch.Tensor, "_lib.C.Array"]:
 
 
 def window_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int, num_sinks: int = 0,
-                   scale: float | None = None, return_lse: bool = False, workspace: Workspace | None = None,
-                   stream: torch.cuda.Stream | None = None):
+                   scale: float | None = None, return_lse: bool = False, return_low: bool = False,
+                   workspace: Workspace | None = None, stream: torch.cuda.Stream | None = None):
     """Causal attention under a sliding window with sinks (``abkv_window_attention``): row i sees keys
     j <= i with j > i - window or j < num_sinks.  q [B, H, S, D], k/v [B, Hkv, S, D] bf16 (any strides;
     what the copy engine cannot address is copied first), D 64 or 128, any S up to 131072, finite values.
-    Returns out [B, H, S, D] (stored as [B, S, H, D]), and lse [B, H, S] fp32 with ``return_lse``."""
+    Returns out [B, H, S, D] (stored as [B, S, H, D]), then lse [B, H, S] fp32 with ``return_lse``, then with
+    ``return_low`` the output's next eight mantissa bits ([B, H, S, D] int8, for ``window_backward``)."""
     window, num_sinks, scale = _window_args(q, k, v, window, num_sinks, scale)
     B, H, S, D = q.shape
     device = q.device
     with call_scope(device, stream):
         out = torch.empty((B, S, H, D), dtype=torch.bfloat16, device=device).transpose(1, 2)
         lse = torch.empty((B, H, S), dtype=torch.float32, device=device) if return_lse else None
+        low = torch.empty((B, H, S, D), dtype=torch.int8, device=device) if return_low else None
         if B * H * S:
             (q, qs), (k, ks), (v, vs), (_, os) = _tma_ready(q), _tma_ready(k), _tma_ready(v), _tma_ready(out)
             ws, raw = call_workspace(device, 256, workspace)
             st = _lib.lib().abkv_window_attention(
                 q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os,
-                lse.data_ptr() if return_lse else None, B, H, k.shape[1], S, D, scale, window, num_sinks, ws.ptr(),
+                low.data_ptr() if return_low else None, lse.data_ptr() if return_lse else None, B, H, k.shape[1], S, D, scale, window, num_sinks, ws.ptr(),
                 ws.nbytes, raw)
             if st:
                 _lib.check("abkv_window_attention", st)
-    return (out, lse) if return_lse else out
+    extra = tuple(t for t in (lse, low) if t is not None)
+    return (out, *extra) if extra else out
 
 
 def window_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, dout: torch.Tensor,
                     lse: torch.Tensor, *, window: int, num_sinks: int = 0, scale: float | None = None,
-                    workspace: Workspace | None = None, stream: torch.cuda.Stream | None = None):
+                    low: torch.Tensor | None = None, workspace: Workspace | None = None,
+                    stream: torch.cuda.Stream | None = None):
     """Gradients (dq, dk, dv) of ``window_forward`` for the upstream gradient ``dout``, from the forward's
-    output and log-sum-exp (``abkv_window_attention_backward``).  dq's parts are added in no fixed order."""
+    output, log-sum-exp and (optionally) the output's low bits (``abkv_window_attention_backward``).  Repeated
+    calls give the same bits."""
     window, num_sinks, scale = _window_args(q, k, v, window, num_sinks, scale)
     B, H, S, D = shape = q.shape
     device = q.device
@@ -252,6 +257,9 @@ def window_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
             raise ValueError("out and dout must be [B, H, S, D] like the query")
     if lse.dtype != torch.float32 or lse.shape != shape[:3] or not lse.is_contiguous() or lse.device != device:
         raise ValueError("lse must be the forward's contiguous float32 [B, H, S] log-sum-exp")
+    if low is not None and (low.dtype != torch.int8 or low.shape != shape or not low.is_contiguous() or
+                            low.device != device):
+        raise ValueError("low must be the forward's contiguous int8 [B, H, S, D] low bits")
     with call_scope(device, stream):
         (q, qs), (k, ks), (v, vs), (out, os), (dout, ds) = (_tma_ready(t) for t in (q, k, v, out, dout))
         dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
@@ -264,9 +272,10 @@ def window_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
         ws, raw = call_workspace(device, need, workspace)
         (_, dqs), (_, dks), (_, dvs) = _tma_ready(dq), _tma_ready(dk), _tma_ready(dv)
         st = lib.abkv_window_attention_backward(
-            q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os, dout.data_ptr(), ds,
-            lse.data_ptr(), dq.data_ptr(), dqs, dk.data_ptr(), dks, dv.data_ptr(), dvs, B, H, k.shape[1], S, D, scale,
-            window, num_sinks, ws.ptr(), ws.nbytes, raw)
+            q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os,
+            low.data_ptr() if low is not None else None, dout.data_ptr(), ds, lse.data_ptr(), dq.data_ptr(), dqs,
+            dk.data_ptr(), dks, dv.data_ptr(), dvs, B, H, k.shape[1], S, D, scale, window, num_sinks, ws.ptr(),
+            ws.nbytes, raw)
     if st:
         _lib.check("abkv_window_attention_backward", st)
     return dq, dk, dv
@@ -277,17 +286,18 @@ class WindowAttention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, window, num_sinks, scale):
-        out, lse = window_forward(q, k, v, window=window, num_sinks=num_sinks, scale=scale, return_lse=True)
-        ctx.save_for_backward(q, k, v, out, lse)
+        out, lse, low = window_forward(q, k, v, window=window, num_sinks=num_sinks, scale=scale, return_lse=True,
+                                       return_low=True)
+        ctx.save_for_backward(q, k, v, out, lse, low)
         ctx.args = (window, num_sinks, scale)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, lse, low = ctx.saved_tensors
         window, num_sinks, scale = ctx.args
-        dq, dk, dv = window_backward(q, k, v, out, dout, lse, window=window, num_sinks=num_sinks, scale=scale)
+        dq, dk, dv = window_backward(q, k, v, out, dout, lse, window=window, num_sinks=num_sinks, scale=scale, low=low)
         return dq, dk, dv, None, None, None
 
 

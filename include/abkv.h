@@ -534,24 +534,27 @@ int abkv_prefill_masked_backward(
  * backward; row i sees keys j <= i with j > i - window or j < num_sinks (window
  * >= 1, so every row sees itself).  Any S from 1 to 131072, head_dim 64 or 128,
  * H <= 128.  All of q, k, v and dout must be finite: a tile multiplies hidden
- * rows by zero.  The backward adds dq's parts in no fixed order (32-bit rounding
- * differs between runs); dk and dv repeat bit for bit.  Its workspace:
+ * rows by zero.  Every sum has a fixed order: results repeat bit for bit.
+ * out_lo (optional): contiguous DEVICE [B][H][S][head_dim] bytes, the eight
+ * mantissa bits of the output after its bf16 ones; given to the backward as well,
+ * rowsum(dout * out) is taken from the longer output (the largest error of dq and
+ * dk after the rounding of their own operands).  The backward's workspace:
  * abkv_window_attention_backward_workspace_size(B, H, S, head_dim) bytes. */
 int abkv_window_attention(const void* q, const int64_t* q_strides, const void* k,
                           const int64_t* k_strides, const void* v,
                           const int64_t* v_strides, void* out,
-                          const int64_t* out_strides, float* lse, int B, int H,
-                          int Hkv, int S, int head_dim, float scale, int window,
-                          int num_sinks, void* workspace, size_t workspace_bytes,
-                          void* stream);
+                          const int64_t* out_strides, void* out_lo, float* lse,
+                          int B, int H, int Hkv, int S, int head_dim, float scale,
+                          int window, int num_sinks, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 size_t abkv_window_attention_backward_workspace_size(int B, int H, int S,
                                                      int head_dim);
 int abkv_window_attention_backward(
     const void* q, const int64_t* q_strides, const void* k,
     const int64_t* k_strides, const void* v, const int64_t* v_strides,
-    const void* out, const int64_t* out_strides, const void* dout,
-    const int64_t* dout_strides, const float* lse, void* dq,
+    const void* out, const int64_t* out_strides, const void* out_lo,
+    const void* dout, const int64_t* dout_strides, const float* lse, void* dq,
     const int64_t* dq_strides, void* dk, const int64_t* dk_strides, void* dv,
     const int64_t* dv_strides, int B, int H, int Hkv, int S, int head_dim,
     float scale, int window, int num_sinks, void* workspace,
