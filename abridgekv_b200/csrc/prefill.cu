@@ -444,10 +444,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
       // O -> the head's half of the Q buffer (no S MMA reads it any more: o_full followed the head's
       // last MMAs), 128B-swizzled like the output map's boxes; then one thread stores the head's tile
       uint8_t* stage = smem + kOffQ + head_slot * kQBytes;
+      uint32_t lo[kWin ? D / 8 : 1];  // kWin: this row's low bits, stored after the output is on its way
       if (o_ok) {
         const bool none = !(l > 0.f);  // no visible key: zeros
         const float inv = none ? 0.f : 1.f / l;
-#pragma unroll 1
+#pragma unroll(kWin ? D / 64 : 1)
         for (int c4 = 0; c4 < D / 64; ++c4) {
           float t[32];
           tmem_ld32(tmem_o + lane_base + (D / 2) * half + c4 * 32, t);
@@ -457,15 +458,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
             for (int i = 0; i < 32; ++i) t[i] = 0.f;
           }
           const int d0 = (D / 2) * half + 32 * c4;  // first dim of these 32
-          if (kWin && p.out_lo && q < p.S) {
-            uint4 lo[2];
-            uint32_t* l = reinterpret_cast<uint32_t*>(lo);
+          if (kWin && p.out_lo) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              l[i] = low_bits4(t[4 * i] * inv, t[4 * i + 1] * inv, t[4 * i + 2] * inv, t[4 * i + 3] * inv);
-            uint4* dst = reinterpret_cast<uint4*>(p.out_lo + (((int64_t)b * p.H + h) * p.S + q) * D + d0);
-            dst[0] = lo[0];
-            dst[1] = lo[1];
+              lo[c4 * 8 + i] = low_bits4(t[4 * i] * inv, t[4 * i + 1] * inv, t[4 * i + 2] * inv, t[4 * i + 3] * inv);
           }
           uint8_t* atom = stage + (d0 / 64) * (kQBytes / kAtoms);
 #pragma unroll
@@ -489,6 +485,12 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
           tma_store_commit();
         }
         tma_store_wait_read();  // the shared memory stays valid until the store has read it
+      }
+      if (kWin && p.out_lo && o_ok && q < p.S) {
+        uint4* dst = reinterpret_cast<uint4*>(p.out_lo + (((int64_t)b * p.H + h) * p.S + q) * D + (D / 2) * half);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+          __stcs(dst + i, make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]));
       }
     }
   }

@@ -14,8 +14,9 @@
 // Both work on 128 x 128 tiles (S and dP products with N = 128: with N = 64 the operands' shared-memory reads,
 // not the tensor core, set the pace).  18 warps: 0 the TMA producer, 1 the issuer of tcgen05.mma and owner of the
 // TMEM, 2..17 threads of TMEM lanes -- warp group cg = (warp - 2) / 4 takes columns [32 cg, 32 cg + 32) of
-// every tile, the warp's lane quarter 32 of its rows.  The four warps of a quarter meet at a named barrier between
-// reading a score tile and writing bf16 operands over it.  The element-wise half of a tile (16,384
+// every tile, the warp's lane quarter 32 of its rows, and puts its bf16 operands (16 columns) over the scores it has
+// read itself, so no warp waits for another: the products take each 16-row step's operand where it lies.  The
+// element-wise half of a tile (16,384
 // exponentials, 1024 clocks) runs beside the products of its neighbours:
 //   dK/dV:  S(0) dP(0) | dV(u) S(u+1) | dK(u) dP(u+1) | ...    threads: P(u) then dS(u)
 //   dQ:     S(0) dP(0) S(1) | dQ(u) dP(u+1) S(u+2) | ...       threads: P(u) in registers, dS(u)
@@ -31,7 +32,7 @@ using namespace tc;
 
 constexpr int kT = 128;          // tile rows (keys and queries)
 constexpr int kThreads = 576;    // 18 warps
-constexpr int kWorkers = 512;    // threads of TMEM lanes
+constexpr int kWorkers = 16;     // warps of TMEM lanes: one arrival each (512 on one barrier cost more than they order)
 constexpr int kLong = 3, kShort = 2;  // ring depth of the operand used twice, and of the one released early
 constexpr uint32_t kIdescS = idesc_bf16_m128(kT, false);
 constexpr float kLog2e = 1.4426950408889634f;
@@ -56,10 +57,10 @@ static_assert(2 * kT * Lay<128>::kRedStride * 4 <= (kLong + kShort) * Lay<128>::
 static_assert(2 * kT * Lay<64>::kRedStride * 4 <= (kLong + kShort) * Lay<64>::kTile, "cluster reduction");
 
 // barriers: stationary operands, long ring full / empty, short ring full / empty, S full (two in the dQ kernel),
-// dP full, P ready, dS ready, accumulators complete, then the TMEM address
+// dP full, P ready, dS ready, accumulators complete, statistics of a column group, then the TMEM address
 constexpr int kBarA = 0, kBarLF = 1, kBarLE = kBarLF + kLong, kBarSF = kBarLE + kLong, kBarSE = kBarSF + kShort,
               kBarS = kBarSE + kShort, kBarDP = kBarS + 2, kBarP = kBarDP + 1, kBarDS = kBarP + 1,
-              kBarAcc = kBarDS + 1, kBarTmem = kBarAcc + 1;
+              kBarAcc = kBarDS + 1, kBarStat = kBarAcc + 1, kBarTmem = kBarStat + 4;
 static_assert((kBarTmem + 1) * 8 <= 256, "barrier area");
 
 struct alignas(64) WinBwdParams {
@@ -93,13 +94,14 @@ __device__ __forceinline__ void issue_scores(uint32_t tmem, uint32_t a, uint32_t
     umma(tmem, desc_advance(da, off), desc_advance(db, off), kIdescS, kk > 0 ? 1u : 0u);
   }
 }
-// D(128 x head_dim) += A B: A bf16 in TMEM (128 x 128), B a [128][D] tile read MN-major.
+// D(128 x head_dim) += A B: A bf16 in TMEM (128 x 128, 32 of its columns in 16 words every 32 words), B a [128][D]
+// tile read MN-major.
 template <int D>
 __device__ __forceinline__ void issue_accumulate(uint32_t tmem, uint32_t a, uint32_t b, bool first) {
   const uint64_t db = desc_mnmajor_sw128(b, Lay<D>::kAtom);
 #pragma unroll
   for (int kk = 0; kk < kT / 16; ++kk)
-    umma_tmem_a(tmem, a + kk * 8, desc_advance(db, kk * 2048), Lay<D>::kIdescAcc, (!first || kk > 0) ? 1u : 0u);
+    umma_tmem_a(tmem, a + (kk >> 1) * 32 + (kk & 1) * 8, desc_advance(db, kk * 2048), Lay<D>::kIdescAcc, (!first || kk > 0) ? 1u : 0u);
 }
 
 __device__ __forceinline__ void alloc_tmem(uint32_t* s_tmem) {
@@ -227,7 +229,6 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
     const int sw = warp - 2, cg = sw >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane, key = kt * kT + row;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const int qbar = 1 + quarter;  // the four warps of this lane quarter
     // the four warps of a column group share its queries' statistics: quarter 0 writes them, two tiles deep
     float* stat = reinterpret_cast<float*>(smem + LY::kOffStat) + cg * 64;
     const float sl2 = p.scale_log2;
@@ -243,24 +244,29 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
       n_di = q < p.S ? __ldg(p.di + r) : 0.f;
     };
     const bool stager = quarter == 0;
-    if (stager && n > 0) fetch(0);
+    auto stage = [&](int u) {  // statistics of pair u into buffer u % 2, then fetch those of pair u + 1
+      stat[(u & 1) * 256 + lane] = n_lse;
+      stat[(u & 1) * 256 + 32 + lane] = n_di;
+      __syncwarp();
+      if (lane == 0) mbar_arrive_one(&bar[kBarStat + cg]);
+      if (u + 1 < n) fetch(u + 1);
+    };
+    if (stager && n > 0) {
+      fetch(0);
+      stage(0);
+    }
     for (int u = 0; u < n; ++u) {
       const uint32_t par = (uint32_t)(u & 1);
       int qt, h;
       pair_at(u, qt, h);
-      float *s_lse = stat + (u & 1) * 256, *s_di = s_lse + 32;
-      if (stager) {
-        s_lse[lane] = n_lse;
-        s_di[lane] = n_di;
-        if (u + 1 < n) fetch(u + 1);
-      }
-      named_bar_sync(5 + cg, 128);
+      const float *s_lse = stat + (u & 1) * 256, *s_di = s_lse + 32;
       // visible queries of this key among the warp's 32: q >= key, q < key + window (or a sink), q < S
       const int q0 = qt * kT + 32 * cg;
       const int e = sink ? p.S : min(p.S, key + p.window);
       const uint32_t mask = below(e - q0) & ~below(key - q0);
       const bool full = __all_sync(0xffffffffu, mask == 0xFFFFFFFFu);
-      bool ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarS], par, dead, p.err));
+      bool ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarStat + cg], par, dead, p.err) &&
+                                            wait_or_abort(&bar[kBarS], par, dead, p.err));
       if (!ok) dead = true;
       tc_fence_after();
       float pv[32];
@@ -283,17 +289,17 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
 #pragma unroll
         for (int c = 0; c < 16; ++c) w[c] = pack_bf16x2(pv[2 * c], pv[2 * c + 1]);
       }
-      tc_fence_before();
-      named_bar_sync(qbar, 128);  // every warp of the quarter has read its columns
-      tc_fence_after();
       if (ok) {
-        tmem_st16(tmem + lane_base + 16 * cg, w);
+        tmem_st16(tmem + lane_base + 32 * cg, w);
         tmem_wait_st();
       }
       tc_fence_before();
-      mbar_arrive_one(&bar[kBarP]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_one(&bar[kBarP]);
       ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarDP], par, dead, p.err));
       if (!ok) dead = true;
+      // dP(u) followed every warp's dS(u - 1): nobody reads the other statistics buffer any more
+      if (stager && u + 1 < n) stage(u + 1);
       tc_fence_after();
       if (ok) {
         float dp[32];
@@ -308,15 +314,13 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
           w[c / 2 + 1] = pack_bf16x2(dp[c + 2], dp[c + 3]);
         }
       }
-      tc_fence_before();
-      named_bar_sync(qbar, 128);
-      tc_fence_after();
       if (ok) {
-        tmem_st16(tmem + lane_base + 128 + 16 * cg, w);
+        tmem_st16(tmem + lane_base + 128 + 32 * cg, w);
         tmem_wait_st();
       }
       tc_fence_before();
-      mbar_arrive_one(&bar[kBarDS]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_one(&bar[kBarDS]);
     }
     if (n > 0) {
       if (!__all_sync(0xffffffffu, wait_or_abort(&bar[kBarAcc], 0, dead, p.err))) dead = true;
@@ -474,7 +478,6 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
     const int sw = warp - 2, cg = sw >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane, q = qt * kT + row;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    const int qbar = 1 + quarter;
     const float sl2 = p.scale_log2;
     const int64_t r = ((int64_t)b * p.H + h) * p.S + q;
     const bool in = q < p.S;
@@ -516,15 +519,13 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
           w[c / 2] = pack_bf16x2(dp[c], dp[c + 1]);
         }
       }
-      tc_fence_before();
-      named_bar_sync(qbar, 128);
-      tc_fence_after();
       if (ok) {
-        tmem_st16(tmem + lane_base + 256 + 16 * cg, w);
+        tmem_st16(tmem + lane_base + 256 + 32 * cg, w);
         tmem_wait_st();
       }
       tc_fence_before();
-      mbar_arrive_one(&bar[kBarDS]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_one(&bar[kBarDS]);
     }
     if (!__all_sync(0xffffffffu, wait_or_abort(&bar[kBarAcc], 0, dead, p.err))) dead = true;
     tc_fence_after();
