@@ -169,16 +169,42 @@ def _window(window, num_sinks) -> tuple[int, int]:
     return w, s
 
 
-def _check_query(query, kv_cache) -> None:
+def _i32(name: str, t, device, dim: int, rows: int) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or not t.is_cuda:
+        raise TypeError(f"{name} must be an int32 CUDA tensor")
+    if t.device != device:
+        raise ValueError(f"{name} must be on the query's device")
+    if t.dim() != dim or t.shape[0] < rows:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _window_rows(query, kv_cache, block_table, seq_lens, query_start_loc, num_kv_heads, num_requests, max_query_len):
+    """Checks the paged arguments of the window entry points -> (R, page, block_table, the C call's arguments
+    from query_start_loc to head_dim, without those of the output)."""
     for name, t in (("query", query), ("kv_cache", kv_cache)):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.bfloat16:
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or not t.is_cuda:
             raise TypeError(f"{name} must be a bf16 CUDA tensor (libabkv has no CPU path)")
-
-
-def _same_device(query, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != query.device:
-            raise ValueError(f"{name} must be on the query's device")
+    if query.dim() != 3 or query.stride(2) != 1:
+        raise ValueError("query must be [T, Hq, D] with a contiguous last dimension")
+    T, Hq, D = query.shape
+    Hkv = int(num_kv_heads)
+    if Hkv <= 0 or Hq % Hkv:
+        raise ValueError("the KV heads must divide the query heads")
+    layout, nb, page = _layout_of(kv_cache, Hkv)
+    if kv_cache.shape[4] != D:
+        raise ValueError(f"the cache's head size {kv_cache.shape[4]} is not the query's {D}")
+    device = query.device
+    if kv_cache.device != device:
+        raise ValueError("kv_cache must be on the query's device")
+    R = block_table.shape[0] if num_requests is None else int(num_requests)
+    if not 0 < max_query_len <= T:
+        raise ValueError(f"max_query_len must be in [1, T={T}]")
+    bt = _i32("block_table", block_table, device, 2, R)
+    sl = _i32("seq_lens", seq_lens, device, 1, R)
+    qs = _i32("query_start_loc", query_start_loc, device, 1, R + 1)
+    tail = (qs.data_ptr(), kv_cache.data_ptr(), layout, nb, page, bt.data_ptr(), bt.shape[1], sl.data_ptr())
+    return R, Hkv, page, (bt, sl, qs), tail
 
 
 def paged_prefill_window(query: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor,
@@ -195,20 +221,23 @@ def paged_prefill_window(query: torch.Tensor, kv_cache: torch.Tensor, block_tabl
     log-sum-exp of each row's scaled scores, which ``paged_prompt_weights`` takes.  Rows of no request
     are left untouched (in lse: undefined)."""
     window, num_sinks = _window(window, num_sinks)
-    _check_query(query, kv_cache)
-    dev = query.device
-    with call_scope(dev, stream):
-        head, out, R, nb, page, T, scale = _prepare(query, kv_cache, block_table, seq_lens, query_start_loc, None,
-                                                    scale, None, num_requests, out, num_kv_heads=num_kv_heads)
-        _same_device(query, kv_cache=kv_cache, block_table=block_table, seq_lens=seq_lens, out=out,
-                     query_start_loc=query_start_loc)
-        if not 0 < max_query_len <= T:
-            raise ValueError(f"max_query_len must be in [1, T={T}]")
-        lse = torch.empty(query.shape[:2], dtype=torch.float32, device=dev) if return_lse else None
-        ws, raw = call_workspace(dev, 256, workspace)
+    if not isinstance(query, torch.Tensor) or not query.is_cuda:
+        raise TypeError("query must be a bf16 CUDA tensor (libabkv has no CPU path)")
+    device, shape = query.device, query.shape
+    with call_scope(device, stream):
+        R, Hkv, _, keep, tail = _window_rows(query, kv_cache, block_table, seq_lens, query_start_loc, num_kv_heads,
+                                             num_requests, max_query_len)
+        if out is None:
+            out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+        elif out.shape != shape or out.dtype != torch.bfloat16 or out.stride(2) != 1 or out.device != device:
+            raise ValueError("out must be a bf16 [T, Hq, D] tensor with a contiguous last dimension on the query's device")
+        lse = torch.empty(shape[:2], dtype=torch.float32, device=device) if return_lse else None
+        ws, raw = call_workspace(device, 256, workspace)
+        T, Hq, D = shape
         st = _lib.lib().abkv_paged_prefill_window(
-            *head[:6], lse.data_ptr() if lse is not None else None, *head[6:], max_query_len, T, scale, window, num_sinks,
-            ws.ptr(), ws.nbytes, raw)
+            query.data_ptr(), query.stride(0), query.stride(1), out.data_ptr(), out.stride(0), out.stride(1),
+            lse.data_ptr() if return_lse else None, *tail, R, Hq, Hkv, D, max_query_len, T,
+            1.0 / math.sqrt(D) if scale is None else scale, window, num_sinks, ws.ptr(), ws.nbytes, raw)
     if st:
         _lib.check("abkv_paged_prefill_window", st)
     return (out, lse) if return_lse else out
@@ -230,35 +259,32 @@ def paged_prompt_weights(query: torch.Tensor, lse: torch.Tensor, kv_cache: torch
     obs = 0 if observe is None else int(observe)
     if observe is not None and obs <= 0:
         raise ValueError(f"observe must be positive (or None for every row), got {observe}")
-    for name, t in (("lse", lse), ("weights", weights)):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32:
-            raise TypeError(f"{name} must be a float32 CUDA tensor")
-    head, _, R, nb, page, T, scale = _prepare(query, kv_cache, block_table, seq_lens, query_start_loc, None, scale,
-                                              None, num_requests, query, num_kv_heads=num_kv_heads)
-    _same_device(query, kv_cache=kv_cache, block_table=block_table, seq_lens=seq_lens, lse=lse, weights=weights,
-                 query_start_loc=query_start_loc)
-    Hq, Hkv, D = query.shape[1], int(num_kv_heads), query.shape[2]
-    if tuple(lse.shape) != (T, Hq) or not lse.is_contiguous():
-        raise ValueError(f"lse must be the attention's contiguous [{T}, {Hq}] log-sum-exp")
-    if weights.dim() != 3 or weights.shape[0] < R or weights.shape[1] not in (1, Hkv) or weights.shape[2] == 0 or \
-            weights.stride(2) != 1:
-        raise ValueError(f"weights must be [>=R, Hkv or 1, rows] with contiguous rows, got {tuple(weights.shape)}")
-    units, rows = int(weights.shape[1]), int(weights.shape[2])
-    if (R > 1 and weights.stride(0) < rows) or (units > 1 and weights.stride(1) < rows):
-        raise ValueError("the rows of weights must not overlap")
-    if int(max_query_len) <= 0 or int(max_query_len) > T:
-        raise ValueError(f"max_query_len must be in [1, T={T}]")
-    dev = query.device
-    lib = _lib.lib()
-    max_rows = min(int(block_table.shape[1]) * page, rows)
-    if R == 0 or max_rows == 0:
-        return weights
-    with call_scope(dev, stream):
-        ws, raw = call_workspace(dev, lib.abkv_prompt_weights_workspace_size(R, Hkv, max_rows, units), workspace)
-        st = lib.abkv_prompt_weights(
-            query.data_ptr(), query.stride(0), query.stride(1), lse.data_ptr(), *head[6:14], weights.data_ptr(),
-            weights.stride(0), weights.stride(1), rows, units, R, Hq, Hkv, D, int(max_query_len), max_rows, T, obs,
-            scale, window, num_sinks, ws.ptr(), ws.nbytes, raw)
+    for name, t in (("query", query), ("lse", lse), ("weights", weights)):
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or (t is not query and t.dtype != torch.float32):
+            raise TypeError(f"{name} must be a {'bf16' if t is query else 'float32'} CUDA tensor")
+    device = query.device
+    with call_scope(device, stream):
+        R, Hkv, page, keep, tail = _window_rows(query, kv_cache, block_table, seq_lens, query_start_loc, num_kv_heads,
+                                                num_requests, max_query_len)
+        T, Hq, D = query.shape
+        if lse.shape != (T, Hq) or not lse.is_contiguous() or lse.device != device:
+            raise ValueError(f"lse must be the attention's contiguous [{T}, {Hq}] log-sum-exp on the query's device")
+        if weights.dim() != 3 or weights.shape[0] < R or weights.shape[1] not in (1, Hkv) or weights.shape[2] == 0 or \
+                weights.stride(2) != 1 or weights.device != device:
+            raise ValueError("weights must be [>=R, Hkv or 1, rows] with contiguous rows on the query's device, "
+                             f"got {tuple(weights.shape)}")
+        units, rows = weights.shape[1], weights.shape[2]
+        if (R > 1 and weights.stride(0) < rows) or (units > 1 and weights.stride(1) < rows):
+            raise ValueError("the rows of weights must not overlap")
+        max_rows = min(keep[0].shape[1] * page, rows)
+        if R == 0 or max_rows == 0:
+            return weights
+        # the workspace holds per-head sums where one unit collects several heads
+        ws, raw = call_workspace(device, 256 + (R * Hkv * max_rows * 4 if units == 1 and Hkv > 1 else 0), workspace)
+        st = _lib.lib().abkv_prompt_weights(
+            query.data_ptr(), query.stride(0), query.stride(1), lse.data_ptr(), *tail, weights.data_ptr(),
+            weights.stride(0), weights.stride(1), rows, units, R, Hq, Hkv, D, max_query_len, max_rows, T, obs,
+            1.0 / math.sqrt(D) if scale is None else scale, window, num_sinks, ws.ptr(), ws.nbytes, raw)
     if st:
         _lib.check("abkv_prompt_weights", st)
     return weights

@@ -218,13 +218,20 @@ __device__ __forceinline__ void softmax_half(const PrefillParams& p, int lim, in
 
 // The eight mantissa bits below the bf16 rounding of four floats: the difference of the bit patterns, in units
 // of 2^8 (bit patterns of one sign are ordered like the values, so adding it back needs no exponent).
-__device__ __forceinline__ uint32_t low_bits4(float a, float b, float c, float d) {
-  auto one = [](float x) -> uint32_t {
-    const int32_t hi = (int32_t)((uint32_t)__bfloat16_as_ushort(__float2bfloat16(x)) << 16);
-    const int32_t diff = (__float_as_int(x) - hi + 128) >> 8;  // in [-128, 128]
-    return (uint32_t)min(diff, 127) & 0xFFu;
+// ab, cd: the packed roundings.
+__device__ __forceinline__ uint32_t low_bits4(float a, float b, float c, float d, uint32_t ab, uint32_t cd) {
+  // byte 1 of (difference + 128), the difference kept below 2^15 - 128
+  auto one = [](float x, uint32_t hi) -> uint32_t {
+    return (uint32_t)(min(__float_as_int(x) - (int32_t)hi, 32639) + 128);
   };
-  return one(a) | one(b) << 8 | one(c) << 16 | one(d) << 24;
+  const uint32_t lo = prmt(one(a, ab << 16), one(b, ab & 0xFFFF0000u), 0x0051u);
+  const uint32_t hi = prmt(one(c, cd << 16), one(d, cd & 0xFFFF0000u), 0x0051u);
+  return prmt(lo, hi, 0x5410u);
+}
+__device__ __forceinline__ void store_32b(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
 __device__ __forceinline__ bool visit_tile(const PrefillParams& p, int hA, int hB, int qt, int kt, int pl) {
@@ -460,8 +467,10 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
           const int d0 = (D / 2) * half + 32 * c4;  // first dim of these 32
           if (kWin && p.out_lo) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              lo[c4 * 8 + i] = low_bits4(t[4 * i] * inv, t[4 * i + 1] * inv, t[4 * i + 2] * inv, t[4 * i + 3] * inv);
+            for (int i = 0; i < 8; ++i) {
+              const float a = t[4 * i] * inv, b4 = t[4 * i + 1] * inv, c = t[4 * i + 2] * inv, d = t[4 * i + 3] * inv;
+              lo[c4 * 8 + i] = low_bits4(a, b4, c, d, pack_bf16x2(a, b4), pack_bf16x2(c, d));
+            }
           }
           uint8_t* atom = stage + (d0 / 64) * (kQBytes / kAtoms);
 #pragma unroll
@@ -487,10 +496,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         tma_store_wait_read();  // the shared memory stays valid until the store has read it
       }
       if (kWin && p.out_lo && o_ok && q < p.S) {
-        uint4* dst = reinterpret_cast<uint4*>(p.out_lo + (((int64_t)b * p.H + h) * p.S + q) * D + (D / 2) * half);
+        int8_t* dst = p.out_lo + (((int64_t)b * p.H + h) * p.S + q) * D + (D / 2) * half;
 #pragma unroll
-        for (int i = 0; i < D / 32; ++i)
-          __stcs(dst + i, make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]));
+        for (int i = 0; i < D / 64; ++i) store_32b(dst + 32 * i, lo + 8 * i);  // whole 32-byte sectors
       }
     }
   }
@@ -588,7 +596,7 @@ extern "C" int abkv_window_attention(const void* q, const int64_t* q_strides, co
   if ((head_dim != 64 && head_dim != 128) || H > kMaxHeads || B > 65535 || S > kMaxKeyTiles * kBN)
     return ABKV_ERR_UNSUPPORTED;
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v) |
-       reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_lo)) & 15)
+       reinterpret_cast<uintptr_t>(out)) & 15 || (reinterpret_cast<uintptr_t>(out_lo) & 31))
     return ABKV_ERR_INVALID_ARG;
   if (!workspace || workspace_bytes < 256 || (reinterpret_cast<uintptr_t>(workspace) & 255))
     return ABKV_ERR_WORKSPACE;

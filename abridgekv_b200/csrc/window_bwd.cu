@@ -168,6 +168,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // the row sums (the previous kernel) are complete; the dQ kernel, which needs nothing of this one, may start
+  asm volatile("griddepcontrol.wait;\ngriddepcontrol.launch_dependents;\n" ::: "memory");
   const uint32_t tmem = *s_tmem;  // S^T [0,128), dP^T [128,256), dV [256,..), dK [384,..)
   bool dead = false;
 
@@ -550,6 +552,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
   __syncthreads();
   tc_fence_after();
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u));
+  // this kernel started beside the dK/dV kernel and must not be over before it: what follows reads both
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
 }
 
 // Di = rowsum(dO * O) in fp32: D / 8 lanes per row, eight dims a lane.  O is the forward's bf16 output with,
@@ -584,8 +588,7 @@ __global__ void __launch_bounds__(256) window_rowdot_kernel(const __nv_bfloat16*
       const int32_t low = (int32_t)(int8_t)((k < 4 ? l.x : l.y) >> (8 * (k & 3)));
       acc = fmaf(__int_as_float((int32_t)xb + (low << 8)), __uint_as_float(yb), acc);
     }
-    (void)rr;
-  }
+    }
 #pragma unroll
   for (int s = kL / 2; s; s >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, s);
   if (live && d0 == 0) {
@@ -622,13 +625,19 @@ int launch(const WinBwdParams& prm, const void* out, const int64_t* os, const in
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = Lay<D>::kSmem;
   cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim = {(unsigned)prm.cluster, 1, 1};
+  // Each kernel may be set up while the one before it drains.  dQ waits for dK/dV at its end only: every CTA
+  // of dK/dV has passed the row sums and is running (or done) before one of dQ's starts.
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim = {(unsigned)prm.cluster, 1, 1};
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   if (cudaLaunchKernelEx(&cfg, window_dkdv_kernel<D>, prm) != cudaSuccess) return ABKV_ERR_CUDA;
-  window_dq_kernel<D><<<dim3(prm.H, prm.B, prm.n_tiles), kThreads, Lay<D>::kSmem, s>>>(prm);
+  cfg.gridDim = dim3(prm.H, prm.B, prm.n_tiles);
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, window_dq_kernel<D>, prm) != cudaSuccess) return ABKV_ERR_CUDA;
   return cudaGetLastError() == cudaSuccess ? ABKV_OK : ABKV_ERR_CUDA;
 }
 

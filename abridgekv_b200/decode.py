@@ -151,11 +151,11 @@ def _window_plan(L, B, Hq, Hkv, D, page, max_pages, chunk_tokens, windows, sinks
                                                         weighted), win, snk
 
 
-def _need(ok: bool, name: str, want: str, t) -> None:
-    if not ok:
-        kind = TypeError if not isinstance(t, torch.Tensor) or not t.is_cuda else ValueError
-        raise kind(f"{name} must be {want}" + (
-            f", got {t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else ""))
+def _refuse(name: str, t, want: str) -> None:
+    kind = TypeError if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in (
+        torch.bfloat16, torch.int32) else ValueError
+    raise kind(f"{name} must be {want}" + (
+        f", got {t.dtype} {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else ""))
 
 
 def _check_weights(weights, L, B, Hkv, device) -> tuple[int, int]:
@@ -197,18 +197,18 @@ def _decode_window(queries, kv_caches, block_tables, seq_lens, weights, window, 
     bf16, i32 = torch.bfloat16, torch.int32
     for l in range(L):
         q, kv, bt, sl = queries[l], kv_caches[l], block_tables[l], seq_lens[l]
-        _need(q.dtype is bf16 and q.device == device and q.shape == q_shape and q.is_contiguous(), "query",
-              f"a contiguous bf16 [{B}, {Hq}, {D}] tensor on {device}", q)
-        _need(kv.dtype is bf16 and kv.device == device and kv.dim() == 5 and kv.shape[1:] == kv_shape[1:] and
-              kv.is_contiguous(), "kv_cache", f"a contiguous bf16 [num_blocks, 2, {page}, {Hkv}, {D}] tensor on {device}", kv)
-        _need(bt.dtype is i32 and bt.device == device and bt.dim() == 2 and bt.shape[0] >= B and bt.is_contiguous(),
-              "block_table", f"a contiguous int32 [>={B}, max_pages] tensor on {device}", bt)
-        _need(sl.dtype is i32 and sl.device == device and sl.dim() == 1 and sl.shape[0] >= B and sl.is_contiguous(),
-              "seq_lens", f"a contiguous int32 [>={B}] tensor on {device}", sl)
+        if not (q.dtype is bf16 and q.device == device and q.shape == q_shape and q.is_contiguous()):
+            _refuse("query", q, f"a contiguous bf16 [{B}, {Hq}, {D}] tensor on {device}")
+        if not (kv.dtype is bf16 and kv.device == device and kv.shape[1:] == kv_shape[1:] and kv.is_contiguous()):
+            _refuse("kv_cache", kv, f"a contiguous bf16 [num_blocks, 2, {page}, {Hkv}, {D}] tensor on {device}")
+        if not (bt.dtype is i32 and bt.device == device and bt.dim() == 2 and bt.shape[0] >= B and bt.is_contiguous()):
+            _refuse("block_table", bt, f"a contiguous int32 [>={B}, max_pages] tensor on {device}")
+        if not (sl.dtype is i32 and sl.device == device and sl.dim() == 1 and sl.shape[0] >= B and sl.is_contiguous()):
+            _refuse("seq_lens", sl, f"a contiguous int32 [>={B}] tensor on {device}")
         if outputs is not None:
             o = outputs[l]
-            _need(o.dtype is bf16 and o.device == device and o.shape == q_shape and o.is_contiguous(), "output",
-                  f"a contiguous bf16 [{B}, {Hq}, {D}] tensor on {device}", o)
+            if not (o.dtype is bf16 and o.device == device and o.shape == q_shape and o.is_contiguous()):
+                _refuse("output", o, f"a contiguous bf16 [{B}, {Hq}, {D}] tensor on {device}")
     windows, sinks = _per_layer("window", window, L), _per_layer("num_sinks", num_sinks, L)
     if max_pages_per_seq is None:
         max_pages_per_seq = max([bt.shape[1] for bt in block_tables])

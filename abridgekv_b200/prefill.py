@@ -18,6 +18,7 @@ it hands each layer its own BlockMask today.
 """
 from __future__ import annotations
 
+import functools
 import math
 from dataclasses import dataclass
 from typing import Sequence
@@ -178,18 +179,18 @@ class WindowMask:
 
 def _window_args(q, k, v, window, num_sinks, scale):
     for name, t in (("query", q), ("key", k), ("value", v)):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.bfloat16:
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or not t.is_cuda:
             raise TypeError(f"{name} must be a bf16 CUDA tensor (libabkv has no CPU path)")
         if t.dim() != 4:
             raise ValueError(f"{name} must be 4-D")
-        if t.device != q.device:
-            raise ValueError(f"{name} must be on the query's device")
     B, H, S, D = q.shape
     Hkv = k.shape[1]
-    if tuple(k.shape) != (B, Hkv, S, D) or tuple(v.shape) != (B, Hkv, S, D):
+    if k.shape != (B, Hkv, S, D) or v.shape != k.shape:
         raise ValueError("key/value must be [B, Hkv, S, D] matching the query")
     if Hkv == 0 or H % Hkv:
         raise ValueError("the KV heads must divide the query heads")
+    if k.device != q.device or v.device != q.device:
+        raise ValueError("key and value must be on the query's device")
     window, num_sinks = int(window), int(num_sinks)
     if not (1 <= window <= 0x7FFFFFFF and 0 <= num_sinks <= 0x7FFFFFFF):
         raise ValueError(f"window must be at least 1 and num_sinks at least 0, got {window} and {num_sinks}")
@@ -228,7 +229,8 @@ def window_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window:
         lse = torch.empty((B, H, S), dtype=torch.float32, device=device) if return_lse else None
         low = torch.empty((B, H, S, D), dtype=torch.int8, device=device) if return_low else None
         if B * H * S:
-            (q, qs), (k, ks), (v, vs), (_, os) = _tma_ready(q), _tma_ready(k), _tma_ready(v), _tma_ready(out)
+            (q, qs), (k, ks), (v, vs) = _tma_ready(q), _tma_ready(k), _tma_ready(v)
+            os = _lib.i64(S * H * D, D, H * D)
             ws, raw = call_workspace(device, 256, workspace)
             st = _lib.lib().abkv_window_attention(
                 q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os,
@@ -248,8 +250,7 @@ def window_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
     output, log-sum-exp and (optionally) the output's low bits (``abkv_window_attention_backward``).  Repeated
     calls give the same bits."""
     window, num_sinks, scale = _window_args(q, k, v, window, num_sinks, scale)
-    B, H, S, D = shape = q.shape
-    device = q.device
+    shape, device = q.shape, q.device
     for name, t in (("out", out), ("dout", dout)):
         if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != torch.bfloat16:
             raise TypeError(f"{name} must be a bf16 tensor on the query's device")
@@ -261,21 +262,35 @@ def window_backward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torc
                             low.device != device):
         raise ValueError("low must be the forward's contiguous int8 [B, H, S, D] low bits")
     with call_scope(device, stream):
-        (q, qs), (k, ks), (v, vs), (out, os), (dout, ds) = (_tma_ready(t) for t in (q, k, v, out, dout))
-        dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-        if B * H * S == 0:
-            return dq, dk, dv
-        lib = _lib.lib()
-        need = lib.abkv_window_attention_backward_workspace_size(B, H, S, D)
-        if need == 0:
-            raise _lib.AbkvError("abkv_window_attention_backward_workspace_size", 3, f"unsupported shape D={D}")
-        ws, raw = call_workspace(device, need, workspace)
-        (_, dqs), (_, dks), (_, dvs) = _tma_ready(dq), _tma_ready(dk), _tma_ready(dv)
-        st = lib.abkv_window_attention_backward(
-            q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os,
-            low.data_ptr() if low is not None else None, dout.data_ptr(), ds, lse.data_ptr(), dq.data_ptr(), dqs,
-            dk.data_ptr(), dks, dv.data_ptr(), dvs, B, H, k.shape[1], S, D, scale, window, num_sinks, ws.ptr(),
-            ws.nbytes, raw)
+        return _window_backward(q, k, v, out, dout, lse, low, window, num_sinks, scale, workspace)
+
+
+@functools.lru_cache(maxsize=256)
+def _window_backward_bytes(B: int, H: int, S: int, D: int) -> int:
+    need = _lib.lib().abkv_window_attention_backward_workspace_size(B, H, S, D)
+    if need == 0:
+        raise _lib.AbkvError("abkv_window_attention_backward_workspace_size", 3, f"unsupported shape D={D}")
+    return need
+
+
+def _window_backward(q, k, v, out, dout, lse, low, window, num_sinks, scale, workspace=None):
+    """The launch, on checked arguments and the current stream."""
+    B, H, S, D = q.shape
+    (q, qs), (k, ks), (v, vs) = _tma_ready(q), _tma_ready(k), _tma_ready(v)
+    (out, os), (dout, ds) = _tma_ready(out), _tma_ready(dout)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    if B * H * S == 0:
+        return dq, dk, dv
+    ws, raw = call_workspace(q.device, _window_backward_bytes(B, H, S, D), workspace)
+    # empty_like keeps the strides of a dense tensor; of others it makes its own
+    dqs = qs if dq.stride() == q.stride() else _tma_ready(dq)[1]
+    dks = ks if dk.stride() == k.stride() else _tma_ready(dk)[1]
+    dvs = vs if dv.stride() == v.stride() else _tma_ready(dv)[1]
+    st = _lib.lib().abkv_window_attention_backward(
+        q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os,
+        low.data_ptr() if low is not None else None, dout.data_ptr(), ds, lse.data_ptr(), dq.data_ptr(), dqs,
+        dk.data_ptr(), dks, dv.data_ptr(), dvs, B, H, k.shape[1], S, D, scale, window, num_sinks, ws.ptr(), ws.nbytes,
+        raw)
     if st:
         _lib.check("abkv_window_attention_backward", st)
     return dq, dk, dv
@@ -289,16 +304,15 @@ class WindowAttention(torch.autograd.Function):
         out, lse, low = window_forward(q, k, v, window=window, num_sinks=num_sinks, scale=scale, return_lse=True,
                                        return_low=True)
         ctx.save_for_backward(q, k, v, out, lse, low)
-        ctx.args = (window, num_sinks, scale)
+        ctx.args = (int(window), int(num_sinks), 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale))
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, low = ctx.saved_tensors
-        window, num_sinks, scale = ctx.args
-        dq, dk, dv = window_backward(q, k, v, out, dout, lse, window=window, num_sinks=num_sinks, scale=scale, low=low)
-        return dq, dk, dv, None, None, None
+        with call_scope(q.device, None):
+            return (*_window_backward(q, k, v, out, dout, lse, low, *ctx.args), None, None, None)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int, num_sinks: int = 0,
