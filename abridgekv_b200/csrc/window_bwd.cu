@@ -48,7 +48,7 @@ struct Lay {
   static constexpr int kOffShort = kOffLong + kLong * kTile;  // dO or V
   static constexpr int kOffStat = kOffShort + kShort * kTile;  // [2 tiles][4 column groups][lse2, di][32]
   static constexpr int kOffBar = kOffStat + 2 * 4 * 2 * 32 * 4;
-  static constexpr int kSmem = kOffBar + 256;      // the base is 1024-byte aligned (checked by the kernels)
+  static constexpr int kSmem = kOffBar + 512;      // the base is 1024-byte aligned (checked by the kernels)
   static constexpr int kRedStride = D + 4;         // fp32 rows of the cluster reduction (in the rings)
   static constexpr uint32_t kIdescAcc = idesc_bf16_m128(D, true);
 };
@@ -57,11 +57,14 @@ static_assert(2 * kT * Lay<128>::kRedStride * 4 <= (kLong + kShort) * Lay<128>::
 static_assert(2 * kT * Lay<64>::kRedStride * 4 <= (kLong + kShort) * Lay<64>::kTile, "cluster reduction");
 
 // barriers: stationary operands, long ring full / empty, short ring full / empty, S full (two in the dQ kernel),
-// dP full, P ready, dS ready, accumulators complete, statistics of a column group, then the TMEM address
+// dP full, P ready, dS ready, accumulators complete / drained, statistics [column group][buffer] (a barrier per buffer:
+// the writer may be a pair ahead of a reader, and a parity wait cannot tell phases 2 apart), stationary operands
+// released, work item full / empty (two deep), then the TMEM address and the items
 constexpr int kBarA = 0, kBarLF = 1, kBarLE = kBarLF + kLong, kBarSF = kBarLE + kLong, kBarSE = kBarSF + kShort,
               kBarS = kBarSE + kShort, kBarDP = kBarS + 2, kBarP = kBarDP + 1, kBarDS = kBarP + 1,
-              kBarAcc = kBarDS + 1, kBarStat = kBarAcc + 1, kBarTmem = kBarStat + 4;
-static_assert((kBarTmem + 1) * 8 <= 256, "barrier area");
+              kBarAcc = kBarDS + 1, kBarDrain = kBarAcc + 1, kBarStat = kBarDrain + 1, kBarAE = kBarStat + 8,
+              kBarIF = kBarAE + 1, kBarIE = kBarIF + 2, kBarTmem = kBarIE + 2, kBarItem = kBarTmem + 1;
+static_assert((kBarItem + 1) * 8 <= 512, "barrier area");
 
 struct alignas(64) WinBwdParams {
   CUtensorMap tm_q, tm_k, tm_v, tm_do;
@@ -70,7 +73,10 @@ struct alignas(64) WinBwdParams {
   __nv_bfloat16 *dq, *dk, *dv;
   int64_t dq_sb, dq_sh, dq_ss, dk_sb, dk_sh, dk_ss, dv_sb, dv_sh, dv_ss;
   int32_t* err;
-  int B, H, Hkv, G, S, n_tiles, window, n_sink, cluster;
+  int32_t* work;     // next work item of the dK/dV launch (zeroed by the row-sum kernel)
+  int B, H, Hkv, G, S, n_tiles, window, n_sink;
+  int cluster, tile0, tiles;  // dK/dV launch: CTAs per key tile; its key tiles
+  int first;                  // the launch that waits for the row sums
   float scale, scale_log2;
 };
 
@@ -136,8 +142,11 @@ __device__ __forceinline__ float4 peer_ld4(uint32_t local, int rank) {
 }
 
 // ---------------------------------------------------------------------------
-// dK and dV of one 128-key tile of one KV head: walks the (query tile, head) pairs that see it.  A cluster of
-// p.cluster CTAs shares the pairs and adds its parts, in rank order, through its shared memory.
+// dK and dV.  A work item is a 128-key tile of one KV head: all (query tile, head) pairs that see it.  Without
+// clusters a CTA per SM takes items from a counter, longest first, and the next item's operands and first scores are
+// under way while the finished accumulators are read out.  With p.cluster > 1 (idle SMs, or the sinks' tiles, which
+// every query tile sees) a cluster takes one item, its CTAs share the pairs and add their parts, in rank order,
+// through shared memory.
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_constant__ WinBwdParams p) {
   using LY = Lay<D>;
@@ -148,218 +157,292 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
   }
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + LY::kOffBar);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar + kBarTmem);
+  volatile int32_t* s_item = reinterpret_cast<volatile int32_t*>(bar + kBarItem);  // [2]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = blockIdx.x % p.cluster, hk = blockIdx.x / p.cluster, b = blockIdx.y, kt = blockIdx.z;
-  // query tiles kt .. last see the key tile (its last key k: queries < k + window); the sinks' tiles: all
-  int last = p.n_tiles - 1;
-  if (kt * kT >= p.n_sink) last = min(last, (min(kt * kT + kT, p.S) - 1 + p.window - 1) / kT);
-  const int pairs = (last - kt + 1) * p.G;
-  const int n = pairs > rank ? (pairs - rank - 1) / p.cluster + 1 : 0;  // this CTA's
-  auto pair_at = [&](int u, int& qt, int& h) {
-    const int i = rank + u * p.cluster;
-    qt = kt + i / p.G;
-    h = hk * p.G + i % p.G;
-  };
+  const int rank = blockIdx.x % p.cluster;
+  const int heads = p.Hkv * p.B, n_items = heads * p.tiles;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBarTmem; ++i) mbar_init(&bar[i], (i == kBarP || i == kBarDS) ? kWorkers : 1);
+    for (int i = 0; i < kBarTmem; ++i)
+      mbar_init(&bar[i], (i == kBarP || i == kBarDS || i == kBarDrain) ? kWorkers
+                                                                       : (i >= kBarIE && i < kBarIE + 2 ? kWorkers + 1 : 1));
   }
   if (warp == 1) alloc_tmem(s_tmem);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  // the row sums (the previous kernel) are complete; the dQ kernel, which needs nothing of this one, may start
-  asm volatile("griddepcontrol.wait;\ngriddepcontrol.launch_dependents;\n" ::: "memory");
+  // The row sums are complete before the first launch goes on, and the others start after all of its CTAs have: they
+  // need nothing of one another.
+  if (p.first) asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");
   const uint32_t tmem = *s_tmem;  // S^T [0,128), dP^T [128,256), dV [256,..), dK [384,..)
   bool dead = false;
 
+  // Work item `it` of this CTA (every role asks in turn): false when there is none.
+  struct Item {
+    int kt, hk, b, n;
+  };
+  auto decode = [&](int i, Item& x) {
+    x.kt = p.tile0 + i / heads;  // longest first
+    const int r = i % heads;
+    x.hk = r % p.Hkv;
+    x.b = r / p.Hkv;
+    // query tiles kt .. last see the key tile (its last key k: queries < k + window); the sinks' tiles: all
+    int last = p.n_tiles - 1;
+    if (x.kt * kT >= p.n_sink) last = min(last, (min(x.kt * kT + kT, p.S) - 1 + p.window - 1) / kT);
+    const int pairs = (last - x.kt + 1) * p.G;
+    x.n = pairs > rank ? (pairs - rank - 1) / p.cluster + 1 : 0;  // this CTA's
+  };
+  auto next_item = [&](int it, Item& x) -> bool {
+    if (p.cluster > 1) {
+      if (it > 0) return false;
+      decode(blockIdx.x / p.cluster, x);
+      return true;
+    }
+    const int slot = it & 1;
+    if (!wait_or_abort(&bar[kBarIF + slot], (uint32_t)((it >> 1) & 1), dead, p.err)) return false;
+    const int i = s_item[slot];
+    if (i < 0) return false;
+    decode(i, x);
+    return true;
+  };
+  auto done_item = [&](int it) {  // by one thread of a role: it has decoded the item
+    if (p.cluster == 1) mbar_arrive_one(&bar[kBarIE + (it & 1)]);
+  };
+  auto pair_at = [&](const Item& x, int u, int& qt, int& h) {
+    const int i = rank + u * p.cluster;
+    qt = x.kt + i / p.G;
+    h = x.hk * p.G + i % p.G;
+  };
+
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
-      mbar_expect_tx(&bar[kBarA], 2 * LY::kTile);
-      load_tile<D>(smem + LY::kOffA, &p.tm_k, kt * kT, hk, b, &bar[kBarA]);
-      load_tile<D>(smem + LY::kOffB, &p.tm_v, kt * kT, hk, b, &bar[kBarA]);
-      for (int u = 0; u < n; ++u) {
-        int qt, h;
-        pair_at(u, qt, h);
-        const int l = u % kLong, s = u % kShort;
-        if (!wait_or_abort(&bar[kBarLE + l], (uint32_t)(((u / kLong) & 1) ^ 1), dead, p.err)) break;
-        mbar_expect_tx(&bar[kBarLF + l], LY::kTile);
-        load_tile<D>(smem + LY::kOffLong + l * LY::kTile, &p.tm_q, qt * kT, h, b, &bar[kBarLF + l]);
-        if (!wait_or_abort(&bar[kBarSE + s], (uint32_t)(((u / kShort) & 1) ^ 1), dead, p.err)) break;
-        mbar_expect_tx(&bar[kBarSF + s], LY::kTile);
-        load_tile<D>(smem + LY::kOffShort + s * LY::kTile, &p.tm_do, qt * kT, h, b, &bar[kBarSF + s]);
+    if (lane == 0) {
+      Item x;
+      int g = 0;  // pairs loaded so far
+      for (int it = 0; !dead; ++it) {
+        if (p.cluster > 1) {
+          if (!next_item(it, x)) break;
+        } else {
+          // take the next item and hand it to the other roles
+          const int slot = it & 1;
+          if (!wait_or_abort(&bar[kBarIE + slot], (uint32_t)(((it >> 1) & 1) ^ 1), dead, p.err)) break;
+          const int i = atomicAdd(p.work, 1);
+          s_item[slot] = i < n_items ? i : -1;
+          mbar_arrive_one(&bar[kBarIF + slot]);
+          if (i >= n_items) break;
+          decode(i, x);
+        }
+        if (x.n == 0) continue;
+        // the previous item's last products over K and V have run
+        if (!wait_or_abort(&bar[kBarAE], (uint32_t)((it & 1) ^ 1), dead, p.err)) break;
+        mbar_expect_tx(&bar[kBarA], 2 * LY::kTile);
+        load_tile<D>(smem + LY::kOffA, &p.tm_k, x.kt * kT, x.hk, x.b, &bar[kBarA]);
+        load_tile<D>(smem + LY::kOffB, &p.tm_v, x.kt * kT, x.hk, x.b, &bar[kBarA]);
+        for (int u = 0; u < x.n; ++u, ++g) {
+          int qt, h;
+          pair_at(x, u, qt, h);
+          const int l = g % kLong, sh = g % kShort;
+          if (!wait_or_abort(&bar[kBarLE + l], (uint32_t)(((g / kLong) & 1) ^ 1), dead, p.err)) break;
+          mbar_expect_tx(&bar[kBarLF + l], LY::kTile);
+          load_tile<D>(smem + LY::kOffLong + l * LY::kTile, &p.tm_q, qt * kT, h, x.b, &bar[kBarLF + l]);
+          if (!wait_or_abort(&bar[kBarSE + sh], (uint32_t)(((g / kShort) & 1) ^ 1), dead, p.err)) break;
+          mbar_expect_tx(&bar[kBarSF + sh], LY::kTile);
+          load_tile<D>(smem + LY::kOffShort + sh * LY::kTile, &p.tm_do, qt * kT, h, x.b, &bar[kBarSF + sh]);
+        }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+    if (lane == 0) {
       const uint32_t k = smem_u32(smem + LY::kOffA), v = smem_u32(smem + LY::kOffB);
-      auto q_at = [&](int u) { return smem_u32(smem + LY::kOffLong + (u % kLong) * LY::kTile); };
-      auto do_at = [&](int u) { return smem_u32(smem + LY::kOffShort + (u % kShort) * LY::kTile); };
-      auto scores = [&](int u) -> bool {  // S^T(u)
-        if (!wait_or_abort(&bar[kBarLF + u % kLong], (uint32_t)((u / kLong) & 1), dead, p.err)) return false;
+      auto q_at = [&](int g) { return smem_u32(smem + LY::kOffLong + (g % kLong) * LY::kTile); };
+      auto do_at = [&](int g) { return smem_u32(smem + LY::kOffShort + (g % kShort) * LY::kTile); };
+      auto scores = [&](int g) -> bool {  // S^T(g)
+        if (!wait_or_abort(&bar[kBarLF + g % kLong], (uint32_t)((g / kLong) & 1), dead, p.err)) return false;
         tc_fence_after();
-        issue_scores<D>(tmem, k, q_at(u));
+        issue_scores<D>(tmem, k, q_at(g));
         umma_commit(&bar[kBarS]);
         return true;
       };
-      auto dscores = [&](int u) -> bool {  // dP^T(u)
-        if (!wait_or_abort(&bar[kBarSF + u % kShort], (uint32_t)((u / kShort) & 1), dead, p.err)) return false;
+      auto dscores = [&](int g) -> bool {  // dP^T(g)
+        if (!wait_or_abort(&bar[kBarSF + g % kShort], (uint32_t)((g / kShort) & 1), dead, p.err)) return false;
         tc_fence_after();
-        issue_scores<D>(tmem + 128, v, do_at(u));
+        issue_scores<D>(tmem + 128, v, do_at(g));
         umma_commit(&bar[kBarDP]);
         return true;
       };
-      if (wait_or_abort(&bar[kBarA], 0, dead, p.err) && scores(0) && dscores(0)) {
-        for (int u = 0; u < n; ++u) {
-          const uint32_t par = (uint32_t)(u & 1);
-          // P^T(u) is ready: dV, then the next scores over it (one thread's MMAs run in issue order)
+      Item x;
+      int g = 0;
+      for (int it = 0; next_item(it, x); ++it) {
+        done_item(it);
+        if (x.n == 0) continue;
+        if (!wait_or_abort(&bar[kBarA], (uint32_t)(it & 1), dead, p.err) || !scores(g) || !dscores(g)) break;
+        if (x.n == 1) umma_commit(&bar[kBarAE]);
+        for (int u = 0; u < x.n; ++u, ++g) {
+          const uint32_t par = (uint32_t)(g & 1);
+          // P^T(g) is ready: dV, then the next scores over it (one thread's MMAs run in issue order)
           if (!wait_or_abort(&bar[kBarP], par, dead, p.err)) break;
+          // the first product of an item overwrites dV and dK: the previous ones have been read out
+          if (u == 0 && it > 0 && !wait_or_abort(&bar[kBarDrain], (uint32_t)((it - 1) & 1), dead, p.err)) break;
           tc_fence_after();
-          issue_accumulate<D>(tmem + 256, tmem, do_at(u), u == 0);
-          umma_commit(&bar[kBarSE + u % kShort]);  // dO(u): its last use
-          if (u + 1 < n && !scores(u + 1)) break;
+          issue_accumulate<D>(tmem + 256, tmem, do_at(g), u == 0);
+          umma_commit(&bar[kBarSE + g % kShort]);  // dO(g): its last use
+          if (u + 1 < x.n && !scores(g + 1)) break;
           if (!wait_or_abort(&bar[kBarDS], par, dead, p.err)) break;
           tc_fence_after();
-          issue_accumulate<D>(tmem + 384, tmem + 128, q_at(u), u == 0);
-          umma_commit(&bar[kBarLE + u % kLong]);
-          if (u + 1 < n && !dscores(u + 1)) break;
+          issue_accumulate<D>(tmem + 384, tmem + 128, q_at(g), u == 0);
+          umma_commit(&bar[kBarLE + g % kLong]);
+          if (u + 1 < x.n && !dscores(g + 1)) break;
+          if (u + 2 == x.n) umma_commit(&bar[kBarAE]);  // the item's last scores are issued: K and V are free then
         }
+        if (dead) break;
+        umma_commit(&bar[kBarAcc]);
       }
-      umma_commit(&bar[kBarAcc]);
     }
   } else {
     const int sw = warp - 2, cg = sw >> 2, quarter = warp & 3;
-    const int row = quarter * 32 + lane, key = kt * kT + row;
+    const int row = quarter * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     // the four warps of a column group share its queries' statistics: quarter 0 writes them, two tiles deep
     float* stat = reinterpret_cast<float*>(smem + LY::kOffStat) + cg * 64;
     const float sl2 = p.scale_log2;
-    const bool sink = key < p.n_sink;
-    // lane c holds the statistics of the next pair's query 32 cg + c
-    float n_lse = 0.f, n_di = 0.f;
-    auto fetch = [&](int u) {
-      int qt, h;
-      pair_at(u, qt, h);
-      const int q = qt * kT + 32 * cg + lane;
-      const int64_t r = ((int64_t)b * p.H + h) * p.S + q;
-      n_lse = q < p.S ? __ldg(p.lse + r) * kLog2e : 0.f;
-      n_di = q < p.S ? __ldg(p.di + r) : 0.f;
-    };
     const bool stager = quarter == 0;
-    auto stage = [&](int u) {  // statistics of pair u into buffer u % 2, then fetch those of pair u + 1
-      stat[(u & 1) * 256 + lane] = n_lse;
-      stat[(u & 1) * 256 + 32 + lane] = n_di;
+    Item x;
+    int g = 0;
+    for (int it = 0;; ++it) {
+      const bool more = next_item(it, x);
+      if (!__all_sync(0xffffffffu, more)) break;
       __syncwarp();
-      if (lane == 0) mbar_arrive_one(&bar[kBarStat + cg]);
-      if (u + 1 < n) fetch(u + 1);
-    };
-    if (stager && n > 0) {
-      fetch(0);
-      stage(0);
-    }
-    for (int u = 0; u < n; ++u) {
-      const uint32_t par = (uint32_t)(u & 1);
-      int qt, h;
-      pair_at(u, qt, h);
-      const float *s_lse = stat + (u & 1) * 256, *s_di = s_lse + 32;
-      // visible queries of this key among the warp's 32: q >= key, q < key + window (or a sink), q < S
-      const int q0 = qt * kT + 32 * cg;
-      const int e = sink ? p.S : min(p.S, key + p.window);
-      const uint32_t mask = below(e - q0) & ~below(key - q0);
-      const bool full = __all_sync(0xffffffffu, mask == 0xFFFFFFFFu);
-      bool ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarStat + cg], par, dead, p.err) &&
-                                            wait_or_abort(&bar[kBarS], par, dead, p.err));
-      if (!ok) dead = true;
-      tc_fence_after();
-      float pv[32];
-      uint32_t w[16];
-      if (ok) {
-        tmem_ld32(tmem + lane_base + 32 * cg, pv);
-        tmem_wait_ld();
+      if (lane == 0) done_item(it);
+      const int key = x.kt * kT + row;
+      const bool sink = key < p.n_sink;
+      // lane c holds the statistics of the next pair's query 32 cg + c
+      float n_lse = 0.f, n_di = 0.f;
+      auto fetch = [&](int u) {
+        int qt, h;
+        pair_at(x, u, qt, h);
+        const int q = qt * kT + 32 * cg + lane;
+        const int64_t r = ((int64_t)x.b * p.H + h) * p.S + q;
+        n_lse = q < p.S ? __ldg(p.lse + r) * kLog2e : 0.f;
+        n_di = q < p.S ? __ldcg(p.di + r) : 0.f;
+      };
+      const int g_item = g;
+      auto stage = [&](int u) {  // statistics of pair u into its buffer, then fetch those of pair u + 1
+        const int buf = (g_item + u) & 1;
+        stat[buf * 256 + lane] = n_lse;
+        stat[buf * 256 + 32 + lane] = n_di;
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&bar[kBarStat + 2 * cg + buf]);
+        if (u + 1 < x.n) fetch(u + 1);
+      };
+      if (stager && x.n > 0) {
+        fetch(0);
+        stage(0);
+      }
+      for (int u = 0; u < x.n; ++u, ++g) {
+        const uint32_t par = (uint32_t)(g & 1);
+        int qt, h;
+        pair_at(x, u, qt, h);
+        const float *s_lse = stat + (g & 1) * 256, *s_di = s_lse + 32;
+        // visible queries of this key among the warp's 32: q >= key, q < key + window (or a sink), q < S
+        const int q0 = qt * kT + 32 * cg;
+        const int e = sink ? p.S : min(p.S, key + p.window);
+        const uint32_t mask = below(e - q0) & ~below(key - q0);
+        const bool full = __all_sync(0xffffffffu, mask == 0xFFFFFFFFu);
+        bool ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarStat + 2 * cg + (g & 1)], (uint32_t)((g >> 1) & 1), dead,
+                                                            p.err) &&
+                                              wait_or_abort(&bar[kBarS], par, dead, p.err));
+        if (!ok) dead = true;
+        tc_fence_after();
+        float pv[32];
+        uint32_t w[16];
+        if (ok) {
+          tmem_ld32(tmem + lane_base + 32 * cg, pv);
+          tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          const float4 l = *reinterpret_cast<const float4*>(s_lse + c);
-          fma_pair(pv[c], pv[c + 1], pv[c], pv[c + 1], sl2, -l.x, -l.y);
-          fma_pair(pv[c + 2], pv[c + 3], pv[c + 2], pv[c + 3], sl2, -l.z, -l.w);
+          for (int c = 0; c < 32; c += 4) {
+            const float4 l = *reinterpret_cast<const float4*>(s_lse + c);
+            fma_pair(pv[c], pv[c + 1], pv[c], pv[c + 1], sl2, -l.x, -l.y);
+            fma_pair(pv[c + 2], pv[c + 3], pv[c + 2], pv[c + 3], sl2, -l.z, -l.w);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) pv[c + j] = fast_exp2(pv[c + j]);
+            for (int j = 0; j < 4; ++j) pv[c + j] = fast_exp2(pv[c + j]);
+          }
+          if (!full) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) pv[c] = (mask >> c) & 1u ? pv[c] : 0.f;
+          }
+#pragma unroll
+          for (int c = 0; c < 16; ++c) w[c] = pack_bf16x2(pv[2 * c], pv[2 * c + 1]);
+          tmem_st16(tmem + lane_base + 32 * cg, w);
+          tmem_wait_st();
         }
-        if (!full) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&bar[kBarP]);
+        ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarDP], par, dead, p.err));
+        if (!ok) dead = true;
+        // dP(u) followed every warp's dS(u - 1): nobody reads the other statistics buffer any more
+        if (stager && u + 1 < x.n) stage(u + 1);
+        tc_fence_after();
+        if (ok) {
+          float dp[32];
+          tmem_ld32(tmem + lane_base + 128 + 32 * cg, dp);
+          tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) pv[c] = (mask >> c) & 1u ? pv[c] : 0.f;
+          for (int c = 0; c < 32; c += 4) {
+            const float4 d = *reinterpret_cast<const float4*>(s_di + c);
+            sub_mul_pair(dp[c], dp[c + 1], dp[c], dp[c + 1], d.x, d.y, pv[c], pv[c + 1]);
+            sub_mul_pair(dp[c + 2], dp[c + 3], dp[c + 2], dp[c + 3], d.z, d.w, pv[c + 2], pv[c + 3]);
+            w[c / 2] = pack_bf16x2(dp[c], dp[c + 1]);
+            w[c / 2 + 1] = pack_bf16x2(dp[c + 2], dp[c + 3]);
+          }
+          tmem_st16(tmem + lane_base + 128 + 32 * cg, w);
+          tmem_wait_st();
         }
-#pragma unroll
-        for (int c = 0; c < 16; ++c) w[c] = pack_bf16x2(pv[2 * c], pv[2 * c + 1]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&bar[kBarDS]);
       }
-      if (ok) {
-        tmem_st16(tmem + lane_base + 32 * cg, w);
-        tmem_wait_st();
+      if (x.n > 0) {
+        if (!__all_sync(0xffffffffu, wait_or_abort(&bar[kBarAcc], (uint32_t)(it & 1), dead, p.err))) dead = true;
+        tc_fence_after();
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_one(&bar[kBarP]);
-      ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarDP], par, dead, p.err));
-      if (!ok) dead = true;
-      // dP(u) followed every warp's dS(u - 1): nobody reads the other statistics buffer any more
-      if (stager && u + 1 < n) stage(u + 1);
-      tc_fence_after();
-      if (ok) {
-        float dp[32];
-        tmem_ld32(tmem + lane_base + 128 + 32 * cg, dp);
-        tmem_wait_ld();
+      // dV (cg 0, 1) and dK (cg 2, 3): this warp's D / 2 columns of its rows
+      const bool is_dk = cg >= 2;
+      const int c0 = (cg & 1) * (D / 2);
+      const uint32_t col = (is_dk ? 384u : 256u) + c0;
+      const float gs = is_dk ? p.scale : 1.f;
+      float* red = reinterpret_cast<float*>(smem + LY::kOffLong) + ((is_dk ? kT : 0) + row) * LY::kRedStride;
+      __nv_bfloat16* out = is_dk ? p.dk + (int64_t)x.b * p.dk_sb + (int64_t)x.hk * p.dk_sh + (int64_t)key * p.dk_ss
+                                 : p.dv + (int64_t)x.b * p.dv_sb + (int64_t)x.hk * p.dv_sh + (int64_t)key * p.dv_ss;
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          const float4 d = *reinterpret_cast<const float4*>(s_di + c);
-          sub_mul_pair(dp[c], dp[c + 1], dp[c], dp[c + 1], d.x, d.y, pv[c], pv[c + 1]);
-          sub_mul_pair(dp[c + 2], dp[c + 3], dp[c + 2], dp[c + 3], d.z, d.w, pv[c + 2], pv[c + 3]);
-          w[c / 2] = pack_bf16x2(dp[c], dp[c + 1]);
-          w[c / 2 + 1] = pack_bf16x2(dp[c + 2], dp[c + 3]);
+      for (int c = 0; c < D / 2; c += 32) {
+        float t[32];
+        if (x.n > 0) {
+          tmem_ld32(tmem + lane_base + col + c, t);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) t[j] = 0.f;
         }
-      }
-      if (ok) {
-        tmem_st16(tmem + lane_base + 128 + 32 * cg, w);
-        tmem_wait_st();
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_one(&bar[kBarDS]);
-    }
-    if (n > 0) {
-      if (!__all_sync(0xffffffffu, wait_or_abort(&bar[kBarAcc], 0, dead, p.err))) dead = true;
-      tc_fence_after();
-    }
-    // dV (cg 0, 1) and dK (cg 2, 3): this warp's D / 2 columns of its rows
-    const bool is_dk = cg >= 2;
-    const int c0 = (cg & 1) * (D / 2);
-    const uint32_t col = (is_dk ? 384u : 256u) + c0;
-    const float gs = is_dk ? p.scale : 1.f;
-    float* red = reinterpret_cast<float*>(smem + LY::kOffLong) + ((is_dk ? kT : 0) + row) * LY::kRedStride;
-    __nv_bfloat16* out = is_dk ? p.dk + (int64_t)b * p.dk_sb + (int64_t)hk * p.dk_sh + (int64_t)key * p.dk_ss
-                               : p.dv + (int64_t)b * p.dv_sb + (int64_t)hk * p.dv_sh + (int64_t)key * p.dv_ss;
-#pragma unroll 1
-    for (int c = 0; c < D / 2; c += 32) {
-      float t[32];
-      if (n > 0) {
-        tmem_ld32(tmem + lane_base + col + c, t);
-        tmem_wait_ld();
-      }
-      if (n == 0) {
+        if (c + 32 == D / 2) {  // the accumulators are in registers
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_one(&bar[kBarDrain]);
+        }
+        if (p.cluster > 1) {
 #pragma unroll
-        for (int j = 0; j < 32; ++j) t[j] = 0.f;
-      }
-      if (p.cluster > 1) {
+          for (int j = 0; j < 32; j += 4)
+            *reinterpret_cast<float4*>(red + c0 + c + j) = make_float4(t[j], t[j + 1], t[j + 2], t[j + 3]);
+        } else if (key < p.S && !dead) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4)
-          *reinterpret_cast<float4*>(red + c0 + c + j) = make_float4(t[j], t[j + 1], t[j + 2], t[j + 3]);
-      } else if (key < p.S && !dead) {
-#pragma unroll
-        for (int v8 = 0; v8 < 4; ++v8) {
-          uint4 pk;
-          pk.x = pack_bf16x2(t[v8 * 8 + 0] * gs, t[v8 * 8 + 1] * gs);
-          pk.y = pack_bf16x2(t[v8 * 8 + 2] * gs, t[v8 * 8 + 3] * gs);
-          pk.z = pack_bf16x2(t[v8 * 8 + 4] * gs, t[v8 * 8 + 5] * gs);
-          pk.w = pack_bf16x2(t[v8 * 8 + 6] * gs, t[v8 * 8 + 7] * gs);
-          *reinterpret_cast<uint4*>(out + c0 + c + v8 * 8) = pk;
+          for (int v8 = 0; v8 < 4; ++v8) {
+            uint4 pk;
+            pk.x = pack_bf16x2(t[v8 * 8 + 0] * gs, t[v8 * 8 + 1] * gs);
+            pk.y = pack_bf16x2(t[v8 * 8 + 2] * gs, t[v8 * 8 + 3] * gs);
+            pk.z = pack_bf16x2(t[v8 * 8 + 4] * gs, t[v8 * 8 + 5] * gs);
+            pk.w = pack_bf16x2(t[v8 * 8 + 6] * gs, t[v8 * 8 + 7] * gs);
+            *reinterpret_cast<uint4*>(out + c0 + c + v8 * 8) = pk;
+          }
         }
       }
     }
@@ -369,6 +452,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
   tc_fence_after();
   if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(512u));
   if (p.cluster > 1) {
+    Item x;
+    decode(blockIdx.x / p.cluster, x);
     cluster_barrier();
     // this CTA's share of the rows of [dV; dK], eight dims a thread, the parts in rank order
     const int rows = 2 * kT / p.cluster;
@@ -376,14 +461,14 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
     for (int i = threadIdx.x; i < rows * (D / 8); i += kThreads) {
       const int rr = rank * rows + i / (D / 8), d0 = (i % (D / 8)) * 8;
       const bool is_dk = rr >= kT;
-      const int key = kt * kT + (is_dk ? rr - kT : rr);
+      const int key = x.kt * kT + (is_dk ? rr - kT : rr);
       if (key >= p.S) continue;
       float a[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       for (int c = 0; c < p.cluster; ++c) {
         const uint32_t at = base + (rr * LY::kRedStride + d0) * 4;
-        const float4 x = peer_ld4(at, c), y = peer_ld4(at + 16, c);
-        a[0] += x.x; a[1] += x.y; a[2] += x.z; a[3] += x.w;
-        a[4] += y.x; a[5] += y.y; a[6] += y.z; a[7] += y.w;
+        const float4 y = peer_ld4(at, c), z = peer_ld4(at + 16, c);
+        a[0] += y.x; a[1] += y.y; a[2] += y.z; a[3] += y.w;
+        a[4] += z.x; a[5] += z.y; a[6] += z.z; a[7] += z.w;
       }
       const float gs = is_dk ? p.scale : 1.f;
       uint4 pk;
@@ -391,16 +476,20 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
       pk.y = pack_bf16x2(a[2] * gs, a[3] * gs);
       pk.z = pack_bf16x2(a[4] * gs, a[5] * gs);
       pk.w = pack_bf16x2(a[6] * gs, a[7] * gs);
-      __nv_bfloat16* out = is_dk ? p.dk + (int64_t)b * p.dk_sb + (int64_t)hk * p.dk_sh + (int64_t)key * p.dk_ss
-                                 : p.dv + (int64_t)b * p.dv_sb + (int64_t)hk * p.dv_sh + (int64_t)key * p.dv_ss;
+      __nv_bfloat16* out = is_dk ? p.dk + (int64_t)x.b * p.dk_sb + (int64_t)x.hk * p.dk_sh + (int64_t)key * p.dk_ss
+                                 : p.dv + (int64_t)x.b * p.dv_sb + (int64_t)x.hk * p.dv_sh + (int64_t)key * p.dv_ss;
       *reinterpret_cast<uint4*>(out + d0) = pk;
     }
     cluster_barrier();  // no CTA leaves while another reads its part
   }
+  // a launch of this kernel that ran beside another one is not over before it
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
 }
 
 // ---------------------------------------------------------------------------
-// dQ of one 128-query tile of one head: walks the key tiles it sees (the sinks', then the window's).
+// dQ.  A work item is a 128-query tile of one head: it walks the key tiles that the tile sees (the sinks', then the
+// window's).  A CTA per SM takes items round robin, the longest first; the next item's operands are loaded and its
+// first scores computed while the finished dQ is read out.
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_constant__ WinBwdParams p) {
   using LY = Lay<D>;
@@ -412,15 +501,10 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + LY::kOffBar);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar + kBarTmem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.x, b = blockIdx.y, qt = p.n_tiles - 1 - (int)blockIdx.z;  // the longest first
-  const int hk = h / p.G;
-  // keys [n_sink, w_lo) are hidden from the whole tile; visited tile i is key tile i < ns ? i : i + shift
-  const int w_lo = max(0, qt * kT - p.window + 1);
-  const int ns = (min(p.n_sink, w_lo) + kT - 1) / kT, shift = max(w_lo / kT - ns, 0);
-  const int n = qt + 1 - shift;
+  const int heads = p.H * p.B, n_items = heads * p.n_tiles;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBarTmem; ++i) mbar_init(&bar[i], i == kBarDS ? kWorkers : 1);
+    for (int i = 0; i < kBarTmem; ++i) mbar_init(&bar[i], (i == kBarDS || i == kBarDrain) ? kWorkers : 1);
   }
   if (warp == 1) alloc_tmem(s_tmem);
   tc_fence_before();
@@ -428,123 +512,162 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
   tc_fence_after();
   const uint32_t tmem = *s_tmem;  // S [0,128) [128,256), dP [256,384), dQ [384,..)
   bool dead = false;
+  struct Item {
+    int qt, h, b, ns, shift, n;
+  };
+  auto decode = [&](int i) -> Item {
+    Item x;
+    x.qt = p.n_tiles - 1 - i / heads;
+    const int r = i % heads;
+    x.h = r % p.H;
+    x.b = r / p.H;
+    // keys [n_sink, w_lo) are hidden from the whole tile; visited tile u is key tile u < ns ? u : u + shift
+    const int w_lo = max(0, x.qt * kT - p.window + 1);
+    x.ns = (min(p.n_sink, w_lo) + kT - 1) / kT;
+    x.shift = max(w_lo / kT - x.ns, 0);
+    x.n = x.qt + 1 - x.shift;
+    return x;
+  };
 
   if (warp == 0) {
     if (lane == 0) {
-      mbar_expect_tx(&bar[kBarA], 2 * LY::kTile);
-      load_tile<D>(smem + LY::kOffA, &p.tm_q, qt * kT, h, b, &bar[kBarA]);
-      load_tile<D>(smem + LY::kOffB, &p.tm_do, qt * kT, h, b, &bar[kBarA]);
-      for (int u = 0; u < n; ++u) {
-        const int row = (u < ns ? u : u + shift) * kT;
-        const int l = u % kLong, s = u % kShort;
-        if (!wait_or_abort(&bar[kBarLE + l], (uint32_t)(((u / kLong) & 1) ^ 1), dead, p.err)) break;
-        mbar_expect_tx(&bar[kBarLF + l], LY::kTile);
-        load_tile<D>(smem + LY::kOffLong + l * LY::kTile, &p.tm_k, row, hk, b, &bar[kBarLF + l]);
-        if (!wait_or_abort(&bar[kBarSE + s], (uint32_t)(((u / kShort) & 1) ^ 1), dead, p.err)) break;
-        mbar_expect_tx(&bar[kBarSF + s], LY::kTile);
-        load_tile<D>(smem + LY::kOffShort + s * LY::kTile, &p.tm_v, row, hk, b, &bar[kBarSF + s]);
+      int g = 0, it = 0;
+      for (int i = blockIdx.x; i < n_items && !dead; i += gridDim.x, ++it) {
+        const Item x = decode(i);
+        const int hk = x.h / p.G;
+        for (int u = 0; u < x.n; ++u, ++g) {
+          const int row = (u < x.ns ? u : u + x.shift) * kT;
+          const int l = g % kLong, sh = g % kShort;
+          if (!wait_or_abort(&bar[kBarLE + l], (uint32_t)(((g / kLong) & 1) ^ 1), dead, p.err)) break;
+          mbar_expect_tx(&bar[kBarLF + l], LY::kTile);
+          load_tile<D>(smem + LY::kOffLong + l * LY::kTile, &p.tm_k, row, hk, x.b, &bar[kBarLF + l]);
+          if (!wait_or_abort(&bar[kBarSE + sh], (uint32_t)(((g / kShort) & 1) ^ 1), dead, p.err)) break;
+          mbar_expect_tx(&bar[kBarSF + sh], LY::kTile);
+          load_tile<D>(smem + LY::kOffShort + sh * LY::kTile, &p.tm_v, row, hk, x.b, &bar[kBarSF + sh]);
+          if (u == 0) {  // the item's Q and dO once the previous item's last scores have run
+            if (!wait_or_abort(&bar[kBarAE], (uint32_t)((it & 1) ^ 1), dead, p.err)) break;
+            mbar_expect_tx(&bar[kBarA], 2 * LY::kTile);
+            load_tile<D>(smem + LY::kOffA, &p.tm_q, x.qt * kT, x.h, x.b, &bar[kBarA]);
+            load_tile<D>(smem + LY::kOffB, &p.tm_do, x.qt * kT, x.h, x.b, &bar[kBarA]);
+          }
+        }
       }
     }
   } else if (warp == 1) {
     if (lane == 0) {
       const uint32_t q = smem_u32(smem + LY::kOffA), dout = smem_u32(smem + LY::kOffB);
-      auto k_at = [&](int u) { return smem_u32(smem + LY::kOffLong + (u % kLong) * LY::kTile); };
-      auto scores = [&](int u) -> bool {  // S(u) into buffer u % 2: dS(u - 2) has been formed from it
-        if (!wait_or_abort(&bar[kBarLF + u % kLong], (uint32_t)((u / kLong) & 1), dead, p.err)) return false;
+      auto k_at = [&](int g) { return smem_u32(smem + LY::kOffLong + (g % kLong) * LY::kTile); };
+      auto scores = [&](int g) -> bool {  // S(g) into buffer g % 2: dS(g - 2) has been formed from it
+        if (!wait_or_abort(&bar[kBarLF + g % kLong], (uint32_t)((g / kLong) & 1), dead, p.err)) return false;
         tc_fence_after();
-        issue_scores<D>(tmem + 128 * (u & 1), q, k_at(u));
-        umma_commit(&bar[kBarS + (u & 1)]);
+        issue_scores<D>(tmem + 128 * (g & 1), q, k_at(g));
+        umma_commit(&bar[kBarS + (g & 1)]);
         return true;
       };
-      auto dscores = [&](int u) -> bool {  // dP(u), over dS(u - 1) which dQ has read
-        if (!wait_or_abort(&bar[kBarSF + u % kShort], (uint32_t)((u / kShort) & 1), dead, p.err)) return false;
+      auto dscores = [&](int g) -> bool {  // dP(g), over dS(g - 1) which dQ has read
+        if (!wait_or_abort(&bar[kBarSF + g % kShort], (uint32_t)((g / kShort) & 1), dead, p.err)) return false;
         tc_fence_after();
-        issue_scores<D>(tmem + 256, dout, smem_u32(smem + LY::kOffShort + (u % kShort) * LY::kTile));
+        issue_scores<D>(tmem + 256, dout, smem_u32(smem + LY::kOffShort + (g % kShort) * LY::kTile));
         umma_commit(&bar[kBarDP]);
-        umma_commit(&bar[kBarSE + u % kShort]);  // V(u): its only use
+        umma_commit(&bar[kBarSE + g % kShort]);  // V(g): its only use
         return true;
       };
-      if (wait_or_abort(&bar[kBarA], 0, dead, p.err) && scores(0) && dscores(0) && (n == 1 || scores(1))) {
-        for (int u = 0; u < n; ++u) {
-          if (!wait_or_abort(&bar[kBarDS], (uint32_t)(u & 1), dead, p.err)) break;
+      int g = 0, it = 0;
+      for (int i = blockIdx.x; i < n_items && !dead; i += gridDim.x, ++it) {
+        const Item x = decode(i);
+        if (!wait_or_abort(&bar[kBarA], (uint32_t)(it & 1), dead, p.err) || !scores(g) || !dscores(g)) break;
+        if (x.n == 1) umma_commit(&bar[kBarAE]);
+        if (x.n > 1 && !scores(g + 1)) break;
+        for (int u = 0; u < x.n; ++u, ++g) {
+          if (!wait_or_abort(&bar[kBarDS], (uint32_t)(g & 1), dead, p.err)) break;
+          // the first product of an item overwrites dQ: the previous one has been read out
+          if (u == 0 && it > 0 && !wait_or_abort(&bar[kBarDrain], (uint32_t)((it - 1) & 1), dead, p.err)) break;
           tc_fence_after();
-          issue_accumulate<D>(tmem + 384, tmem + 256, k_at(u), u == 0);
-          umma_commit(&bar[kBarLE + u % kLong]);
-          if (u + 1 < n && !dscores(u + 1)) break;
-          if (u + 2 < n && !scores(u + 2)) break;
+          issue_accumulate<D>(tmem + 384, tmem + 256, k_at(g), u == 0);
+          umma_commit(&bar[kBarLE + g % kLong]);
+          if (u + 1 < x.n && !dscores(g + 1)) break;
+          if (u + 2 == x.n) umma_commit(&bar[kBarAE]);  // the item's last scores are issued: Q and dO are free then
+          if (u + 2 < x.n && !scores(g + 2)) break;
         }
+        if (dead) break;
+        umma_commit(&bar[kBarAcc]);
       }
-      umma_commit(&bar[kBarAcc]);
     }
   } else {
     const int sw = warp - 2, cg = sw >> 2, quarter = warp & 3;
-    const int row = quarter * 32 + lane, q = qt * kT + row;
+    const int row = quarter * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
     const float sl2 = p.scale_log2;
-    const int64_t r = ((int64_t)b * p.H + h) * p.S + q;
-    const bool in = q < p.S;
-    const float nl = in ? -__ldg(p.lse + r) * kLog2e : 0.f, di = in ? __ldg(p.di + r) : 0.f;
-    for (int u = 0; u < n; ++u) {
-      const int k0 = (u < ns ? u : u + shift) * kT + 32 * cg;
-      // visible keys of this row among the warp's 32: k <= q without [n_sink, q - window + 1)
-      const uint32_t mask = in ? below(q + 1 - k0) & (below(p.n_sink - k0) | ~below(q - p.window + 1 - k0)) : 0u;
-      const bool full = __all_sync(0xffffffffu, mask == 0xFFFFFFFFu);
-      bool ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarS + (u & 1)], (uint32_t)((u >> 1) & 1), dead, p.err));
-      if (!ok) dead = true;
+    int g = 0, it = 0;
+    for (int i = blockIdx.x; i < n_items; i += gridDim.x, ++it) {
+      const Item x = decode(i);
+      const int q = x.qt * kT + row;
+      const int64_t r = ((int64_t)x.b * p.H + x.h) * p.S + q;
+      const bool in = q < p.S;
+      const float nl = in ? -__ldg(p.lse + r) * kLog2e : 0.f, di = in ? __ldcg(p.di + r) : 0.f;
+      for (int u = 0; u < x.n; ++u, ++g) {
+        const int k0 = (u < x.ns ? u : u + x.shift) * kT + 32 * cg;
+        // visible keys of this row among the warp's 32: k <= q without [n_sink, q - window + 1)
+        const uint32_t mask = in ? below(q + 1 - k0) & (below(p.n_sink - k0) | ~below(q - p.window + 1 - k0)) : 0u;
+        const bool full = __all_sync(0xffffffffu, mask == 0xFFFFFFFFu);
+        bool ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarS + (g & 1)], (uint32_t)((g >> 1) & 1), dead, p.err));
+        if (!ok) dead = true;
+        tc_fence_after();
+        float pv[32];
+        if (ok) {
+          tmem_ld32(tmem + lane_base + 128 * (g & 1) + 32 * cg, pv);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            ffma2(pv[c], pv[c + 1], pv[c], pv[c + 1], sl2, nl);
+            pv[c] = fast_exp2(pv[c]);
+            pv[c + 1] = fast_exp2(pv[c + 1]);
+          }
+          if (!full) {
+#pragma unroll
+            for (int c = 0; c < 32; ++c) pv[c] = (mask >> c) & 1u ? pv[c] : 0.f;
+          }
+        }
+        ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarDP], (uint32_t)(g & 1), dead, p.err));
+        if (!ok) dead = true;
+        tc_fence_after();
+        if (ok) {
+          float dp[32];
+          uint32_t w[16];
+          tmem_ld32(tmem + lane_base + 256 + 32 * cg, dp);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            sub_mul_pair(dp[c], dp[c + 1], dp[c], dp[c + 1], di, di, pv[c], pv[c + 1]);
+            w[c / 2] = pack_bf16x2(dp[c], dp[c + 1]);
+          }
+          tmem_st16(tmem + lane_base + 256 + 32 * cg, w);
+          tmem_wait_st();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&bar[kBarDS]);
+      }
+      if (!__all_sync(0xffffffffu, wait_or_abort(&bar[kBarAcc], (uint32_t)(it & 1), dead, p.err))) dead = true;
       tc_fence_after();
-      float pv[32];
-      if (ok) {
-        tmem_ld32(tmem + lane_base + 128 * (u & 1) + 32 * cg, pv);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          ffma2(pv[c], pv[c + 1], pv[c], pv[c + 1], sl2, nl);
-          pv[c] = fast_exp2(pv[c]);
-          pv[c + 1] = fast_exp2(pv[c + 1]);
-        }
-        if (!full) {
-#pragma unroll
-          for (int c = 0; c < 32; ++c) pv[c] = (mask >> c) & 1u ? pv[c] : 0.f;
-        }
-      }
-      ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarDP], (uint32_t)(u & 1), dead, p.err));
-      if (!ok) dead = true;
-      tc_fence_after();
-      uint32_t w[16];
-      if (ok) {
-        float dp[32];
-        tmem_ld32(tmem + lane_base + 256 + 32 * cg, dp);
-        tmem_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          sub_mul_pair(dp[c], dp[c + 1], dp[c], dp[c + 1], di, di, pv[c], pv[c + 1]);
-          w[c / 2] = pack_bf16x2(dp[c], dp[c + 1]);
-        }
-      }
-      if (ok) {
-        tmem_st16(tmem + lane_base + 256 + 32 * cg, w);
-        tmem_wait_st();
-      }
+      // this warp's D / 4 columns of its rows
+      __nv_bfloat16* out = p.dq + (int64_t)x.b * p.dq_sb + (int64_t)x.h * p.dq_sh + (int64_t)q * p.dq_ss + cg * (D / 4);
+      float t[32];
+      tmem_ld32(tmem + lane_base + 384 + cg * (D / 4), t);  // D 64: the upper 16 columns are not this warp's
+      tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_one(&bar[kBarDS]);
-    }
-    if (!__all_sync(0xffffffffu, wait_or_abort(&bar[kBarAcc], 0, dead, p.err))) dead = true;
-    tc_fence_after();
-    // this warp's D / 4 columns of its rows
-    __nv_bfloat16* out = p.dq + (int64_t)b * p.dq_sb + (int64_t)h * p.dq_sh + (int64_t)q * p.dq_ss + cg * (D / 4);
-    float t[32];
-    tmem_ld32(tmem + lane_base + 384 + cg * (D / 4), t);  // D 64: the upper 16 columns are the next group's
-    tmem_wait_ld();
-    if (in && !dead) {
+      if (lane == 0) mbar_arrive_one(&bar[kBarDrain]);
+      if (in && !dead) {
 #pragma unroll
-      for (int v8 = 0; v8 < D / 32; ++v8) {
-        uint4 pk;
-        pk.x = pack_bf16x2(t[v8 * 8 + 0] * p.scale, t[v8 * 8 + 1] * p.scale);
-        pk.y = pack_bf16x2(t[v8 * 8 + 2] * p.scale, t[v8 * 8 + 3] * p.scale);
-        pk.z = pack_bf16x2(t[v8 * 8 + 4] * p.scale, t[v8 * 8 + 5] * p.scale);
-        pk.w = pack_bf16x2(t[v8 * 8 + 6] * p.scale, t[v8 * 8 + 7] * p.scale);
-        *reinterpret_cast<uint4*>(out + v8 * 8) = pk;
+        for (int v8 = 0; v8 < D / 32; ++v8) {
+          uint4 pk;
+          pk.x = pack_bf16x2(t[v8 * 8 + 0] * p.scale, t[v8 * 8 + 1] * p.scale);
+          pk.y = pack_bf16x2(t[v8 * 8 + 2] * p.scale, t[v8 * 8 + 3] * p.scale);
+          pk.z = pack_bf16x2(t[v8 * 8 + 4] * p.scale, t[v8 * 8 + 5] * p.scale);
+          pk.w = pack_bf16x2(t[v8 * 8 + 6] * p.scale, t[v8 * 8 + 7] * p.scale);
+          *reinterpret_cast<uint4*>(out + v8 * 8) = pk;
+        }
       }
     }
   }
@@ -563,8 +686,10 @@ template <int D>
 __global__ void __launch_bounds__(256) window_rowdot_kernel(const __nv_bfloat16* __restrict__ o, int64_t o_sb,
                                                             int64_t o_sh, int64_t o_ss, const int8_t* __restrict__ lo,
                                                             const __nv_bfloat16* __restrict__ dout, int64_t d_sb,
-                                                            int64_t d_sh, int64_t d_ss, float* di, int B, int H, int S) {
+                                                            int64_t d_sh, int64_t d_ss, float* di, int32_t* work, int B,
+                                                            int H, int S) {
   constexpr int kL = D / 8;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *work = 0;  // the dK/dV launch's item counter
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int64_t r = i / kL;
   const int d0 = (int)(i % kL) * 8;
@@ -609,49 +734,62 @@ constexpr size_t kWsHeader = 256;
 constexpr int kSms = 148;
 
 template <int D>
-int launch(const WinBwdParams& prm, const void* out, const int64_t* os, const int8_t* lo, const void* dout,
+int launch(WinBwdParams& prm, const void* out, const int64_t* os, const int8_t* lo, const void* dout,
            const int64_t* ds, float* di, cudaStream_t s) {
   const int64_t threads = (int64_t)prm.B * prm.H * prm.S * (D / 8);
   window_rowdot_kernel<D><<<(unsigned)((threads + 255) / 256), 256, 0, s>>>(
       static_cast<const __nv_bfloat16*>(out), os[0], os[1], os[2], lo, static_cast<const __nv_bfloat16*>(dout), ds[0],
-      ds[1], ds[2], di, prm.B, prm.H, prm.S);
+      ds[1], ds[2], di, prm.work, prm.B, prm.H, prm.S);
   if (cudaFuncSetAttribute(window_dkdv_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::kSmem) !=
           cudaSuccess ||
       cudaFuncSetAttribute(window_dq_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::kSmem) !=
           cudaSuccess)
     return ABKV_ERR_CUDA;
+  // Each kernel may be set up while the one before it drains; the last ones run beside one another.
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(prm.Hkv * prm.cluster, prm.B, prm.n_tiles);
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = Lay<D>::kSmem;
   cfg.stream = s;
-  // Each kernel may be set up while the one before it drains.  dQ waits for dK/dV at its end only: every CTA
-  // of dK/dV has passed the row sums and is running (or done) before one of dQ's starts.
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim = {(unsigned)prm.cluster, 1, 1};
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  if (cudaLaunchKernelEx(&cfg, window_dkdv_kernel<D>, prm) != cudaSuccess) return ABKV_ERR_CUDA;
-  cfg.gridDim = dim3(prm.H, prm.B, prm.n_tiles);
+  auto dkdv = [&](int tile0, int tiles, int cluster, bool first) -> bool {
+    prm.tile0 = tile0;
+    prm.tiles = tiles;
+    prm.cluster = cluster;
+    prm.first = first ? 1 : 0;
+    const int64_t items = (int64_t)prm.Hkv * prm.B * tiles;
+    attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
+    cfg.gridDim = dim3((unsigned)(cluster > 1 ? items * cluster : std::min<int64_t>(items, kSms)));
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, window_dkdv_kernel<D>, prm) == cudaSuccess;
+  };
+  // Key tiles as (sinks', others), pairs per tile and in all.
+  const int64_t heads = (int64_t)prm.Hkv * prm.B;
+  const int sink_tiles = std::min(prm.n_tiles, (prm.n_sink + kT - 1) / kT);
+  const int64_t most = (int64_t)prm.n_tiles * prm.G;
+  const int64_t usual = (int64_t)std::min(prm.n_tiles, (prm.window + kT - 2) / kT + 1) * prm.G;
+  const int64_t share = heads * (sink_tiles * most + (prm.n_tiles - sink_tiles) * usual) / kSms;  // pairs per SM
+  if (heads * prm.n_tiles * 2 <= kSms) {
+    // few key tiles: a cluster of CTAs for each, up to one CTA per SM
+    const int64_t pairs = sink_tiles ? most : usual;
+    int cs = 1;
+    while (cs < 8 && pairs >= 2 * cs && heads * prm.n_tiles * 2 * cs <= kSms) cs *= 2;
+    if (!dkdv(0, prm.n_tiles, cs, true)) return ABKV_ERR_CUDA;
+  } else if (sink_tiles && sink_tiles < prm.n_tiles && 10 * most > 11 * share) {
+    // the sinks' tiles would outlast the rest: clusters for them, beside the others
+    int cs = 2;
+    while (cs < 8 && most > cs * std::max(usual, share / 2)) cs *= 2;
+    if (!dkdv(0, sink_tiles, cs, true) || !dkdv(sink_tiles, prm.n_tiles - sink_tiles, 1, false)) return ABKV_ERR_CUDA;
+  } else {
+    if (!dkdv(0, prm.n_tiles, 1, true)) return ABKV_ERR_CUDA;
+  }
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>((int64_t)prm.H * prm.B * prm.n_tiles, kSms));
   cfg.numAttrs = 1;
   if (cudaLaunchKernelEx(&cfg, window_dq_kernel<D>, prm) != cudaSuccess) return ABKV_ERR_CUDA;
   return cudaGetLastError() == cudaSuccess ? ABKV_OK : ABKV_ERR_CUDA;
-}
-
-// CTAs that share a key tile's pairs: while the launch leaves SMs idle, or the sinks' tile (which every query tile
-// sees) would outlast the rest of the launch.
-int pick_cluster(const WinBwdParams& p) {
-  const int64_t most = (int64_t)(p.n_sink > 0 ? p.n_tiles : std::min(p.n_tiles, (p.window + kT - 2) / kT + 1)) * p.G;
-  const int64_t usual = (int64_t)std::min(p.n_tiles, (p.window + kT - 2) / kT + 1) * p.G;
-  const int64_t ctas = (int64_t)p.n_tiles * p.Hkv * p.B;
-  int cs = 1;
-  while (cs < 8 && most >= 2 * cs &&
-         (ctas * 2 * cs <= kSms || 4 * most > 5 * cs * std::max<int64_t>(usual, ctas * usual / kSms)))
-    cs *= 2;
-  return cs;
 }
 
 }  // namespace
@@ -712,6 +850,7 @@ extern "C" int abkv_window_attention_backward(
   prm.dv_sh = dv_strides[1];
   prm.dv_ss = dv_strides[2];
   prm.err = static_cast<int32_t*>(workspace);
+  prm.work = static_cast<int32_t*>(workspace) + 32;  // inside the header
   prm.B = B;
   prm.H = H;
   prm.Hkv = Hkv;
@@ -723,7 +862,6 @@ extern "C" int abkv_window_attention_backward(
   // a window past S hides nothing, sinks past S are every key: keep the tile arithmetic in 32 bits
   prm.window = window < S ? window : S;
   prm.n_sink = num_sinks < S ? num_sinks : S;
-  prm.cluster = pick_cluster(prm);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int8_t* lo = static_cast<const int8_t*>(out_lo);
   return head_dim == 64 ? launch<64>(prm, out, out_strides, lo, dout, dout_strides, di, s)
