@@ -12,15 +12,16 @@
 // cache rows, so the sum over queries is a sum over a thread's own registers, no reduction across lanes
 // and no second product.  The 128 columns are 4 units of 32 consecutive query rows of one head (so a
 // group of 4 heads x 32 observed rows is one full tile).  19 warps:
-//   warp 0      K tiles (eight 16-row page slices, 2-stage ring) by cp.async.bulk.tensor, 128B swizzle
-//   warp 18     Q tiles (four 32-row boxes, 4-stage ring); where every counted row of a request fits one
-//               tile, it is loaded once for all cache tiles of a (request, head) run
+//   warp 0      K tiles (eight 16-row page slices) by cp.async.bulk.tensor, 128B swizzle
+//   warp 18     Q tiles (four 32-row boxes); where every counted row of a request fits one
+//               tile, it is loaded once for all cache tiles of a (request, head) run, and the six ring slots go to K
+//               (4) rather than Q (4 otherwise)
 //   warp 1      TMEM owner (4 S^T buffers) and issuer of tcgen05.mma
-//   warps 2..17 thread = one cache row and one unit's 32 columns: x = S scale log2(e) - lse log2(e), 2^x, sum
+//   warps 2..17 thread = one cache row of every fourth step: x = S scale log2(e) - lse log2(e), 2^x, sum
 // The exponentials bound it: 128 x 128 of them take 1024 clocks of the SM's 16 a clock, the tile's MMAs
 // 256 (head_dim 128).  Work items are (cache tile, KV head, request); a CTA per SM takes them round
-// robin, the cache tiles that the most rows see first -- or, where Q stays resident, a contiguous run.
-// The sum's order is fixed (units, then the four column groups), so results repeat bit for bit.
+// robin to and fro, the cache tiles that the most rows see first -- or, where Q stays resident, a contiguous run.
+// The sum's order is fixed (steps, then the four warp groups), so results repeat bit for bit.
 // With one accumulator row for all heads, per-head sums go through the workspace and are added in head order.
 // Every mbarrier wait is bounded and records ABKV_DEVERR_TIMEOUT on expiry.
 #include <algorithm>
@@ -36,16 +37,21 @@ constexpr int kM = 128, kN = 128, kD = 128;  // cache rows, query columns, head_
 constexpr int kUnit = 32;                    // query rows of a unit
 constexpr int kThreads = 608;
 constexpr int kWarpQ = 18;
-constexpr int kKStages = 2, kQStages = 4, kSBufs = 4;
+constexpr int kStages = 6, kSBufs = 4;  // 32 KiB ring slots, shared out between K and Q
+__host__ __device__ constexpr int k_stages(bool resident) { return resident ? 4 : 2; }
+__host__ __device__ constexpr int q_stages(bool resident) { return kStages - k_stages(resident); }
+constexpr int kMaxK = 4, kMaxQ = 4;
 constexpr uint32_t kIdescS = idesc_bf16_m128(kN, false);
 constexpr int kTileBytes = kM * kD * 2;  // 2 atoms of [128 rows][128 B]
 constexpr int kOffK = 0;
-constexpr int kOffQ = kOffK + kKStages * kTileBytes;
-constexpr int kOffLse = kOffQ + kQStages * kTileBytes;  // 16 warps x 32 floats
-constexpr int kOffAcc = kOffLse + 16 * 32 * 4;          // [2 items][4 column groups][128 rows] partial sums
-constexpr int kOffBar = kOffAcc + 2 * 4 * kM * 4;
-constexpr int kBarKFull = 0, kBarKEmpty = kBarKFull + kKStages, kBarQFull = kBarKEmpty + kKStages,
-              kBarQEmpty = kBarQFull + kQStages, kBarSFull = kBarQEmpty + kQStages, kBarSEmpty = kBarSFull + kSBufs,
+constexpr int kOffLse = kOffK + kStages * kTileBytes;   // 16 warps x [128] floats
+constexpr int kOffAcc = kOffLse + 16 * kN * 4;          // [2 items][4 groups][128 rows] partial sums
+constexpr int kMaxPref = 1024;
+constexpr int kOffPref = kOffAcc + 2 * 4 * kM * 4;      // [R + 1] running tile counts
+constexpr int kOffBar = kOffPref + (kMaxPref + 2) * 4;
+static_assert(kOffBar % 8 == 0, "barriers");
+constexpr int kBarKFull = 0, kBarKEmpty = kBarKFull + kMaxK, kBarQFull = kBarKEmpty + kMaxK,
+              kBarQEmpty = kBarQFull + kMaxQ, kBarSFull = kBarQEmpty + kMaxQ, kBarSEmpty = kBarSFull + kSBufs,
               kBarTmem = kBarSEmpty + kSBufs;
 constexpr int kSmemBytes = kOffBar + 8 * (kBarTmem + 1) + 1024;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory");
@@ -123,37 +129,63 @@ __device__ __forceinline__ void item_units(const PromptParams& p, const Req& x, 
   u1 = resident ? chunks * p.G : c1 * p.G;
 }
 
-// Item sequence of a CTA; resident: Q of a whole request fits one tile (same answer for every request,
-// from the host's bound on the counted rows).
+// Item sequence of a CTA; resident: every request's counted rows fit one Q tile (by the host's bound on them).
 struct Items {
-  int i, end, step;
+  int first, n;         // items k = 0 .. n - 1 of this CTA
+  const int32_t* pref;  // resident: [R + 1] visible cache tiles of the requests before, in shared memory
 };
-__device__ __forceinline__ Items my_items(const PromptParams& p, bool resident) {
-  Items t;
-  if (resident) {  // contiguous: (request, head) outermost
-    const int per = (p.n_items + (int)gridDim.x - 1) / (int)gridDim.x;
-    t.i = min(p.n_items, (int)blockIdx.x * per);
-    t.end = min(p.n_items, t.i + per);
-    t.step = 1;
-  } else {
-    t.i = blockIdx.x;
-    t.end = p.n_items;
-    t.step = gridDim.x;
-  }
+// The visible cache tiles of a request: tile v of `count` is cache tile v < ns ? v : v + shift.
+struct Tiles {
+  int ns, shift, count;
+};
+__device__ __forceinline__ Tiles req_tiles(const PromptParams& p, const Req& x) {
+  Tiles t;
+  const int lo = p.window > 0 ? max(0, x.p0 - p.window + 1) : 0;
+  t.ns = (min(p.n_sink, lo) + kM - 1) / kM;
+  t.shift = max(lo / kM - t.ns, 0);
+  t.count = x.nq > 0 ? (x.n + kM - 1) / kM - t.shift : 0;
   return t;
 }
-__device__ __forceinline__ void item_at(const PromptParams& p, bool resident, int i, int& r, int& hk, int& kt) {
-  const int rh = p.R * p.Hkv;
-  int g;
-  if (resident) {
-    g = i / p.max_tiles;
-    kt = i - g * p.max_tiles;
-  } else {
-    kt = i / rh;
-    g = i - kt * rh;
+// k-th item of this CTA -> false past the end.  Resident: every item is one tile of work, a contiguous run of the
+// requests' visible tiles, (request, head) outermost.  Else the cache tiles in order (under causality the first see
+// the most rows), dealt out to and fro so that the CTAs' shares of long and short items come out alike.
+__device__ __forceinline__ bool item_at(const PromptParams& p, const Items& it, int k, int& r, int& hk, int& kt) {
+  if (it.pref) {
+    int i = it.first + k;
+    if (k >= it.n) return false;
+    int lo = 0, hi = p.R;  // pref[lo] * Hkv <= i < pref[hi] * Hkv
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (it.pref[mid] * p.Hkv <= i)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    r = lo;
+    i -= it.pref[r] * p.Hkv;
+    const int count = it.pref[r + 1] - it.pref[r];
+    hk = i / count;
+    const Tiles t = req_tiles(p, load_req(p, r, false));
+    const int v = i - hk * count;
+    kt = v < t.ns ? v : v + t.shift;
+    return true;
   }
+  const int rh = p.R * p.Hkv;
+  const int i = k * (int)gridDim.x + ((k & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x);
+  if (i >= p.n_items) return false;
+  kt = i / rh;
+  const int g = i - kt * rh;
   r = g / p.Hkv;
   hk = g - r * p.Hkv;
+  return true;
+}
+
+// a * b + c on a pair with one b.
+__device__ __forceinline__ void scale_add(float& d0, float& d1, float a0, float a1, float b, float c0, float c1) {
+  asm("{\n .reg .b64 x, y, z, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mov.b64 z, {%5, %6};\n"
+      " fma.rn.f32x2 r, x, y, z;\n mov.b64 {%0, %1}, r;\n}\n"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b), "f"(c0), "f"(c1));
 }
 
 __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __grid_constant__ PromptParams p) {
@@ -162,10 +194,27 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + kOffBar);
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar + kBarTmem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const bool resident = (int64_t)((most_rows(p) + kUnit - 1) / kUnit) * p.G <= kN / kUnit;
+  const bool resident = (int64_t)((most_rows(p) + kUnit - 1) / kUnit) * p.G <= kN / kUnit && p.R <= kMaxPref;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBarTmem; ++i) mbar_init(&bar[i], i >= kBarSEmpty ? 16 : 1);
+    for (int i = 0; i < kBarTmem; ++i) mbar_init(&bar[i], i >= kBarSEmpty ? 4 : 1);  // the four warps of a group
+  }
+  int32_t* s_pref = reinterpret_cast<int32_t*>(smem + kOffPref);
+  if (resident && warp == 2) {  // running count of the requests' visible tiles
+    int run = 0;
+    for (int r0 = 0; r0 < p.R; r0 += 32) {
+      int v = 0;
+      if (r0 + lane < p.R) v = req_tiles(p, load_req(p, r0 + lane, blockIdx.x == 0)).count;
+      int incl = v;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += o;
+      }
+      if (r0 + lane < p.R) s_pref[r0 + lane + 1] = run + incl;
+      run += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) s_pref[0] = 0;
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(s_tmem)),
@@ -177,53 +226,76 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
   bool dead = false;
-  const Items it = my_items(p, resident);
+  Items it;
+  it.pref = nullptr;
+  it.first = 0;
+  it.n = (p.n_items + (int)gridDim.x - 1) / (int)gridDim.x;  // the last one may be past the end
+  if (resident) {
+    const int total = s_pref[p.R] * p.Hkv, per = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+    it.pref = s_pref;
+    it.first = blockIdx.x * per;
+    it.n = max(0, min(per, total - it.first));
+  }
+  const int kKStages = k_stages(resident), kQStages = q_stages(resident);
+  uint8_t* const s_k = smem + kOffK;
+  uint8_t* const s_q = smem + kOffK + kKStages * kTileBytes;
 
   if (warp == 0) {
-    // ---------------- K producer: lane i < 8 owns 16-row slice i ----------------
+    // ---------------- K producer: four items at a time, lane = 8 x item + 16-row slice, so that the
+    // look-ups of four items (request, page) are under way together ----------------
     int kc = 0;
-    for (int i = it.i; i < it.end && !dead; i += it.step) {
-      int r, hk, kt, u0, u1;
-      item_at(p, resident, i, r, hk, kt);
-      const Req x = load_req(p, r, kt == 0 && hk == 0 && lane == 0);
-      item_units(p, x, kt, resident, u0, u1);
-      if (u0 >= u1) continue;
-      const int row0 = kt * kM + 16 * lane;
-      int pg = -1;
-      if (lane < 8 && row0 < x.n) {
-        // a slice hidden from every counted row is not looked up: its page may be freed
-        const bool hidden = p.window > 0 && row0 >= p.n_sink && row0 + 16 <= x.p0 - p.window + 1;
-        if (!hidden) {
-          pg = __ldg(p.bt + (int64_t)r * p.bt_stride + row0 / p.page);
-          if (pg < 0 || (int64_t)pg >= p.num_blocks) {
-            set_error(p.err, ABKV_DEVERR_PAGE_OOB);
-            pg = -1;
+    for (int base = 0; base < it.n && !dead; base += 4) {
+      const int k = base + (lane >> 3), slice = lane & 7;
+      int pg = -1, hk = 0, off = 0;
+      bool busy = false;  // the item has work
+      int r, kt, u0, u1;
+      if (k < it.n && item_at(p, it, k, r, hk, kt)) {
+        const Req x = load_req(p, r, !resident && kt == 0 && hk == 0 && slice == 0);
+        item_units(p, x, kt, resident, u0, u1);
+        busy = u0 < u1;
+        const int row0 = kt * kM + 16 * slice;
+        if (busy && row0 < x.n) {
+          // a slice hidden from every counted row is not looked up: its page may be freed
+          const bool hidden = p.window > 0 && row0 >= p.n_sink && row0 + 16 <= x.p0 - p.window + 1;
+          if (!hidden) {
+            pg = __ldg(p.bt + (int64_t)r * p.bt_stride + row0 / p.page);
+            off = row0 % p.page;
+            if (pg < 0 || (int64_t)pg >= p.num_blocks) {
+              set_error(p.err, ABKV_DEVERR_PAGE_OOB);
+              pg = -1;
+            }
           }
         }
       }
-      const int st = kc % kKStages;
-      const uint32_t valid = __ballot_sync(0xffffffffu, pg >= 0);
-      bool ok = true;
-      if (lane == 0) {
-        ok = wait_or_abort(&bar[kBarKEmpty + st], (uint32_t)(((kc / kKStages) & 1) ^ 1), dead, p.err);
-        if (ok) mbar_expect_tx(&bar[kBarKFull + st], (uint32_t)__popc(valid) * 2u * 2048u);
+      const uint32_t valid = __ballot_sync(0xffffffffu, pg >= 0), work = __ballot_sync(0xffffffffu, busy);
+      for (int j = 0; j < 4; ++j) {
+        if (!((work >> (8 * j)) & 1u)) continue;
+        const int st = kc % kKStages;
+        bool ok = true;
+        if (lane == 0) {
+          ok = wait_or_abort(&bar[kBarKEmpty + st], (uint32_t)(((kc / kKStages) & 1) ^ 1), dead, p.err);
+          if (ok) mbar_expect_tx(&bar[kBarKFull + st], (uint32_t)__popc((valid >> (8 * j)) & 0xFFu) * 2u * 2048u);
+        }
+        if (!__shfl_sync(0xffffffffu, ok, 0)) {
+          dead = true;
+          break;
+        }
+        if ((lane >> 3) == j && pg >= 0) {
+          uint8_t* kb = s_k + st * kTileBytes + slice * 2048;
+          const int plane = p.fa_layout ? pg : 2 * pg;
+          tma_load_4d(kb, &p.tm_k, 0, hk, off, plane, &bar[kBarKFull + st]);
+          tma_load_4d(kb + kTileBytes / 2, &p.tm_k, 64, hk, off, plane, &bar[kBarKFull + st]);
+        }
+        ++kc;
       }
-      if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-      if (pg >= 0) {
-        uint8_t* kb = smem + kOffK + st * kTileBytes + lane * 2048;
-        const int plane = p.fa_layout ? pg : 2 * pg;
-        tma_load_4d(kb, &p.tm_k, 0, hk, row0 % p.page, plane, &bar[kBarKFull + st]);
-        tma_load_4d(kb + kTileBytes / 2, &p.tm_k, 64, hk, row0 % p.page, plane, &bar[kBarKFull + st]);
-      }
-      ++kc;
     }
   } else if (warp == kWarpQ) {
     // ---------------- Q producer ----------------
     if (lane == 0) {
       int qc = 0, last_g = -1;
-      for (int i = it.i; i < it.end && !dead; i += it.step) {
+      for (int k = 0; k < it.n && !dead; ++k) {
         int r, hk, kt, u0, u1;
-        item_at(p, resident, i, r, hk, kt);
+        if (!item_at(p, it, k, r, hk, kt)) break;
         const Req x = load_req(p, r, false);
         item_units(p, x, kt, resident, u0, u1);
         if (u0 >= u1) continue;
@@ -235,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
           mbar_expect_tx(&bar[kBarQFull + st], (uint32_t)nu * 2u * 4096u);
           for (int c = 0; c < nu; ++c) {
             const int chunk = (u + c) / p.G, h = hk * p.G + (u + c) % p.G;
-            uint8_t* qb = smem + kOffQ + st * kTileBytes + c * 4096;
+            uint8_t* qb = s_q + st * kTileBytes + c * 4096;
             tma_load_4d(qb, &p.tm_q, 0, h, x.q0 + chunk * kUnit, 0, &bar[kBarQFull + st]);
             tma_load_4d(qb + kTileBytes / 2, &p.tm_q, 64, h, x.q0 + chunk * kUnit, 0, &bar[kBarQFull + st]);
           }
@@ -246,15 +318,15 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
     // ---------------- MMA issuer ----------------
     if (lane == 0) {
       int kc = 0, qc = 0, sc = 0, last_g = -1;
-      for (int i = it.i; i < it.end && !dead; i += it.step) {
+      for (int k = 0; k < it.n && !dead; ++k) {
         int r, hk, kt, u0, u1;
-        item_at(p, resident, i, r, hk, kt);
+        if (!item_at(p, it, k, r, hk, kt)) break;
         const Req x = load_req(p, r, false);
         item_units(p, x, kt, resident, u0, u1);
         if (u0 >= u1) continue;
         const int ks = kc % kKStages;
         if (!wait_or_abort(&bar[kBarKFull + ks], (uint32_t)((kc / kKStages) & 1), dead, p.err)) break;
-        const uint64_t dk = desc_kmajor_sw128(smem_u32(smem + kOffK + ks * kTileBytes));
+        const uint64_t dk = desc_kmajor_sw128(smem_u32(s_k + ks * kTileBytes));
         const bool fresh = !resident || last_g != r * p.Hkv + hk;
         if (resident && fresh && last_g >= 0) {
           umma_commit(&bar[kBarQEmpty + qc % kQStages]);  // the previous run's Q tile
@@ -266,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
           if (fresh && !wait_or_abort(&bar[kBarQFull + qs], (uint32_t)((qc / kQStages) & 1), dead, p.err)) break;
           if (!wait_or_abort(&bar[kBarSEmpty + sb], (uint32_t)(((sc / kSBufs) & 1) ^ 1), dead, p.err)) break;
           tc_fence_after();
-          const uint64_t dq = desc_kmajor_sw128(smem_u32(smem + kOffQ + qs * kTileBytes));
+          const uint64_t dq = desc_kmajor_sw128(smem_u32(s_q + qs * kTileBytes));
 #pragma unroll
           for (int kk = 0; kk < kD / 16; ++kk) {
             const uint32_t off = (kk >> 2) * (kTileBytes / 2) + (kk & 3) * 32;
@@ -284,79 +356,115 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
       }
     }
   } else {
-    // ---------------- exponentials and sums: lane = cache row, warp group = unit of the tile ----------------
+    // ---------------- exponentials and sums: lane = cache row; group cg of four warps (one per lane quarter)
+    // takes every fourth step, all of its 128 columns, so that four steps are under way at a time ----------------
     const int sw = warp - 2, cg = sw >> 2, quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-    float* s_lse = reinterpret_cast<float*>(smem + kOffLse) + sw * 32;
+    float* s_lse = reinterpret_cast<float*>(smem + kOffLse) + sw * kN;  // this warp's: a step's 128 rows
     float* s_acc = reinterpret_cast<float*>(smem + kOffAcc);
     const float sl2 = p.scale_log2;
     int sc = 0, ic = 0;
-    for (int i = it.i; i < it.end; i += it.step) {
+    for (int k = 0; k < it.n; ++k) {
       int r, hk, kt, u0, u1;
-      item_at(p, resident, i, r, hk, kt);
+      if (!item_at(p, it, k, r, hk, kt)) break;
+      if (resident && (sc & 3) != cg) {  // one step, another group's
+        ++sc;
+        continue;
+      }
       const Req x = load_req(p, r, false);
       item_units(p, x, kt, resident, u0, u1);
       if (u0 >= u1) continue;
       const int key = kt * kM + row;
       float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int u = u0; u < u1; u += 4, ++sc) {
-        const int sb = sc % kSBufs, un = u + cg;
-        const bool live = un < u1;  // warp-uniform: the tile has this unit
-        const int chunk = un / p.G, h = hk * p.G + un % p.G;
-        if (live) {
+      // log-sum-exp (negated, log2 units) of a step's rows, lane = row of each of its four units
+      float n_lse[4];
+      auto fetch = [&](int u) {
+        int chunk = u / p.G, h = u - chunk * p.G;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
           const int t = min(x.q0 + chunk * kUnit + lane, p.T - 1);
-          s_lse[lane] = __ldg(p.lse + (int64_t)t * p.H + h) * 1.4426950408889634f;
+          n_lse[j] = u + j < u1 ? __ldg(p.lse + (int64_t)t * p.H + hk * p.G + h) * -1.4426950408889634f : 0.f;
+          if (++h == p.G) {
+            h = 0;
+            ++chunk;
+          }
         }
+      };
+      int mine = u0 + 4 * ((cg - sc) & 3);  // the group's first step of the item
+      if (mine < u1) fetch(mine);
+      for (int u = u0; u < u1; u += 4, ++sc) {
+        if (u != mine) continue;
+        const int sb = sc % kSBufs;
+        __syncwarp();  // every lane is past its reads of the previous step's values
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s_lse[32 * j + lane] = n_lse[j];
         __syncwarp();
+        mine += 16;
+        if (mine < u1) fetch(mine);
         const bool ok = __all_sync(0xffffffffu,
                                    wait_or_abort(&bar[kBarSFull + sb], (uint32_t)((sc / kSBufs) & 1), dead, p.err));
         if (!ok) dead = true;
         tc_fence_after();
-        if (ok && live) {
-          float s[32];
-          tmem_ld32(tmem + lane_base + 128 * sb + 32 * cg, s);
-          tmem_wait_ld();
-          tc_fence_before();
-          if (lane == 0) mbar_arrive_one(&bar[kBarSEmpty + sb]);  // the buffer's columns are in registers
-          // visible columns [a, e): rows at or past the key, inside its window, and counted
-          const int pc = x.p0 + chunk * kUnit;
-          const int a = max(key - pc, 0);
-          int e = min(kUnit, x.nq - chunk * kUnit);
-          if (p.window > 0 && key >= p.n_sink) e = (int)min((int64_t)e, (int64_t)key + p.window - pc);
-          const uint32_t mask = (a >= e || e <= 0) ? 0u : (0xFFFFFFFFu >> (32 - e)) & (0xFFFFFFFFu << a);
-          const bool full = __all_sync(0xffffffffu, mask == 0xFFFFFFFFu);
-          if (full) {
+        int chunk = u / p.G, h = u - chunk * p.G;
 #pragma unroll
-            for (int c = 0; c < 32; c += 4) {
-              const float4 l = *reinterpret_cast<const float4*>(s_lse + c);
-              acc[0] += fast_exp2(fmaf(s[c], sl2, -l.x));
-              acc[1] += fast_exp2(fmaf(s[c + 1], sl2, -l.y));
-              acc[2] += fast_exp2(fmaf(s[c + 2], sl2, -l.z));
-              acc[3] += fast_exp2(fmaf(s[c + 3], sl2, -l.w));
-            }
-          } else {
+        for (int j = 0; j < 4; ++j) {
+          if (ok && u + j < u1) {
+            float s[32];
+            tmem_ld32(tmem + lane_base + 128 * sb + 32 * j, s);
+            tmem_wait_ld();
+            // visible columns [a, e): rows at or past the key, inside its window, and counted
+            const int pc = x.p0 + chunk * kUnit;
+            const int a = max(key - pc, 0);
+            int e = min(kUnit, x.nq - chunk * kUnit);
+            if (p.window > 0 && key >= p.n_sink) e = (int)min((int64_t)e, (int64_t)key + p.window - pc);
+            const uint32_t mask = (a >= e || e <= 0) ? 0u : (0xFFFFFFFFu >> (32 - e)) & (0xFFFFFFFFu << a);
+            const bool full = __all_sync(0xffffffffu, mask == 0xFFFFFFFFu);
+            const float* l4 = s_lse + 32 * j;
+            if (full) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const float v = fast_exp2(fmaf(s[c], sl2, -s_lse[c]));
-              acc[c & 3] += (mask >> c) & 1u ? v : 0.f;
+              for (int c = 0; c < 32; c += 4) {
+                const float4 l = *reinterpret_cast<const float4*>(l4 + c);
+                float x0, x1, x2, x3;
+                scale_add(x0, x1, s[c], s[c + 1], sl2, l.x, l.y);
+                scale_add(x2, x3, s[c + 2], s[c + 3], sl2, l.z, l.w);
+                fadd2(acc[0], acc[1], fast_exp2(x0), fast_exp2(x1));
+                fadd2(acc[2], acc[3], fast_exp2(x2), fast_exp2(x3));
+              }
+            } else if (__any_sync(0xffffffffu, mask != 0u)) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c) {
+                const float v = fast_exp2(fmaf(s[c], sl2, l4[c]));
+                acc[c & 3] += (mask >> c) & 1u ? v : 0.f;
+              }
             }
           }
-        } else {
-          if (lane == 0) mbar_arrive_one(&bar[kBarSEmpty + sb]);
+          if (++h == p.G) {
+            h = 0;
+            ++chunk;
+          }
         }
-        __syncwarp();  // s_lse is rewritten by the next step
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&bar[kBarSEmpty + sb]);
       }
-      // the four column groups of a cache row, added in order
-      float* sa = s_acc + (ic & 1) * 4 * kM;
-      sa[cg * kM + row] = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-      named_bar_sync(1, 512);
-      if (cg == 0 && key < x.n && !dead) {
+      float add = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+      if (!resident) {
+        // the four groups' parts of a cache row, added in order
+        float* sa = s_acc + (ic & 1) * 4 * kM;
+        sa[cg * kM + row] = add;
+        named_bar_sync(1, 512);
+        add = (sa[row] + sa[kM + row]) + (sa[2 * kM + row] + sa[3 * kM + row]);
+        ++ic;
+      }
+      if ((resident || cg == 0) && key < x.n && !dead) {
         float* w = p.w + (int64_t)r * p.w_sb + (int64_t)hk * p.w_su + key;
-        const float add = (sa[row] + sa[kM + row]) + (sa[2 * kM + row] + sa[3 * kM + row]);
-        *w = p.w_out ? add : *w + add;
+        // one addition per element and launch: without waiting for the old value
+        if (p.w_out)
+          *w = add;
+        else
+          atomicAdd(w, add);
       }
-      ++ic;
     }
   }
   tc_fence_before();

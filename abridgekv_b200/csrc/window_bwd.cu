@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
         pair_at(x, u, qt, h);
         const int q = qt * kT + 32 * cg + lane;
         const int64_t r = ((int64_t)x.b * p.H + h) * p.S + q;
-        n_lse = q < p.S ? __ldg(p.lse + r) * kLog2e : 0.f;
+        n_lse = q < p.S ? __ldg(p.lse + r) * -kLog2e : 0.f;  // staged negated: an addend of the exponent
         n_di = q < p.S ? __ldcg(p.di + r) : 0.f;
       };
       const int g_item = g;
@@ -361,8 +361,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
             const float4 l = *reinterpret_cast<const float4*>(s_lse + c);
-            fma_pair(pv[c], pv[c + 1], pv[c], pv[c + 1], sl2, -l.x, -l.y);
-            fma_pair(pv[c + 2], pv[c + 3], pv[c + 2], pv[c + 3], sl2, -l.z, -l.w);
+            fma_pair(pv[c], pv[c + 1], pv[c], pv[c + 1], sl2, l.x, l.y);
+            fma_pair(pv[c + 2], pv[c + 3], pv[c + 2], pv[c + 3], sl2, l.z, l.w);
 #pragma unroll
             for (int j = 0; j < 4; ++j) pv[c + j] = fast_exp2(pv[c + j]);
           }
