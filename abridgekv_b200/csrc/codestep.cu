@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
     // wait behind the tcgen05.mma operand reads it has queued, so while one issuer waits
     // the other's queued MMAs keep the tensor core busy.
     const int hs = warp == 1 ? 0 : 1;
-    if (lane == 0 && (hs == 0 || hB >= 0)) {
+    if ((kWin ? elect_one() : lane == 0) && (hs == 0 || hB >= 0)) {
       // head B's P.V of a partial tile (the last sidecar tile, the last cache tile) waits
       // until head A's softmax warps have zeroed its V rows past the valid rows; the two
       // tile indices, read before any MMA is issued

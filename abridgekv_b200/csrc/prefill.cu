@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
 
   if (warp == 0) {
     // ---------------- TMA producer ----------------
-    if (lane == 0) {
+    if (kWin ? elect_one() : lane == 0) {
       for (int j = 0; j < n_tiles; ++j) {
         const int e = s_list[j];
         const int k0 = kWin ? e * kBN : (e >> 16) * p.per + (e & 0xFFFF);
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   } else if (warp == 1 || warp == kWarpIssuerB) {
     // ---------------- MMA issuers: warp 1 head A, warp 18 head B ----------------
     const int hs = warp == 1 ? 0 : 1;
-    if (lane == 0 && (hs == 0 || hB >= 0)) {
+    if ((kWin ? elect_one() : lane == 0) && (hs == 0 || hB >= 0)) {
       wait_or_abort(q_full, 0, dead, p.err);
       const uint32_t qaddr = smem_u32(smem + kOffQ) + hs * kQBytes;
       const uint32_t sbase = tmem + 256 * hs, obase = sbase + 128;

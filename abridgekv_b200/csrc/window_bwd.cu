@@ -90,10 +90,22 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
   for (int a = 0; a < Lay<D>::kAtoms; ++a) tma_load_4d(dst + a * Lay<D>::kAtom, map, 64 * a, row, head, b, bar);
 }
 
-// D(128 x 128) = A B^T over head_dim, both K-major tiles in shared memory.
+// Position in a ring of N slots and the parity of its use.
+template <int N>
+struct Pos {
+  int i = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void step() {
+    if (++i == N) {
+      i = 0;
+      ph ^= 1u;
+    }
+  }
+};
+
+// D(128 x 128) = A B^T over head_dim, both K-major tiles in shared memory (descriptors).
 template <int D>
-__device__ __forceinline__ void issue_scores(uint32_t tmem, uint32_t a, uint32_t b) {
-  const uint64_t da = desc_kmajor_sw128(a), db = desc_kmajor_sw128(b);
+__device__ __forceinline__ void issue_scores(uint32_t tmem, uint64_t da, uint64_t db) {
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) {
     const uint32_t off = (kk >> 2) * Lay<D>::kAtom + (kk & 3) * 32;
@@ -101,13 +113,13 @@ __device__ __forceinline__ void issue_scores(uint32_t tmem, uint32_t a, uint32_t
   }
 }
 // D(128 x head_dim) += A B: A bf16 in TMEM (128 x 128, 32 of its columns in 16 words every 32 words), B a [128][D]
-// tile read MN-major.
+// tile read MN-major (descriptor).
 template <int D>
-__device__ __forceinline__ void issue_accumulate(uint32_t tmem, uint32_t a, uint32_t b, bool first) {
-  const uint64_t db = desc_mnmajor_sw128(b, Lay<D>::kAtom);
+__device__ __forceinline__ void issue_accumulate(uint32_t tmem, uint32_t a, uint64_t db, bool first) {
 #pragma unroll
   for (int kk = 0; kk < kT / 16; ++kk)
-    umma_tmem_a(tmem, a + (kk >> 1) * 32 + (kk & 1) * 8, desc_advance(db, kk * 2048), Lay<D>::kIdescAcc, (!first || kk > 0) ? 1u : 0u);
+    umma_tmem_a(tmem, a + (kk >> 1) * 32 + (kk & 1) * 8, desc_advance(db, kk * 2048), Lay<D>::kIdescAcc,
+                (!first || kk > 0) ? 1u : 0u);
 }
 
 __device__ __forceinline__ void alloc_tmem(uint32_t* s_tmem) {
@@ -216,9 +228,10 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
   };
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       Item x;
-      int g = 0;  // pairs loaded so far
+      Pos<kLong> l;
+      Pos<kShort> sh;
       for (int it = 0; !dead; ++it) {
         if (p.cluster > 1) {
           if (!next_item(it, x)) break;
@@ -238,64 +251,75 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
         mbar_expect_tx(&bar[kBarA], 2 * LY::kTile);
         load_tile<D>(smem + LY::kOffA, &p.tm_k, x.kt * kT, x.hk, x.b, &bar[kBarA]);
         load_tile<D>(smem + LY::kOffB, &p.tm_v, x.kt * kT, x.hk, x.b, &bar[kBarA]);
-        for (int u = 0; u < x.n; ++u, ++g) {
+        for (int u = 0; u < x.n; ++u) {
           int qt, h;
           pair_at(x, u, qt, h);
-          const int l = g % kLong, sh = g % kShort;
-          if (!wait_or_abort(&bar[kBarLE + l], (uint32_t)(((g / kLong) & 1) ^ 1), dead, p.err)) break;
-          mbar_expect_tx(&bar[kBarLF + l], LY::kTile);
-          load_tile<D>(smem + LY::kOffLong + l * LY::kTile, &p.tm_q, qt * kT, h, x.b, &bar[kBarLF + l]);
-          if (!wait_or_abort(&bar[kBarSE + sh], (uint32_t)(((g / kShort) & 1) ^ 1), dead, p.err)) break;
-          mbar_expect_tx(&bar[kBarSF + sh], LY::kTile);
-          load_tile<D>(smem + LY::kOffShort + sh * LY::kTile, &p.tm_do, qt * kT, h, x.b, &bar[kBarSF + sh]);
+          if (!wait_or_abort(&bar[kBarLE + l.i], l.ph ^ 1u, dead, p.err)) break;
+          mbar_expect_tx(&bar[kBarLF + l.i], LY::kTile);
+          load_tile<D>(smem + LY::kOffLong + l.i * LY::kTile, &p.tm_q, qt * kT, h, x.b, &bar[kBarLF + l.i]);
+          l.step();
+          if (!wait_or_abort(&bar[kBarSE + sh.i], sh.ph ^ 1u, dead, p.err)) break;
+          mbar_expect_tx(&bar[kBarSF + sh.i], LY::kTile);
+          load_tile<D>(smem + LY::kOffShort + sh.i * LY::kTile, &p.tm_do, qt * kT, h, x.b, &bar[kBarSF + sh.i]);
+          sh.step();
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t k = smem_u32(smem + LY::kOffA), v = smem_u32(smem + LY::kOffB);
-      auto q_at = [&](int g) { return smem_u32(smem + LY::kOffLong + (g % kLong) * LY::kTile); };
-      auto do_at = [&](int g) { return smem_u32(smem + LY::kOffShort + (g % kShort) * LY::kTile); };
-      auto scores = [&](int g) -> bool {  // S^T(g)
-        if (!wait_or_abort(&bar[kBarLF + g % kLong], (uint32_t)((g / kLong) & 1), dead, p.err)) return false;
+    if (elect_one()) {
+      constexpr uint64_t kStep = LY::kTile >> 4;  // a ring slot on, in a descriptor
+      const uint64_t dk = desc_kmajor_sw128(smem_u32(smem + LY::kOffA));
+      const uint64_t dv = desc_kmajor_sw128(smem_u32(smem + LY::kOffB));
+      const uint64_t q_k = desc_kmajor_sw128(smem_u32(smem + LY::kOffLong));
+      const uint64_t do_k = desc_kmajor_sw128(smem_u32(smem + LY::kOffShort));
+      const uint64_t q_mn = desc_mnmajor_sw128(smem_u32(smem + LY::kOffLong), LY::kAtom);
+      const uint64_t do_mn = desc_mnmajor_sw128(smem_u32(smem + LY::kOffShort), LY::kAtom);
+      Pos<kLong> qf, qe;    // next Q to read for scores; Q of the current pair
+      Pos<kShort> df, de;   // likewise dO
+      uint32_t par = 0, it_par = 0;
+      auto scores = [&]() -> bool {  // S^T of the next pair
+        if (!wait_or_abort(&bar[kBarLF + qf.i], qf.ph, dead, p.err)) return false;
         tc_fence_after();
-        issue_scores<D>(tmem, k, q_at(g));
+        issue_scores<D>(tmem, dk, q_k + qf.i * kStep);
         umma_commit(&bar[kBarS]);
+        qf.step();
         return true;
       };
-      auto dscores = [&](int g) -> bool {  // dP^T(g)
-        if (!wait_or_abort(&bar[kBarSF + g % kShort], (uint32_t)((g / kShort) & 1), dead, p.err)) return false;
+      auto dscores = [&]() -> bool {  // dP^T of the next pair
+        if (!wait_or_abort(&bar[kBarSF + df.i], df.ph, dead, p.err)) return false;
         tc_fence_after();
-        issue_scores<D>(tmem + 128, v, do_at(g));
+        issue_scores<D>(tmem + 128, dv, do_k + df.i * kStep);
         umma_commit(&bar[kBarDP]);
+        df.step();
         return true;
       };
       Item x;
-      int g = 0;
       for (int it = 0; next_item(it, x); ++it) {
         done_item(it);
         if (x.n == 0) continue;
-        if (!wait_or_abort(&bar[kBarA], (uint32_t)(it & 1), dead, p.err) || !scores(g) || !dscores(g)) break;
+        if (!wait_or_abort(&bar[kBarA], it_par, dead, p.err) || !scores() || !dscores()) break;
         if (x.n == 1) umma_commit(&bar[kBarAE]);
-        for (int u = 0; u < x.n; ++u, ++g) {
-          const uint32_t par = (uint32_t)(g & 1);
-          // P^T(g) is ready: dV, then the next scores over it (one thread's MMAs run in issue order)
+        for (int u = 0; u < x.n; ++u, par ^= 1u) {
+          // P^T is ready: dV, then the next scores over it (one thread's MMAs run in issue order)
           if (!wait_or_abort(&bar[kBarP], par, dead, p.err)) break;
           // the first product of an item overwrites dV and dK: the previous ones have been read out
-          if (u == 0 && it > 0 && !wait_or_abort(&bar[kBarDrain], (uint32_t)((it - 1) & 1), dead, p.err)) break;
+          if (u == 0 && it > 0 && !wait_or_abort(&bar[kBarDrain], it_par ^ 1u, dead, p.err)) break;
           tc_fence_after();
-          issue_accumulate<D>(tmem + 256, tmem, do_at(g), u == 0);
-          umma_commit(&bar[kBarSE + g % kShort]);  // dO(g): its last use
-          if (u + 1 < x.n && !scores(g + 1)) break;
+          issue_accumulate<D>(tmem + 256, tmem, do_mn + de.i * kStep, u == 0);
+          umma_commit(&bar[kBarSE + de.i]);  // dO's last use
+          de.step();
+          if (u + 1 < x.n && !scores()) break;
           if (!wait_or_abort(&bar[kBarDS], par, dead, p.err)) break;
           tc_fence_after();
-          issue_accumulate<D>(tmem + 384, tmem + 128, q_at(g), u == 0);
-          umma_commit(&bar[kBarLE + g % kLong]);
-          if (u + 1 < x.n && !dscores(g + 1)) break;
+          issue_accumulate<D>(tmem + 384, tmem + 128, q_mn + qe.i * kStep, u == 0);
+          umma_commit(&bar[kBarLE + qe.i]);
+          qe.step();
+          if (u + 1 < x.n && !dscores()) break;
           if (u + 2 == x.n) umma_commit(&bar[kBarAE]);  // the item's last scores are issued: K and V are free then
         }
         if (dead) break;
         umma_commit(&bar[kBarAcc]);
+        it_par ^= 1u;
       }
     }
   } else {
@@ -530,20 +554,23 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
   };
 
   if (warp == 0) {
-    if (lane == 0) {
-      int g = 0, it = 0;
+    if (elect_one()) {
+      Pos<kLong> l;
+      Pos<kShort> sh;
+      int it = 0;
       for (int i = blockIdx.x; i < n_items && !dead; i += gridDim.x, ++it) {
         const Item x = decode(i);
         const int hk = x.h / p.G;
-        for (int u = 0; u < x.n; ++u, ++g) {
+        for (int u = 0; u < x.n; ++u) {
           const int row = (u < x.ns ? u : u + x.shift) * kT;
-          const int l = g % kLong, sh = g % kShort;
-          if (!wait_or_abort(&bar[kBarLE + l], (uint32_t)(((g / kLong) & 1) ^ 1), dead, p.err)) break;
-          mbar_expect_tx(&bar[kBarLF + l], LY::kTile);
-          load_tile<D>(smem + LY::kOffLong + l * LY::kTile, &p.tm_k, row, hk, x.b, &bar[kBarLF + l]);
-          if (!wait_or_abort(&bar[kBarSE + sh], (uint32_t)(((g / kShort) & 1) ^ 1), dead, p.err)) break;
-          mbar_expect_tx(&bar[kBarSF + sh], LY::kTile);
-          load_tile<D>(smem + LY::kOffShort + sh * LY::kTile, &p.tm_v, row, hk, x.b, &bar[kBarSF + sh]);
+          if (!wait_or_abort(&bar[kBarLE + l.i], l.ph ^ 1u, dead, p.err)) break;
+          mbar_expect_tx(&bar[kBarLF + l.i], LY::kTile);
+          load_tile<D>(smem + LY::kOffLong + l.i * LY::kTile, &p.tm_k, row, hk, x.b, &bar[kBarLF + l.i]);
+          l.step();
+          if (!wait_or_abort(&bar[kBarSE + sh.i], sh.ph ^ 1u, dead, p.err)) break;
+          mbar_expect_tx(&bar[kBarSF + sh.i], LY::kTile);
+          load_tile<D>(smem + LY::kOffShort + sh.i * LY::kTile, &p.tm_v, row, hk, x.b, &bar[kBarSF + sh.i]);
+          sh.step();
           if (u == 0) {  // the item's Q and dO once the previous item's last scores have run
             if (!wait_or_abort(&bar[kBarAE], (uint32_t)((it & 1) ^ 1), dead, p.err)) break;
             mbar_expect_tx(&bar[kBarA], 2 * LY::kTile);
@@ -554,43 +581,55 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      const uint32_t q = smem_u32(smem + LY::kOffA), dout = smem_u32(smem + LY::kOffB);
-      auto k_at = [&](int g) { return smem_u32(smem + LY::kOffLong + (g % kLong) * LY::kTile); };
-      auto scores = [&](int g) -> bool {  // S(g) into buffer g % 2: dS(g - 2) has been formed from it
-        if (!wait_or_abort(&bar[kBarLF + g % kLong], (uint32_t)((g / kLong) & 1), dead, p.err)) return false;
+    if (elect_one()) {
+      constexpr uint64_t kStep = LY::kTile >> 4;
+      const uint64_t dq = desc_kmajor_sw128(smem_u32(smem + LY::kOffA));
+      const uint64_t ddo = desc_kmajor_sw128(smem_u32(smem + LY::kOffB));
+      const uint64_t k_k = desc_kmajor_sw128(smem_u32(smem + LY::kOffLong));
+      const uint64_t v_k = desc_kmajor_sw128(smem_u32(smem + LY::kOffShort));
+      const uint64_t k_mn = desc_mnmajor_sw128(smem_u32(smem + LY::kOffLong), LY::kAtom);
+      Pos<kLong> kf, ke;  // next K to read for scores; K of the current tile
+      Pos<kShort> vf;
+      uint32_t par = 0, sbuf = 0, it_par = 0;
+      auto scores = [&]() -> bool {  // S of the next tile into its buffer: dS of two tiles ago has been formed from it
+        if (!wait_or_abort(&bar[kBarLF + kf.i], kf.ph, dead, p.err)) return false;
         tc_fence_after();
-        issue_scores<D>(tmem + 128 * (g & 1), q, k_at(g));
-        umma_commit(&bar[kBarS + (g & 1)]);
+        issue_scores<D>(tmem + 128 * sbuf, dq, k_k + kf.i * kStep);
+        umma_commit(&bar[kBarS + sbuf]);
+        kf.step();
+        sbuf ^= 1u;
         return true;
       };
-      auto dscores = [&](int g) -> bool {  // dP(g), over dS(g - 1) which dQ has read
-        if (!wait_or_abort(&bar[kBarSF + g % kShort], (uint32_t)((g / kShort) & 1), dead, p.err)) return false;
+      auto dscores = [&]() -> bool {  // dP of the next tile, over the last dS, which dQ has read
+        if (!wait_or_abort(&bar[kBarSF + vf.i], vf.ph, dead, p.err)) return false;
         tc_fence_after();
-        issue_scores<D>(tmem + 256, dout, smem_u32(smem + LY::kOffShort + (g % kShort) * LY::kTile));
+        issue_scores<D>(tmem + 256, ddo, v_k + vf.i * kStep);
         umma_commit(&bar[kBarDP]);
-        umma_commit(&bar[kBarSE + g % kShort]);  // V(g): its only use
+        umma_commit(&bar[kBarSE + vf.i]);  // V's only use
+        vf.step();
         return true;
       };
-      int g = 0, it = 0;
+      int it = 0;
       for (int i = blockIdx.x; i < n_items && !dead; i += gridDim.x, ++it) {
         const Item x = decode(i);
-        if (!wait_or_abort(&bar[kBarA], (uint32_t)(it & 1), dead, p.err) || !scores(g) || !dscores(g)) break;
+        if (!wait_or_abort(&bar[kBarA], it_par, dead, p.err) || !scores() || !dscores()) break;
         if (x.n == 1) umma_commit(&bar[kBarAE]);
-        if (x.n > 1 && !scores(g + 1)) break;
-        for (int u = 0; u < x.n; ++u, ++g) {
-          if (!wait_or_abort(&bar[kBarDS], (uint32_t)(g & 1), dead, p.err)) break;
+        if (x.n > 1 && !scores()) break;
+        for (int u = 0; u < x.n; ++u, par ^= 1u) {
+          if (!wait_or_abort(&bar[kBarDS], par, dead, p.err)) break;
           // the first product of an item overwrites dQ: the previous one has been read out
-          if (u == 0 && it > 0 && !wait_or_abort(&bar[kBarDrain], (uint32_t)((it - 1) & 1), dead, p.err)) break;
+          if (u == 0 && it > 0 && !wait_or_abort(&bar[kBarDrain], it_par ^ 1u, dead, p.err)) break;
           tc_fence_after();
-          issue_accumulate<D>(tmem + 384, tmem + 256, k_at(g), u == 0);
-          umma_commit(&bar[kBarLE + g % kLong]);
-          if (u + 1 < x.n && !dscores(g + 1)) break;
+          issue_accumulate<D>(tmem + 384, tmem + 256, k_mn + ke.i * kStep, u == 0);
+          umma_commit(&bar[kBarLE + ke.i]);
+          ke.step();
+          if (u + 1 < x.n && !dscores()) break;
           if (u + 2 == x.n) umma_commit(&bar[kBarAE]);  // the item's last scores are issued: Q and dO are free then
-          if (u + 2 < x.n && !scores(g + 2)) break;
+          if (u + 2 < x.n && !scores()) break;
         }
         if (dead) break;
         umma_commit(&bar[kBarAcc]);
+        it_par ^= 1u;
       }
     }
   } else {
