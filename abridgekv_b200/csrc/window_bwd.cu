@@ -19,7 +19,7 @@
 // element-wise half of a tile (16,384
 // exponentials, 1024 clocks) runs beside the products of its neighbours:
 //   dK/dV:  S(0) dP(0) | dV(u) S(u+1) | dK(u) dP(u+1) | ...    threads: P(u) then dS(u)
-//   dQ:     S(0) dP(0) S(1) | dQ(u) dP(u+1) S(u+2) | ...       threads: P(u) in registers, dS(u)
+//   dQ:     S(0) dP(0) S(1) | dP(u+1) | dQ(u) S(u+2) | ...     threads: P(u), dP(u) in registers, dS(u) over S(u)
 // Every mbarrier wait is bounded and records ABKV_DEVERR_TIMEOUT on expiry.
 #include <algorithm>
 #include <cstring>
@@ -32,7 +32,7 @@ using namespace tc;
 
 constexpr int kT = 128;          // tile rows (keys and queries)
 constexpr int kThreads = 576;    // 18 warps
-constexpr int kWorkers = 16;     // warps of TMEM lanes: one arrival each (512 on one barrier cost more than they order)
+constexpr int kWorkers = 16;     // warps of TMEM lanes, one arrival each
 constexpr int kLong = 3, kShort = 2;  // ring depth of the operand used twice, and of the one released early
 constexpr uint32_t kIdescS = idesc_bf16_m128(kT, false);
 constexpr float kLog2e = 1.4426950408889634f;
@@ -57,7 +57,7 @@ static_assert(2 * kT * Lay<128>::kRedStride * 4 <= (kLong + kShort) * Lay<128>::
 static_assert(2 * kT * Lay<64>::kRedStride * 4 <= (kLong + kShort) * Lay<64>::kTile, "cluster reduction");
 
 // barriers: stationary operands, long ring full / empty, short ring full / empty, S full (two in the dQ kernel),
-// dP full, P ready, dS ready, accumulators complete / drained, statistics [column group][buffer] (a barrier per buffer:
+// dP full, P ready (dQ: dP read), dS ready, accumulators complete / drained, statistics [column group][buffer] (a barrier per buffer:
 // the writer may be a pair ahead of a reader, and a parity wait cannot tell phases 2 apart), stationary operands
 // released, work item full / empty (two deep), then the TMEM address and the items
 constexpr int kBarA = 0, kBarLF = 1, kBarLE = kBarLF + kLong, kBarSF = kBarLE + kLong, kBarSE = kBarSF + kShort,
@@ -528,7 +528,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
   const int heads = p.H * p.B, n_items = heads * p.n_tiles;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBarTmem; ++i) mbar_init(&bar[i], (i == kBarDS || i == kBarDrain) ? kWorkers : 1);
+    for (int i = 0; i < kBarTmem; ++i)
+      mbar_init(&bar[i], (i == kBarDS || i == kBarP || i == kBarDrain) ? kWorkers : 1);
   }
   if (warp == 1) alloc_tmem(s_tmem);
   tc_fence_before();
@@ -591,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
       Pos<kLong> kf, ke;  // next K to read for scores; K of the current tile
       Pos<kShort> vf;
       uint32_t par = 0, sbuf = 0, it_par = 0;
-      auto scores = [&]() -> bool {  // S of the next tile into its buffer: dS of two tiles ago has been formed from it
+      auto scores = [&]() -> bool {  // S of the next tile into its buffer, over the dS that dQ has read
         if (!wait_or_abort(&bar[kBarLF + kf.i], kf.ph, dead, p.err)) return false;
         tc_fence_after();
         issue_scores<D>(tmem + 128 * sbuf, dq, k_k + kf.i * kStep);
@@ -600,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
         sbuf ^= 1u;
         return true;
       };
-      auto dscores = [&]() -> bool {  // dP of the next tile, over the last dS, which dQ has read
+      auto dscores = [&]() -> bool {  // dP of the next tile
         if (!wait_or_abort(&bar[kBarSF + vf.i], vf.ph, dead, p.err)) return false;
         tc_fence_after();
         issue_scores<D>(tmem + 256, ddo, v_k + vf.i * kStep);
@@ -610,21 +611,26 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
         return true;
       };
       int it = 0;
+      uint32_t buf = 0;  // S buffer of the current tile, which dS takes over
       for (int i = blockIdx.x; i < n_items && !dead; i += gridDim.x, ++it) {
         const Item x = decode(i);
-        if (!wait_or_abort(&bar[kBarA], it_par, dead, p.err) || !scores() || !dscores()) break;
+        if (!wait_or_abort(&bar[kBarA], it_par, dead, p.err) || !scores()) break;
+        // the last dP of the previous item has been read
+        if (it > 0 && !wait_or_abort(&bar[kBarP], par ^ 1u, dead, p.err)) break;
+        if (!dscores()) break;
         if (x.n == 1) umma_commit(&bar[kBarAE]);
         if (x.n > 1 && !scores()) break;
-        for (int u = 0; u < x.n; ++u, par ^= 1u) {
+        for (int u = 0; u < x.n; ++u, par ^= 1u, buf ^= 1u) {
+          // dP has been read: the next one, beside the forming of dS
+          if (u + 1 < x.n && (!wait_or_abort(&bar[kBarP], par, dead, p.err) || !dscores())) break;
+          if (u + 2 == x.n) umma_commit(&bar[kBarAE]);  // the item's last scores are issued: Q and dO are free then
           if (!wait_or_abort(&bar[kBarDS], par, dead, p.err)) break;
           // the first product of an item overwrites dQ: the previous one has been read out
           if (u == 0 && it > 0 && !wait_or_abort(&bar[kBarDrain], it_par ^ 1u, dead, p.err)) break;
           tc_fence_after();
-          issue_accumulate<D>(tmem + 384, tmem + 256, k_mn + ke.i * kStep, u == 0);
+          issue_accumulate<D>(tmem + 384, tmem + 128 * buf, k_mn + ke.i * kStep, u == 0);
           umma_commit(&bar[kBarLE + ke.i]);
           ke.step();
-          if (u + 1 < x.n && !dscores()) break;
-          if (u + 2 == x.n) umma_commit(&bar[kBarAE]);  // the item's last scores are issued: Q and dO are free then
           if (u + 2 < x.n && !scores()) break;
         }
         if (dead) break;
@@ -675,13 +681,18 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
           uint32_t w[16];
           tmem_ld32(tmem + lane_base + 256 + 32 * cg, dp);
           tmem_wait_ld();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_one(&bar[kBarP]);  // dP is in registers
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
             sub_mul_pair(dp[c], dp[c + 1], dp[c], dp[c + 1], di, di, pv[c], pv[c + 1]);
             w[c / 2] = pack_bf16x2(dp[c], dp[c + 1]);
           }
-          tmem_st16(tmem + lane_base + 256 + 32 * cg, w);
+          tmem_st16(tmem + lane_base + 128 * (g & 1) + 32 * cg, w);
           tmem_wait_st();
+        } else if (lane == 0) {
+          mbar_arrive_one(&bar[kBarP]);
         }
         tc_fence_before();
         __syncwarp();
