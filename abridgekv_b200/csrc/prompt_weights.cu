@@ -12,7 +12,8 @@
 // cache rows, so the sum over queries is a sum over a thread's own registers, no reduction across lanes
 // and no second product.  The 128 columns are 4 units of 32 consecutive query rows of one head (so a
 // group of 4 heads x 32 observed rows is one full tile).  19 warps:
-//   warp 0      K tiles (eight 16-row page slices) by cp.async.bulk.tensor, 128B swizzle
+//   warp 0      the items' descriptors (request, tile, units), passed on through a ring in shared memory, and
+//               their K tiles (eight 16-row page slices) by cp.async.bulk.tensor, 128B swizzle
 //   warp 18     Q tiles (four 32-row boxes); where every counted row of a request fits one
 //               tile, it is loaded once for all cache tiles of a (request, head) run, and the six ring slots go to K
 //               (4) rather than Q (4 otherwise)
@@ -48,11 +49,14 @@ constexpr int kOffLse = kOffK + kStages * kTileBytes;   // 16 warps x [128] floa
 constexpr int kOffAcc = kOffLse + 16 * kN * 4;          // [2 items][4 groups][128 rows] partial sums
 constexpr int kMaxPref = 1024;
 constexpr int kOffPref = kOffAcc + 2 * 4 * kM * 4;      // [R + 1] running tile counts
-constexpr int kOffBar = kOffPref + (kMaxPref + 2) * 4;
-static_assert(kOffBar % 8 == 0, "barriers");
+constexpr int kItemGroup = 4, kItemGroups = 4;          // items are described four at a time, four groups ahead
+constexpr int kOffItems = kOffPref + (kMaxPref + 4) * 4;
+constexpr int kOffBar = kOffItems + kItemGroup * kItemGroups * 48;
+static_assert(kOffItems % 16 == 0 && kOffBar % 8 == 0, "descriptors and barriers");
 constexpr int kBarKFull = 0, kBarKEmpty = kBarKFull + kMaxK, kBarQFull = kBarKEmpty + kMaxK,
               kBarQEmpty = kBarQFull + kMaxQ, kBarSFull = kBarQEmpty + kMaxQ, kBarSEmpty = kBarSFull + kSBufs,
-              kBarTmem = kBarSEmpty + kSBufs;
+              kBarAccFull = kBarSEmpty + kSBufs, kBarAccEmpty = kBarAccFull + 2, kBarItemFull = kBarAccEmpty + 2,
+              kBarItemEmpty = kBarItemFull + kItemGroups, kBarTmem = kBarItemEmpty + kItemGroups;
 constexpr int kSmemBytes = kOffBar + 8 * (kBarTmem + 1) + 1024;
 static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 
@@ -180,6 +184,14 @@ __device__ __forceinline__ bool item_at(const PromptParams& p, const Items& it, 
   return true;
 }
 
+// What every role has to know of an item; units [u0, u1) may be empty.
+struct alignas(16) Desc {
+  int r, hk, kt, u0;
+  int u1, q0, nq, n;
+  int p0, valid, pad[2];
+};
+static_assert(sizeof(Desc) == 48, "ring of descriptors");
+
 // a * b + c on a pair with one b.
 __device__ __forceinline__ void scale_add(float& d0, float& d1, float a0, float a1, float b, float c0, float c1) {
   asm("{\n .reg .b64 x, y, z, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mov.b64 z, {%5, %6};\n"
@@ -197,7 +209,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
   const bool resident = (int64_t)((most_rows(p) + kUnit - 1) / kUnit) * p.G <= kN / kUnit && p.R <= kMaxPref;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBarTmem; ++i) mbar_init(&bar[i], i >= kBarSEmpty ? 4 : 1);  // the four warps of a group
+    for (int i = 0; i < kBarTmem; ++i) {
+      int n = 1;
+      if ((i >= kBarSEmpty && i < kBarSEmpty + kSBufs) || (i >= kBarAccEmpty && i < kBarAccEmpty + 2))
+        n = 4;  // the four warps of a group
+      else if (i >= kBarAccFull && i < kBarAccFull + 2)
+        n = 16;
+      else if (i >= kBarItemEmpty)
+        n = 16 + 2;  // the groups' warps, the issuer, the Q producer
+      mbar_init(&bar[i], n);
+    }
   }
   int32_t* s_pref = reinterpret_cast<int32_t*>(smem + kOffPref);
   if (resident && warp == 2) {  // running count of the requests' visible tiles
@@ -236,7 +257,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
     it.first = blockIdx.x * per;
     it.n = max(0, min(per, total - it.first));
   }
+  // ring lengths are 2 or 4: slot and phase of a running count
   const int kKStages = k_stages(resident), kQStages = q_stages(resident);
+  const int k_shift = kKStages >> 1, q_shift = kQStages >> 1;
+  const Desc* const s_items = reinterpret_cast<const Desc*>(smem + kOffItems);
+  auto items_ready = [&](int grp) -> bool {
+    return wait_or_abort(&bar[kBarItemFull + (grp & (kItemGroups - 1))], (uint32_t)(grp / kItemGroups) & 1u, dead, p.err);
+  };
   uint8_t* const s_k = smem + kOffK;
   uint8_t* const s_q = smem + kOffK + kKStages * kTileBytes;
 
@@ -246,19 +273,23 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
     int kc = 0;
     for (int base = 0; base < it.n && !dead; base += 4) {
       const int k = base + (lane >> 3), slice = lane & 7;
-      int pg = -1, hk = 0, off = 0;
-      bool busy = false;  // the item has work
-      int r, kt, u0, u1;
-      if (k < it.n && item_at(p, it, k, r, hk, kt)) {
-        const Req x = load_req(p, r, !resident && kt == 0 && hk == 0 && slice == 0);
-        item_units(p, x, kt, resident, u0, u1);
-        busy = u0 < u1;
-        const int row0 = kt * kM + 16 * slice;
-        if (busy && row0 < x.n) {
+      int pg = -1, off = 0;
+      Desc d;
+      d.r = d.hk = d.kt = d.u0 = d.u1 = d.q0 = d.nq = d.n = d.p0 = d.valid = d.pad[0] = d.pad[1] = 0;
+      if (k < it.n && item_at(p, it, k, d.r, d.hk, d.kt)) {
+        const Req x = load_req(p, d.r, !resident && d.kt == 0 && d.hk == 0 && slice == 0);
+        item_units(p, x, d.kt, resident, d.u0, d.u1);
+        d.q0 = x.q0;
+        d.nq = x.nq;
+        d.n = x.n;
+        d.p0 = x.p0;
+        d.valid = 1;
+        const int row0 = d.kt * kM + 16 * slice;
+        if (d.u0 < d.u1 && row0 < x.n) {
           // a slice hidden from every counted row is not looked up: its page may be freed
           const bool hidden = p.window > 0 && row0 >= p.n_sink && row0 + 16 <= x.p0 - p.window + 1;
           if (!hidden) {
-            pg = __ldg(p.bt + (int64_t)r * p.bt_stride + row0 / p.page);
+            pg = __ldg(p.bt + (int64_t)d.r * p.bt_stride + row0 / p.page);
             off = row0 % p.page;
             if (pg < 0 || (int64_t)pg >= p.num_blocks) {
               set_error(p.err, ABKV_DEVERR_PAGE_OOB);
@@ -267,13 +298,22 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
           }
         }
       }
-      const uint32_t valid = __ballot_sync(0xffffffffu, pg >= 0), work = __ballot_sync(0xffffffffu, busy);
+      const uint32_t valid = __ballot_sync(0xffffffffu, pg >= 0), work = __ballot_sync(0xffffffffu, d.u0 < d.u1);
+      const int grp = base / kItemGroup, gs = grp & (kItemGroups - 1);
+      if (!__all_sync(0xffffffffu, wait_or_abort(&bar[kBarItemEmpty + gs], ((uint32_t)(grp / kItemGroups) & 1u) ^ 1u,
+                                                 dead, p.err))) {
+        dead = true;
+        break;
+      }
+      if (slice == 0) *reinterpret_cast<Desc*>(smem + kOffItems + (gs * kItemGroup + (lane >> 3)) * 48) = d;
+      __syncwarp();
+      if (lane == 0) mbar_arrive_one(&bar[kBarItemFull + gs]);
       for (int j = 0; j < 4; ++j) {
         if (!((work >> (8 * j)) & 1u)) continue;
-        const int st = kc % kKStages;
+        const int st = kc & (kKStages - 1);
         bool ok = true;
         if (lane == 0) {
-          ok = wait_or_abort(&bar[kBarKEmpty + st], (uint32_t)(((kc / kKStages) & 1) ^ 1), dead, p.err);
+          ok = wait_or_abort(&bar[kBarKEmpty + st], (uint32_t)(((kc >> k_shift) & 1) ^ 1), dead, p.err);
           if (ok) mbar_expect_tx(&bar[kBarKFull + st], (uint32_t)__popc((valid >> (8 * j)) & 0xFFu) * 2u * 2048u);
         }
         if (!__shfl_sync(0xffffffffu, ok, 0)) {
@@ -283,76 +323,85 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
         if ((lane >> 3) == j && pg >= 0) {
           uint8_t* kb = s_k + st * kTileBytes + slice * 2048;
           const int plane = p.fa_layout ? pg : 2 * pg;
-          tma_load_4d(kb, &p.tm_k, 0, hk, off, plane, &bar[kBarKFull + st]);
-          tma_load_4d(kb + kTileBytes / 2, &p.tm_k, 64, hk, off, plane, &bar[kBarKFull + st]);
+          tma_load_4d(kb, &p.tm_k, 0, d.hk, off, plane, &bar[kBarKFull + st]);
+          tma_load_4d(kb + kTileBytes / 2, &p.tm_k, 64, d.hk, off, plane, &bar[kBarKFull + st]);
         }
         ++kc;
       }
     }
   } else if (warp == kWarpQ) {
     // ---------------- Q producer ----------------
-    if (lane == 0) {
+    if (elect_one()) {
       int qc = 0, last_g = -1;
-      for (int k = 0; k < it.n && !dead; ++k) {
-        int r, hk, kt, u0, u1;
-        if (!item_at(p, it, k, r, hk, kt)) break;
-        const Req x = load_req(p, r, false);
-        item_units(p, x, kt, resident, u0, u1);
-        if (u0 >= u1) continue;
-        if (resident && last_g == r * p.Hkv + hk) continue;  // this tile is loaded
-        last_g = r * p.Hkv + hk;
-        for (int u = u0; u < u1; u += 4, ++qc) {
-          const int st = qc % kQStages, nu = min(4, u1 - u);
-          if (!wait_or_abort(&bar[kBarQEmpty + st], (uint32_t)(((qc / kQStages) & 1) ^ 1), dead, p.err)) break;
-          mbar_expect_tx(&bar[kBarQFull + st], (uint32_t)nu * 2u * 4096u);
-          for (int c = 0; c < nu; ++c) {
-            const int chunk = (u + c) / p.G, h = hk * p.G + (u + c) % p.G;
-            uint8_t* qb = s_q + st * kTileBytes + c * 4096;
-            tma_load_4d(qb, &p.tm_q, 0, h, x.q0 + chunk * kUnit, 0, &bar[kBarQFull + st]);
-            tma_load_4d(qb + kTileBytes / 2, &p.tm_q, 64, h, x.q0 + chunk * kUnit, 0, &bar[kBarQFull + st]);
+      for (int base = 0, grp = 0; base < it.n && !dead; base += kItemGroup, ++grp) {
+        if (!items_ready(grp)) break;
+        for (int j = 0; j < kItemGroup && !dead; ++j) {
+          const Desc x = s_items[(grp & (kItemGroups - 1)) * kItemGroup + j];
+          if (x.u0 >= x.u1) continue;
+          if (resident && last_g == x.r * p.Hkv + x.hk) continue;  // this tile is loaded
+          last_g = x.r * p.Hkv + x.hk;
+          int chunk = x.u0 / p.G, g = x.u0 - chunk * p.G;
+          for (int u = x.u0; u < x.u1; u += 4, ++qc) {
+            const int st = qc & (kQStages - 1), nu = min(4, x.u1 - u);
+            if (!wait_or_abort(&bar[kBarQEmpty + st], (uint32_t)(((qc >> q_shift) & 1) ^ 1), dead, p.err)) break;
+            mbar_expect_tx(&bar[kBarQFull + st], (uint32_t)nu * 2u * 4096u);
+            for (int c = 0; c < nu; ++c) {
+              uint8_t* qb = s_q + st * kTileBytes + c * 4096;
+              const int h = x.hk * p.G + g, t = x.q0 + chunk * kUnit;
+              tma_load_4d(qb, &p.tm_q, 0, h, t, 0, &bar[kBarQFull + st]);
+              tma_load_4d(qb + kTileBytes / 2, &p.tm_q, 64, h, t, 0, &bar[kBarQFull + st]);
+              if (++g == p.G) {
+                g = 0;
+                ++chunk;
+              }
+            }
           }
         }
+        mbar_arrive_one(&bar[kBarItemEmpty + (grp & (kItemGroups - 1))]);
       }
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
-    if (lane == 0) {
+    if (elect_one()) {
+      const uint64_t dk0 = desc_kmajor_sw128(smem_u32(s_k)), dq0 = desc_kmajor_sw128(smem_u32(s_q));
+      constexpr uint64_t kStep = kTileBytes >> 4;  // descriptors count 16 bytes
       int kc = 0, qc = 0, sc = 0, last_g = -1;
-      for (int k = 0; k < it.n && !dead; ++k) {
-        int r, hk, kt, u0, u1;
-        if (!item_at(p, it, k, r, hk, kt)) break;
-        const Req x = load_req(p, r, false);
-        item_units(p, x, kt, resident, u0, u1);
-        if (u0 >= u1) continue;
-        const int ks = kc % kKStages;
-        if (!wait_or_abort(&bar[kBarKFull + ks], (uint32_t)((kc / kKStages) & 1), dead, p.err)) break;
-        const uint64_t dk = desc_kmajor_sw128(smem_u32(s_k + ks * kTileBytes));
-        const bool fresh = !resident || last_g != r * p.Hkv + hk;
-        if (resident && fresh && last_g >= 0) {
-          umma_commit(&bar[kBarQEmpty + qc % kQStages]);  // the previous run's Q tile
-          ++qc;
-        }
-        last_g = r * p.Hkv + hk;
-        for (int u = u0; u < u1 && !dead; u += 4) {
-          const int qs = qc % kQStages, sb = sc % kSBufs;
-          if (fresh && !wait_or_abort(&bar[kBarQFull + qs], (uint32_t)((qc / kQStages) & 1), dead, p.err)) break;
-          if (!wait_or_abort(&bar[kBarSEmpty + sb], (uint32_t)(((sc / kSBufs) & 1) ^ 1), dead, p.err)) break;
-          tc_fence_after();
-          const uint64_t dq = desc_kmajor_sw128(smem_u32(s_q + qs * kTileBytes));
-#pragma unroll
-          for (int kk = 0; kk < kD / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * (kTileBytes / 2) + (kk & 3) * 32;
-            umma(tmem + 128 * sb, desc_advance(dk, off), desc_advance(dq, off), kIdescS, kk > 0 ? 1u : 0u);
-          }
-          umma_commit(&bar[kBarSFull + sb]);
-          ++sc;
-          if (!resident) {
-            umma_commit(&bar[kBarQEmpty + qs]);
+      for (int base = 0, grp = 0; base < it.n && !dead; base += kItemGroup, ++grp) {
+        if (!items_ready(grp)) break;
+        for (int j = 0; j < kItemGroup && !dead; ++j) {
+          const Desc x = s_items[(grp & (kItemGroups - 1)) * kItemGroup + j];
+          if (x.u0 >= x.u1) continue;
+          const int ks = kc & (kKStages - 1), g = x.r * p.Hkv + x.hk;
+          const bool fresh = !resident || last_g != g;
+          if (resident && fresh && last_g >= 0) {
+            umma_commit(&bar[kBarQEmpty + (qc & (kQStages - 1))]);  // the previous run's Q tile
             ++qc;
           }
+          last_g = g;
+          if (!wait_or_abort(&bar[kBarKFull + ks], (uint32_t)((kc >> k_shift) & 1), dead, p.err)) break;
+          const uint64_t dk = dk0 + ks * kStep;
+          for (int u = x.u0; u < x.u1; u += 4) {
+            const int qs = qc & (kQStages - 1), sb = sc & (kSBufs - 1);
+            if (fresh && !wait_or_abort(&bar[kBarQFull + qs], (uint32_t)((qc >> q_shift) & 1), dead, p.err)) break;
+            if (!wait_or_abort(&bar[kBarSEmpty + sb], (uint32_t)(((sc / kSBufs) & 1) ^ 1), dead, p.err)) break;
+            tc_fence_after();
+            const uint64_t dq = dq0 + qs * kStep;
+#pragma unroll
+            for (int kk = 0; kk < kD / 16; ++kk) {
+              const uint32_t off = (kk >> 2) * (kTileBytes / 2) + (kk & 3) * 32;
+              umma(tmem + 128 * sb, desc_advance(dk, off), desc_advance(dq, off), kIdescS, kk > 0 ? 1u : 0u);
+            }
+            umma_commit(&bar[kBarSFull + sb]);
+            ++sc;
+            if (!resident) {
+              umma_commit(&bar[kBarQEmpty + qs]);
+              ++qc;
+            }
+          }
+          umma_commit(&bar[kBarKEmpty + ks]);
+          ++kc;
         }
-        umma_commit(&bar[kBarKEmpty + ks]);
-        ++kc;
+        mbar_arrive_one(&bar[kBarItemEmpty + (grp & (kItemGroups - 1))]);
       }
     }
   } else {
@@ -365,106 +414,123 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
     float* s_acc = reinterpret_cast<float*>(smem + kOffAcc);
     const float sl2 = p.scale_log2;
     int sc = 0, ic = 0;
-    for (int k = 0; k < it.n; ++k) {
-      int r, hk, kt, u0, u1;
-      if (!item_at(p, it, k, r, hk, kt)) break;
-      if (resident && (sc & 3) != cg) {  // one step, another group's
-        ++sc;
-        continue;
+    for (int base = 0, grp = 0; base < it.n && !dead; base += kItemGroup, ++grp) {
+      if (!__all_sync(0xffffffffu, items_ready(grp))) {
+        dead = true;
+        break;
       }
-      const Req x = load_req(p, r, false);
-      item_units(p, x, kt, resident, u0, u1);
-      if (u0 >= u1) continue;
-      const int key = kt * kM + row;
-      float acc[4] = {0.f, 0.f, 0.f, 0.f};
-      // log-sum-exp (negated, log2 units) of a step's rows, lane = row of each of its four units
-      float n_lse[4];
-      auto fetch = [&](int u) {
-        int chunk = u / p.G, h = u - chunk * p.G;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int t = min(x.q0 + chunk * kUnit + lane, p.T - 1);
-          n_lse[j] = u + j < u1 ? __ldg(p.lse + (int64_t)t * p.H + hk * p.G + h) * -1.4426950408889634f : 0.f;
-          if (++h == p.G) {
-            h = 0;
-            ++chunk;
-          }
+      for (int i = 0; i < kItemGroup && !dead; ++i) {
+        const Desc& x = s_items[(grp & (kItemGroups - 1)) * kItemGroup + i];
+        const int u0 = x.u0, u1 = x.u1;
+        if (u0 >= u1) continue;
+        if (resident && (sc & 3) != cg) {  // one step, another group's
+          ++sc;
+          continue;
         }
-      };
-      int mine = u0 + 4 * ((cg - sc) & 3);  // the group's first step of the item
-      if (mine < u1) fetch(mine);
-      for (int u = u0; u < u1; u += 4, ++sc) {
-        if (u != mine) continue;
-        const int sb = sc % kSBufs;
-        __syncwarp();  // every lane is past its reads of the previous step's values
+        const int key = x.kt * kM + row;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        // log-sum-exp (negated, log2 units) of a step's rows, lane = row of each of its four units
+        float n_lse[4];
+        auto fetch = [&](int u) {
+          int chunk = u / p.G, h = u - chunk * p.G;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s_lse[32 * j + lane] = n_lse[j];
-        __syncwarp();
-        mine += 16;
-        if (mine < u1) fetch(mine);
-        const bool ok = __all_sync(0xffffffffu,
-                                   wait_or_abort(&bar[kBarSFull + sb], (uint32_t)((sc / kSBufs) & 1), dead, p.err));
-        if (!ok) dead = true;
-        tc_fence_after();
-        int chunk = u / p.G, h = u - chunk * p.G;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (ok && u + j < u1) {
-            float s[32];
-            tmem_ld32(tmem + lane_base + 128 * sb + 32 * j, s);
-            tmem_wait_ld();
-            // visible columns [a, e): rows at or past the key, inside its window, and counted
-            const int pc = x.p0 + chunk * kUnit;
-            const int a = max(key - pc, 0);
-            int e = min(kUnit, x.nq - chunk * kUnit);
-            if (p.window > 0 && key >= p.n_sink) e = (int)min((int64_t)e, (int64_t)key + p.window - pc);
-            const uint32_t mask = (a >= e || e <= 0) ? 0u : (0xFFFFFFFFu >> (32 - e)) & (0xFFFFFFFFu << a);
-            const bool full = __all_sync(0xffffffffu, mask == 0xFFFFFFFFu);
-            const float* l4 = s_lse + 32 * j;
-            if (full) {
-#pragma unroll
-              for (int c = 0; c < 32; c += 4) {
-                const float4 l = *reinterpret_cast<const float4*>(l4 + c);
-                float x0, x1, x2, x3;
-                scale_add(x0, x1, s[c], s[c + 1], sl2, l.x, l.y);
-                scale_add(x2, x3, s[c + 2], s[c + 3], sl2, l.z, l.w);
-                fadd2(acc[0], acc[1], fast_exp2(x0), fast_exp2(x1));
-                fadd2(acc[2], acc[3], fast_exp2(x2), fast_exp2(x3));
-              }
-            } else if (__any_sync(0xffffffffu, mask != 0u)) {
-#pragma unroll
-              for (int c = 0; c < 32; ++c) {
-                const float v = fast_exp2(fmaf(s[c], sl2, l4[c]));
-                acc[c & 3] += (mask >> c) & 1u ? v : 0.f;
-              }
+          for (int j = 0; j < 4; ++j) {
+            const int t = min(x.q0 + chunk * kUnit + lane, p.T - 1);
+            n_lse[j] = u + j < u1 ? __ldg(p.lse + (int64_t)t * p.H + x.hk * p.G + h) * -1.4426950408889634f : 0.f;
+            if (++h == p.G) {
+              h = 0;
+              ++chunk;
             }
           }
-          if (++h == p.G) {
-            h = 0;
-            ++chunk;
+        };
+        int mine = u0 + 4 * ((cg - sc) & 3);  // the group's first step of the item
+        if (mine < u1) fetch(mine);
+        for (int u = u0; u < u1; u += 4, ++sc) {
+          if (u != mine) continue;
+          const int sb = sc % kSBufs;
+          __syncwarp();  // every lane is past its reads of the previous step's values
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s_lse[32 * j + lane] = n_lse[j];
+          __syncwarp();
+          mine += 16;
+          if (mine < u1) fetch(mine);
+          const bool ok = __all_sync(0xffffffffu,
+                                     wait_or_abort(&bar[kBarSFull + sb], (uint32_t)((sc / kSBufs) & 1), dead, p.err));
+          if (!ok) dead = true;
+          tc_fence_after();
+          int chunk = u / p.G, h = u - chunk * p.G;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (ok && u + j < u1) {
+              float s[32];
+              tmem_ld32(tmem + lane_base + 128 * sb + 32 * j, s);
+              tmem_wait_ld();
+              // visible columns [a, e): rows at or past the key, inside its window, and counted
+              const int pc = x.p0 + chunk * kUnit;
+              const int a = max(key - pc, 0);
+              int e = min(kUnit, x.nq - chunk * kUnit);
+              if (p.window > 0 && key >= p.n_sink) e = (int)min((int64_t)e, (int64_t)key + p.window - pc);
+              const uint32_t mask = (a >= e || e <= 0) ? 0u : (0xFFFFFFFFu >> (32 - e)) & (0xFFFFFFFFu << a);
+              const bool full = __all_sync(0xffffffffu, mask == 0xFFFFFFFFu);
+              const float* l4 = s_lse + 32 * j;
+              if (full) {
+#pragma unroll
+                for (int c = 0; c < 32; c += 4) {
+                  const float4 l = *reinterpret_cast<const float4*>(l4 + c);
+                  float x0, x1, x2, x3;
+                  scale_add(x0, x1, s[c], s[c + 1], sl2, l.x, l.y);
+                  scale_add(x2, x3, s[c + 2], s[c + 3], sl2, l.z, l.w);
+                  fadd2(acc[0], acc[1], fast_exp2(x0), fast_exp2(x1));
+                  fadd2(acc[2], acc[3], fast_exp2(x2), fast_exp2(x3));
+                }
+              } else if (__any_sync(0xffffffffu, mask != 0u)) {
+#pragma unroll
+                for (int c = 0; c < 32; ++c) {
+                  const float v = fast_exp2(fmaf(s[c], sl2, l4[c]));
+                  acc[c & 3] += (mask >> c) & 1u ? v : 0.f;
+                }
+              }
+            }
+            if (++h == p.G) {
+              h = 0;
+              ++chunk;
+            }
           }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_one(&bar[kBarSEmpty + sb]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_one(&bar[kBarSEmpty + sb]);
+        float add = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+        bool writer = true;
+        if (!resident) {
+          // the four groups' parts of a cache row, added in group order by one group (in turn)
+          const int b = ic & 1;
+          const uint32_t ph = (uint32_t)(ic >> 1) & 1u;
+          float* sa = s_acc + b * 4 * kM;
+          if (!__all_sync(0xffffffffu, wait_or_abort(&bar[kBarAccEmpty + b], ph ^ 1u, dead, p.err))) dead = true;
+          if (!dead) sa[cg * kM + row] = add;
+          __syncwarp();
+          if (lane == 0) mbar_arrive_one(&bar[kBarAccFull + b]);
+          writer = (ic & 3) == cg;
+          if (writer) {
+            if (!__all_sync(0xffffffffu, wait_or_abort(&bar[kBarAccFull + b], ph, dead, p.err))) dead = true;
+            add = (sa[row] + sa[kM + row]) + (sa[2 * kM + row] + sa[3 * kM + row]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive_one(&bar[kBarAccEmpty + b]);
+          }
+          ++ic;
+        }
+        if (writer && key < x.n && !dead) {
+          float* w = p.w + (int64_t)x.r * p.w_sb + (int64_t)x.hk * p.w_su + key;
+          // one addition per element and launch: without waiting for the old value
+          if (p.w_out)
+            *w = add;
+          else
+            atomicAdd(w, add);
+        }
       }
-      float add = (acc[0] + acc[1]) + (acc[2] + acc[3]);
-      if (!resident) {
-        // the four groups' parts of a cache row, added in order
-        float* sa = s_acc + (ic & 1) * 4 * kM;
-        sa[cg * kM + row] = add;
-        named_bar_sync(1, 512);
-        add = (sa[row] + sa[kM + row]) + (sa[2 * kM + row] + sa[3 * kM + row]);
-        ++ic;
-      }
-      if ((resident || cg == 0) && key < x.n && !dead) {
-        float* w = p.w + (int64_t)r * p.w_sb + (int64_t)hk * p.w_su + key;
-        // one addition per element and launch: without waiting for the old value
-        if (p.w_out)
-          *w = add;
-        else
-          atomicAdd(w, add);
-      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_one(&bar[kBarItemEmpty + (grp & (kItemGroups - 1))]);
     }
   }
   tc_fence_before();
