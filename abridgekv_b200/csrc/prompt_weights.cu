@@ -43,6 +43,7 @@ __host__ __device__ constexpr int k_stages(bool resident) { return resident ? 4 
 __host__ __device__ constexpr int q_stages(bool resident) { return kStages - k_stages(resident); }
 constexpr int kMaxK = 4, kMaxQ = 4;
 constexpr uint32_t kIdescS = idesc_bf16_m128(kN, false);
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTileBytes = kM * kD * 2;  // 2 atoms of [128 rows][128 B]
 constexpr int kOffK = 0;
 constexpr int kOffLse = kOffK + kStages * kTileBytes;   // 16 warps x [128] floats
@@ -413,6 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
     float* s_lse = reinterpret_cast<float*>(smem + kOffLse) + sw * kN;  // this warp's: a step's 128 rows
     float* s_acc = reinterpret_cast<float*>(smem + kOffAcc);
     const float sl2 = p.scale_log2;
+    const int ahead = 16 / p.G;  // whole chunks from a group's step to its next
     int sc = 0, ic = 0;
     for (int base = 0, grp = 0; base < it.n && !dead; base += kItemGroup, ++grp) {
       if (!__all_sync(0xffffffffu, items_ready(grp))) {
@@ -429,36 +431,43 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
         }
         const int key = x.kt * kM + row;
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        // log-sum-exp (negated, log2 units) of a step's rows, lane = row of each of its four units
+        // log-sum-exp of a step's rows, lane = row of each of its four units
         float n_lse[4];
-        auto fetch = [&](int u) {
-          int chunk = u / p.G, h = u - chunk * p.G;
+        int mine = u0 + 4 * ((cg - sc) & 3);  // the group's first step of the item
+        int f_chunk = mine / p.G, f_h = mine - f_chunk * p.G;  // chunk and head of unit `mine`
+        auto fetch = [&]() {
+          int chunk = f_chunk, h = f_h;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int t = min(x.q0 + chunk * kUnit + lane, p.T - 1);
-            n_lse[j] = u + j < u1 ? __ldg(p.lse + (int64_t)t * p.H + x.hk * p.G + h) * -1.4426950408889634f : 0.f;
+            n_lse[j] = mine + j < u1 ? __ldg(p.lse + (int64_t)t * p.H + x.hk * p.G + h) : 0.f;
             if (++h == p.G) {
               h = 0;
               ++chunk;
             }
           }
         };
-        int mine = u0 + 4 * ((cg - sc) & 3);  // the group's first step of the item
-        if (mine < u1) fetch(mine);
+        if (mine < u1) fetch();
         for (int u = u0; u < u1; u += 4, ++sc) {
           if (u != mine) continue;
           const int sb = sc % kSBufs;
           __syncwarp();  // every lane is past its reads of the previous step's values
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s_lse[32 * j + lane] = n_lse[j];
+          for (int j = 0; j < 4; ++j) s_lse[32 * j + lane] = n_lse[j] * -kLog2e;
           __syncwarp();
+          int chunk = f_chunk, h = f_h;
           mine += 16;
-          if (mine < u1) fetch(mine);
+          f_chunk += ahead;
+          f_h += 16 - ahead * p.G;
+          if (f_h >= p.G) {
+            f_h -= p.G;
+            ++f_chunk;
+          }
+          if (mine < u1) fetch();
           const bool ok = __all_sync(0xffffffffu,
                                      wait_or_abort(&bar[kBarSFull + sb], (uint32_t)((sc / kSBufs) & 1), dead, p.err));
           if (!ok) dead = true;
           tc_fence_after();
-          int chunk = u / p.G, h = u - chunk * p.G;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (ok && u + j < u1) {
@@ -634,7 +643,7 @@ extern "C" int abkv_prompt_weights(const void* q, int64_t q_row_stride, int64_t 
   prm.window = window;
   prm.n_sink = num_sinks;
   prm.max_query_len = max_query_len;
-  prm.scale_log2 = scale * 1.4426950408889634f;
+  prm.scale_log2 = scale * kLog2e;
   int dev = 0, num_sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess ||
       cudaDeviceGetAttribute(&num_sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || num_sms <= 0)
