@@ -56,13 +56,15 @@ static_assert(Lay<128>::kSmem <= 227 * 1024, "shared memory");
 static_assert(2 * kT * Lay<128>::kRedStride * 4 <= (kLong + kShort) * Lay<128>::kTile, "cluster reduction");
 static_assert(2 * kT * Lay<64>::kRedStride * 4 <= (kLong + kShort) * Lay<64>::kTile, "cluster reduction");
 
-// barriers: stationary operands, long ring full / empty, short ring full / empty, S full (two in the dQ kernel),
-// dP full, P ready (dQ: dP read), dS ready, accumulators complete / drained, statistics [column group][buffer] (a barrier per buffer:
-// the writer may be a pair ahead of a reader, and a parity wait cannot tell phases 2 apart), stationary operands
-// released, work item full / empty (two deep), then the TMEM address and the items
+// barriers: stationary operands, long ring full / empty, short ring full / empty, S full (two in the dQ kernel), dP
+// full, P ready (dQ: dP read), dS ready (two in the dQ kernel), accumulators complete / drained, statistics [column
+// group][buffer], stationary operands released, work item full / empty (two deep), then the TMEM address and the
+// items.  One barrier per buffer wherever an arrival may be a pair ahead of a wait (a parity wait cannot tell phases 2
+// apart): the statistics' writer runs ahead of their readers, and dS(u+1) may be ready before the issuer, which put
+// dP(u+1) under way before it, has looked at dS(u).
 constexpr int kBarA = 0, kBarLF = 1, kBarLE = kBarLF + kLong, kBarSF = kBarLE + kLong, kBarSE = kBarSF + kShort,
               kBarS = kBarSE + kShort, kBarDP = kBarS + 2, kBarP = kBarDP + 1, kBarDS = kBarP + 1,
-              kBarAcc = kBarDS + 1, kBarDrain = kBarAcc + 1, kBarStat = kBarDrain + 1, kBarAE = kBarStat + 8,
+              kBarAcc = kBarDS + 2, kBarDrain = kBarAcc + 1, kBarStat = kBarDrain + 1, kBarAE = kBarStat + 8,
               kBarIF = kBarAE + 1, kBarIE = kBarIF + 2, kBarTmem = kBarIE + 2, kBarItem = kBarTmem + 1;
 static_assert((kBarItem + 1) * 8 <= 512, "barrier area");
 
@@ -529,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBarTmem; ++i)
-      mbar_init(&bar[i], (i == kBarDS || i == kBarP || i == kBarDrain) ? kWorkers : 1);
+      mbar_init(&bar[i], (i == kBarDS || i == kBarDS + 1 || i == kBarP || i == kBarDrain) ? kWorkers : 1);
   }
   if (warp == 1) alloc_tmem(s_tmem);
   tc_fence_before();
@@ -591,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
       const uint64_t k_mn = desc_mnmajor_sw128(smem_u32(smem + LY::kOffLong), LY::kAtom);
       Pos<kLong> kf, ke;  // next K to read for scores; K of the current tile
       Pos<kShort> vf;
-      uint32_t par = 0, sbuf = 0, it_par = 0;
+      uint32_t sbuf = 0, it_par = 0;
       auto scores = [&]() -> bool {  // S of the next tile into its buffer, over the dS that dQ has read
         if (!wait_or_abort(&bar[kBarLF + kf.i], kf.ph, dead, p.err)) return false;
         tc_fence_after();
@@ -611,20 +613,21 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
         return true;
       };
       int it = 0;
-      uint32_t buf = 0;  // S buffer of the current tile, which dS takes over
+      uint32_t g = 0;  // tiles so far; tile g's S buffer, which dS takes over, is g & 1
       for (int i = blockIdx.x; i < n_items && !dead; i += gridDim.x, ++it) {
         const Item x = decode(i);
         if (!wait_or_abort(&bar[kBarA], it_par, dead, p.err) || !scores()) break;
         // the last dP of the previous item has been read
-        if (it > 0 && !wait_or_abort(&bar[kBarP], par ^ 1u, dead, p.err)) break;
+        if (it > 0 && !wait_or_abort(&bar[kBarP], (g & 1u) ^ 1u, dead, p.err)) break;
         if (!dscores()) break;
         if (x.n == 1) umma_commit(&bar[kBarAE]);
         if (x.n > 1 && !scores()) break;
-        for (int u = 0; u < x.n; ++u, par ^= 1u, buf ^= 1u) {
+        for (int u = 0; u < x.n; ++u, ++g) {
+          const uint32_t buf = g & 1u;
           // dP has been read: the next one, beside the forming of dS
-          if (u + 1 < x.n && (!wait_or_abort(&bar[kBarP], par, dead, p.err) || !dscores())) break;
+          if (u + 1 < x.n && (!wait_or_abort(&bar[kBarP], buf, dead, p.err) || !dscores())) break;
           if (u + 2 == x.n) umma_commit(&bar[kBarAE]);  // the item's last scores are issued: Q and dO are free then
-          if (!wait_or_abort(&bar[kBarDS], par, dead, p.err)) break;
+          if (!wait_or_abort(&bar[kBarDS + buf], (g >> 1) & 1u, dead, p.err)) break;
           // the first product of an item overwrites dQ: the previous one has been read out
           if (u == 0 && it > 0 && !wait_or_abort(&bar[kBarDrain], it_par ^ 1u, dead, p.err)) break;
           tc_fence_after();
@@ -696,7 +699,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_one(&bar[kBarDS]);
+        if (lane == 0) mbar_arrive_one(&bar[kBarDS + (g & 1)]);
       }
       if (!__all_sync(0xffffffffu, wait_or_abort(&bar[kBarAcc], (uint32_t)(it & 1), dead, p.err))) dead = true;
       tc_fence_after();
