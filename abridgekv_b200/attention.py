@@ -34,6 +34,10 @@ Every attention call runs a libabkv kernel (abkv_decode, abkv_decode_packed,
 abkv_paged_prefill[_packed], abkv_code_step_attention[_packed], abkv_store_kv).
 There is no CPU path and no fallback.  Masked (non-physical) per-layer quotas,
 which the kernels do not serve, raise ``NotImplementedError``.
+
+A layer with a sliding window (``sliding_window``, and ``num_sinks`` leading rows
+that stay visible) runs its causal steps through ``abkv_decode_window`` and
+``abkv_paged_prefill_window``.  The code step and the packed hook have no window.
 """
 from __future__ import annotations
 
@@ -201,15 +205,25 @@ class AbkvAttentionImpl:
     ``forward(layer, query, key, value, kv_cache, attn_metadata, output)``: query ``[T, Hq, D]``
     (or ``[T, Hq*D]``), key / value ``[T, Hkv, D]`` (the step's new rows; None to skip the cache
     write), kv_cache ``[num_blocks, 2, page, Hkv, D]`` bf16, output ``[T, Hq*D]`` (written in place
-    for the step's ``num_actual_tokens`` rows and returned)."""
+    for the step's ``num_actual_tokens`` rows and returned).
+
+    ``sliding_window`` rows (None or -1: all), the query's own among them, and the first ``num_sinks``
+    rows of the cache are seen by a causal step's query."""
 
     def __init__(self, num_heads: int, head_size: int, scale: float, num_kv_heads: int | None = None,
                  alibi_slopes: Any = None, sliding_window: int | None = None, kv_cache_dtype: str = "auto",
                  logits_soft_cap: float | None = None, attn_type: str = "decoder",
-                 kv_sharing_target_layer_name: str | None = None, workspace: Workspace | None = None):
-        if alibi_slopes is not None or sliding_window not in (None, -1) or logits_soft_cap:
-            raise NotImplementedError("alibi, sliding windows and logit soft-capping are not part of the "
+                 kv_sharing_target_layer_name: str | None = None, workspace: Workspace | None = None,
+                 num_sinks: int = 0):
+        if alibi_slopes is not None or logits_soft_cap:
+            raise NotImplementedError("alibi and logit soft-capping are not part of the "
                                       "compressed-cache attention path")
+        self.window = None if sliding_window in (None, -1) else int(sliding_window)
+        self.num_sinks = int(num_sinks)
+        if self.window is not None and self.window < 1:
+            raise ValueError(f"sliding_window must be at least 1 (None or -1: no window), got {sliding_window}")
+        if self.num_sinks < 0 or (self.num_sinks and self.window is None):
+            raise ValueError(f"num_sinks={num_sinks} needs a sliding_window and must not be negative")
         if kv_cache_dtype not in ("auto", "bfloat16"):
             raise NotImplementedError(f"kv_cache_dtype {kv_cache_dtype!r}: the kernels read bf16 caches")
         self.num_heads = int(num_heads)
@@ -241,18 +255,24 @@ class AbkvAttentionImpl:
                      workspace=ws)
         q = query[:T].view(T, Hq, D)
         out = output[:T].view(T, Hq, D)
-        attend(q, kv_cache, md, out, num_kv_heads=Hkv, scale=self.scale, workspace=ws)
+        attend(q, kv_cache, md, out, num_kv_heads=Hkv, scale=self.scale, workspace=ws, window=self.window,
+               num_sinks=self.num_sinks)
         return output
 
 
 def attend(q: torch.Tensor, kv_cache: torch.Tensor, md: AbkvAttentionMetadata, out: torch.Tensor, *,
            num_kv_heads: int, scale: float, workspace: Workspace | None = None,
            k_max: int | None = None, quota_per_kv_head: Sequence[int] | None = None,
-           excluded: torch.Tensor | None = None, sidecar: SidecarPool | None = None) -> None:
+           excluded: torch.Tensor | None = None, sidecar: SidecarPool | None = None,
+           window: int | None = None, num_sinks: int = 0) -> None:
     """Attention of one layer's step over its KV-cache group (the dispatch of AbkvAttentionImpl and of
     the sidecar hook): decode, causal paged prefill, or the code step; with a sidecar pool, the causal
-    prefill and the code step read the requests' packed pages first.  q / out ``[T, Hq, D]``."""
+    prefill and the code step read the requests' packed pages first.  q / out ``[T, Hq, D]``.
+    ``window`` / ``num_sinks``: a sliding window with sinks, in causal steps without a sidecar."""
     R = md.num_reqs
+    if window is not None and (not md.causal or sidecar is not None):
+        raise NotImplementedError("a sliding window is served in causal steps over the paged cache alone, "
+                                  "not in the code step nor over packed pages")
     if R == 0 or md.num_actual_tokens == 0:
         return
     if md.causal:
@@ -260,10 +280,20 @@ def attend(q: torch.Tensor, kv_cache: torch.Tensor, md: AbkvAttentionMetadata, o
             qc = q if q.is_contiguous() else q.contiguous()
             direct = out.is_contiguous()
             o = out if direct else torch.empty_like(qc)
-            decode.paged_decode([qc[:R]], [kv_cache], [md.block_table], [md.seq_lens], scale=scale,
-                                outputs=[o[:R]], workspace=workspace)
+            if window is not None:
+                decode.paged_decode_window([qc[:R]], [kv_cache], [md.block_table], [md.seq_lens], window=window,
+                                           num_sinks=num_sinks, scale=scale, outputs=[o[:R]], workspace=workspace)
+            else:
+                decode.paged_decode([qc[:R]], [kv_cache], [md.block_table], [md.seq_lens], scale=scale,
+                                    outputs=[o[:R]], workspace=workspace)
             if not direct:
                 out.copy_(o)
+            return
+        if window is not None:
+            codestep.paged_prefill_window(q, kv_cache, md.block_table, md.seq_lens, md.query_start_loc,
+                                          max_query_len=md.max_query_len, num_kv_heads=num_kv_heads, window=window,
+                                          num_sinks=num_sinks, scale=scale, num_requests=R, out=out,
+                                          kv_layout=0, workspace=workspace)
             return
         codestep.paged_prefill(q, kv_cache, md.block_table, md.seq_lens, md.query_start_loc,
                                max_query_len=md.max_query_len, num_kv_heads=num_kv_heads, scale=scale,
@@ -424,6 +454,8 @@ class CompressedKVSidecar:
             return
         if query.dtype != torch.bfloat16:
             raise RuntimeError(f"packed KV attention on libabkv needs bf16 queries, got {query.dtype}")
+        if getattr(layer.impl, "window", None) is not None:
+            raise NotImplementedError("packed KV attention has no sliding window")
         common = self.common_attn_metadata
         if common is None:
             raise RuntimeError("packed KV common attention metadata is absent")

@@ -179,7 +179,24 @@ def _i32(name: str, t, device, dim: int, rows: int) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _window_rows(query, kv_cache, block_table, seq_lens, query_start_loc, num_kv_heads, num_requests, max_query_len):
+def _given_layout(kv: torch.Tensor, kv_layout: int | None) -> int:
+    """kv_layout, or the layout that the shape of a paged cache shows: 0 [blocks, 2, ...], 1 [2, blocks, ...]."""
+    if kv_layout not in (None, 0, 1):
+        raise ValueError("kv_layout must be 0 ([blocks, 2, page, Hkv, D]) or 1 ([2, blocks, page, Hkv, D]), "
+                         f"got {kv_layout}")
+    if kv.dim() != 5 or not kv.is_contiguous():
+        raise ValueError("kv_cache must be a contiguous 5-D paged cache")
+    if kv_layout is None:
+        if kv.shape[0] == kv.shape[1] == 2:
+            raise ValueError("a cache of two blocks fits both layouts: say which with kv_layout")
+        kv_layout = 0 if kv.shape[1] == 2 else 1
+    if kv.shape[1 - kv_layout] != 2:
+        raise ValueError(f"unrecognised paged KV layout {tuple(kv.shape)}")
+    return kv_layout
+
+
+def _window_rows(query, kv_cache, block_table, seq_lens, query_start_loc, num_kv_heads, num_requests, max_query_len,
+                 kv_layout):
     """Checks the paged arguments of the window entry points -> (R, page, block_table, the C call's arguments
     from query_start_loc to head_dim, without those of the output)."""
     for name, t in (("query", query), ("kv_cache", kv_cache)):
@@ -191,7 +208,10 @@ def _window_rows(query, kv_cache, block_table, seq_lens, query_start_loc, num_kv
     Hkv = int(num_kv_heads)
     if Hkv <= 0 or Hq % Hkv:
         raise ValueError("the KV heads must divide the query heads")
-    layout, nb, page = _layout_of(kv_cache, Hkv)
+    layout = _given_layout(kv_cache, kv_layout)
+    nb, page = kv_cache.shape[layout], kv_cache.shape[2]
+    if kv_cache.shape[3] != Hkv:
+        raise ValueError(f"the cache holds {kv_cache.shape[3]} heads, not {Hkv}")
     if kv_cache.shape[4] != D:
         raise ValueError(f"the cache's head size {kv_cache.shape[4]} is not the query's {D}")
     device = query.device
@@ -211,11 +231,14 @@ def paged_prefill_window(query: torch.Tensor, kv_cache: torch.Tensor, block_tabl
                          seq_lens: torch.Tensor, query_start_loc: torch.Tensor, *, max_query_len: int,
                          num_kv_heads: int, window: int | None, num_sinks: int = 0, scale: float | None = None,
                          num_requests: int | None = None, out: torch.Tensor | None = None, return_lse: bool = False,
-                         workspace: Workspace | None = None, stream: torch.cuda.Stream | None = None):
+                         kv_layout: int | None = None, workspace: Workspace | None = None,
+                         stream: torch.cuda.Stream | None = None):
     """``paged_prefill`` under a sliding window with sinks (``abkv_paged_prefill_window``): the row at
     position p of its request sees cache rows j <= p with j > p - window or j < num_sinks.  A window
     of None or 0 shows every row j <= p.  Pages that hold no visible row are never read, and their
-    block-table entries may be stale (freed pages).
+    block-table entries may be stale (freed pages).  ``kv_layout``: 0 for a cache [blocks, 2, page, Hkv,
+    D], 1 for [2, blocks, page, Hkv, D]; None reads it off the shape, which a cache of two blocks does
+    not show.
 
     Returns out [T, Hq, D], or (out, lse) with ``return_lse``: lse [T, Hq] fp32, the natural-log
     log-sum-exp of each row's scaled scores, which ``paged_prompt_weights`` takes.  Rows of no request
@@ -226,7 +249,7 @@ def paged_prefill_window(query: torch.Tensor, kv_cache: torch.Tensor, block_tabl
     device, shape = query.device, query.shape
     with call_scope(device, stream):
         R, Hkv, _, keep, tail = _window_rows(query, kv_cache, block_table, seq_lens, query_start_loc, num_kv_heads,
-                                             num_requests, max_query_len)
+                                             num_requests, max_query_len, kv_layout)
         if out is None:
             out = torch.empty(shape, dtype=torch.bfloat16, device=device)
         elif out.shape != shape or out.dtype != torch.bfloat16 or out.stride(2) != 1 or out.device != device:
@@ -247,11 +270,11 @@ def paged_prompt_weights(query: torch.Tensor, lse: torch.Tensor, kv_cache: torch
                          seq_lens: torch.Tensor, query_start_loc: torch.Tensor, weights: torch.Tensor, *,
                          max_query_len: int, num_kv_heads: int, observe: int | None = None, window: int | None = None,
                          num_sinks: int = 0, scale: float | None = None, num_requests: int | None = None,
-                         workspace: Workspace | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+                         kv_layout: int | None = None, workspace: Workspace | None = None, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
     """Add the attention weights of prompt rows to per-row accumulators (``abkv_prompt_weights``).
 
-    The arguments of ``paged_prefill_window`` (same window, num_sinks and scale) plus the ``lse`` [T, Hq] it
-    returned.  Request r's counted rows are its last ``observe`` query rows (None: all of them); every
+    The arguments of ``paged_prefill_window`` (same window, num_sinks and scale) plus the ``lse`` [T, Hq]
+    that it returned.  Request r's counted rows are its last ``observe`` query rows (None: all of them); every
     cache row that they see collects their softmax weight in ``weights`` [>=R, units, rows] fp32 (rows
     contiguous, at least as many as the longest sequence): unit u = KV head u's query heads, or one unit
     for all heads.  The sums' order is fixed, so repeated calls give the same bits.  Returns weights."""
@@ -265,7 +288,7 @@ def paged_prompt_weights(query: torch.Tensor, lse: torch.Tensor, kv_cache: torch
     device = query.device
     with call_scope(device, stream):
         R, Hkv, page, keep, tail = _window_rows(query, kv_cache, block_table, seq_lens, query_start_loc, num_kv_heads,
-                                                num_requests, max_query_len)
+                                                num_requests, max_query_len, kv_layout)
         T, Hq, D = query.shape
         if lse.shape != (T, Hq) or not lse.is_contiguous() or lse.device != device:
             raise ValueError(f"lse must be the attention's contiguous [{T}, {Hq}] log-sum-exp on the query's device")

@@ -29,6 +29,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .codestep import _given_layout
 from .workspace import Workspace, call_scope, call_workspace, default_workspace
 
 
@@ -248,7 +249,7 @@ def evict_by_weight(kv_caches: Sequence[torch.Tensor], block_tables: Sequence[to
                     seq_lens: Sequence[torch.Tensor], weights: Sequence[torch.Tensor], *,
                     budget: int | Sequence[int], num_sinks: int = 0, num_recent: int = 0,
                     dst_block_tables: Sequence[torch.Tensor] | None = None, return_keep: bool = False,
-                    in_place_weights: bool = False, workspace: Workspace | None = None,
+                    in_place_weights: bool = False, kv_layout: int | None = None, workspace: Workspace | None = None,
                     stream: torch.cuda.Stream | None = None) -> Evicted:
     """Bring every sequence back to ``budget`` rows by accumulated attention weight (``abkv_evict_by_weight``).
 
@@ -262,7 +263,9 @@ def evict_by_weight(kv_caches: Sequence[torch.Tensor], block_tables: Sequence[to
     Rows move inside the sequence's own pages (the pages past the new length are then free), or,
     with ``dst_block_tables``, into the pages of those tables, which must be other pages of the same
     caches.  The new weights are new tensors of ``weights``' shape, or ``weights`` themselves with
-    ``in_place_weights``.  ``seq_lens`` stays as it was; go on with the returned lengths."""
+    ``in_place_weights``.  ``seq_lens`` stays as it was; go on with the returned lengths.  In place, a
+    page that two sequences share (a cached prefix) would be moved for both: evict into other pages then.
+    ``kv_layout``: as in ``codestep.paged_prefill_window``."""
     L = len(kv_caches)
     if L == 0 or not (L == len(block_tables) == len(seq_lens) == len(weights)):
         raise ValueError("per-layer argument lists must be non-empty and of equal length")
@@ -276,7 +279,8 @@ def evict_by_weight(kv_caches: Sequence[torch.Tensor], block_tables: Sequence[to
         raise ValueError("every budget must be positive and hold num_sinks + num_recent rows (both >= 0), "
                          f"got budget {budgets}, num_sinks {num_sinks}, num_recent {num_recent}")
     dev = kv_caches[0].device
-    layout, _, page, hkv, d = _layout_of(kv_caches[0])
+    layout = _given_layout(kv_caches[0], kv_layout)
+    page, hkv, d = kv_caches[0].shape[2:]
     B = int(seq_lens[0].shape[0])
     units, rows = int(weights[0].shape[1]) if weights[0].dim() == 3 else 0, int(weights[0].shape[-1])
 

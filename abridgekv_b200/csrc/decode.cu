@@ -1664,7 +1664,8 @@ int plan_window(int num_layers, int num_seqs, int num_q_heads, int num_kv_heads,
                 int max_pages, int chunk_tokens, const int32_t* windows, const int32_t* sinks, int weighted,
                 WindowPlan* plan) {
   if (num_layers <= 0 || num_seqs <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || page_size <= 0 ||
-      max_pages <= 0 || num_q_heads % num_kv_heads || chunk_tokens < 0 || chunk_tokens % kTile)
+      max_pages <= 0 || num_q_heads % num_kv_heads || chunk_tokens < 0 || chunk_tokens % kTile ||
+      (weighted != 0 && weighted != 1 && weighted != num_kv_heads))
     return ABKV_ERR_INVALID_ARG;
   if ((head_dim != 64 && head_dim != kD) || page_size % kTile != 0 || num_seqs > 65535 ||
       kWarps % num_kv_heads != 0 || num_q_heads / num_kv_heads > kMaxG)
