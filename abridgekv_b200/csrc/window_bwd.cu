@@ -144,6 +144,11 @@ __device__ __forceinline__ void sub_mul_pair(float& d0, float& d1, float a0, flo
       : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
 }
 
+// w = bf16 roundings of the pair a, b; returns those of what they leave out.
+__device__ __forceinline__ uint32_t pack_rest(uint32_t w, float a, float b) {
+  return pack_bf16x2(a - __uint_as_float(w << 16), b - __uint_as_float(w & 0xFFFF0000u));
+}
+
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;\n" ::: "memory");
 }
@@ -161,7 +166,7 @@ __device__ __forceinline__ float4 peer_ld4(uint32_t local, int rank) {
 // under way while the finished accumulators are read out.  With p.cluster > 1 (idle SMs, or the sinks' tiles, which
 // every query tile sees) a cluster takes one item, its CTAs share the pairs and add their parts, in rank order,
 // through shared memory.
-template <int D>
+template <int D, bool kRest>
 __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_constant__ WinBwdParams p) {
   using LY = Lay<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -314,6 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
           if (!wait_or_abort(&bar[kBarDS], par, dead, p.err)) break;
           tc_fence_after();
           issue_accumulate<D>(tmem + 384, tmem + 128, q_mn + qe.i * kStep, u == 0);
+          if (kRest) issue_accumulate<D>(tmem + 384, tmem + 128 + 16, q_mn + qe.i * kStep, false);
           umma_commit(&bar[kBarLE + qe.i]);
           qe.step();
           if (u + 1 < x.n && !dscores()) break;
@@ -420,8 +426,17 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
             sub_mul_pair(dp[c + 2], dp[c + 3], dp[c + 2], dp[c + 3], d.z, d.w, pv[c + 2], pv[c + 3]);
             w[c / 2] = pack_bf16x2(dp[c], dp[c + 1]);
             w[c / 2 + 1] = pack_bf16x2(dp[c + 2], dp[c + 3]);
+            if (kRest) {
+              dp[c / 2] = __uint_as_float(pack_rest(w[c / 2], dp[c], dp[c + 1]));
+              dp[c / 2 + 1] = __uint_as_float(pack_rest(w[c / 2 + 1], dp[c + 2], dp[c + 3]));
+            }
           }
           tmem_st16(tmem + lane_base + 128 + 32 * cg, w);
+          if (kRest) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) w[c] = __float_as_uint(dp[c]);
+            tmem_st16(tmem + lane_base + 128 + 16 + 32 * cg, w);
+          }
           tmem_wait_st();
         }
         tc_fence_before();
@@ -513,10 +528,13 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
 }
 
 // ---------------------------------------------------------------------------
+// kRest in either kernel: dS = bf16 part + bf16 rest, one product each; the rest takes the 16 words of TMEM that the bf16
+// part leaves of its 32.
+//
 // dQ.  A work item is a 128-query tile of one head: it walks the key tiles that the tile sees (the sinks', then the
 // window's).  A CTA per SM takes items round robin, the longest first; the next item's operands are loaded and its
 // first scores computed while the finished dQ is read out.
-template <int D>
+template <int D, bool kRest>
 __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_constant__ WinBwdParams p) {
   using LY = Lay<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -632,6 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
           if (u == 0 && it > 0 && !wait_or_abort(&bar[kBarDrain], it_par ^ 1u, dead, p.err)) break;
           tc_fence_after();
           issue_accumulate<D>(tmem + 384, tmem + 128 * buf, k_mn + ke.i * kStep, u == 0);
+          if (kRest) issue_accumulate<D>(tmem + 384, tmem + 128 * buf + 16, k_mn + ke.i * kStep, false);
           umma_commit(&bar[kBarLE + ke.i]);
           ke.step();
           if (u + 2 < x.n && !scores()) break;
@@ -691,8 +710,14 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
           for (int c = 0; c < 32; c += 2) {
             sub_mul_pair(dp[c], dp[c + 1], dp[c], dp[c + 1], di, di, pv[c], pv[c + 1]);
             w[c / 2] = pack_bf16x2(dp[c], dp[c + 1]);
+            if (kRest) dp[c / 2] = __uint_as_float(pack_rest(w[c / 2], dp[c], dp[c + 1]));
           }
           tmem_st16(tmem + lane_base + 128 * (g & 1) + 32 * cg, w);
+          if (kRest) {
+#pragma unroll
+            for (int c = 0; c < 16; ++c) w[c] = __float_as_uint(dp[c]);
+            tmem_st16(tmem + lane_base + 128 * (g & 1) + 16 + 32 * cg, w);
+          }
           tmem_wait_st();
         } else if (lane == 0) {
           mbar_arrive_one(&bar[kBarP]);
@@ -785,17 +810,23 @@ int make_map(CUtensorMap* m, const void* base, int B, int heads, int S, int D, c
 
 constexpr size_t kWsHeader = 256;
 constexpr int kSms = 148;
+// dS is rounded to bf16 for the products of dQ and dK: one more error beside the rounding of the result, sqrt(2) of
+// that one alone where many terms average it (1.43 measured with windows of 512 to 2000).  Rows of few terms, of which
+// some dominate, come out worse (up to 1.7 over 60 random shapes), so those launches add a second product with what
+// the rounding left out (kRest: 1.25 at most).  It costs 33.0 -> 33.1 us at 333 rows of 8 heads, 377 -> 441 us at
+// 2 x 4096 rows of 32 heads with a window of 256, and would cost 497 -> 594 us with one of 1024.
+constexpr int kRestKeys = 512;
 
-template <int D>
+template <int D, bool kRest>
 int launch(WinBwdParams& prm, const void* out, const int64_t* os, const int8_t* lo, const void* dout,
            const int64_t* ds, float* di, cudaStream_t s) {
   const int64_t threads = (int64_t)prm.B * prm.H * prm.S * (D / 8);
   window_rowdot_kernel<D><<<(unsigned)((threads + 255) / 256), 256, 0, s>>>(
       static_cast<const __nv_bfloat16*>(out), os[0], os[1], os[2], lo, static_cast<const __nv_bfloat16*>(dout), ds[0],
       ds[1], ds[2], di, prm.work, prm.B, prm.H, prm.S);
-  if (cudaFuncSetAttribute(window_dkdv_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::kSmem) !=
+  if (cudaFuncSetAttribute(window_dkdv_kernel<D, kRest>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::kSmem) !=
           cudaSuccess ||
-      cudaFuncSetAttribute(window_dq_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::kSmem) !=
+      cudaFuncSetAttribute(window_dq_kernel<D, kRest>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<D>::kSmem) !=
           cudaSuccess)
     return ABKV_ERR_CUDA;
   // Each kernel may be set up while the one before it drains; the last ones run beside one another.
@@ -817,7 +848,7 @@ int launch(WinBwdParams& prm, const void* out, const int64_t* os, const int8_t* 
     attr[1].val.clusterDim = {(unsigned)cluster, 1, 1};
     cfg.gridDim = dim3((unsigned)(cluster > 1 ? items * cluster : std::min<int64_t>(items, kSms)));
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, window_dkdv_kernel<D>, prm) == cudaSuccess;
+    return cudaLaunchKernelEx(&cfg, window_dkdv_kernel<D, kRest>, prm) == cudaSuccess;
   };
   // Key tiles as (sinks', others), pairs per tile and in all.
   const int64_t heads = (int64_t)prm.Hkv * prm.B;
@@ -841,7 +872,7 @@ int launch(WinBwdParams& prm, const void* out, const int64_t* os, const int8_t* 
   }
   cfg.gridDim = dim3((unsigned)std::min<int64_t>((int64_t)prm.H * prm.B * prm.n_tiles, kSms));
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, window_dq_kernel<D>, prm) != cudaSuccess) return ABKV_ERR_CUDA;
+  if (cudaLaunchKernelEx(&cfg, window_dq_kernel<D, kRest>, prm) != cudaSuccess) return ABKV_ERR_CUDA;
   return cudaGetLastError() == cudaSuccess ? ABKV_OK : ABKV_ERR_CUDA;
 }
 
@@ -917,6 +948,9 @@ extern "C" int abkv_window_attention_backward(
   prm.n_sink = num_sinks < S ? num_sinks : S;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int8_t* lo = static_cast<const int8_t*>(out_lo);
-  return head_dim == 64 ? launch<64>(prm, out, out_strides, lo, dout, dout_strides, di, s)
-                        : launch<128>(prm, out, out_strides, lo, dout, dout_strides, di, s);
+  // Rows that see few keys: dS in two bf16 parts (kRestKeys).
+  const bool rest = std::min<int64_t>(S, (int64_t)window + num_sinks) <= kRestKeys;
+  auto run = head_dim == 64 ? (rest ? launch<64, true> : launch<64, false>)
+                            : (rest ? launch<128, true> : launch<128, false>);
+  return run(prm, out, out_strides, lo, dout, dout_strides, di, s);
 }
