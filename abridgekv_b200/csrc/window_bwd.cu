@@ -404,6 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
           }
 #pragma unroll
           for (int c = 0; c < 16; ++c) w[c] = pack_bf16x2(pv[2 * c], pv[2 * c + 1]);
+          if (q0 == 0) pv[0] = 0.f;  // query 0 sees one key: P = 1, dS = 0 exactly (also where every query does: scale)
           tmem_st16(tmem + lane_base + 32 * cg, w);
           tmem_wait_st();
         }
@@ -671,11 +672,12 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_kernel(const __grid_con
       const int q = x.qt * kT + row;
       const int64_t r = ((int64_t)x.b * p.H + x.h) * p.S + q;
       const bool in = q < p.S;
+      const bool live = in && q > 0;  // query 0 sees one key: P = 1, dS = 0 exactly
       const float nl = in ? -__ldg(p.lse + r) * kLog2e : 0.f, di = in ? __ldcg(p.di + r) : 0.f;
       for (int u = 0; u < x.n; ++u, ++g) {
         const int k0 = (u < x.ns ? u : u + x.shift) * kT + 32 * cg;
         // visible keys of this row among the warp's 32: k <= q without [n_sink, q - window + 1)
-        const uint32_t mask = in ? below(q + 1 - k0) & (below(p.n_sink - k0) | ~below(q - p.window + 1 - k0)) : 0u;
+        const uint32_t mask = live ? below(q + 1 - k0) & (below(p.n_sink - k0) | ~below(q - p.window + 1 - k0)) : 0u;
         const bool full = __all_sync(0xffffffffu, mask == 0xFFFFFFFFu);
         bool ok = __all_sync(0xffffffffu, wait_or_abort(&bar[kBarS + (g & 1)], (uint32_t)((g >> 1) & 1), dead, p.err));
         if (!ok) dead = true;
@@ -941,7 +943,8 @@ extern "C" int abkv_window_attention_backward(
   prm.G = H / Hkv;
   prm.S = S;
   prm.n_tiles = (S + kT - 1) / kT;
-  prm.scale = scale;
+  // where every query sees its own key alone the scores have no gradient: exactly, not as the difference of two sums
+  prm.scale = window == 1 && num_sinks == 0 ? 0.f : scale;
   prm.scale_log2 = scale * kLog2e;
   // a window past S hides nothing, sinks past S are every key: keep the tile arithmetic in 32 bits
   prm.window = window < S ? window : S;

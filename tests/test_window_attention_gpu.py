@@ -209,3 +209,23 @@ def test_refusals():
         prefill.window_backward(q, k, v, q, do, torch.zeros((1, 4, 39), device="cuda"), window=4)
     with pytest.raises(RuntimeError):
         prefill.window_forward(q, k, v, window=4, scale=-1.0, workspace=Workspace("cuda:0"))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("S,window,sinks,alone", [(1, 5, 0, 1), (1, 5, 3, 1), (150, 1, 0, 150), (150, 1, 2, 1), (150, 40, 0, 1),
+                                                  (700, 600, 4, 1)])
+def test_rows_that_see_one_key_have_no_score_gradient(D, S, window, sinks, alone):
+    """Their weight is 1 whatever the score, so dq is exactly 0 there, and dk where no other row sees the key."""
+    g = torch.Generator().manual_seed(S + D)
+    q, k, v, do = (torch.randn((2, h, S, D), generator=g).bfloat16().cuda() for h in (4, 2, 2, 4))
+    for t in (q, k, v):
+        t.requires_grad_()
+    out = prefill.window_attention(q, k, v, window=window, num_sinks=sinks)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), do)
+    assert torch.equal(out[:, :, :alone], v.repeat_interleave(2, 1)[:, :, :alone])
+    assert (dq[:, :, :alone] == 0).all() and (alone == S or (dq[:, :, alone:] != 0).any())
+    if alone == S:
+        assert (dk == 0).all()
+        # each key has its own row's gradient, summed over the two heads that share it
+        want = do.double().view(2, 2, 2, S, D).sum(2)
+        assert (dv.double() - want).abs().le(2.0 ** -8 * want.abs() + 1e-30).all()
