@@ -202,8 +202,8 @@ __device__ __noinline__ void commit_request_ops(const CodeStepParams& p, bool de
 // so both take the same lazy-rescale decision and reference maximum; each keeps
 // the row sum of its own columns and rescales its own half of O.  P (bf16,
 // 16 words) goes into this half's columns of the upper half of the S buffer.
-// kHole: columns [hs, he) are hidden as well (the code step's tail exclusion).
-template <bool kHole>
+// kHole: columns [hs, he) are hidden as well (the code step's tail exclusion).  kFull: none is hidden.
+template <bool kHole, bool kFull = false>
 __device__ __forceinline__ void softmax_half(const CodeStepParams& p, int lim, int hs, int he, int half, int row,
                                              uint32_t tmem_s, uint32_t tmem_o, uint32_t lane_base, int j,
                                              uint64_t* o_done, bool& dead, SoftmaxState& st, float* xm_mine,
@@ -226,7 +226,7 @@ __device__ __forceinline__ void softmax_half(const CodeStepParams& p, int lim, i
     const uint32_t lo = (1u << a) - 1u;  // a < 32 here
     return hi & ~lo;
   };
-  const bool full = lim == kBN && (!kHole || he <= 0 || hs >= kBN);
+  const bool full = kFull || (lim == kBN && (!kHole || he <= 0 || hs >= kBN));
   uint32_t vm = 0xFFFFFFFFu;  // only a partial tile needs the mask
   if (!full) {
     vm = span(0, lim - c0);
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
       mbar_init(&kv_empty[i], hB >= 0 ? 2 : 1);
     }
     for (int i = 0; i < 4; ++i) mbar_init(&s_full[i], 1);
-    for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 256);  // the 8 softmax warps of a head
+    for (int i = 0; i < 4; ++i) mbar_init(&p_full[i], 8);  // the softmax warps of a head
     for (int i = 0; i < 2; ++i) {
       mbar_init(&o_done[i], 1);
       mbar_init(&o_full[i], 1);
@@ -652,8 +652,31 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
         hole_e = leff - p.window;
       }
       int nz = 0;
+      // kWin: a key tile from full_lo on (or among the sinks) and up to full_hi is seen by every row of the query tile:
+      // most tiles, which skip the masks and the V rows to zero below
+      int full_lo = 0, full_hi = 0;
+      if constexpr (kWin) {
+        full_hi = seq_len - qlen + qt * kBM + 1;
+        const int last = seq_len - qlen + min(qt * kBM + kBM, qlen);
+        if (p.window > 0 && last - p.window > p.n_sink) full_lo = last - p.window;
+      }
       for (int j = 0; j < n_tiles; ++j) {
         const int e = s_list[j];
+        if constexpr (kWin) {
+          if (e * kBN + kBN <= full_hi && (e * kBN >= full_lo || e * kBN + kBN <= p.n_sink)) {
+            const bool ok = __all_sync(
+                0xffffffffu, wait_or_abort(&s_full[2 * head_slot + (j & 1)], (uint32_t)((j >> 1) & 1), dead, p.err));
+            if (!ok) dead = true;
+            tc_fence_after();
+            float* xm = xmax + ((j & 1) * 2 + head_slot) * 256;
+            softmax_half<false, true>(p, kBN, 0, 0, half, row, tmem_h + 64 * (j & 1), tmem_o, lane_base, j,
+                                      &o_done[head_slot], dead, st, xm + half * 128, xm + (1 - half) * 128, pair_bar, ok);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_one(&p_full[2 * head_slot + (j & 1)]);
+            continue;
+          }
+        }
         const bool side = !kWin && e < 0;  // sidecar tile -(e + 1): every query row sees its rows
         const int lim = side ? min(max(n_side - (-e - 1) * kBN, 0), kBN) : min(max(leff - e * kBN, 0), kBN);
         // valid rows of the tile: the rest was not loaded (V zeroed below)
@@ -701,7 +724,8 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
                            tmem_h + 64 * (j & 1), tmem_o, lane_base, j, &o_done[head_slot], dead, st,
                            xm + half * 128, xm + (1 - half) * 128, pair_bar, ok);
         tc_fence_before();  // P's tcgen05.st completed (wait::st) before the arrival
-        mbar_arrive_one(&p_full[2 * head_slot + (j & 1)]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&p_full[2 * head_slot + (j & 1)]);
       }
       // epilogue: this warp writes dims [64 half, 64 half + 64) of its rows
       const bool o_ok =

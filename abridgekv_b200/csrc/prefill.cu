@@ -129,8 +129,8 @@ struct alignas(64) PrefillParams {
 // so both take the same lazy-rescale decision and reference maximum; each keeps
 // the row sum of its own columns and rescales its own half of O (D / 2 columns).
 // P (bf16, 16 words) goes into this half's columns of the upper half of the S buffer.
-// kHole: columns [hs, he) are hidden as well.
-template <int D, bool kHole>
+// kHole: columns [hs, he) are hidden as well.  kFull: none is hidden.
+template <int D, bool kHole, bool kFull = false>
 __device__ __forceinline__ void softmax_half(const PrefillParams& p, int lim, int hs, int he, int half, int row, uint32_t tmem_s,
                                              uint32_t tmem_o, uint32_t lane_base, int j, uint64_t* o_done,
                                              bool& dead, SoftmaxState& st, float* xm_mine, const float* xm_other,
@@ -146,10 +146,10 @@ __device__ __forceinline__ void softmax_half(const PrefillParams& p, int lim, in
   tmem_wait_ld();
   // visible columns of this half as a bit mask (bit i: column c0 + i visible, i.e. c0 + i < lim)
   auto below = [](int n) -> uint32_t { return n >= 32 ? 0xFFFFFFFFu : (n <= 0 ? 0u : ((1u << n) - 1u)); };
-  uint32_t vm = below(lim - c0);
+  uint32_t vm = kFull ? 0xFFFFFFFFu : below(lim - c0);
   if (kHole) vm &= below(hs - c0) | ~below(he - c0);
   auto vis = [&](int c) { return ((vm >> (c - c0)) & 1u) != 0u; };
-  const bool full = kHole ? __all_sync(0xffffffffu, vm == 0xFFFFFFFFu) : lim == kBN;
+  const bool full = kFull ? true : kHole ? __all_sync(0xffffffffu, vm == 0xFFFFFFFFu) : lim == kBN;
   float mxa[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // independent chains
   if (full) {
 #pragma unroll
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
     }
     for (int i = 0; i < 4; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 256);  // the 8 softmax warps of a head
+      mbar_init(&p_full[i], 8);  // the softmax warps of a head
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&o_done[i], 1);
@@ -419,6 +419,23 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
       const int qbr = kWin ? 0 : q / p.per, qwr = kWin ? 0 : q - qbr * p.per, quota = kWin ? 0 : p.quota[h];
       for (int j = 0; j < n_tiles; ++j) {
         const int e = s_list[j];
+        if constexpr (kWin) {
+          // seen by every row of the query tile (most tiles): no masks
+          if (e * kBN + kBN <= qt * kBM + 1 && (e * kBN > qt * kBM + kBM - 1 - p.window || e * kBN + kBN <= p.n_sink)) {
+            const bool ok = __all_sync(
+                0xffffffffu, wait_or_abort(&s_full[2 * head_slot + (j & 1)], (uint32_t)((j >> 1) & 1), dead, p.err));
+            if (!ok) dead = true;
+            tc_fence_after();
+            float* xm = xmax + ((j & 1) * 2 + head_slot) * 256;
+            softmax_half<D, false, true>(p, kBN, 0, 0, half, row, tmem_h + 64 * (j & 1), tmem_o, lane_base, j,
+                                         &o_done[head_slot], dead, st, xm + half * 128, xm + (1 - half) * 128, pair_bar,
+                                         ok);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_one(&p_full[2 * head_slot + (j & 1)]);
+            continue;
+          }
+        }
         int lim, hs = 0, he = 0;
         if constexpr (kWin) {
           lim = min(max(q + 1 - e * kBN, 0), kBN);
@@ -439,7 +456,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
         softmax_half<D, kWin>(p, lim, hs, he, half, row, tmem_h + 64 * (j & 1), tmem_o, lane_base, j, &o_done[head_slot], dead,
                         st, xm + half * 128, xm + (1 - half) * 128, pair_bar, ok);
         tc_fence_before();  // P's tcgen05.st completed (wait::st) before the arrival
-        mbar_arrive_one(&p_full[2 * head_slot + (j & 1)]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive_one(&p_full[2 * head_slot + (j & 1)]);
       }
       // epilogue: this warp writes dims [D/2 half, D/2 half + D/2) of its row
       const bool o_ok =
