@@ -6,14 +6,17 @@
 // row i becomes row i of the destination table (the source pages themselves, or other pages of the
 // pool), its weight becomes weight i, and weights past the new length become 0.
 //
-// Two kernels.  select: one CTA per unit.  The weights become order-preserving 32-bit keys (-0 as
-// +0, NaN as -inf), are held in shared memory, and the (m - sinks - recent)-th largest key is found by
-// histogram passes over 11, 11 and 10 key bits, of which the last are left out once they decide nothing
-// (plain shared-memory adds, one per warp where its rows share the digit; grouping equal digits first with
-// match.any was 1.3 to 3 us slower on 1311 and 8190 rows).  Then every warp walks its contiguous share of the rows twice, counting and emitting by
-// ballot, so the kept list comes out in row order with one scan over the warps.
+// Two kernels.  select: one CTA per unit.  The weights become order-preserving 32-bit keys (-0 as +0, NaN as -inf),
+// are held in shared memory, and the (m - sinks - recent)-th largest key is found by histogram passes over 11, 11
+// and 10 key bits, of which the last are left out once they decide nothing (plain shared-memory adds, one per warp
+// where its rows share the digit; grouping equal digits first with match.any was 1.3 to 3 us slower on 1311 and
+// 8190 rows).  Then every warp walks its contiguous share of the rows twice, counting and emitting by ballot, so
+// the kept list comes out in row order with one scan over the warps.
 // move: bound by memory, so as many bytes in flight as fit: rows go through a shared-memory ring (see
 // evict_move_kernel).
+// Measured: 4 layers x 16 sequences of 5003 to 8190 rows to 4096 (2.15 GB with both directions) 392 us, 5.5 TB/s
+// of 6.53 measured for a copy; one sequence of 1311 rows to 1024 15 us, which is two launches and the selection's
+// three passes, one after another.
 #include <algorithm>
 #include <cstring>
 

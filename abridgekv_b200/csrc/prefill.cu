@@ -51,7 +51,10 @@
 // kWin (abkv_window_attention): the same kernel under a causal sliding window with sinks instead of the
 // block mask, for any S: row q sees keys j <= q with j > q - window or j < n_sink.  Key tiles hidden from
 // the whole query tile are not visited; inside a tile a row's hidden keys are its causal tail and the hole
-// [n_sink, q - window + 1).  Rows past S are read as zeros and clipped by the output's tensor map.
+// [n_sink, q - window + 1).  Rows past S are read as zeros and clipped by the output's tensor map.  Measured at
+// 2 x 32 heads (8 KV heads) x 4096 rows x 128 dims: window 1024 177 us (189 with out_lo), no window 292 us.  Bound by the
+// softmax warps' latencies, like the paged form: their exponentials (74 us of them with the window) and the rest of
+// a tile's work take turns.  Tiles that every row sees skip the masks: 192 -> 177 us.
 #include <cstring>
 
 #include "prefill_mask.cuh"

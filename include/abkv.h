@@ -428,7 +428,7 @@ int abkv_gather_rows(const void* const* src, void* const* dst, int num_tensors,
  *   weights[l][b * weight_strides[2l] + u * weight_strides[2l+1] + row] up to
  *   budgets[l] rows in all (ties to the lower row; NaN counts as -inf).
  * Kept rows stay in order: kept row i moves to row i of block_tables[l] (in
- * place) or, with dst_block_tables, to row i of that table's pages in the same
+ * place: its live pages then belong to one sequence each; not checked) or, with dst_block_tables, to row i of that table's pages in the same
  * cache, which must not be pages of any source table (not checked).
  * new_lens[l][b] = min(n, budget) (another buffer than seq_lens[l]).
  * weights_out[l] (weights[l] itself with the same strides, or a buffer that does
@@ -535,10 +535,11 @@ int abkv_prefill_masked_backward(
  * >= 1, so every row sees itself).  Any S from 1 to 131072, head_dim 64 or 128,
  * H <= 128.  All of q, k, v and dout must be finite: a tile multiplies hidden
  * rows by zero.  Every sum has a fixed order: results repeat bit for bit.
- * out_lo (optional): contiguous DEVICE [B][H][S][head_dim] bytes, the eight
- * mantissa bits of the output after its bf16 ones; given to the backward as well,
- * rowsum(dout * out) is taken from the longer output (the largest error of dq and
- * dk after the rounding of their own operands).  The backward's workspace:
+ * out_lo (optional): contiguous DEVICE [B][H][S][head_dim] bytes that start on a
+ * 32-byte boundary, the eight mantissa bits of the output after its bf16 ones; given
+ * to the backward as well, rowsum(dout * out) is taken from the longer output (the
+ * largest error of dq and dk after the rounding of their own operands).  Rows that
+ * see one key get a dq of exactly zero.  The backward's workspace:
  * abkv_window_attention_backward_workspace_size(B, H, S, head_dim) bytes. */
 int abkv_window_attention(const void* q, const int64_t* q_strides, const void* k,
                           const int64_t* k_strides, const void* v,
