@@ -9,7 +9,7 @@
 // (dQ: three) recompute S and dP once each -- seven products a tile instead of five -- but every sum stays in TMEM:
 // no fp32 accumulator of dQ in memory (its zeroing, a 64 KiB reduction per tile pair, its conversion) and no order-
 // dependent additions, so all gradients repeat bit for bit.  Measured at 2 x 32 heads (8 KV heads) x 4096 rows x
-// 128 dims: window 1024, row sums 42 us, dK/dV 261 us, dQ 206 us; no window, dK/dV 486 us, dQ 378 us (0.9 PFLOP/s
+// 128 dims: window 1024, row sums 29 us, dK/dV 265 us, dQ 200 us; no window, dK/dV 486 us, dQ 378 us (0.9 PFLOP/s
 // of the visible pairs' products with the window, 1.1 without, of 1.63 for a library product).  A tile takes a dQ
 // CTA about 4000 clocks against 1536 of products: the hand-overs between the issuer and the threads (about 200
 // clocks each way) and the threads' element-wise work in between bound both kernels, not a pipe.
@@ -772,19 +772,18 @@ __global__ void __launch_bounds__(256) window_rowdot_kernel(const __nv_bfloat16*
                                                             int H, int S) {
   constexpr int kL = D / 8;
   if (blockIdx.x == 0 && threadIdx.x == 0) *work = 0;  // the dK/dV launch's item counter
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t r = i / kL;
-  const int d0 = (int)(i % kL) * 8;
-  const bool live = r < (int64_t)B * H * S;
+  // at most 2^31 rows (the entry checks), counted in 32 bits: 64-bit divisions took longer than the loads
+  const uint32_t r = blockIdx.x * (256u / kL) + threadIdx.x / kL;
+  const int d0 = (int)(threadIdx.x % kL) * 8;
+  const bool live = r < (uint32_t)B * H * S;
+  // rows in memory order of [B][S][H]: neighbouring rows of a warp are neighbours there
+  const uint32_t bs = r / (uint32_t)H;
+  const int h = (int)(r - bs * H), b = (int)(bs / (uint32_t)S), q = (int)(bs - (uint32_t)b * S);
+  const int64_t rr = ((int64_t)b * H + h) * S + q;
   float acc = 0.f;
   if (live) {
-    // rows in memory order of [B][S][H]: neighbouring rows of a warp are neighbours there
-    const int h = (int)(r % H);
-    const int64_t bs = r / H;
-    const int q = (int)(bs % S), b = (int)(bs / S);
     const uint4 x = ld_stream_v4(o + b * o_sb + h * o_sh + q * o_ss + d0);
     const uint4 y = ld_stream_v4(dout + b * d_sb + h * d_sh + q * d_ss + d0);
-    const int64_t rr = ((int64_t)b * H + h) * S + q;
     uint2 l = make_uint2(0, 0);
     if (lo) l = __ldcs(reinterpret_cast<const uint2*>(lo + rr * D + d0));
     const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
@@ -795,14 +794,10 @@ __global__ void __launch_bounds__(256) window_rowdot_kernel(const __nv_bfloat16*
       const int32_t low = (int32_t)(int8_t)((k < 4 ? l.x : l.y) >> (8 * (k & 3)));
       acc = fmaf(__int_as_float((int32_t)xb + (low << 8)), __uint_as_float(yb), acc);
     }
-    }
+  }
 #pragma unroll
   for (int s = kL / 2; s; s >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, s);
-  if (live && d0 == 0) {
-    const int h = (int)(r % H);
-    const int64_t bs = r / H;
-    di[((bs / S) * H + h) * S + bs % S] = acc;
-  }
+  if (live && d0 == 0) di[rr] = acc;
 }
 
 int make_map(CUtensorMap* m, const void* base, int B, int heads, int S, int D, const int64_t* strides) {
