@@ -329,6 +329,10 @@ def evict_by_weight(kv_caches: Sequence[torch.Tensor], block_tables: Sequence[to
             return result
         if rows == 0:
             raise ValueError("weights must hold at least one row")
+        if not return_keep:
+            # no sequence is longer than its weights, so a larger budget keeps every row all the same, without a list of
+            # kept rows of its length in the workspace
+            budgets = [min(m, max(rows, num_sinks + num_recent)) for m in budgets]
         c_budget = _lib.i32_array(budgets)
         need = 256 if return_keep else lib.abkv_evict_by_weight_workspace_size(L, B, units, c_budget)
         ws, raw = call_workspace(dev, need, workspace)

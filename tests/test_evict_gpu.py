@@ -186,3 +186,15 @@ def test_refusals():
         ev(kv, bt, sl, w, budget=8, dst_block_tables=bt)
     with pytest.raises(_lib.AbkvError):
         ev([torch.zeros((4, 2, 16, 2, 32), dtype=torch.bfloat16, device="cuda")], bt, sl, w, budget=8)
+
+
+def test_a_budget_far_above_the_rows_needs_no_memory_for_it():
+    c = R.Paged([40, 7], 2, 64, 16, 0, seed=4)
+    kv, bt, seq = c.kv.cuda(), c.table.cuda(), c.seq.cuda()
+    before, w = kv.clone(), torch.rand((2, 2, 48), device="cuda")
+    ws = Workspace("cuda", 4096)
+    e = compaction.evict_by_weight([kv], [bt], [seq], [w], budget=1 << 30, num_sinks=4, num_recent=100, workspace=ws)
+    assert ws.nbytes < 1 << 20 and e.seq_lens[0].tolist() == [40, 7]
+    assert torch.equal(kv.nan_to_num(7.0), before.nan_to_num(7.0))
+    for b, n in enumerate((40, 7)):
+        assert torch.equal(e.weights[0][b, :, :n], w[b, :, :n]) and (e.weights[0][b, :, n:] == 0).all()
