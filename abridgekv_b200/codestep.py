@@ -251,10 +251,10 @@ def paged_prefill_window(query: torch.Tensor, kv_cache: torch.Tensor, block_tabl
         R, Hkv, _, keep, tail = _window_rows(query, kv_cache, block_table, seq_lens, query_start_loc, num_kv_heads,
                                              num_requests, max_query_len, kv_layout)
         if out is None:
-            out = torch.empty(shape, dtype=torch.bfloat16, device=device)
+            out = query.new_empty(shape)
         elif out.shape != shape or out.dtype != torch.bfloat16 or out.stride(2) != 1 or out.device != device:
             raise ValueError("out must be a bf16 [T, Hq, D] tensor with a contiguous last dimension on the query's device")
-        lse = torch.empty(shape[:2], dtype=torch.float32, device=device) if return_lse else None
+        lse = query.new_empty(shape[:2], dtype=torch.float32) if return_lse else None
         ws, raw = call_workspace(device, 256, workspace)
         T, Hq, D = shape
         st = _lib.lib().abkv_paged_prefill_window(

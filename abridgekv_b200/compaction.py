@@ -320,10 +320,9 @@ def evict_by_weight(kv_caches: Sequence[torch.Tensor], block_tables: Sequence[to
         raise ValueError("every layer needs its own weights tensor")
     lib = _lib.lib()
     with call_scope(dev, stream):
-        new = [torch.empty(B, dtype=torch.int32, device=dev) for _ in range(L)]
-        outs = list(weights) if in_place_weights else [torch.empty((B, units, rows), dtype=torch.float32, device=dev)
-                                                       for _ in range(L)]
-        keep = [torch.empty((B, units, m), dtype=torch.int32, device=dev) for m in budgets] if return_keep else None
+        new = [torch.empty_like(t) for t in seq_lens]
+        outs = list(weights) if in_place_weights else [t.new_empty((B, units, rows)) for t in weights]
+        keep = [t.new_empty((B, units, m)) for t, m in zip(seq_lens, budgets)] if return_keep else None
         result = Evicted(new, outs, keep)
         if B == 0:
             return result

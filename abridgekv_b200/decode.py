@@ -214,8 +214,7 @@ def _decode_window(queries, kv_caches, block_tables, seq_lens, weights, window, 
         max_pages_per_seq = max([bt.shape[1] for bt in block_tables])
     units, rows = (1, 0) if weights is None else _check_weights(weights, L, B, Hkv, device)
     with call_scope(device, stream):
-        outs = list(outputs) if outputs is not None else [torch.empty(q_shape, dtype=bf16, device=device)
-                                                          for _ in range(L)]
+        outs = list(outputs) if outputs is not None else [torch.empty_like(q) for q in queries]
         if B == 0:
             return outs
         need, win, snk = _window_plan(L, B, Hq, Hkv, D, page, max_pages_per_seq, chunk_tokens, windows, sinks,

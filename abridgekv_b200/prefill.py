@@ -225,17 +225,17 @@ def window_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window:
     B, H, S, D = q.shape
     device = q.device
     with call_scope(device, stream):
-        out = torch.empty((B, S, H, D), dtype=torch.bfloat16, device=device).transpose(1, 2)
-        lse = torch.empty((B, H, S), dtype=torch.float32, device=device) if return_lse else None
-        low = torch.empty((B, H, S, D), dtype=torch.int8, device=device) if return_low else None
+        out = q.new_empty((B, S, H, D)).transpose(1, 2)
+        lse = q.new_empty((B, H, S), dtype=torch.float32) if return_lse else None
+        low = q.new_empty((B, H, S, D), dtype=torch.int8) if return_low else None
         if B * H * S:
             (q, qs), (k, ks), (v, vs) = _tma_ready(q), _tma_ready(k), _tma_ready(v)
             os = _lib.i64(S * H * D, D, H * D)
             ws, raw = call_workspace(device, 256, workspace)
             st = _lib.lib().abkv_window_attention(
                 q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, out.data_ptr(), os,
-                low.data_ptr() if return_low else None, lse.data_ptr() if return_lse else None, B, H, k.shape[1], S, D, scale, window, num_sinks, ws.ptr(),
-                ws.nbytes, raw)
+                low.data_ptr() if return_low else None, lse.data_ptr() if return_lse else None, B, H, k.shape[1], S, D,
+                scale, window, num_sinks, ws.ptr(), ws.nbytes, raw)
             if st:
                 _lib.check("abkv_window_attention", st)
     extra = tuple(t for t in (lse, low) if t is not None)
