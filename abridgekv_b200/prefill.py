@@ -307,12 +307,17 @@ class WindowAttention(torch.autograd.Function):
         ctx.args = (int(window), int(num_sinks), 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale))
         return out
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
+    def _gradients(ctx, dout):
         q, k, v, out, lse, low = ctx.saved_tensors
         with call_scope(q.device, None):
             return (*_window_backward(q, k, v, out, dout, lse, low, *ctx.args), None, None, None)
+
+    _once = staticmethod(torch.autograd.function.once_differentiable(_gradients))
+
+    @staticmethod
+    def backward(ctx, dout):
+        # what marks the gradients as not differentiable again is only needed under create_graph
+        return WindowAttention._once(ctx, dout) if torch.is_grad_enabled() else WindowAttention._gradients(ctx, dout)
 
 
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int, num_sinks: int = 0,

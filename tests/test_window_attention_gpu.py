@@ -229,3 +229,20 @@ def test_rows_that_see_one_key_have_no_score_gradient(D, S, window, sinks, alone
         # each key has its own row's gradient, summed over the two heads that share it
         want = do.double().view(2, 2, 2, S, D).sum(2)
         assert (dv.double() - want).abs().le(2.0 ** -8 * want.abs() + 1e-30).all()
+
+
+def test_gradients_are_not_differentiable_again():
+    """Under create_graph the gradients come out, and a second derivative is refused rather than left out."""
+    g = torch.Generator().manual_seed(2)
+    q, k, v, do = (torch.randn((1, h, 70, 64), generator=g).bfloat16().cuda() for h in (4, 2, 2, 4))
+    for t in (q, k, v):
+        t.requires_grad_()
+    plain = torch.autograd.grad(prefill.window_attention(q, k, v, window=9), (q, k, v), do)
+    again = torch.autograd.grad(prefill.window_attention(q, k, v, window=9), (q, k, v), do, create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, again))
+    with pytest.raises(RuntimeError):  # (torch: of a dout without a gradient of its own the result has none either)
+        torch.autograd.grad(again[0].float().sum(), q)
+    do.requires_grad_()
+    again = torch.autograd.grad(prefill.window_attention(q, k, v, window=9), (q, k, v), do, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        again[0].float().sum().backward()
