@@ -387,19 +387,19 @@ def run(state):
     if k == "prompt_window":
         return codestep.paged_prefill_window(state["q"], state["kv"], state["bt"], state["sl"], state["qs"],
                                              max_query_len=c["qhi"], num_kv_heads=c["Hkv"], window=c["window"],
-                                             num_sinks=c["sinks"], return_lse=True, kv_layout=c["layout"])
+                                             num_sinks=c["sinks"], return_lse=True)
     if k == "prompt_weights":
         w = state["w"].clone()
         return codestep.paged_prompt_weights(state["q"], state["lse"], state["kv"], state["bt"], state["sl"],
                                              state["qs"], w, num_kv_heads=c["Hkv"], max_query_len=c["qhi"],
                                              observe=c["observe"] or None, window=c["window"] or None,
-                                             num_sinks=c["sinks"], kv_layout=c["layout"])
+                                             num_sinks=c["sinks"])
     if k == "train_window":
         out = prefill.window_attention(state["q"], state["k"], state["v"], window=c["window"], num_sinks=c["sinks"])
         return (out.detach(), *torch.autograd.grad(out, (state["q"], state["k"], state["v"]), state["do"]))
     res = compaction.evict_by_weight(state["kv"], state["bt"], state["sl"], state["w"], budget=c["budget"],
                                      num_sinks=c["sinks"], num_recent=c["recent"], dst_block_tables=state["dst"],
-                                     return_keep=True, kv_layout=0)
+                                     return_keep=True)
     return dict(kv=state["kv"], new_lens=res.seq_lens, weights=res.weights, keep=res.keep)
 
 
