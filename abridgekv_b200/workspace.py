@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import threading
 
 import torch
 
@@ -67,25 +68,36 @@ def call_scope(device: torch.device, stream: torch.cuda.Stream | None):
     return _here if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
 
-_per_stream: dict[tuple[int, int], Workspace] = {}
+_own = threading.local()  # .table: {(device index, raw stream): Workspace} of this thread
+
+
+def stream_workspace(device: torch.device, stream: torch.cuda.Stream | None = None) -> Workspace:
+    """The workspace that this thread's calls without one of their own use on ``stream`` (None: the current
+    stream) outside a capture.  Its error word is theirs: ``stream_workspace(device, s).read_error(s)``."""
+    with call_scope(device, stream):
+        return _stream_workspace(device, torch._C._cuda_getCurrentRawStream(device.index), 256)
+
+
+def _stream_workspace(device: torch.device, raw: int, nbytes: int) -> Workspace:
+    table = _own.__dict__.setdefault("table", {})
+    ws = table.get((device.index, raw))
+    if ws is None:
+        ws = table[(device.index, raw)] = Workspace(device, nbytes)
+    return ws.ensure(nbytes)
 
 
 def call_workspace(device: torch.device, nbytes: int, workspace: Workspace | None = None) -> tuple[Workspace, int]:
     """(workspace, raw current stream) of one call, inside its ``call_scope``: the caller's workspace,
-    else one that no other stream and no CUDA graph uses.
+    else one that no other stream, no other thread and no CUDA graph uses.
 
-    The device's default stream takes ``default_workspace`` (whose error word the caller reads there); any other
-    stream has its own.  A call under stream capture gets a fresh one from the graph's memory pool, zeroed
-    at every replay: two graphs never share it, and no later growth frees it under them.  (To read the
-    error word of a captured or side-stream call, pass a workspace of your own.)"""
+    A call may be several launches with data in the workspace between them, and another thread's launches may
+    come in between on the same stream, so every thread has a buffer per stream (``stream_workspace``), apart from
+    ``default_workspace``, which other entries use on any stream.  A call under stream capture gets a fresh one from the graph's memory pool, zeroed at every replay: two graphs never share it,
+    and no later growth frees it under them.  (To read the error word of a captured call, pass a workspace
+    of your own.)"""
     raw = torch._C._cuda_getCurrentRawStream(device.index)
     if workspace is not None:
         return workspace.ensure(nbytes), raw
     if torch._C._cuda_isCurrentStreamCapturing():
         return Workspace(device, nbytes), raw
-    if raw == 0:
-        return default_workspace(device).ensure(nbytes), raw
-    ws = _per_stream.get((device.index, raw))
-    if ws is None:
-        ws = _per_stream[(device.index, raw)] = Workspace(device, nbytes)
-    return ws.ensure(nbytes), raw
+    return _stream_workspace(device, raw, nbytes), raw

@@ -1,0 +1,57 @@
+"""Which workspace a call gets, without a GPU: the streams and the capture state are faked, the buffers are host tensors."""
+import threading
+
+import pytest
+import torch
+
+from abridgekv_b200 import workspace as W
+
+DEV = torch.device("cuda", 0)
+
+
+class Stream:
+    """The current stream as the fakes see it."""
+    raw, capturing = 0, False
+
+
+@pytest.fixture
+def now(monkeypatch):
+    s = Stream()
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: s.raw, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: s.capturing, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    real = W.Workspace.__init__
+    monkeypatch.setattr(W.Workspace, "__init__", lambda self, device=None, *a, **kw: real(self, "cpu", *a, **kw))
+    monkeypatch.setattr(W, "_per_device", {})
+    return s
+
+
+def in_thread(fn):
+    out = []
+    t = threading.Thread(target=lambda: out.append(fn()))
+    t.start()
+    t.join()
+    return out[0]
+
+
+def test_a_call_shares_its_buffer_with_no_other_stream_thread_or_entry(now):
+    first = W.call_workspace(DEV, 300)[0]
+    assert W.call_workspace(DEV, 200)[0] is first and first.nbytes >= 300
+    assert first is not W.default_workspace(DEV)  # which older entries take on any stream and inside captures
+    other = in_thread(lambda: W.call_workspace(DEV, 300)[0])
+    assert other is not first and W.call_workspace(DEV, 300)[0] is first
+    now.raw = 77
+    side, raw = W.call_workspace(DEV, 300)
+    assert raw == 77 and side not in (first, other) and W.call_workspace(DEV, 300)[0] is side
+    now.capturing = True
+    graphs = [W.call_workspace(DEV, 300)[0] for _ in range(2)]
+    assert graphs[0] is not graphs[1] and not {id(g) for g in graphs} & {id(first), id(other), id(side)}
+    mine = W.Workspace(DEV, 256)
+    assert W.call_workspace(DEV, 512, mine)[0] is mine and mine.nbytes == 512
+
+
+def test_the_buffer_of_a_stream_can_be_found(now):
+    first = W.call_workspace(DEV, 4096)[0]
+    assert W.stream_workspace(DEV) is first and first.nbytes == 4096
+    now.raw = 5
+    assert W.stream_workspace(DEV) is W.call_workspace(DEV, 256)[0] is not first

@@ -1,0 +1,93 @@
+"""Calls at once with the workspaces that they get by themselves: on two streams, from two threads on one stream.
+Every comparison is of bits: no call's result may depend on what ran beside it."""
+import threading
+
+import pytest
+import torch
+
+import bounded_ref as ref
+from abridgekv_b200 import codestep, compaction, decode, prefill
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+HKV, G, D, PAGE = 2, 2, 128, 16
+
+
+class Job:
+    """A paged cache with what the entries over it need."""
+
+    def __init__(self, lens, seed):
+        c = ref.Paged(lens, HKV, D, PAGE, 0, seed=seed)
+        g = torch.Generator().manual_seed(seed)
+        self.kv, self.bt, self.seq = c.kv.to(DEV), c.table.to(DEV), c.seq.to(DEV)
+        self.q = torch.randn((len(lens), HKV * G, D), generator=g).bfloat16().to(DEV)
+        self.w = torch.rand((len(lens), HKV, c.width * PAGE), generator=g).to(DEV)
+        self.pages = (self.bt,), (self.seq,)
+
+    def decode(self, stream=None):
+        return decode.paged_decode([self.q], [self.kv], *self.pages, chunk_tokens=64, stream=stream)
+
+    def weighted(self):
+        w = self.w.clone()
+        return decode.paged_decode_weighted([self.q], [self.kv], *self.pages, [w], chunk_tokens=64) + [w]
+
+    def one_unit(self):
+        w = torch.zeros((len(self.seq), 1, self.w.shape[2]), device=DEV)
+        starts = torch.arange(len(self.seq) + 1, dtype=torch.int32, device=DEV)
+        out, lse = codestep.paged_prefill_window(self.q, self.kv, self.bt, self.seq, starts, max_query_len=1,
+                                                 num_kv_heads=HKV, window=None, return_lse=True)
+        codestep.paged_prompt_weights(self.q, lse, self.kv, self.bt, self.seq, starts, w, max_query_len=1,
+                                      num_kv_heads=HKV)
+        return [out, lse, w]
+
+    def evict(self):
+        kv = self.kv.clone()
+        e = compaction.evict_by_weight([kv], *self.pages, [self.w], budget=300, num_sinks=4, num_recent=8)
+        return [kv.view(torch.int16), e.seq_lens[0], e.weights[0]]
+
+
+def backward(seed):
+    g = torch.Generator().manual_seed(seed)
+    q, k, v, do = (torch.randn((1, h, 300, 64), generator=g).bfloat16().to(DEV) for h in (4, 2, 2, 4))
+    out, lse = prefill.window_forward(q, k, v, window=70, num_sinks=2, return_lse=True)
+    return lambda: list(prefill.window_backward(q, k, v, out, do, lse, window=70, num_sinks=2))
+
+
+def equal(got, want):
+    return all(torch.equal(a, b) for a, b in zip(got, want, strict=True))
+
+
+def test_an_older_entry_on_a_side_stream_beside_new_ones_on_the_default_stream():
+    a, b, bwd = Job([2000, 1500, 700], 1), Job([900, 1100], 2), backward(3)
+    calls = [b.weighted, b.evict, bwd, b.one_unit]
+    alone, decoded = [f() for f in calls], a.decode()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for _ in range(10):
+        beside = [a.decode(stream=s) for _ in range(12)]
+        got = [f() for f in calls for _ in range(2)]
+        beside += [a.decode(stream=s) for _ in range(12)]
+        torch.cuda.synchronize()
+        assert all(equal(x, decoded) for x in beside)
+        assert all(equal(x, alone[i // 2]) for i, x in enumerate(got))
+
+
+def test_two_threads_on_one_stream():
+    jobs = [Job([900, 1100], 4), Job([1300, 650], 5)]
+    calls = [[j.weighted, j.evict, backward(6 + i), j.one_unit] for i, j in enumerate(jobs)]
+    alone = [[f() for f in fs] for fs in calls]
+    torch.cuda.synchronize()
+    start, wrong = threading.Barrier(2), []
+
+    def work(fs, want):
+        start.wait()
+        got = [[f() for f in fs] for _ in range(20)]
+        torch.cuda.synchronize()
+        wrong.extend(i for r in got for i, x in enumerate(r) if not equal(x, want[i]))
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(calls, alone)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
