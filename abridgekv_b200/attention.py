@@ -235,9 +235,6 @@ class AbkvAttentionImpl:
         self.kv_sharing_target_layer_name = kv_sharing_target_layer_name
         self.workspace = workspace
 
-    def _ws(self, device) -> Workspace:
-        return self.workspace or default_workspace(device)
-
     def forward(self, layer: Any, query: torch.Tensor, key: torch.Tensor | None, value: torch.Tensor | None,
                 kv_cache: torch.Tensor, attn_metadata: AbkvAttentionMetadata | None,
                 output: torch.Tensor | None = None, output_scale: Any = None,
@@ -249,7 +246,7 @@ class AbkvAttentionImpl:
             return output.fill_(0)
         md = attn_metadata
         T = md.num_actual_tokens
-        ws = self._ws(query.device)
+        ws = self.workspace  # None: every entry takes its own (a windowed one per stream, thread and capture)
         if key is not None and value is not None and self.kv_sharing_target_layer_name is None:
             store_kv(key[:T].view(T, Hkv, D), value[:T].view(T, Hkv, D), kv_cache, md.slot_mapping[:T],
                      workspace=ws)

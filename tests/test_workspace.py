@@ -55,3 +55,20 @@ def test_the_buffer_of_a_stream_can_be_found(now):
     assert W.stream_workspace(DEV) is first and first.nbytes == 4096
     now.raw = 5
     assert W.stream_workspace(DEV) is W.call_workspace(DEV, 256)[0] is not first
+
+
+@pytest.mark.parametrize("qlens", [[1, 1], [3, 2]])
+def test_a_windowed_layer_leaves_the_choice_to_the_entries(monkeypatch, qlens):
+    """The attention backend without a workspace hands none on: a shared one would meet another stream's calls."""
+    from test_bounded_host import attention, codestep, decode, impl, metadata
+
+    seen = []
+    for mod, name in ((decode, "paged_decode_window"), (codestep, "paged_prefill_window")):
+        monkeypatch.setattr(mod, name, lambda *a, **kw: seen.append(kw["workspace"]))
+    monkeypatch.setattr(attention, "store_kv", lambda *a, **kw: None)
+    monkeypatch.setattr(attention, "default_workspace", lambda device: W.Workspace("cpu"))
+    T = sum(qlens)
+    q, kv = torch.zeros(T, 1024, dtype=torch.bfloat16), torch.zeros(4, 2, 16, 2, 128, dtype=torch.bfloat16)
+    new = torch.zeros(T, 256, dtype=torch.bfloat16)
+    impl(sliding_window=32).forward(None, q, new, new, kv, metadata(qlens), q.clone())
+    assert seen == [None]

@@ -91,3 +91,48 @@ def test_two_threads_on_one_stream():
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_a_windowed_layer_on_two_streams_and_in_a_graph():
+    """The attention backend without a workspace of its own: layers at once on two streams, and a captured step that is
+    replayed after eager calls have needed larger workspaces."""
+    from types import SimpleNamespace
+
+    from abridgekv_b200 import attention
+
+    impl = attention.AbkvAttentionImpl(HKV * G, D, D ** -0.5, num_kv_heads=HKV, sliding_window=700, num_sinks=3)
+
+    def layer(j):
+        B = len(j.seq)
+        starts = torch.arange(B + 1, dtype=torch.int32)
+        md = attention.AbkvMetadataBuilder().build(0, SimpleNamespace(
+            num_reqs=B, num_actual_tokens=B, query_start_loc=starts.to(DEV), query_start_loc_cpu=starts, seq_lens=j.seq,
+            _seq_lens_cpu=j.seq.cpu(), block_table_tensor=j.bt, slot_mapping=torch.full((B,), -1, device=DEV),
+            max_query_len=1, causal=True))
+        new = torch.zeros((B, HKV, D), dtype=torch.bfloat16, device=DEV)
+        out = torch.zeros((B, HKV * G * D), dtype=torch.bfloat16, device=DEV)
+        return lambda: impl.forward(None, j.q.view(B, -1), new, new, j.kv, md, out)
+
+    # enough (sequence, KV head) pairs for the split kernel, whose partial results lie in the workspace
+    layers = [layer(Job([1500] * 150 + [20] * i, 11 + i)) for i in range(2)]
+    alone = [f().clone() for f in layers]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in layers]
+    for _ in range(10):
+        got = []
+        for f, s in zip(layers * 3, streams * 3):
+            with torch.cuda.stream(s):
+                got.append(f().clone())
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, alone[i % 2]) for i, x in enumerate(got))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = layers[0]()
+    big = Job([1500] * 400, 13)
+    want = big.weighted()
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        assert equal(big.weighted(), want)
+        torch.cuda.synchronize()
+        assert torch.equal(out, alone[0])
