@@ -3,7 +3,10 @@
 The C ABI never allocates: every call receives a workspace whose first four
 bytes hold the device error word.  This helper keeps one zero-initialised,
 256-byte aligned buffer per device and grows it on demand (growth happens
-outside any kernel; a grown buffer starts with a clean error word).
+outside any kernel and keeps the error word; a buffer that a captured call used
+stays allocated as long as the workspace, for the graph's replays).  Give a
+workspace its size before a capture: one that grows inside is zeroed by the
+replays only.
 """
 from __future__ import annotations
 
@@ -20,6 +23,8 @@ class Workspace:
     def __init__(self, device: torch.device | int | str | None = None, nbytes: int = 1 << 20):
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self._buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=self.device)
+        self._in_graph = False  # a CUDA graph holds the buffer's address
+        self._kept: list[torch.Tensor] = []
 
     @property
     def nbytes(self) -> int:
@@ -29,11 +34,16 @@ class Workspace:
         if nbytes > self._buf.numel():
             # keep the error word of the old buffer visible to the caller
             old_err = self._buf[:4].clone()
+            if self._in_graph:  # its replays go on writing there: the memory is not given back
+                self._kept.append(self._buf)
+                self._in_graph = False
             self._buf = torch.zeros(nbytes, dtype=torch.uint8, device=self.device)
             self._buf[:4].copy_(old_err)
         return self
 
     def ptr(self) -> int:
+        if not self._in_graph:
+            self._in_graph = torch._C._cuda_isCurrentStreamCapturing()
         return self._buf.data_ptr()
 
     def read_error(self, stream: torch.cuda.Stream | None = None) -> int:

@@ -1,5 +1,7 @@
 """Which workspace a call gets, without a GPU: the streams and the capture state are faked, the buffers are host tensors."""
+import gc
 import threading
+import weakref
 
 import pytest
 import torch
@@ -72,3 +74,22 @@ def test_a_windowed_layer_leaves_the_choice_to_the_entries(monkeypatch, qlens):
     new = torch.zeros(T, 256, dtype=torch.bfloat16)
     impl(sliding_window=32).forward(None, q, new, new, kv, metadata(qlens), q.clone())
     assert seen == [None]
+
+
+def test_a_buffer_that_a_graph_uses_outlives_its_growth(now):
+    ws = W.Workspace(DEV, 256)
+    ws.ptr()
+    ref = weakref.ref(ws._buf.untyped_storage())
+    ws.ensure(512)
+    gc.collect()
+    assert ref() is None  # no graph: given back
+    now.capturing = True
+    at, storage = ws.ptr(), weakref.ref(ws._buf.untyped_storage())
+    now.capturing = False
+    ws._buf[0] = 4
+    ws.ensure(4096)
+    assert ws.ptr() != at and ws._buf[0] == 4 and ws.nbytes == 4096
+    gc.collect()
+    assert storage() is not None and [b.data_ptr() for b in ws._kept] == [at]
+    ws.ensure(8192)  # the second buffer was in no graph
+    assert [b.data_ptr() for b in ws._kept] == [at]

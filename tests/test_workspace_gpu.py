@@ -136,3 +136,34 @@ def test_a_windowed_layer_on_two_streams_and_in_a_graph():
         assert equal(big.weighted(), want)
         torch.cuda.synchronize()
         assert torch.equal(out, alone[0])
+
+
+def test_a_graph_with_a_workspace_that_grows_afterwards():
+    """Older and newer entries captured with the caller's workspace, which eager calls then outgrow; memory of the old
+    buffer's size is taken and filled between the replays."""
+    from abridgekv_b200.workspace import Workspace
+
+    j, big, ws = Job([900, 1100], 21), Job([1500] * 60, 22), Workspace(DEV, 1 << 18)
+    w = torch.zeros_like(j.w)
+
+    def step():
+        return (decode.paged_decode([j.q], [j.kv], *j.pages, chunk_tokens=64, workspace=ws) +
+                decode.paged_decode_weighted([j.q], [j.kv], *j.pages, [w], chunk_tokens=64, workspace=ws))
+
+    want = [t.clone() for t in step()]
+    want_w, size = w.clone(), ws.nbytes
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    bw = torch.zeros_like(big.w)
+    decode.paged_decode_weighted([big.q], [big.kv], *big.pages, [bw], chunk_tokens=64, workspace=ws)
+    assert ws.nbytes > size
+    others = [torch.full((size,), 85, dtype=torch.uint8, device=DEV) for _ in range(4)]
+    for _ in range(3):
+        w.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert equal(got, want) and torch.equal(w, want_w)
+        assert all((x == 85).all() for x in others)
+    assert ws.read_error() == 0
