@@ -20,9 +20,12 @@ from . import _lib
 
 
 class Workspace:
-    def __init__(self, device: torch.device | int | str | None = None, nbytes: int = 1 << 20):
+    def __init__(self, device: torch.device | int | str | None = None, nbytes: int = 1 << 20,
+                 zeroed: int | None = None):
+        """``zeroed``: leading bytes that start at zero (None: all)."""
         self.device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-        self._buf = torch.zeros(max(nbytes, 256), dtype=torch.uint8, device=self.device)
+        self._buf = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=self.device)
+        self._buf[:zeroed].zero_()
         self._in_graph = False  # a CUDA graph holds the buffer's address
         self._kept: list[torch.Tensor] = []
 
@@ -102,12 +105,12 @@ def call_workspace(device: torch.device, nbytes: int, workspace: Workspace | Non
 
     A call may be several launches with data in the workspace between them, and another thread's launches may
     come in between on the same stream, so every thread has a buffer per stream (``stream_workspace``), apart from
-    ``default_workspace``, which other entries use on any stream.  A call under stream capture gets a fresh one from the graph's memory pool, zeroed at every replay: two graphs never share it,
-    and no later growth frees it under them.  (To read the error word of a captured call, pass a workspace
+    ``default_workspace``, which other entries use on any stream.  A call under stream capture gets a fresh one from the graph's memory pool, its header zeroed at every replay (the entries that
+    come here write the rest before they read it): two graphs never share it, and no later growth frees it under them.  (To read the error word of a captured call, pass a workspace
     of your own.)"""
     raw = torch._C._cuda_getCurrentRawStream(device.index)
     if workspace is not None:
         return workspace.ensure(nbytes), raw
     if torch._C._cuda_isCurrentStreamCapturing():
-        return Workspace(device, nbytes), raw
+        return Workspace(device, nbytes, zeroed=256), raw
     return _stream_workspace(device, raw, nbytes), raw

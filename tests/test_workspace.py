@@ -93,3 +93,17 @@ def test_a_buffer_that_a_graph_uses_outlives_its_growth(now):
     assert storage() is not None and [b.data_ptr() for b in ws._kept] == [at]
     ws.ensure(8192)  # the second buffer was in no graph
     assert [b.data_ptr() for b in ws._kept] == [at]
+
+
+def test_a_captured_call_zeroes_its_header_alone(now, monkeypatch):
+    """What is zeroed under capture is zeroed at every replay, scores of a hundred megabytes too."""
+    sizes = []
+    zero, zeros = torch.Tensor.zero_, torch.zeros
+    monkeypatch.setattr(torch.Tensor, "zero_", lambda t: (sizes.append(t.numel()), zero(t))[1])
+    monkeypatch.setattr(torch, "zeros", lambda n, **kw: (sizes.append(n), zeros(n, **kw))[1])
+    now.capturing = True
+    ws = W.call_workspace(DEV, 1 << 20)[0]
+    assert sizes == [256] and ws.nbytes == 1 << 20 and not ws._buf[:256].any()
+    now.capturing = False
+    sizes.clear()
+    assert not W.Workspace(DEV, 4096)._buf.any() and sizes == [4096]
