@@ -1713,8 +1713,12 @@ int launch_cluster(const WinDecodeParams& prm, const WindowPlan& plan, int head_
   auto kernel = head_dim == 64 ? decode_cluster_kernel<64> : decode_cluster_kernel<kD>;
   const size_t scores = prm.win[0].weights && !plan.logits
                             ? (size_t)plan.warp_tiles * kClusterWarps * prm.G * kTile * 4 : 0;
-  const size_t smem = (head_dim == 64 ? sizeof(ClusterSmem<64>) : sizeof(ClusterSmem<kD>)) + scores;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+  const size_t base = head_dim == 64 ? sizeof(ClusterSmem<64>) : sizeof(ClusterSmem<kD>), smem = base + scores;
+  // The attribute is the process's, not the call's: every call sets the most that any call asks for, so that a call
+  // of another thread between this line and the launch cannot take it below what this launch needs.
+  constexpr size_t most = (size_t)kMaxClusterTiles * kClusterWarps * kMaxG * kTile * 4;
+  static_assert(sizeof(ClusterSmem<kD>) + most <= 227 * 1024, "shared memory");
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(base + most)) != cudaSuccess)
     return ABKV_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(plan.cluster, prm.Hkv, prm.nl * prm.B);

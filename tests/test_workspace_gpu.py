@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import bounded_ref as ref
-from abridgekv_b200 import codestep, compaction, decode, prefill
+from abridgekv_b200 import _lib, codestep, compaction, decode, prefill
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -16,11 +16,11 @@ HKV, G, D, PAGE = 2, 2, 128, 16
 class Job:
     """A paged cache with what the entries over it need."""
 
-    def __init__(self, lens, seed):
+    def __init__(self, lens, seed, group=G):
         c = ref.Paged(lens, HKV, D, PAGE, 0, seed=seed)
         g = torch.Generator().manual_seed(seed)
         self.kv, self.bt, self.seq = c.kv.to(DEV), c.table.to(DEV), c.seq.to(DEV)
-        self.q = torch.randn((len(lens), HKV * G, D), generator=g).bfloat16().to(DEV)
+        self.q = torch.randn((len(lens), HKV * group, D), generator=g).bfloat16().to(DEV)
         self.w = torch.rand((len(lens), HKV, c.width * PAGE), generator=g).to(DEV)
         self.pages = (self.bt,), (self.seq,)
 
@@ -167,3 +167,43 @@ def test_a_graph_with_a_workspace_that_grows_afterwards():
         assert equal(got, want) and torch.equal(w, want_w)
         assert all((x == 85).all() for x in others)
     assert ws.read_error() == 0
+
+
+def test_threads_whose_cluster_kernels_need_different_shared_memory(monkeypatch):
+    """One sequence with accumulators (scores in shared memory) in one thread, one without in others, each on its own
+    stream: they share the kernel, whose limit of shared memory is the process's.  The bare C calls, so that the
+    threads meet inside them."""
+    jobs = [Job([9000], 31, group=8), Job([200], 32, group=8)]
+    w = torch.zeros_like(jobs[0].w)  # 73 KB of shared memory against 37
+    calls = [lambda: decode.paged_decode_weighted([jobs[0].q], [jobs[0].kv], *jobs[0].pages, [w]),
+             lambda: decode.paged_decode_window([jobs[1].q], [jobs[1].kv], *jobs[1].pages, window=100)]
+    entry, args = _lib.lib().abkv_decode_window, []
+
+    class Recorder:
+        def __getattr__(self, name):
+            return getattr(real, name) if name != "abkv_decode_window" else lambda *a: args.append(a) or entry(*a)
+
+    real = _lib.lib()
+    monkeypatch.setattr(_lib, "lib", Recorder)
+    streams, keep = [], []
+    for f in (calls[0], calls[1], calls[1], calls[1]):
+        streams.append(torch.cuda.Stream())
+        with torch.cuda.stream(streams[-1]):
+            keep.append(f())
+    torch.cuda.synchronize()
+    start, status = threading.Barrier(4), [set() for _ in args]
+
+    def work(i):
+        start.wait()
+        for k in range(20000):
+            status[i].add(entry(*args[i]))
+            if k % 500 == 499:
+                streams[i].synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert status == [{0}] * 4
