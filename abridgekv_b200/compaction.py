@@ -262,7 +262,8 @@ def evict_by_weight(kv_caches: Sequence[torch.Tensor], block_tables: Sequence[to
 
     Rows move inside the sequence's own pages (the pages past the new length are then free), or,
     with ``dst_block_tables``, into the pages of those tables, which must be other pages of the same
-    caches.  The new weights are new tensors of ``weights``' shape, or ``weights`` themselves with
+    caches, with room for what a sequence may keep (the least of the budget, the source table's rows and the
+    weights' rows).  The new weights are new tensors of ``weights``' shape, or ``weights`` themselves with
     ``in_place_weights``.  ``seq_lens`` stays as it was; go on with the returned lengths.  In place, a
     page that two sequences share (a cached prefix) would be moved for both: evict into other pages then.
     ``kv_layout``: as in ``codestep.paged_prefill_window``."""
@@ -303,6 +304,11 @@ def evict_by_weight(kv_caches: Sequence[torch.Tensor], block_tables: Sequence[to
             check(name, bt, torch.int32)
             if bt.dim() != 2 or bt.shape[0] < B or not bt.is_contiguous():
                 raise ValueError(f"{name} must be a contiguous [>=B, max_pages] tensor")
+        if dst_block_tables is not None:
+            most = min(budgets[l], rows, block_tables[l].shape[1] * page)
+            if dst_block_tables[l].shape[1] * page < most:
+                raise ValueError(f"dst_block_table has {dst_block_tables[l].shape[1] * page} rows for the {most} that a "
+                                 "sequence may keep")
         check("seq_lens", seq_lens[l], torch.int32)
         if tuple(seq_lens[l].shape) != (B,) or not seq_lens[l].is_contiguous():
             raise ValueError("seq_lens must be a contiguous [B] tensor, the same B for every layer")

@@ -471,6 +471,10 @@ extern "C" int abkv_evict_by_weight(void* const* kv, const int32_t* const* block
         (dst_block_tables && dst_strides[l] <= 0))
       return ABKV_ERR_INVALID_ARG;
     if (dst_block_tables && dst_block_tables[l] == block_tables[l]) return ABKV_ERR_INVALID_ARG;
+    // rows that a sequence may keep need a place: one without would be lost with its length reported
+    const int64_t most = std::min({(int64_t)budgets[l], (int64_t)weight_rows, bt_strides[l] * page_size,
+                                   (int64_t)max_pages_per_seq * page_size});
+    if (dst_block_tables && dst_strides[l] < (most + page_size - 1) / page_size) return ABKV_ERR_INVALID_ARG;
     if (budgets[l] <= 0 || (int64_t)num_sinks + num_recent > budgets[l]) return ABKV_ERR_INVALID_ARG;
     if (new_lens[l] == seq_lens[l]) return ABKV_ERR_INVALID_ARG;  // other CTAs still read the old lengths
     if (num_blocks[l] > INT32_MAX) return ABKV_ERR_UNSUPPORTED;

@@ -428,8 +428,11 @@ int abkv_gather_rows(const void* const* src, void* const* dst, int num_tensors,
  *   weights[l][b * weight_strides[2l] + u * weight_strides[2l+1] + row] up to
  *   budgets[l] rows in all (ties to the lower row; NaN counts as -inf).
  * Kept rows stay in order: kept row i moves to row i of block_tables[l] (in
- * place: its live pages then belong to one sequence each; not checked) or, with dst_block_tables, to row i of that table's pages in the same
- * cache, which must not be pages of any source table (not checked).
+ * place: its live pages then belong to one sequence each; not checked) or, with
+ * dst_block_tables, to row i of that table's pages in the same cache, which must
+ * not be pages of any source table (not checked).  A destination table is wide
+ * enough for what a sequence may keep: the least of the budget, the source table's
+ * rows and weight_rows.
  * new_lens[l][b] = min(n, budget) (another buffer than seq_lens[l]).
  * weights_out[l] (weights[l] itself with the same strides, or a buffer that does
  * not overlap it) gets the kept rows' weights, then zeros up to weight_out_rows.

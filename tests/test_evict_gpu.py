@@ -198,3 +198,13 @@ def test_a_budget_far_above_the_rows_needs_no_memory_for_it():
     assert torch.equal(kv.nan_to_num(7.0), before.nan_to_num(7.0))
     for b, n in enumerate((40, 7)):
         assert torch.equal(e.weights[0][b, :, :n], w[b, :, :n]) and (e.weights[0][b, :, n:] == 0).all()
+
+
+def test_a_destination_without_room_is_refused():
+    c = R.Paged([40], 2, 64, 16, seed=7)
+    kv, bt, sl, w = [c.kv.cuda()], [c.table.cuda()], [c.seq.cuda()], [torch.rand((1, 2, 48)).cuda()]
+    before = bits(kv[0]).clone()
+    for width, budget in ((1, 17), (2, 33), (2, 1000)):
+        with pytest.raises(ValueError, match="dst_block_table"):
+            compaction.evict_by_weight(kv, bt, sl, w, budget=budget, dst_block_tables=[bt[0][:, :width].contiguous()])
+    assert torch.equal(bits(kv[0]), before)
