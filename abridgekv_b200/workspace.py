@@ -30,6 +30,11 @@ class Workspace:
         self._kept: list[torch.Tensor] = []
 
     @property
+    def on(self) -> torch.device:
+        """The device of the buffer (``device`` may leave its index open)."""
+        return self._buf.device
+
+    @property
     def nbytes(self) -> int:
         return self._buf.numel()
 
@@ -77,6 +82,8 @@ def call_scope(device: torch.device, stream: torch.cuda.Stream | None):
     given) its current stream, so that what the call allocates belongs to the stream that uses it.
     No context is entered where both hold already (a context costs a few microseconds)."""
     if stream is not None:
+        if stream.device != device:
+            raise ValueError(f"the stream is on {stream.device}, the call's tensors are on {device}")
         return torch.cuda.stream(stream)
     return _here if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
 
@@ -110,6 +117,8 @@ def call_workspace(device: torch.device, nbytes: int, workspace: Workspace | Non
     of your own.)"""
     raw = torch._C._cuda_getCurrentRawStream(device.index)
     if workspace is not None:
+        if workspace.on != device:
+            raise ValueError(f"the workspace is on {workspace.on}, the call's tensors are on {device}")
         return workspace.ensure(nbytes), raw
     if torch._C._cuda_isCurrentStreamCapturing():
         return Workspace(device, nbytes, zeroed=256), raw

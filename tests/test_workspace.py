@@ -2,6 +2,7 @@
 import gc
 import threading
 import weakref
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -24,6 +25,7 @@ def now(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
     real = W.Workspace.__init__
     monkeypatch.setattr(W.Workspace, "__init__", lambda self, device=None, *a, **kw: real(self, "cpu", *a, **kw))
+    monkeypatch.setattr(W.Workspace, "on", property(lambda self: DEV), raising=False)
     monkeypatch.setattr(W, "_per_device", {})
     return s
 
@@ -107,3 +109,20 @@ def test_a_captured_call_zeroes_its_header_alone(now, monkeypatch):
     now.capturing = False
     sizes.clear()
     assert not W.Workspace(DEV, 4096)._buf.any() and sizes == [4096]
+
+
+def test_streams_and_workspaces_of_another_device_are_refused(now, monkeypatch):
+    """Their kernels would run where the call's tensors are not."""
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: s)
+    here, there = (SimpleNamespace(device=torch.device("cuda", i)) for i in (0, 1))
+    assert W.call_scope(DEV, here) is here
+    with pytest.raises(ValueError, match="stream"):
+        W.call_scope(DEV, there)
+    ws = W.Workspace()
+    assert W.call_workspace(DEV, 256, ws)[0] is ws
+    with pytest.raises(ValueError, match="workspace"):
+        W.call_workspace(there.device, 256, ws)
+
+
+def test_the_device_of_a_workspace():
+    assert W.Workspace("cpu").on == torch.device("cpu")
