@@ -116,6 +116,11 @@ __device__ __forceinline__ Req load_req(const PromptParams& p, int r, bool repor
   return x;
 }
 
+// A 16-row slice hidden from every counted row is not looked up: its page may be freed.
+__device__ __forceinline__ bool hidden_slice(const PromptParams& p, const Req& x, int row0) {
+  return p.window > 0 && row0 >= p.n_sink && row0 + 16 <= x.p0 - p.window + 1;
+}
+
 // Work of one item: the contiguous range [u0, u1) of units (unit = chunk * G + head) whose rows see a row
 // of cache tile kt; empty when there is none.
 __device__ __forceinline__ void item_units(const PromptParams& p, const Req& x, int kt, bool resident, int& u0,
@@ -193,8 +198,8 @@ __device__ __forceinline__ bool item_at(const PromptParams& p, const Items& it, 
 // What every role has to know of an item; units [u0, u1) may be empty.
 struct alignas(16) Desc {
   int r, hk, kt, u0;
-  int u1, q0, nq, n;
-  int p0, valid, pad[2];
+  int u1, q0, nq, n;  // n: the request's rows, cut before the tile's first bad page
+  int p0, pad[3];
 };
 static_assert(sizeof(Desc) == 48, "ring of descriptors");
 
@@ -280,8 +285,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
     for (int base = 0; base < it.n && !dead; base += 4) {
       const int k = base + (lane >> 3), slice = lane & 7;
       int pg = -1, off = 0;
+      bool bad = false;
       Desc d;
-      d.r = d.hk = d.kt = d.u0 = d.u1 = d.q0 = d.nq = d.n = d.p0 = d.valid = d.pad[0] = d.pad[1] = 0;
+      d.r = d.hk = d.kt = d.u0 = d.u1 = d.q0 = d.nq = d.n = d.p0 = 0;
       if (k < it.n && item_at(p, it, k, d.r, d.hk, d.kt)) {
         const Req x = load_req(p, d.r, !resident && d.kt == 0 && d.hk == 0 && slice == 0);
         item_units(p, x, d.kt, resident, d.u0, d.u1);
@@ -289,22 +295,25 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
         d.nq = x.nq;
         d.n = x.n;
         d.p0 = x.p0;
-        d.valid = 1;
         const int row0 = d.kt * kM + 16 * slice;
         if (d.u0 < d.u1 && row0 < x.n) {
-          // a slice hidden from every counted row is not looked up: its page may be freed
-          const bool hidden = p.window > 0 && row0 >= p.n_sink && row0 + 16 <= x.p0 - p.window + 1;
-          if (!hidden) {
+          if (!hidden_slice(p, x, row0)) {
             pg = __ldg(p.bt + (int64_t)d.r * p.bt_stride + row0 / p.page);
             off = row0 % p.page;
             if (pg < 0 || (int64_t)pg >= p.num_blocks) {
               set_error(p.err, ABKV_DEVERR_PAGE_OOB);
               pg = -1;
+              bad = true;
             }
           }
         }
       }
       const uint32_t valid = __ballot_sync(0xffffffffu, pg >= 0), work = __ballot_sync(0xffffffffu, d.u0 < d.u1);
+      // Scores of a slice without its page are of what the ring held before.  Its rows must not collect them, and the rows
+      // behind it in the tile go without as well: a limit that the writers read anyway (checking each row's own slice
+      // there took 2 to 6% of the kernel's time).
+      const uint32_t bad8 = __ballot_sync(0xffffffffu, bad) >> (lane & 24) & 0xFFu;
+      if (bad8) d.n = min(d.n, d.kt * kM + 16 * (__ffs(bad8) - 1));
       const int grp = base / kItemGroup, gs = grp & (kItemGroups - 1);
       if (!__all_sync(0xffffffffu, wait_or_abort(&bar[kBarItemEmpty + gs], ((uint32_t)(grp / kItemGroups) & 1u) ^ 1u,
                                                  dead, p.err))) {
@@ -561,6 +570,12 @@ __global__ void prompt_weights_heads_kernel(const __grid_constant__ PromptParams
   const Req x = load_req(p, r, false);
   const int row = blockIdx.x * blockDim.x + threadIdx.x;
   if (row >= x.n || x.nq == 0) return;
+  // nor were the rows from a tile's first bad page on
+  for (int row0 = row / kM * kM; row0 <= row; row0 += 16) {
+    if (hidden_slice(p, x, row0)) continue;
+    const int pg = __ldg(p.bt + (int64_t)r * p.bt_stride + row0 / p.page);
+    if (pg < 0 || (int64_t)pg >= p.num_blocks) return;
+  }
   float acc = 0.f;
   for (int h = 0; h < p.Hkv; ++h) {
     // a tile no counted row sees was not written

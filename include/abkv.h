@@ -668,7 +668,9 @@ int abkv_paged_prefill_window(const void* q, int64_t q_row_stride,
  * (weight_units = Hkv, or 1 for all heads).  The order of the sum is fixed.
  * max_query_len >= every qlen, max_rows >= every seq_lens[r] (they bound the launch);
  * a request with seq_lens[r] < qlen, or more rows than the table, max_rows or
- * weight_rows hold, sets ABKV_DEVERR_SEQ_OOB and is not counted.  head_dim 128,
+ * weight_rows hold, sets ABKV_DEVERR_SEQ_OOB and is not counted; from a page id
+ * out of range (ABKV_DEVERR_PAGE_OOB) to the end of its 128-row tile, rows collect
+ * nothing.  head_dim 128,
  * page_size a multiple of 16. */
 size_t abkv_prompt_weights_workspace_size(int R, int num_kv_heads, int64_t max_rows,
                                           int weight_units);

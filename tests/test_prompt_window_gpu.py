@@ -204,3 +204,28 @@ def test_refusals():
         pw(case.args[0], lse, *case.args[1:], torch.zeros((1, 3, 90), device="cuda"), **kw)
     with pytest.raises(ValueError, match="overlap"):
         pw(case.args[0], lse, *case.args[1:], torch.zeros((1, 1, 90), device="cuda").expand(1, 2, 90), **kw)
+
+
+@pytest.mark.parametrize("observe", [None, 32])
+def test_rows_of_a_bad_page_collect_nothing(observe):
+    """Their scores come from whatever was loaded there before, and the accumulators outlive the call.  (Nor do the rows
+    behind it in its tile of 128.)"""
+    case = Case([300, 40], [700, 333], 2, 2, seed=12)
+    q, kv, bt, sl, qs = case.args
+    kw = dict(max_query_len=300, num_kv_heads=2, window=None, observe=observe)
+    ws = Workspace("cuda:0")
+    _, lse = codestep.paged_prefill_window(*case.args, max_query_len=300, num_kv_heads=2, window=None, return_lse=True)
+    bad = bt.clone()
+    holes = [(0, 2), (0, 30), (1, 0), (1, 20)]
+    for r, slot in holes:
+        bad[r, slot] = 10 ** 6
+    for units in (2, 1):
+        w0 = torch.rand((2, units, 720), generator=torch.Generator().manual_seed(1)).cuda()
+        want, w = w0.clone(), w0.clone()
+        codestep.paged_prompt_weights(q, lse, kv, bt, sl, qs, want, **kw)
+        codestep.paged_prompt_weights(q, lse, kv, bad, sl, qs, w, workspace=ws, **kw)
+        assert ws.read_error() == 1
+        for r, slot in holes:
+            s = slice(16 * slot, (16 * slot // 128 + 1) * 128)
+            want[r, :, s] = w0[r, :, s]
+        assert torch.equal(w, want)
