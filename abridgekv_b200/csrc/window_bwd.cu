@@ -809,11 +809,14 @@ int make_map(CUtensorMap* m, const void* base, int B, int heads, int S, int D, c
 
 constexpr size_t kWsHeader = 256;
 constexpr int kSms = 148;
-// dS is rounded to bf16 for the products of dQ and dK: one more error beside the rounding of the result, sqrt(2) of
-// that one alone where many terms average it (1.43 measured with windows of 512 to 2000).  Rows of few terms, of which
-// some dominate, come out worse (up to 1.7 over 60 random shapes), so those launches add a second product with what
-// the rounding left out (kRest: 1.25 at most).  It costs 33.0 -> 33.1 us at 333 rows of 8 heads, 377 -> 441 us at
-// 2 x 4096 rows of 32 heads with a window of 256, and would cost 497 -> 594 us with one of 1024.
+// dS is rounded to bf16 for the products of dQ and dK: one more error beside the rounding of the result, together sqrt(2)
+// of the latter alone (1.43 rms measured for rows of 128 keys and more, 1.46 for the first 128 rows of a sequence; up to
+// 1.7 for single outputs over 60 random shapes).  A launch none of whose rows sees more than kRestKeys keys adds a second product
+// with what the rounding left out (kRest: 1.04 rms, 1.25 at most).  It costs 33.0 -> 33.1 us at 333 rows of 8 heads, 377 ->
+// 441 us at 2 x 4096 rows of 32 heads with a window of 256, and would cost 497 -> 594 us with one of 1024.  The choice is
+// the launch's: the first rows of a longer one see as few keys and get one part, like its other rows.  Made by query tile it
+// gave those rows' dq 1.04 and dk 1.05, and took a step of 2 x 4096 rows with a window of 1024 from 652 to 665 us (as
+// launches of their own) or 669 (as a branch): the second part's registers, for 4% of the tiles.
 constexpr int kRestKeys = 512;
 
 template <int D, bool kRest>
