@@ -88,3 +88,50 @@ def test_gradients_from_an_output_with_its_low_bits(D, B, H, Hkv, S, window, sin
         bare = prefill.window_backward(q.cuda(), k.cuda(), v.cuda(), out, do.cuda(), lse.float().cuda(), window=window,
                                        num_sinks=sinks)
         assert ((bare[0].double().cpu() - dq).abs() > bq).any()
+
+
+def step(B, H, Hkv, S, D, window, sinks, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    leaves = [bf16((B, h, S, D), g).cuda().requires_grad_(True) for h in (H, Hkv, Hkv)]
+    do = bf16((B, H, S, D), g).cuda()
+
+    def run():
+        out = prefill.window_attention(*leaves, window=window, num_sinks=sinks)
+        return [out.detach(), *torch.autograd.grad(out, leaves, do)]
+
+    return run
+
+
+# more query tiles x heads than SMs (several items a CTA), short (clusters for dK / dV), sinks' tiles of their own launch
+REPEATS = [(2, 16, 4, 1300, 128, 300, 4), (1, 8, 2, 333, 64, 128, 1), (1, 8, 2, 4200, 64, 50, 2), (2, 8, 8, 700, 128, 1000, 0)]
+
+
+@pytest.mark.parametrize("shape", REPEATS)
+def test_gradients_repeat_bit_for_bit(shape):
+    run = step(*shape)
+    first = run()
+    for _ in range(60):
+        assert all(torch.equal(a, b) for a, b in zip(run(), first))
+
+
+def test_gradients_of_a_graph_and_of_two_streams_are_the_same_bits():
+    runs = [step(1, 16, 4, 1500, 128, 200, 3, seed=i) for i in range(2)]
+    first = [r() for r in runs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in runs]
+    for _ in range(5):
+        got = []
+        for r, s in zip(runs * 2, streams * 2):
+            with torch.cuda.stream(s):
+                got.append(r())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for i, t in enumerate(got) for a, b in zip(t, first[i % 2]))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = runs[0]()
+    for _ in range(5):
+        for t in out:
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, first[0]))
