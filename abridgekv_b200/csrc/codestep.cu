@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1) codestep_kernel(const __grid_cons
   uint64_t* p_full = bar + kBarPFull;      // [head][S buffer]
   uint64_t* o_done = bar + kBarODone;      // [head]: one phase per P.V
   uint64_t* o_full = bar + kBarOFull;      // [head]
-  uint64_t* v_zero = bar + kBarVZero;      // [sidecar, cache]: used at most once each
+  uint64_t* v_zero = bar + kBarVZero;      // [sidecar, cache], kWin: [its zeroed tiles in order]; each used at most once
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar + kBarTmem);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

@@ -88,7 +88,7 @@ __device__ __forceinline__ int evict_len(const EvictParams& p, const EvictLayer&
   return s;
 }
 
-// Exclusive prefix over the block of one value per warp's lane 0 pattern: v summed over warps before this one.
+// Inclusive prefix sum over the lanes of a warp.
 __device__ __forceinline__ int warp_incl_scan(int v) {
   const int lane = threadIdx.x & 31;
 #pragma unroll

@@ -64,9 +64,8 @@ constexpr uint32_t idesc_bf16_m128(uint32_t n, bool b_mn_major) {
          ((128u >> 4) << 24);
 }
 
-// One lane of the warp, the same every time.  Unlike lane == 0 the compiler knows that a single thread is active and
-// keeps the operands of tcgen05 and TMA instructions in uniform registers: the window backward's issuers ran 5-9%
-// faster with it.
+// One lane of the warp, the same every time.  In place of lane == 0 as the condition of a role's single thread it took the 4K
+// training step under a window from 734 to 694 us (with ring positions that are counted on instead of divided).
 static __device__ __forceinline__ bool elect_one() {
   uint32_t p;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xFFFFFFFF;\n selp.b32 %0, 1, 0, p;\n}\n" : "=r"(p));
