@@ -208,7 +208,8 @@ class AbkvAttentionImpl:
     for the step's ``num_actual_tokens`` rows and returned).
 
     ``sliding_window`` rows (None or -1: all), the query's own among them, and the first ``num_sinks``
-    rows of the cache are seen by a causal step's query."""
+    rows of the cache are seen by a causal step's query.  Such a layer's decode steps take a head_size of 64 or
+    128, its prompt rows 128 alone (NotImplementedError)."""
 
     def __init__(self, num_heads: int, head_size: int, scale: float, num_kv_heads: int | None = None,
                  alibi_slopes: Any = None, sliding_window: int | None = None, kv_cache_dtype: str = "auto",

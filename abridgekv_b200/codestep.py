@@ -205,6 +205,8 @@ def _window_rows(query, kv_cache, block_table, seq_lens, query_start_loc, num_kv
     if query.dim() != 3 or query.stride(2) != 1:
         raise ValueError("query must be [T, Hq, D] with a contiguous last dimension")
     T, Hq, D = query.shape
+    if D != 128:
+        raise NotImplementedError(f"prompt rows under a window and their weights need a head size of 128, got {D}")
     Hkv = int(num_kv_heads)
     if Hkv <= 0 or Hq % Hkv:
         raise ValueError("the KV heads must divide the query heads")
@@ -238,7 +240,7 @@ def paged_prefill_window(query: torch.Tensor, kv_cache: torch.Tensor, block_tabl
     of None or 0 shows every row j <= p.  Pages that hold no visible row are never read, and their
     block-table entries may be stale (freed pages).  ``kv_layout``: 0 for a cache [blocks, 2, page, Hkv,
     D], 1 for [2, blocks, page, Hkv, D]; None reads it off the shape, which a cache of two blocks does
-    not show.
+    not show.  Head size 128, pages of a multiple of 16 rows.
 
     Returns out [T, Hq, D], or (out, lse) with ``return_lse``: lse [T, Hq] fp32, the natural-log
     log-sum-exp of each row's scaled scores, which ``paged_prompt_weights`` takes.  Rows of no request
@@ -277,7 +279,8 @@ def paged_prompt_weights(query: torch.Tensor, lse: torch.Tensor, kv_cache: torch
     that it returned.  Request r's counted rows are its last ``observe`` query rows (None: all of them); every
     cache row that they see collects their softmax weight in ``weights`` [>=R, units, rows] fp32 (rows
     contiguous, at least as many as the longest sequence): unit u = KV head u's query heads, or one unit
-    for all heads.  The sums' order is fixed, so repeated calls give the same bits.  Returns weights."""
+    for all heads.  The sums' order is fixed, so repeated calls give the same bits.  Head size 128, pages of a
+    multiple of 16 rows.  Returns weights."""
     window, num_sinks = _window(window, num_sinks)
     obs = 0 if observe is None else int(observe)
     if observe is not None and obs <= 0:

@@ -256,7 +256,12 @@ def paged_decode_window(
     sequence of n rows sees its last ``window`` rows (its own among them) and its first
     ``num_sinks`` rows.  ``window`` and ``num_sinks`` are one number, or one per layer; a window of
     None or 0 shows every row, so layers with and without a window share a launch.  Pages that hold
-    no visible row are never read, and their block-table entries may be stale (freed pages)."""
+    no visible row are never read, and their block-table entries may be stale (freed pages).
+
+    The launch is laid out for the most rows that a sequence can show: the window and the sinks, or without a window
+    ``max_pages_per_seq`` pages (None: the block tables' width).  Where the tables are much wider than the
+    longest sequence, pass that sequence's pages (a longer one would be cut): the work is then split for them, and a weighted call's scores take
+    4 x sequences x query heads x those rows bytes of workspace a layer instead of the table's."""
     return _decode_window(queries, kv_caches, block_tables, seq_lens, None, window, num_sinks, scale, outputs,
                           max_pages_per_seq, chunk_tokens, workspace, stream)
 
@@ -282,7 +287,8 @@ def paged_decode_weighted(
     weights[l]: fp32 [>=B, units, rows], rows contiguous and at least as many as the longest
     sequence (a longer sequence sets the workspace's SEQ_OOB bit and is cut): with units = Hkv,
     unit u collects KV head u's query heads; with units = 1, all query heads.  The sums are taken in
-    head order, so repeated calls give the same bits.  ``compaction.evict_by_weight`` reads them."""
+    head order, so repeated calls give the same bits.  ``compaction.evict_by_weight`` reads them.
+    ``max_pages_per_seq``: see ``paged_decode_window``; it matters most here."""
     return _decode_window(queries, kv_caches, block_tables, seq_lens, list(weights), window, num_sinks, scale,
                           outputs, max_pages_per_seq, chunk_tokens, workspace, stream)
 

@@ -91,9 +91,12 @@ def call_scope(device: torch.device, stream: torch.cuda.Stream | None):
 _own = threading.local()  # .table: {(device index, raw stream): Workspace} of this thread
 
 
-def stream_workspace(device: torch.device, stream: torch.cuda.Stream | None = None) -> Workspace:
+def stream_workspace(device: torch.device | str, stream: torch.cuda.Stream | None = None) -> Workspace:
     """The workspace that this thread's calls without one of their own use on ``stream`` (None: the current
     stream) outside a capture.  Its error word is theirs: ``stream_workspace(device, s).read_error(s)``."""
+    device = torch.device(device)
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     with call_scope(device, stream):
         return _stream_workspace(device, torch._C._cuda_getCurrentRawStream(device.index), 256)
 

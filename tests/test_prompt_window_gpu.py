@@ -229,3 +229,14 @@ def test_rows_of_a_bad_page_collect_nothing(observe):
             s = slice(16 * slot, (16 * slot // 128 + 1) * 128)
             want[r, :, s] = w0[r, :, s]
         assert torch.equal(w, want)
+
+
+def test_other_head_sizes_are_refused_before_the_launch():
+    q = torch.zeros((4, 4, 64), dtype=torch.bfloat16, device="cuda")
+    kv = torch.zeros((5, 2, 16, 2, 64), dtype=torch.bfloat16, device="cuda")
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    args, kw = (kv, i32(1).view(1, 1), i32(4), i32(0, 4)), dict(max_query_len=4, num_kv_heads=2, window=3)
+    with pytest.raises(NotImplementedError, match="128"):
+        codestep.paged_prefill_window(q, *args, **kw)
+    with pytest.raises(NotImplementedError, match="128"):
+        codestep.paged_prompt_weights(q, torch.zeros((4, 4), device="cuda"), *args, torch.zeros((1, 2, 16), device="cuda"), **kw)
