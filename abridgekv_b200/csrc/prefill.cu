@@ -531,17 +531,6 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_kernel(const __grid_const
   }
 }
 
-// ---------------------------------------------------------------------------
-// [B][heads][S][D] bf16 with element strides (sb, sh, ss) -> 4D tensor map,
-// box = 64 dims x box_rows rows, 128B swizzle.
-int make_map(CUtensorMap* m, const void* base, int B, int heads, int S, int D, const int64_t* strides,
-             int box_rows) {
-  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)heads, (cuuint64_t)B};
-  const cuuint64_t gstr[3] = {(cuuint64_t)strides[2] * 2, (cuuint64_t)strides[1] * 2, (cuuint64_t)strides[0] * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
-  return tc::encode_tiled_4d(m, base, dims, gstr, box);
-}
-
 }  // namespace
 }  // namespace abkv
 
@@ -566,10 +555,10 @@ extern "C" int abkv_prefill_masked(const void* q, const int64_t* q_strides, cons
     return ABKV_ERR_WORKSPACE;
   PrefillParams prm;
   std::memset(&prm, 0, sizeof(prm));
-  int st = make_map(&prm.tm_q, q, B, H, S, head_dim, q_strides, kBM);
-  if (st == ABKV_OK) st = make_map(&prm.tm_k, k, B, Hkv, S, head_dim, k_strides, kBN);
-  if (st == ABKV_OK) st = make_map(&prm.tm_v, v, B, Hkv, S, head_dim, v_strides, kBN);
-  if (st == ABKV_OK) st = make_map(&prm.tm_out, out, B, H, S, head_dim, out_strides, kBM);
+  int st = tc::encode_bhsd(&prm.tm_q, q, B, H, S, head_dim, q_strides, kBM);
+  if (st == ABKV_OK) st = tc::encode_bhsd(&prm.tm_k, k, B, Hkv, S, head_dim, k_strides, kBN);
+  if (st == ABKV_OK) st = tc::encode_bhsd(&prm.tm_v, v, B, Hkv, S, head_dim, v_strides, kBN);
+  if (st == ABKV_OK) st = tc::encode_bhsd(&prm.tm_out, out, B, H, S, head_dim, out_strides, kBM);
   if (st != ABKV_OK) return st;
   prm.out = static_cast<__nv_bfloat16*>(out);
   prm.o_sb = out_strides[0];
@@ -623,10 +612,10 @@ extern "C" int abkv_window_attention(const void* q, const int64_t* q_strides, co
     return ABKV_ERR_WORKSPACE;
   PrefillParams prm;
   std::memset(&prm, 0, sizeof(prm));
-  int st = make_map(&prm.tm_q, q, B, H, S, head_dim, q_strides, kBM);
-  if (st == ABKV_OK) st = make_map(&prm.tm_k, k, B, Hkv, S, head_dim, k_strides, kBN);
-  if (st == ABKV_OK) st = make_map(&prm.tm_v, v, B, Hkv, S, head_dim, v_strides, kBN);
-  if (st == ABKV_OK) st = make_map(&prm.tm_out, out, B, H, S, head_dim, out_strides, kBM);
+  int st = tc::encode_bhsd(&prm.tm_q, q, B, H, S, head_dim, q_strides, kBM);
+  if (st == ABKV_OK) st = tc::encode_bhsd(&prm.tm_k, k, B, Hkv, S, head_dim, k_strides, kBN);
+  if (st == ABKV_OK) st = tc::encode_bhsd(&prm.tm_v, v, B, Hkv, S, head_dim, v_strides, kBN);
+  if (st == ABKV_OK) st = tc::encode_bhsd(&prm.tm_out, out, B, H, S, head_dim, out_strides, kBM);
   if (st != ABKV_OK) return st;
   prm.lse = lse;
   prm.out_lo = static_cast<int8_t*>(out_lo);

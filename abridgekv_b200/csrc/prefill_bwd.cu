@@ -850,14 +850,6 @@ __global__ void dq_store_kernel(const float* __restrict__ acc, __nv_bfloat16* dq
   *reinterpret_cast<uint4*>(dq + b * sb + h * sh + q * ss + d0) = pk;
 }
 
-int make_map(CUtensorMap* m, const void* base, int B, int heads, int S, int D, const int64_t* strides,
-             int box_rows) {
-  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)heads, (cuuint64_t)B};
-  const cuuint64_t gstr[3] = {(cuuint64_t)strides[2] * 2, (cuuint64_t)strides[1] * 2, (cuuint64_t)strides[0] * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
-  return tc::encode_tiled_4d(m, base, dims, gstr, box);
-}
-
 constexpr size_t kWsHeader = 256;
 size_t bwd_workspace(int B, int H, int S, int D) {
   const size_t rows = (size_t)B * H * S;
@@ -911,10 +903,10 @@ extern "C" int abkv_prefill_masked_backward(
   std::memset(&prm, 0, sizeof(prm));
   // head_dim 128 runs the 64-query-unit kernel: Q, dO and dQ move in 64-row boxes
   const int qrows = head_dim == 128 ? kU : kT;
-  int st = make_map(&prm.tm_q, q, B, H, S, head_dim, q_strides, qrows);
-  if (st == ABKV_OK) st = make_map(&prm.tm_do, dout, B, H, S, head_dim, dout_strides, qrows);
-  if (st == ABKV_OK) st = make_map(&prm.tm_k, k, B, Hkv, S, head_dim, k_strides, kT);
-  if (st == ABKV_OK) st = make_map(&prm.tm_v, v, B, Hkv, S, head_dim, v_strides, kT);
+  int st = tc::encode_bhsd(&prm.tm_q, q, B, H, S, head_dim, q_strides, qrows);
+  if (st == ABKV_OK) st = tc::encode_bhsd(&prm.tm_do, dout, B, H, S, head_dim, dout_strides, qrows);
+  if (st == ABKV_OK) st = tc::encode_bhsd(&prm.tm_k, k, B, Hkv, S, head_dim, k_strides, kT);
+  if (st == ABKV_OK) st = tc::encode_bhsd(&prm.tm_v, v, B, Hkv, S, head_dim, v_strides, kT);
   if (st == ABKV_OK) {
     const cuuint64_t dims[2] = {(cuuint64_t)head_dim, (cuuint64_t)rows};
     const cuuint64_t gstr[1] = {(cuuint64_t)head_dim * 4};

@@ -203,14 +203,6 @@ struct alignas(16) Desc {
 };
 static_assert(sizeof(Desc) == 48, "ring of descriptors");
 
-// a * b + c on a pair with one b.
-__device__ __forceinline__ void scale_add(float& d0, float& d1, float a0, float a1, float b, float c0, float c1) {
-  asm("{\n .reg .b64 x, y, z, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mov.b64 z, {%5, %6};\n"
-      " fma.rn.f32x2 r, x, y, z;\n mov.b64 {%0, %1}, r;\n}\n"
-      : "=f"(d0), "=f"(d1)
-      : "f"(a0), "f"(a1), "f"(b), "f"(c0), "f"(c1));
-}
-
 __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __grid_constant__ PromptParams p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -501,8 +493,8 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_weights_kernel(const __gri
                 for (int c = 0; c < 32; c += 4) {
                   const float4 l = *reinterpret_cast<const float4*>(l4 + c);
                   float x0, x1, x2, x3;
-                  scale_add(x0, x1, s[c], s[c + 1], sl2, l.x, l.y);
-                  scale_add(x2, x3, s[c + 2], s[c + 3], sl2, l.z, l.w);
+                  ffma2(x0, x1, s[c], s[c + 1], sl2, l.x, l.y);
+                  ffma2(x2, x3, s[c + 2], s[c + 3], sl2, l.z, l.w);
                   fadd2(acc[0], acc[1], fast_exp2(x0), fast_exp2(x1));
                   fadd2(acc[2], acc[3], fast_exp2(x2), fast_exp2(x3));
                 }

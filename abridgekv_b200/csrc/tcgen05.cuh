@@ -20,6 +20,12 @@ static __device__ __forceinline__ void ffma2(float& d0, float& d1, float a0, flo
       : "=f"(d0), "=f"(d1)
       : "f"(a0), "f"(a1), "f"(b), "f"(c));
 }
+static __device__ __forceinline__ void ffma2(float& d0, float& d1, float a0, float a1, float b, float c0, float c1) {
+  asm("{\n .reg .b64 x, y, z, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mov.b64 z, {%5, %6};\n"
+      " fma.rn.f32x2 r, x, y, z;\n mov.b64 {%0, %1}, r;\n}\n"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b), "f"(c0), "f"(c1));
+}
 static __device__ __forceinline__ void fadd2(float& d0, float& d1, float a0, float a1) {
   asm("{\n .reg .b64 x, y, r;\n mov.b64 x, {%0, %1};\n mov.b64 y, {%2, %3};\n"
       " add.rn.f32x2 r, x, y;\n mov.b64 {%0, %1}, r;\n}\n"
@@ -272,6 +278,15 @@ static inline int encode_tiled(CUtensorMap* m, CUtensorMapDataType dtype, int ra
 static inline int encode_tiled_4d(CUtensorMap* m, const void* base, const cuuint64_t (&dims)[4],
                                   const cuuint64_t (&gstr)[3], const cuuint32_t (&box)[4]) {
   return encode_tiled(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, gstr, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Map of a bf16 [B][heads][S][D] tensor with element strides (batch, head, row): boxes of box_rows rows x 64 dims.
+static inline int encode_bhsd(CUtensorMap* m, const void* base, int B, int heads, int S, int D, const int64_t* strides,
+                              int box_rows) {
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)heads, (cuuint64_t)B};
+  const cuuint64_t gstr[3] = {(cuuint64_t)strides[2] * 2, (cuuint64_t)strides[1] * 2, (cuuint64_t)strides[0] * 2};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  return encode_tiled_4d(m, base, dims, gstr, box);
 }
 
 }  // namespace tc

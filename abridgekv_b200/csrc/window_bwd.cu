@@ -131,13 +131,7 @@ __device__ __forceinline__ void alloc_tmem(uint32_t* s_tmem) {
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n");
 }
 
-// x = a * b + c on a pair with one b and a pair of c; (a - b) * c on pairs.
-__device__ __forceinline__ void fma_pair(float& d0, float& d1, float a0, float a1, float b, float c0, float c1) {
-  asm("{\n .reg .b64 x, y, z, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %4};\n mov.b64 z, {%5, %6};\n"
-      " fma.rn.f32x2 r, x, y, z;\n mov.b64 {%0, %1}, r;\n}\n"
-      : "=f"(d0), "=f"(d1)
-      : "f"(a0), "f"(a1), "f"(b), "f"(c0), "f"(c1));
-}
+// (a - b) * c on pairs.
 __device__ __forceinline__ void sub_mul_pair(float& d0, float& d1, float a0, float a1, float b0, float b1, float c0,
                                              float c1) {
   asm("{\n .reg .b64 x, y, z, r;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
@@ -395,8 +389,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkdv_kernel(const __grid_c
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
             const float4 l = *reinterpret_cast<const float4*>(s_lse + c);
-            fma_pair(pv[c], pv[c + 1], pv[c], pv[c + 1], sl2, l.x, l.y);
-            fma_pair(pv[c + 2], pv[c + 3], pv[c + 2], pv[c + 3], sl2, l.z, l.w);
+            ffma2(pv[c], pv[c + 1], pv[c], pv[c + 1], sl2, l.x, l.y);
+            ffma2(pv[c + 2], pv[c + 3], pv[c + 2], pv[c + 3], sl2, l.z, l.w);
 #pragma unroll
             for (int j = 0; j < 4; ++j) pv[c + j] = fast_exp2(pv[c + j]);
           }
@@ -800,13 +794,6 @@ __global__ void __launch_bounds__(256) window_rowdot_kernel(const __nv_bfloat16*
   if (live && d0 == 0) di[rr] = acc;
 }
 
-int make_map(CUtensorMap* m, const void* base, int B, int heads, int S, int D, const int64_t* strides) {
-  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)S, (cuuint64_t)heads, (cuuint64_t)B};
-  const cuuint64_t gstr[3] = {(cuuint64_t)strides[2] * 2, (cuuint64_t)strides[1] * 2, (cuuint64_t)strides[0] * 2};
-  const cuuint32_t box[4] = {64, (cuuint32_t)kT, 1, 1};
-  return tc::encode_tiled_4d(m, base, dims, gstr, box);
-}
-
 constexpr size_t kWsHeader = 256;
 constexpr int kSms = 148;
 // dS is rounded to bf16 for the products of dQ and dK: one more error beside the rounding of the result, together sqrt(2)
@@ -915,10 +902,10 @@ extern "C" int abkv_window_attention_backward(
     return ABKV_ERR_WORKSPACE;
   WinBwdParams prm;
   std::memset(&prm, 0, sizeof(prm));
-  int st = make_map(&prm.tm_q, q, B, H, S, head_dim, q_strides);
-  if (st == ABKV_OK) st = make_map(&prm.tm_do, dout, B, H, S, head_dim, dout_strides);
-  if (st == ABKV_OK) st = make_map(&prm.tm_k, k, B, Hkv, S, head_dim, k_strides);
-  if (st == ABKV_OK) st = make_map(&prm.tm_v, v, B, Hkv, S, head_dim, v_strides);
+  int st = tc::encode_bhsd(&prm.tm_q, q, B, H, S, head_dim, q_strides, kT);
+  if (st == ABKV_OK) st = tc::encode_bhsd(&prm.tm_do, dout, B, H, S, head_dim, dout_strides, kT);
+  if (st == ABKV_OK) st = tc::encode_bhsd(&prm.tm_k, k, B, Hkv, S, head_dim, k_strides, kT);
+  if (st == ABKV_OK) st = tc::encode_bhsd(&prm.tm_v, v, B, Hkv, S, head_dim, v_strides, kT);
   if (st != ABKV_OK) return st;
   float* di = reinterpret_cast<float*>(static_cast<char*>(workspace) + kWsHeader);
   prm.lse = lse;

@@ -260,8 +260,9 @@ def paged_decode_window(
 
     The launch is laid out for the most rows that a sequence can show: the window and the sinks, or without a window
     ``max_pages_per_seq`` pages (None: the block tables' width).  Where the tables are much wider than the
-    longest sequence, pass that sequence's pages (a longer one would be cut): the work is then split for them, and a weighted call's scores take
-    4 x sequences x query heads x those rows bytes of workspace a layer instead of the table's."""
+    longest sequence, pass that sequence's pages (a longer one would be cut): the work is then split for
+    them, and a weighted call's scores take 4 x sequences x query heads x those rows bytes of workspace a layer
+    instead of the table's."""
     return _decode_window(queries, kv_caches, block_tables, seq_lens, None, window, num_sinks, scale, outputs,
                           max_pages_per_seq, chunk_tokens, workspace, stream)
 

@@ -114,10 +114,11 @@ def call_workspace(device: torch.device, nbytes: int, workspace: Workspace | Non
     else one that no other stream, no other thread and no CUDA graph uses.
 
     A call may be several launches with data in the workspace between them, and another thread's launches may
-    come in between on the same stream, so every thread has a buffer per stream (``stream_workspace``), apart from
-    ``default_workspace``, which other entries use on any stream.  A call under stream capture gets a fresh one from the graph's memory pool, its header zeroed at every replay (the entries that
-    come here write the rest before they read it): two graphs never share it, and no later growth frees it under them.  (To read the error word of a captured call, pass a workspace
-    of your own.)"""
+    come in between on the same stream, so every thread has a buffer per stream (``stream_workspace``), apart
+    from ``default_workspace``, which other entries use on any stream.  A call under stream capture gets a
+    fresh one from the graph's memory pool, its header zeroed at every replay (the entries that come here write
+    the rest before they read it): two graphs never share it, and no later growth frees it under them.  (To read
+    the error word of a captured call, pass a workspace of your own.)"""
     raw = torch._C._cuda_getCurrentRawStream(device.index)
     if workspace is not None:
         if workspace.on != device:
