@@ -15,7 +15,7 @@
 // move: bound by memory, so as many bytes in flight as fit: rows go through a shared-memory ring (see
 // evict_move_kernel).
 // Measured: 4 layers x 16 sequences of 5003 to 8190 rows to 4096 (2.15 GB with both directions) 392 us, 5.5 TB/s
-// of 6.53 measured for a copy; one sequence of 1311 rows to 1024 15 us, which is two launches and the selection's
+// of 6.53 measured for a copy; one sequence of 1311 rows to 1024 16 us, which is two launches and the selection's
 // three passes, one after another.
 #include <algorithm>
 #include <cstring>

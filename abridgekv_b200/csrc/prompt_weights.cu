@@ -22,7 +22,7 @@
 // The exponentials bound it: 128 x 128 of them take 1024 clocks of the SM's 16 a clock, the tile's MMAs 512
 // (head_dim 128); a step takes about 1800, as four warps an SM quarter do not hide each other's loads and
 // hand-overs.  Measured: 2 x 4050 rows, 32 heads, all counted 219 us (117 of exponentials); the last 32 rows
-// of 4 requests over 8065 rows 23 us.  Tried and no faster: half of the exponentials, or a quarter, as
+// of 4 requests over 8065 rows 24 us.  Tried and no faster: half of the exponentials, or a quarter, as
 // polynomials on the FMA pipe (238 and 222 us), scores in halves of 64 columns with an issuer for every
 // second step (246 us), the next 32 columns loaded ahead (343 us, out of registers).
 // Work items are (cache tile, KV head, request); a CTA per SM takes them round robin to and fro, the cache
